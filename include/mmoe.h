@@ -20,7 +20,8 @@ extern "C" {
 
 /* Version of the structures and functions below, raised whenever one of them changes: a structure that grows is written past
  * its end for a host compiled against the earlier header.  Compare with mmoe_abi_version() before anything else.
- * 3: MmoeOptions.residual.  4: MmoeLayout.shared_tile_sf, mmoe_split_halves. */
+ * 3: MmoeOptions.residual.  4: MmoeLayout.shared_tile_sf, mmoe_split_halves; since then the dense feed-forward operators have come, which
+ * change nothing for a host that does not call them. */
 #define MMOE_ABI_VERSION 4
 
 enum {
@@ -280,6 +281,68 @@ int mmoe_split_halves(const void* src, void* dst, int32_t num_groups, int64_t ha
  * and 22 GEMM1 / GEMM2 on CTA pairs (role: the warp), 10 + b barrier b of the peer exchange (role: the rank that did not arrive).
  * A call that gave up leaves the workspace fit for the next one.  Replaces the reference's device `trap` after a 300 s spin (backend/kernel/comm.py:229-250). */
 int mmoe_read_status(const MmoeGeometry* geo, void* workspace, int32_t* words8, void* stream);
+
+/* ---- Dense feed-forward operators (no counterpart in the reference): the gated block of a model's dense layers, or of a shared expert that is
+ * not MXFP8, in 16 bits with its gradients, and its products in 8-bit integers.  They need no workspace and no geometry.  `status` of each
+ * call: int32 [8] device words, zero before their first use, in which a wait that expired is recorded as in a workspace (kernels 31 and
+ * 32); kept by the caller, one set per device is enough.  Pointers are 16-byte aligned, and so is the start of every row. */
+enum { MMOE_BF16 = 0, MMOE_FP16 = 1, MMOE_INT8 = 2, MMOE_FP32 = 3 };
+
+/* Once per device, with that device current and outside stream capture, before any of the calls below but mmoe_quantize_int8 there. */
+int mmoe_dense_prepare(void* stream);
+
+/* y = h w2^T with h = silu(min(x wg^T, clamp)) * clip(x wu^T, -clamp, clamp), w13 = [wg; wu] in checkpoint order (no interleave). */
+typedef struct MmoeFeedForward {
+  int32_t type;               /* MMOE_BF16 or MMOE_FP16: x, w13, w2, h, y and their gradients */
+  int32_t hidden;             /* H, a multiple of 8 */
+  int32_t intermediate;       /* I, a multiple of 8 */
+  int32_t num_tokens;         /* M */
+  float clamp;                /* +inf: none */
+  int32_t timeout_ms;         /* bound of every device-side wait; <= 0 selects the default (2000) */
+  int64_t x_stride;           /* elements between the rows of x, >= H and a multiple of 8 */
+  const void* x;              /* [M, H] */
+  const void* w13;            /* [2I, H] */
+  const void* w2;             /* [H, I] */
+  void* h;                    /* [M, I], rounded to the type: the second product's operand */
+  float* preact;              /* float [M, 2I]: x w13^T, unrounded, for the backward call; NULL: not kept */
+  void* y;                    /* [M, H] */
+  int32_t* status;
+} MmoeFeedForward;
+int mmoe_feed_forward(const MmoeFeedForward* ff, void* stream);
+/* Gradients, from the h and preact that mmoe_feed_forward left and dy [M, H] (contiguous).  dpre [M, 2I]: scratch, the gradients of the
+ * two products rounded to the type; needed where dx or dw13 are asked for.  dx [M, H], dw13 [2I, H], dw2 [H, I]: NULL where not
+ * wanted (ff->preact may be NULL where only dw2 is, ff->h where it is not). */
+int mmoe_feed_forward_grad(const MmoeFeedForward* ff, const void* dy, void* dpre, void* dx, void* dw13, void* dw2, void* stream);
+
+/* Per-token quantiser: scale = max|x| / 127 (1 for a row of zeros), q = x / scale to the nearest whole number, ties to even, by that scale
+ * as it is in FP32.  A row that holds an infinity or a NaN gets the scale NaN and zeros.  x: `type` BF16 or FP16, [M, K] with
+ * `x_stride` elements between rows, any K; q int8 [M, K]; scales float [M]. */
+int mmoe_quantize_int8(const void* x, int32_t type, int64_t x_stride, void* q, float* scales, int32_t num_tokens, int32_t width, void* stream);
+
+/* Products of 8-bit integers with a scale per token and per channel; the sums are exact. */
+typedef struct MmoeInt8Product {
+  int32_t num_tokens;         /* M */
+  int32_t width;              /* K, a multiple of 16, at most 131072 */
+  int32_t channels;           /* N: rows of w (projection), or half of them (gated) */
+  int32_t out_type;           /* MMOE_BF16, MMOE_FP16 or MMOE_FP32 */
+  float clamp;                /* gated only; +inf: none */
+  int32_t timeout_ms;
+  int64_t x_stride;           /* bytes between the rows of x, >= K and a multiple of 16 */
+  const void* x;              /* int8 [M, K] */
+  const float* x_scales;      /* [M] */
+  const void* w;              /* int8 [N, K]; gated: [2N, K], the gate's rows first */
+  const float* w_scales;      /* one per row of w */
+  const float* bias;          /* projection only: [N] or NULL */
+  void* out;                  /* [M, N], contiguous */
+  int32_t* status;
+} MmoeInt8Product;
+/* out = (x w^T) * x_scales[m] * w_scales[n] + bias[n] */
+int mmoe_int8_projection(const MmoeInt8Product* p, void* stream);
+/* g and u as above without bias; out = silu(min(g, clamp)) * clip(u, -clamp, clamp) */
+int mmoe_int8_gated_projection(const MmoeInt8Product* p, void* stream);
+
+/* mmoe_read_status for the words of these calls. */
+int mmoe_dense_read_status(int32_t* status, int32_t* words8, void* stream);
 
 /* Process-wide tuning of the tensor-core kernels (the reference keeps such knobs in `KernelOptions`,
  * backend/frontend.py:72-116).  `max_stages`: cap on the shared-memory pipeline depth of the weights-as-A kernels (0: no

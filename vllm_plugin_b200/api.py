@@ -106,6 +106,62 @@ def prepare_megamoe_nvfp4_inputs(hidden_states, global_scale: float, out=None):
     return _impl(hidden_states, global_scale, out)
 
 
+def gated_feed_forward(x, w13, w2, *, activation_clamp: Optional[float] = None):
+    """Gated feed-forward block of a dense layer, or of a shared expert that is not MXFP8, with its gradients (no counterpart in
+    the reference): ``y = h w2^T`` with ``h = silu(min(g, c)) * clip(u, -c, c)``, ``g = x wg^T``, ``u = x wu^T``.
+
+    ``x``: BF16 or FP16 ``(..., H)``, any strides (rows that are not dense or do not start on 16 bytes are copied).  ``w13``: ``(2 I, H)``
+    in checkpoint order, the gate's rows first; ``w2``: ``(H, I)``; both contiguous and of x's type; H and I multiples of 8.
+    ``activation_clamp``: ``c``, none by default.  Returns ``(..., H)`` of the same type.
+
+    Sums are FP32.  ``h`` is rounded to the type, as the second product's operand, and so are the gradients of g and u in the backward
+    pass; g and u themselves are kept for it in FP32.  A value on the border of the clamp passes its gradient, one beyond it does not.
+    First derivatives only.  A training step can be captured into a CUDA graph behind a first call, but not while the graph of an eager
+    call with the same leaves is alive (``RuntimeError``)."""
+    from .backend.dense import gated_feed_forward as _impl
+
+    return _impl(x, w13, w2, activation_clamp=activation_clamp)
+
+
+def prepare_int8_inputs(hidden_states, out=None):
+    """Per-token 8-bit quantiser of BF16 or FP16 hidden states ``(..., K)``; returns ``(int8 (..., K), float32 scales (...))``.
+    ``scale = max|x| / 127`` (1 for a row of zeros), values ``x / scale`` rounded to the nearest, ties to even.  A row that holds an infinity or
+    a NaN gets the scale NaN and zeros, so that what is computed from it is NaN.  ``out``: the two tensors, contiguous."""
+    from .backend.dense import prepare_int8_inputs as _impl
+
+    return _impl(hidden_states, out)
+
+
+def int8_projection(x, x_scales, w, w_scales, *, bias=None, out_dtype=None):
+    """``(x w^T) * x_scales[..., None] * w_scales + bias`` with exact integer sums: ``x`` int8 ``(..., K)`` with float32 scales ``(...)``, ``w`` int8
+    ``(N, K)`` with ``(N,)``, optional ``bias`` float32 ``(N,)``; K a multiple of 16 below 131072.  ``out_dtype``: BF16 (default), FP16 or
+    FP32.  No gradient."""
+    import torch
+
+    from .backend.dense import int8_projection as _impl
+
+    return _impl(x, x_scales, w, w_scales, bias=bias, out_dtype=torch.bfloat16 if out_dtype is None else out_dtype)
+
+
+def int8_gated_projection(x, x_scales, w13, w13_scales, *, activation_clamp: Optional[float] = None, out_dtype=None):
+    """The first half of a gated feed-forward block in 8-bit integers: both products (``w13`` int8 ``(2 I, K)``, the gate's rows first, scales
+    ``(2 I,)``), the activation and their product in one kernel, ``silu(min(g, c)) * clip(u, -c, c)`` in ``(..., I)``.  Quantise it with
+    :func:`prepare_int8_inputs` for :func:`int8_projection`.  Otherwise as there."""
+    import torch
+
+    from .backend.dense import int8_gated_projection as _impl
+
+    return _impl(x, x_scales, w13, w13_scales, activation_clamp=activation_clamp,
+                 out_dtype=torch.bfloat16 if out_dtype is None else out_dtype)
+
+
+def read_dense_status(device=None) -> None:
+    """:func:`read_status` of the dense operators' calls on ``device`` (default: the current one)."""
+    from .backend.dense import read_dense_status as _impl
+
+    return _impl(device)
+
+
 def precompile_mega_moe_variants(num_ranks: int, num_experts: int, num_max_tokens_per_rank: int, num_topk: int,
                                  hidden: int, intermediate_hidden: int, num_shared_experts: int = 0, *,
                                  activation_clamp: Optional[float] = None, activation_alpha: float = 1.0,
@@ -180,4 +236,5 @@ __all__ = [
     "route_and_stage_inputs_for_mega_moe", "prepare_megamoe_nvfp4_inputs",
     "precompile_mega_moe_variants", "set_kernel_options", "get_kernel_options", "is_localization_available",
     "get_balanced_sm_locality_domains", "localize", "localize_mega_moe_weights", "read_status", "SymmBuffer",
+    "gated_feed_forward", "prepare_int8_inputs", "int8_projection", "int8_gated_projection", "read_dense_status",
 ]

@@ -4,7 +4,7 @@ Sub-modules are imported on first use so that importing the package needs neithe
 import importlib
 from typing import Any
 
-_SUBMODULES = ("heuristics", "workspace", "weights", "staging", "frontend", "locality", "_native")
+_SUBMODULES = ("heuristics", "workspace", "weights", "staging", "frontend", "dense", "locality", "_native")
 
 
 def __getattr__(name: str) -> Any:

@@ -34,6 +34,8 @@ EXPORTED_SYMBOLS = (
     "mmoe_experts_ep_return", "mmoe_forward_ep", "mmoe_transform_weights",
     "mmoe_plan_shared", "mmoe_experts_select", "mmoe_route_stage_inputs", "mmoe_stage_inputs_nvfp4",
     "mmoe_combine_residual", "mmoe_split_halves",
+    "mmoe_dense_prepare", "mmoe_feed_forward", "mmoe_feed_forward_grad", "mmoe_quantize_int8", "mmoe_int8_projection",
+    "mmoe_int8_gated_projection", "mmoe_dense_read_status",
 )
 
 
@@ -65,6 +67,20 @@ class MmoeOptions(ctypes.Structure):
     _fields_ = [("activation_clamp", ctypes.c_float), ("fast_math", ctypes.c_int32), ("engine", ctypes.c_int32),
                 ("timeout_ms", ctypes.c_int32), ("layer_mask", ctypes.c_int32), ("residual", ctypes.c_void_p)]
 
+
+class MmoeFeedForward(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("type", "hidden", "intermediate", "num_tokens")] + [
+        ("clamp", ctypes.c_float), ("timeout_ms", ctypes.c_int32), ("x_stride", ctypes.c_int64)] + [
+        (n, ctypes.c_void_p) for n in ("x", "w13", "w2", "h", "preact", "y", "status")]
+
+
+class MmoeInt8Product(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("num_tokens", "width", "channels", "out_type")] + [
+        ("clamp", ctypes.c_float), ("timeout_ms", ctypes.c_int32), ("x_stride", ctypes.c_int64)] + [
+        (n, ctypes.c_void_p) for n in ("x", "x_scales", "w", "w_scales", "bias", "out", "status")]
+
+
+MMOE_BF16, MMOE_FP16, MMOE_INT8, MMOE_FP32 = range(4)
 
 _lib: Optional[ctypes.CDLL] = None
 _raw_stream = None
@@ -121,6 +137,14 @@ def load() -> ctypes.CDLL:
     lib.mmoe_experts_ep_return.argtypes = [geo_p, vp, ctypes.POINTER(vp), ctypes.POINTER(MmoeWeights),
                                            ctypes.POINTER(MmoeOptions), i32, i32, vp]
     lib.mmoe_route_order_noalloc.argtypes = [vp, i32, i32, i32, vp, vp, vp, vp, vp]
+    ff_p, i8_p = ctypes.POINTER(MmoeFeedForward), ctypes.POINTER(MmoeInt8Product)
+    lib.mmoe_dense_prepare.argtypes = [vp]
+    lib.mmoe_feed_forward.argtypes = [ff_p, vp]
+    lib.mmoe_feed_forward_grad.argtypes = [ff_p, vp, vp, vp, vp, vp, vp]
+    lib.mmoe_quantize_int8.argtypes = [vp, i32, ctypes.c_int64, vp, vp, i32, i32, vp]
+    lib.mmoe_int8_projection.argtypes = [i8_p, vp]
+    lib.mmoe_int8_gated_projection.argtypes = [i8_p, vp]
+    lib.mmoe_dense_read_status.argtypes = [vp, ctypes.POINTER(i32), vp]
     for name in EXPORTED_SYMBOLS:
         fn = getattr(lib, name)
         if fn.restype is not ctypes.c_char_p:

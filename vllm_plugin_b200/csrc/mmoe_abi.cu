@@ -126,6 +126,8 @@ float bf16_round_host(float v) {
 
 }  // namespace
 
+int mmoe::record_failure(int code, const char* detail) { return fail(code, "%s", detail); }
+
 extern "C" {
 
 int mmoe_abi_version(void) { return MMOE_ABI_VERSION; }

@@ -443,6 +443,7 @@ cudaError_t launch_combine(const Ctx& c, void* y, const void* residual, int m, c
 cudaError_t zero_counters(const Ctx& c, cudaStream_t s);   // what the combine of a single-GPU call zeroes, for a call whose combine was not launched
 cudaError_t launch_experts_simt(const Ctx& c, const MmoeWeights& w, const MmoeOptions& o, int m, int block_m, cudaStream_t s);
 cudaError_t launch_experts_umma(const Ctx& c, const MmoeWeights& w, const MmoeOptions& o, int m, int block_m, cudaStream_t s);
+int record_failure(int code, const char* detail);   // what mmoe_last_error() returns on this thread from now on; returns the code
 int prepare_umma(const MmoeGeometry& geo);   // returns an MMOE_* code
 bool tc_ready();                             // prepare_umma() has run on the current device
 void set_tuning(int max_stages, int orientation);

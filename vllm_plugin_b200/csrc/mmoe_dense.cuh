@@ -1,0 +1,150 @@
+// Products of the dense feed-forward operators: D[m, n] = sum_k A[m, k] B[n, k] in 16 bits (FP32 sums) or in 8-bit integers (exact
+// 32-bit sums), with the arithmetic that follows a product done on its sums before they leave the SM.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "mmoe_common.cuh"
+
+namespace mmoe {
+
+enum DenseType { kDenseBf16 = 0, kDenseFp16 = 1, kDenseInt8 = 2, kDenseFp32 = 3 };
+
+// What becomes of the sums.
+//   kLinear     out[m, n] = s [* row_scale[m] * col_scale[n]] [+ bias[n]]
+//   kGated      B holds `inter` gate rows and then `inter` up rows; out[m, i] = silu(min(g, c)) * clip(u, -c, c), and, for a backward
+//               pass, preact[m, i] = g, preact[m, inter + i] = u
+//   kGatedGrad  the sums are the gradient of kGated's output: out[m, i] = that of g, out[m, inter + i] = that of u
+enum DenseEpilogueKind { kLinear = 0, kGated = 1, kGatedGrad = 2 };
+
+struct DenseEpilogue {
+  void* out;
+  int64_t ld_out;
+  int32_t out_type;
+  int32_t inter;             // kGated, kGatedGrad
+  const float* row_scale;    // 8-bit integers: one per row of A ...
+  const float* col_scale;    // ... and of B
+  const float* bias;
+  float* preact;             // float [m, 2 inter]; written by kGated unless null, read by kGatedGrad
+  float clamp;               // +inf: none
+};
+
+// An operand [rows, k]: row-major with `ld` elements between rows, or (k_rows) stored as its transpose, `ld` elements between the k's.
+struct DenseOperand {
+  const void* p;
+  int64_t ld;
+  bool k_rows;
+};
+
+struct DenseProduct {
+  DenseOperand a, b;
+  int32_t m, n, k;           // n: columns of the output; kGated multiplies 2 n rows of B
+  int32_t type;              // of both operands
+  int32_t kind;
+  DenseEpilogue epi;
+  int32_t* status;           // int32 [8], see kStatusTimeout
+  int32_t timeout_ms;        // of every wait; <= 0: the default
+};
+
+cudaError_t prepare_dense();   // once per device, outside stream capture
+
+cudaError_t launch_dense(const DenseProduct& p, cudaStream_t s);
+cudaError_t launch_quantize_int8(const void* x, int type, int64_t ld, int8_t* q, float* scales, int m, int k, cudaStream_t s);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float clip_above(float v, float c) { return v > c ? c : v; }                    // NaN stays NaN
+__device__ __forceinline__ float clip_both(float v, float c) { return v > c ? c : (v < -c ? -c : v); }
+
+// silu(min(g, c)) * clip(u, -c, c)
+__device__ __forceinline__ float gated_value(float g, float u, float c) {
+  const float gc = clip_above(g, c);
+  return __fdividef(gc, 1.f + __expf(-gc)) * clip_both(u, c);
+}
+
+// Its derivatives, times the gradient dh of its value.  A clipped input has none; one on the border has.
+__device__ __forceinline__ void gated_grad(float dh, float g, float u, float c, float& dg, float& du) {
+  const float gc = clip_above(g, c), s = __fdividef(1.f, 1.f + __expf(-gc));
+  dg = g > c ? 0.f : dh * clip_both(u, c) * (s * (1.f + gc * (1.f - s)));
+  du = fabsf(u) > c ? 0.f : dh * (gc * s);
+}
+
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Eight neighbouring values of one row, of which the first `valid` exist.  16-byte stores where all do and the place allows it.
+template <typename T>
+__device__ __forceinline__ void store8(T* dst, const float (&v)[8], int valid) {
+  constexpr int kBytes = 8 * sizeof(T);
+  if (valid >= 8 && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+    __align__(16) T t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = from_float<T>(v[j]);
+#pragma unroll
+    for (int j = 0; j < kBytes / 16; ++j) reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(t)[j];
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < valid) dst[j] = from_float<T>(v[j]);
+}
+
+// What follows a product, for eight neighbouring columns of a row: `a` the sums (kGated: the gate's, and `b` the up row's).
+template <int kKind>
+__device__ __forceinline__ void dense_finish8(const DenseEpilogue& e, int n, int row, int col, float (&a)[8], float (&b)[8]) {
+  const int valid = n - col;
+  if (valid <= 0) return;
+  const auto load8 = [&](const float* src, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < valid ? __ldg(src + j) : 0.f;
+  };
+  const auto scale8 = [&](float (&v)[8], const float* col_scale) {
+    const float rs = __ldg(e.row_scale + row);
+    float cs[8];
+    load8(col_scale, cs);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * rs * cs[j];
+  };
+  const auto put = [&](int64_t at, const float (&v)[8]) {
+    if (e.out_type == kDenseBf16) store8(static_cast<__nv_bfloat16*>(e.out) + at, v, valid);
+    else if (e.out_type == kDenseFp16) store8(static_cast<__half*>(e.out) + at, v, valid);
+    else store8(static_cast<float*>(e.out) + at, v, valid);
+  };
+  const int64_t at = row * e.ld_out + col;
+  if (kKind == kLinear) {
+    if (e.col_scale != nullptr) scale8(a, e.col_scale + col);
+    if (e.bias != nullptr) {
+      float bias[8];
+      load8(e.bias + col, bias);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] += bias[j];
+    }
+    put(at, a);
+  } else if (kKind == kGated) {
+    if (e.col_scale != nullptr) {
+      scale8(a, e.col_scale + col);
+      scale8(b, e.col_scale + e.inter + col);
+    }
+    if (e.preact != nullptr) {
+      float* keep = e.preact + (int64_t)row * 2 * e.inter + col;
+      store8(keep, a, valid);
+      store8(keep + e.inter, b, valid);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = gated_value(a[j], b[j], e.clamp);
+    put(at, a);
+  } else {
+    const float* keep = e.preact + (int64_t)row * 2 * e.inter + col;
+    float g[8], u[8];
+    load8(keep, g);
+    load8(keep + e.inter, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) gated_grad(a[j], g[j], u[j], e.clamp, g[j], u[j]);
+    put(at, g);
+    put(at + e.inter, u);
+  }
+}
+#endif
+
+}  // namespace mmoe
