@@ -1,64 +1,331 @@
 // Products of the dense feed-forward operators for sm_100a (see mmoe_dense.cuh).
+#include <algorithm>
+#include <atomic>
+
 #include "mmoe_dense.cuh"
+#include "mmoe_tc.cuh"
 
 namespace mmoe {
 
 namespace {
 
-// A block per 64 x 64 sums, 2 x 8 of them a thread, operands through shared memory 16 k's at a time.
-constexpr int kTile = 64, kDepth = 16;
+// ---------------------------------------------------------------------------------------------------------------------
+// Products on CTA pairs: a persistent pair takes tiles of 256 rows of A by up to 256 rows of B (tcgen05.mma.cta_group::2, M = 256), of
+// which each CTA stages 128 rows of A and half of B, 128 bytes of K a stage.  One warp of the leader issues for both SMs; the
+// accumulators of two tiles alternate in tensor memory, so that a tile's epilogue runs beside the next one's products.
+// kGated: the leader stages gate rows and its peer the up rows of the same channels, so the two values of a channel are half a tile of
+// columns apart in one lane.
+// An operand whose rows run along K is staged as such; one that is stored transposed (k_rows) as 64 x 64 blocks with its own rows along the
+// 128 bytes, which the tensor core reads just as well (MN-major descriptors): no transposed copy is made.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int kPairRows = 128;                        // rows of A per CTA
+constexpr int kPairCols = 256;                        // most rows of B per tile
+constexpr int kStageA = kPairRows * 128;              // bytes
+constexpr int kStageB = kPairCols / 2 * 128;
+constexpr int kStageBytes = kStageA + kStageB;
+constexpr int kStages = 6;
+constexpr int kEpiWarps = 4;
+constexpr int kEpiBlock = 32 * 64 * 4;                // a warp's 32 rows x 64 sums on their way from lanes to rows
+constexpr int kPairThreads = 32 * (2 + kEpiWarps);
+constexpr int kPairSmem = 1024 + 1024 + kStages * kStageBytes + kEpiWarps * kEpiBlock;
+static_assert(kPairSmem <= 227 * 1024, "shared memory budget");
+constexpr int kStatusDense = 31;
 
-template <typename T> struct Sum { using type = float; };
-template <> struct Sum<int8_t> { using type = int; };
-template <typename T> __device__ __forceinline__ typename Sum<T>::type widen(T v) { return static_cast<float>(v); }
-template <> __device__ __forceinline__ int widen<int8_t>(int8_t v) { return v; }
+struct DenseParams {
+  CUtensorMap map_a, map_b;
+  int32_t m, n, k_stages;
+  int32_t cols;              // rows of B per tile (kGated: half of them gate rows)
+  int32_t m_tiles, n_tiles;
+  uint32_t idesc;
+  DenseEpilogue epi;
+  int32_t* status;
+  int64_t timeout_ns;
+};
 
-template <typename T, int kKind>
-__global__ void __launch_bounds__(256) dense_kernel(const DenseProduct p) {
-  using S = typename Sum<T>::type;
-  constexpr int kParts = kKind == kGated ? 2 : 1;
-  __shared__ S sa[kDepth][kTile + 1], sb[kParts][kDepth][kTile + 1];
-  const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile, t = threadIdx.x;
-  S acc[kParts][2][8] = {};
-  const auto at = [&](const DenseOperand& o, int64_t row, int64_t k) {
-    return widen(static_cast<const T*>(o.p)[o.k_rows ? k * o.ld + row : row * o.ld + k]);
-  };
-  for (int k0 = 0; k0 < p.k; k0 += kDepth) {
-    for (int i = t; i < kTile * kDepth; i += 256) {
-      const int r = i / kDepth, k = i % kDepth;
-      const bool in = k0 + k < p.k;
-      sa[k][r] = in && m0 + r < p.m ? at(p.a, m0 + r, k0 + k) : S(0);
-      for (int c = 0; c < kParts; ++c) sb[c][k][r] = in && n0 + r < p.n ? at(p.b, n0 + r + (int64_t)c * p.n, k0 + k) : S(0);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kDepth; ++k)
-#pragma unroll
-      for (int c = 0; c < kParts; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) acc[c][i][j] += sa[k][(t >> 3) * 2 + i] * sb[c][k][(t & 7) * 8 + j];
-    __syncthreads();
-  }
-  for (int i = 0; i < 2; ++i) {
-    const int row = m0 + (t >> 3) * 2 + i;
-    if (row >= p.m) break;
-    float a[8], b[8];
-    for (int j = 0; j < 8; ++j) {
-      a[j] = static_cast<float>(acc[0][i][j]);
-      b[j] = static_cast<float>(acc[kParts - 1][i][j]);
-    }
-    dense_finish8<kKind>(p.epi, p.n, row, n0 + (t & 7) * 8, a, b);
-  }
+struct PairControl {
+  uint64_t full[kStages];       // leader only: every copy of the stage, in both CTAs, has landed
+  uint64_t empty[kStages];      // issuer -> producers of both CTAs
+  uint64_t acc_full[2];         // issuer -> epilogues of both CTAs
+  uint64_t acc_empty[2];        // leader only: epilogue warps of both CTAs -> issuer
+  uint32_t tmem_base;
+  volatile int32_t abort_flag;
+};
+
+// descriptor without its address: 128-byte swizzle; K-major: eight-row groups 1024 bytes apart.  MN-major: groups of eight k's 1024 bytes
+// apart, blocks of 64 rows `block` bytes apart.
+__device__ __forceinline__ uint64_t operand_desc(bool mn_major, uint32_t block) {
+  return desc_hi_sw128() | (mn_major ? static_cast<uint64_t>(block >> 4) << 16 : 0ull);
 }
 
-template <typename T>
-cudaError_t launch_typed(const DenseProduct& p, cudaStream_t s) {
-  const dim3 grid((p.n + kTile - 1) / kTile, (p.m + kTile - 1) / kTile);
-  if (p.kind == kGated) return launch_plain(dense_kernel<T, kGated>, grid, dim3(256), 0, s, p);
-  if (p.kind == kGatedGrad) return launch_plain(dense_kernel<T, kGatedGrad>, grid, dim3(256), 0, s, p);
-  return launch_plain(dense_kernel<T, kLinear>, grid, dim3(256), 0, s, p);
+template <bool kInt8>
+__device__ __forceinline__ void pair_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (kInt8)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// The t-th tile: eight tiles of rows at a time, all columns of those before the next eight, so that what runs at once reads few
+// different rows of either operand.
+struct TilePlace {
+  int m, n;
+};
+__device__ __forceinline__ TilePlace place_tile(int t, int m_tiles, int n_tiles) {
+  const int group = t / (8 * n_tiles), first = group * 8, rows = min(8, m_tiles - first), in = t - group * 8 * n_tiles;
+  return TilePlace{first + in % rows, in / rows};
+}
+
+// A warp's 32 x 64 block of sums, turned from one row per lane to eight columns per lane.  16-byte piece g of row r lies at g ^ (r & 7);
+// both directions are free of bank conflicts.
+__device__ __forceinline__ void block_write(uint8_t* block, int lane, const uint32_t (&v)[64]) {
+#pragma unroll
+  for (int g = 0; g < 16; ++g)
+    *reinterpret_cast<uint4*>(block + lane * 256 + ((g ^ (lane & 7)) << 4)) = make_uint4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+}
+__device__ __forceinline__ void block_read8(const uint8_t* block, int row, int piece, bool swap, float (&v)[8]) {
+  const float4 p = *reinterpret_cast<const float4*>(block + row * 256 + (((piece + (swap ? 1 : 0)) ^ (row & 7)) << 4));
+  const float4 q = *reinterpret_cast<const float4*>(block + row * 256 + (((piece + (swap ? 0 : 1)) ^ (row & 7)) << 4));
+  const float4 lo = swap ? q : p, hi = swap ? p : q;
+  v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+}
+
+template <bool kInt8, bool kAmn, bool kBmn, int kKind>
+__global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __grid_constant__ DenseParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the same offset in both CTAs
+  PairControl* ctl = reinterpret_cast<PairControl*>(smem);
+  uint8_t* stages = smem + 1024;
+  uint8_t* blocks = stages + kStages * kStageBytes;
+  constexpr int kDepth = kInt8 ? 128 : 64;              // k's per stage
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_ctarank();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem_u32(&ctl->full[i]), 1);
+      mbar_init(smem_u32(&ctl->empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&ctl->acc_full[i]), 1);
+      mbar_init(smem_u32(&ctl->acc_empty[i]), 2 * kEpiWarps);
+    }
+    ctl->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                       // the peer's barriers are initialised before anything arrives on them
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+  const int tiles = p.m_tiles * p.n_tiles, step = gridDim.x / 2, half = p.cols / 2;
+  Waiter waiter{&ctl->abort_flag, p.status, global_timer() + static_cast<uint64_t>(p.timeout_ns), kStatusDense, warp};
+  const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
+
+  if (warp == 0) {
+    // --------------------------------------------------------------------------------------------- producer
+    uint32_t stage = 0, phase = 0;
+    const uint32_t leader_full0 = map_to_cta(full0, 0), base = smem_u32(stages);
+    const int b_blocks = (half + 63) / 64;
+    const uint32_t tx = 2 * (kStageA + (kBmn ? b_blocks * 8192 : half * 128));
+    bool ok = true;
+    for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
+      const TilePlace at = place_tile(t, p.m_tiles, p.n_tiles);
+      const int a_row = at.m * 2 * kPairRows + static_cast<int>(cta) * kPairRows;
+      const int b_row = kKind == kGated ? at.n * half + static_cast<int>(cta) * p.epi.inter : at.n * p.cols + static_cast<int>(cta) * half;
+      for (int kb = 0; kb < p.k_stages; ++kb) {
+        if (!waiter.wait_uniform(empty0 + 8 * stage, phase ^ 1u)) { ok = false; break; }
+        const uint32_t bar = leader_full0 + 8 * stage, a = base + stage * kStageBytes, b = a + kStageA;
+        if (elect_one()) {
+          if (cta == 0) mbar_expect_tx(full0 + 8 * stage, tx);
+          if (kAmn) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) pair_load_2d(a + j * 8192, &p.map_a, a_row + 64 * j, kb * kDepth, bar);
+          } else {
+            pair_load_2d(a, &p.map_a, kb * kDepth, a_row, bar);
+          }
+          if (kBmn) {
+            for (int j = 0; j < b_blocks; ++j) pair_load_2d(b + j * 8192, &p.map_b, b_row + 64 * j, kb * kDepth, bar);
+          } else {
+            pair_load_2d(b, &p.map_b, kb * kDepth, b_row, bar);
+          }
+        }
+        __syncwarp();
+        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      }
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------------------------------------------------- issuer
+    if (cta == 0) {
+      uint32_t stage = 0, phase = 0, it = 0;
+      bool ok = true;
+      const uint64_t a_hi = operand_desc(kAmn, 8192), b_hi = operand_desc(kBmn, 8192);
+      const uint32_t lo0 = (smem_u32(stages) & 0x3FFFFu) >> 4;
+      // a K of 32 bytes further: along the 128 bytes, or 16 rows of them
+      constexpr uint32_t kStepA = kAmn ? 2048 >> 4 : 2, kStepB = kBmn ? 2048 >> 4 : 2;
+      for (int t = blockIdx.x / 2; ok && t < tiles; t += step, ++it) {
+        const uint32_t acc = it & 1u, d = tmem_base + acc * kPairCols;
+        if (!waiter.wait_uniform(smem_u32(&ctl->acc_empty[acc]), ((it >> 1) & 1u) ^ 1u)) break;
+        tc_fence_after();
+        for (int kb = 0; kb < p.k_stages; ++kb) {
+          if (!waiter.wait_uniform(full0 + 8 * stage, phase)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a = lo0 + stage * (kStageBytes >> 4), b = a + (kStageA >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              pair_product<kInt8>(d, a_hi | (a + kStepA * k), b_hi | (b + kStepB * k), p.idesc, (kb | k) != 0 ? 1u : 0u);
+            pair_commit(empty0 + 8 * stage);
+          }
+          __syncwarp();
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+        if (ok && elect_one()) pair_commit(smem_u32(&ctl->acc_full[acc]));
+        __syncwarp();
+      }
+    }
+  } else {
+    // --------------------------------------------------------------------------------------------- epilogue
+    const int q = warp & 3;                       // TMEM lane quadrant this warp may read
+    const uint32_t leader_empty = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
+    uint8_t* block = blocks + (warp - 2) * kEpiBlock;
+    uint32_t it = 0;
+    for (int t = blockIdx.x / 2; t < tiles; t += step, ++it) {
+      const TilePlace at = place_tile(t, p.m_tiles, p.n_tiles);
+      const uint32_t acc = it & 1u;
+      const int row0 = at.m * 2 * kPairRows + static_cast<int>(cta) * kPairRows + q * 32, rows = min(32, p.m - row0);
+      const int width = kKind == kGated ? half : p.cols, col0 = at.n * width;
+      constexpr int kChunk = kKind == kGated ? 32 : 64;
+      if (!waiter.wait_warp(smem_u32(&ctl->acc_full[acc]), (it >> 1) & 1u)) break;
+      tc_fence_after();
+      const uint32_t d = tmem_base + acc * kPairCols + (static_cast<uint32_t>(q * 32) << 16);
+      const int chunks = rows > 0 ? (min(width, p.n - col0) + kChunk - 1) / kChunk : 0;
+#pragma unroll 1
+      for (int c = 0; c < chunks; ++c) {
+        uint32_t v[64];
+        tc_ld32(d + kChunk * c, v);
+        tc_ld32(kKind == kGated ? d + half + 32 * c : d + 64 * c + 32, v + 32);
+        tc_ld_wait();
+        if (kInt8) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] = __float_as_uint(static_cast<float>(static_cast<int32_t>(v[j])));
+        }
+        if (c + 1 == chunks) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_pair(leader_empty + 8 * acc);
+        }
+        __syncwarp();                             // the previous block has been read
+        block_write(block, lane, v);
+        __syncwarp();
+        constexpr int kLanes = kChunk / 8, kRowsAtOnce = 32 / kLanes;
+        const int sub = lane / kLanes, piece = lane % kLanes;
+        const int col = col0 + kChunk * c + 8 * piece;
+        const int last = min(p.n, col0 + width);
+#pragma unroll 2
+        for (int r = sub; r < rows; r += kRowsAtOnce) {
+          float a[8], b[8];
+          block_read8(block, r, 2 * piece, kKind != kGated && piece >= 4, a);
+          if (kKind == kGated) block_read8(block, r, 8 + 2 * piece, false, b);
+          dense_finish8<kKind>(p.epi, last, row0 + r, col, a, b);
+        }
+      }
+      if (chunks == 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_pair(leader_empty + 8 * acc);
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------------------------------------------- teardown
+  __syncwarp();
+  if (ctl->abort_flag != 0) {               // copies still in flight land before this CTA's shared memory goes
+    const uint64_t t0 = global_timer();
+    while (global_timer() - t0 < 200000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                       // no CTA leaves while its peer may still arrive on its barriers
+  tc_fence_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------------
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+std::atomic<EncodeFn> g_encode{nullptr};
+constexpr int kMaxDevices = 64;
+std::atomic<int> g_sms[kMaxDevices];        // per device, 0: prepare_dense() has not run there
+
+int prepared_sms() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? g_sms[dev].load() : 0;
+}
+
+// `rows` x k matrix; boxes of 128 bytes of K by `box` rows, or (stored transposed) of 64 rows by 64 k's
+bool encode(CUtensorMap* map, const DenseOperand& o, int type, uint64_t rows, uint64_t k, uint32_t box) {
+  const uint64_t size = type == kDenseInt8 ? 1 : 2;
+  const cuuint64_t dims[2] = {o.k_rows ? rows : k, o.k_rows ? k : rows};
+  const cuuint64_t strides[1] = {static_cast<uint64_t>(o.ld) * size};
+  const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(128 / size), o.k_rows ? 64u : box};
+  const cuuint32_t one[2] = {1, 1};
+  const CUtensorMapDataType t = type == kDenseInt8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type == kDenseBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return g_encode.load()(map, t, 2, const_cast<void*>(o.p), dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Instruction descriptor: [4,6) sums (1 FP32, 2 32-bit integers), [7,10) and [10,13) operands (16 bits: 0 FP16, 1 BF16; 8 bits: 1 signed),
+// [15], [16] MN-major operands, [17,23) N >> 3, [24,29) M >> 4.
+uint32_t product_idesc(const DenseProduct& p, int rows, int cols) {
+  const uint32_t format = p.type == kDenseFp16 ? 0 : 1;
+  return ((p.type == kDenseInt8 ? 2u : 1u) << 4) | (format << 7) | (format << 10) | ((p.a.k_rows ? 1u : 0u) << 15) | ((p.b.k_rows ? 1u : 0u) << 16) |
+         (static_cast<uint32_t>(cols >> 3) << 17) | (static_cast<uint32_t>(rows >> 4) << 24);
+}
+
+template <typename F>
+cudaError_t for_each_pair_kernel(F f) {
+  cudaError_t e = f(dense_pair_kernel<false, false, false, kGated>, kDenseBf16, false, false, kGated);
+  if (e == cudaSuccess) e = f(dense_pair_kernel<false, false, false, kLinear>, kDenseBf16, false, false, kLinear);
+  if (e == cudaSuccess) e = f(dense_pair_kernel<false, false, true, kGatedGrad>, kDenseBf16, false, true, kGatedGrad);
+  if (e == cudaSuccess) e = f(dense_pair_kernel<false, false, true, kLinear>, kDenseBf16, false, true, kLinear);
+  if (e == cudaSuccess) e = f(dense_pair_kernel<false, true, true, kLinear>, kDenseBf16, true, true, kLinear);
+  if (e == cudaSuccess) e = f(dense_pair_kernel<true, false, false, kGated>, kDenseInt8, false, false, kGated);
+  if (e == cudaSuccess) e = f(dense_pair_kernel<true, false, false, kLinear>, kDenseInt8, false, false, kLinear);
+  return e;
+}
+
+cudaError_t launch_pairs(const DenseProduct& p, int sms, cudaStream_t s) {
+  DenseParams d;
+  d.m = p.m, d.n = p.n;
+  const int depth = p.type == kDenseInt8 ? 128 : 64;
+  d.k_stages = (p.k + depth - 1) / depth;
+  d.cols = kPairCols;
+  const int width = p.kind == kGated ? d.cols / 2 : d.cols;
+  d.m_tiles = (p.m + 2 * kPairRows - 1) / (2 * kPairRows);
+  d.n_tiles = (p.n + width - 1) / width;
+  if ((int64_t)d.m_tiles * d.n_tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
+  d.idesc = product_idesc(p, 2 * kPairRows, d.cols);
+  d.epi = p.epi;
+  d.status = p.status;
+  d.timeout_ns = (p.timeout_ms > 0 ? (int64_t)p.timeout_ms : 2000) * 1000000ll;
+  if (!encode(&d.map_a, p.a, p.type, p.m, p.k, kPairRows) || !encode(&d.map_b, p.b, p.type, p.kind == kGated ? 2 * (uint64_t)p.n : p.n, p.k, d.cols / 2))
+    return cudaErrorInvalidValue;
+  const int grid = 2 * std::min(sms / 2, d.m_tiles * d.n_tiles);
+  bool found = false;
+  const cudaError_t e = for_each_pair_kernel([&](auto kernel, int type, bool a_mn, bool b_mn, int kind) {
+    if ((type == kDenseInt8) != (p.type == kDenseInt8) || a_mn != p.a.k_rows || b_mn != p.b.k_rows || kind != p.kind) return cudaSuccess;
+    found = true;
+    return launch_clustered(kernel, dim3(grid), dim3(kPairThreads), kPairSmem, 2, s, d);
+  });
+  return found ? e : cudaErrorInvalidValue;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -138,12 +405,32 @@ cudaError_t launch_quantize(const void* x, int64_t ld, int8_t* q, float* scales,
 
 }  // namespace
 
-cudaError_t prepare_dense() { return cudaSuccess; }
+cudaError_t prepare_dense() {
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  if (g_sms[dev].load() > 0) return cudaSuccess;
+  if (g_encode.load() == nullptr) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found);
+    if (e != cudaSuccess) return e;
+    if (found != cudaDriverEntryPointSuccess || fn == nullptr) return cudaErrorSymbolNotFound;
+    g_encode.store(reinterpret_cast<EncodeFn>(fn));
+  }
+  e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess)
+    e = for_each_pair_kernel([](auto kernel, int, bool, bool, int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem); });
+  if (e == cudaSuccess) g_sms[dev].store(sms);
+  return e;
+}
 
 cudaError_t launch_dense(const DenseProduct& p, cudaStream_t s) {
   if (p.m <= 0 || p.n <= 0) return cudaSuccess;
-  if (p.type == kDenseInt8) return launch_typed<int8_t>(p, s);
-  return p.type == kDenseBf16 ? launch_typed<__nv_bfloat16>(p, s) : launch_typed<__half>(p, s);
+  const int sms = prepared_sms();
+  if (sms == 0) return cudaErrorNotReady;
+  return launch_pairs(p, sms, s);
 }
 
 cudaError_t launch_quantize_int8(const void* x, int type, int64_t ld, int8_t* q, float* scales, int m, int k, cudaStream_t s) {

@@ -87,36 +87,8 @@ struct TmControl {        // lives at the start of shared memory (same layout in
 static_assert(sizeof(TmControl) <= 1024, "control block");
 
 // ---------------------------------------------------------------------------------------------------------------
-// cluster / CTA-pair helpers
+// CTA-pair helpers
 // ---------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// shared::cluster address of the same shared-memory location in CTA `rank` of the cluster
-__device__ __forceinline__ uint32_t map_to_cta(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-// Arrival on the barrier that hands columns of tensor memory back, in either CTA of the pair: ordered by the tcgen05 fences on
-// either side, and no memory access rides on it (the queue of tasks has arrivals of its own).  So the default release, of CTA scope, is enough: one of cluster scope first waits for
-// this warp's outstanding stores to global memory, which stood between every two tasks of the issuer.  Cluster scope -> CTA scope, one card: 3840
-// tokens of 48 experts 930 -> 908 us repeated for seconds (at the power limit), 819 -> 800 in bursts of 30 calls; 2560 of 16 376 -> 369 and
-// 333 -> 326, 3001 of 96 skewed 884 -> 870 and 778 -> 765, 1021 of 384 skewed 456 -> 451 and 410 -> 405.
-__device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// arrives on the barrier at this offset in both CTAs of the pair when everything issued so far has completed
-__device__ __forceinline__ void pair_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-               ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
-}
 __device__ __forceinline__ void pair_cp_sf(uint32_t tmem_addr, uint64_t sdesc) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem_addr), "l"(sdesc) : "memory");
 }
@@ -129,20 +101,6 @@ __device__ __forceinline__ void pair_mma(uint32_t d, uint64_t adesc, uint64_t bd
       ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
       : "memory");
 }
-// tile loads into this CTA's shared memory whose completion is counted on a barrier of either CTA of the pair
-__device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
-      : "memory");
-}
-
 // What the queue of claimed tasks is made of (mmoe_pair_queue.h); every function by the whole warp.
 template <bool kOneLanePolls>
 struct PairPort {
