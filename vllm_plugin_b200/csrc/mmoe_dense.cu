@@ -257,6 +257,205 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
+// Products of few tokens, bound by the bytes of B (the weights): 128 of its rows are operand A of the tensor core and the tokens, padded to 16,
+// operand B, so that few tokens cost little.  kGated: 64 gate and 64 up rows.  K is split over the CTAs of a cluster, whose partial sums meet
+// in shared memory, added in the order of the CTAs: no atomics, no workspace, and the same bits in every call.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int kFewRows = 128;                         // rows of B per tile
+constexpr int kFewThreads = 192;
+constexpr int kFewMaxStages = 12;
+constexpr int kFewChunk = 64;                         // tokens whose partial sums are in shared memory at a time
+constexpr int kFewPartBytes = kFewChunk * kFewRows * 4;
+constexpr int kFewMaxTokens = 256;                    // per tile
+
+struct FewParams {
+  CUtensorMap map_w, map_t;
+  int32_t m, n, k_stages;
+  int32_t tokens;            // per tile, a multiple of 16
+  int32_t split;             // CTAs of a cluster
+  int32_t stages;
+  uint32_t idesc;
+  int32_t tmem_cols;
+  DenseEpilogue epi;
+  int32_t* status;
+  int64_t timeout_ns;
+};
+
+struct FewControl {
+  uint64_t full[kFewMaxStages], empty[kFewMaxStages];
+  uint64_t acc_full;
+  uint32_t tmem_base;
+  volatile int32_t abort_flag;
+};
+static_assert(sizeof(FewControl) <= 1024, "control block");
+
+template <bool kInt8>
+__device__ __forceinline__ void single_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (kInt8)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+__device__ __forceinline__ float4 cluster_load(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// eight neighbouring sums of a token over the CTAs of the cluster
+template <bool kInt8>
+__device__ __forceinline__ void add_parts(uint32_t addr, int split, float (&v)[8]) {
+  int32_t whole[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f, whole[j] = 0;
+  for (int r = 0; r < split; ++r) {
+    const uint32_t from = map_to_cta(addr, r);
+    const float4 lo = cluster_load(from), hi = cluster_load(from + 16);
+    const float part[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (kInt8) whole[j] += __float_as_int(part[j]);
+      else v[j] += part[j];
+    }
+  }
+  if (kInt8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(whole[j]);
+  }
+}
+
+template <bool kInt8, bool kWmn, int kKind>
+__global__ void __launch_bounds__(kFewThreads, 2) dense_few_kernel(const __grid_constant__ FewParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the same offset in all CTAs
+  FewControl* ctl = reinterpret_cast<FewControl*>(smem);
+  uint8_t* stages = smem + 1024;
+  constexpr int kDepth = kInt8 ? 128 : 64;
+  constexpr int kWBytes = kFewRows * 128;
+  const int t_bytes = p.tokens * 128, stage_bytes = kWBytes + t_bytes;
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int tile = blockIdx.x / p.split, tok0 = blockIdx.y * p.tokens;
+  const int k0 = static_cast<int>((int64_t)p.k_stages * rank / p.split), k1 = static_cast<int>((int64_t)p.k_stages * (rank + 1) / p.split);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(smem_u32(&ctl->full[i]), 1);
+      mbar_init(smem_u32(&ctl->empty[i]), 1);
+    }
+    mbar_init(smem_u32(&ctl->acc_full), 1);
+    ctl->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)), "r"(p.tmem_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+  Waiter waiter{&ctl->abort_flag, p.status, global_timer() + static_cast<uint64_t>(p.timeout_ns), kStatusDense + 1, warp};
+  const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]), base = smem_u32(stages);
+  const int n_stages = p.stages;
+
+  if (warp == 0) {
+    // --------------------------------------------------------------------------------------------- producer
+    int stage = 0;
+    uint32_t phase = 0;
+    const int w_row = tile * (kKind == kGated ? kFewRows / 2 : kFewRows);
+    for (int kb = k0; kb < k1; ++kb) {
+      if (!waiter.wait_uniform(empty0 + 8 * stage, phase ^ 1u)) break;
+      const uint32_t bar = full0 + 8 * stage, w = base + stage * stage_bytes;
+      if (elect_one()) {
+        mbar_expect_tx(bar, stage_bytes);
+        if (kKind == kGated) {
+          tma_load_2d(w, &p.map_w, kb * kDepth, w_row, bar);
+          tma_load_2d(w + 8192, &p.map_w, kb * kDepth, p.epi.inter + w_row, bar);
+        } else if (kWmn) {
+          tma_load_2d(w, &p.map_w, w_row, kb * kDepth, bar);
+          tma_load_2d(w + 8192, &p.map_w, w_row + 64, kb * kDepth, bar);
+        } else {
+          tma_load_2d(w, &p.map_w, kb * kDepth, w_row, bar);
+        }
+        tma_load_2d(w + kWBytes, &p.map_t, kb * kDepth, tok0, bar);
+      }
+      __syncwarp();
+      if (++stage == n_stages) { stage = 0; phase ^= 1u; }
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------------------------------------------------- issuer
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint64_t w_hi = operand_desc(kWmn, 8192), t_hi = operand_desc(false, 0);
+    constexpr uint32_t kStepW = kWmn ? 2048 >> 4 : 2;
+    for (int kb = k0; kb < k1; ++kb) {
+      if (!waiter.wait_uniform(full0 + 8 * stage, phase)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t w = ((base + stage * stage_bytes) & 0x3FFFFu) >> 4, t = w + (kWBytes >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) single_product<kInt8>(tmem_base, w_hi | (w + kStepW * k), t_hi | (t + 2 * k), p.idesc, kb > k0 || k > 0 ? 1u : 0u);
+        tc_commit(empty0 + 8 * stage);
+      }
+      __syncwarp();
+      if (++stage == n_stages) { stage = 0; phase ^= 1u; }
+    }
+    if (ok && elect_one()) tc_commit(smem_u32(&ctl->acc_full));
+    __syncwarp();
+  }
+
+  // ------------------------------------------------------------------------------------------------- sums
+  // everything staged has been multiplied when the accumulator is complete, so the partial sums may take its place: [token][128 rows]
+  bool ok = true;
+  if (warp >= 2) {
+    ok = waiter.wait_warp(smem_u32(&ctl->acc_full), 0);
+    tc_fence_after();
+  }
+  constexpr int kGroups = kKind == kGated ? kFewRows / 16 : kFewRows / 8;     // eight channels each
+  const int tokens = min(p.tokens, p.m - tok0);
+  for (int c0 = 0; c0 < tokens; c0 += kFewChunk) {
+    const int here = min(kFewChunk, tokens - c0);
+    if (warp >= 2 && ok) {
+      const int row = (warp & 3) * 32 + lane;
+      const uint32_t d = tmem_base + c0 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+      for (int j0 = 0; j0 < here; j0 += 16) {
+        uint32_t v[16];
+        tc_ld16(d + j0, v);
+        tc_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) reinterpret_cast<uint32_t*>(stages)[(j0 + j) * kFewRows + row] = v[j];
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    for (int i = rank * kFewThreads + static_cast<int>(threadIdx.x); i < here * kGroups; i += p.split * kFewThreads) {
+      const int t = i / kGroups, g = i - t * kGroups;
+      float a[8], b[8];
+      add_parts<kInt8>(base + (t * kFewRows + 8 * g) * 4, p.split, a);
+      if (kKind == kGated) add_parts<kInt8>(base + (t * kFewRows + kFewRows / 2 + 8 * g) * 4, p.split, b);
+      dense_finish8<kKind>(p.epi, p.n, tok0 + c0 + t, tile * 8 * kGroups + 8 * g, a, b);
+    }
+    __syncwarp();
+    cluster_sync_all();                     // read by all, before the next sums or the end of this CTA
+  }
+
+  // ---------------------------------------------------------------------------------------------------- teardown
+  if (ctl->abort_flag != 0) {
+    const uint64_t t0 = global_timer();
+    while (global_timer() - t0 < 200000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(p.tmem_cols) : "memory");
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------------
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -284,9 +483,9 @@ bool encode(CUtensorMap* map, const DenseOperand& o, int type, uint64_t rows, ui
 
 // Instruction descriptor: [4,6) sums (1 FP32, 2 32-bit integers), [7,10) and [10,13) operands (16 bits: 0 FP16, 1 BF16; 8 bits: 1 signed),
 // [15], [16] MN-major operands, [17,23) N >> 3, [24,29) M >> 4.
-uint32_t product_idesc(const DenseProduct& p, int rows, int cols) {
-  const uint32_t format = p.type == kDenseFp16 ? 0 : 1;
-  return ((p.type == kDenseInt8 ? 2u : 1u) << 4) | (format << 7) | (format << 10) | ((p.a.k_rows ? 1u : 0u) << 15) | ((p.b.k_rows ? 1u : 0u) << 16) |
+uint32_t product_idesc(int type, bool a_mn, bool b_mn, int rows, int cols) {
+  const uint32_t format = type == kDenseFp16 ? 0 : 1;
+  return ((type == kDenseInt8 ? 2u : 1u) << 4) | (format << 7) | (format << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
          (static_cast<uint32_t>(cols >> 3) << 17) | (static_cast<uint32_t>(rows >> 4) << 24);
 }
 
@@ -302,6 +501,48 @@ cudaError_t for_each_pair_kernel(F f) {
   return e;
 }
 
+template <typename F>
+cudaError_t for_each_few_kernel(F f) {
+  cudaError_t e = f(dense_few_kernel<false, false, kGated>, kDenseBf16, false, kGated);
+  if (e == cudaSuccess) e = f(dense_few_kernel<false, false, kLinear>, kDenseBf16, false, kLinear);
+  if (e == cudaSuccess) e = f(dense_few_kernel<false, true, kGatedGrad>, kDenseBf16, true, kGatedGrad);
+  if (e == cudaSuccess) e = f(dense_few_kernel<false, true, kLinear>, kDenseBf16, true, kLinear);
+  if (e == cudaSuccess) e = f(dense_few_kernel<true, false, kGated>, kDenseInt8, false, kGated);
+  if (e == cudaSuccess) e = f(dense_few_kernel<true, false, kLinear>, kDenseInt8, false, kLinear);
+  return e;
+}
+
+constexpr int kFewSmemHalf = 113 * 1024, kFewSmemFull = 227 * 1024;     // two CTAs to an SM, or one
+
+cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
+  FewParams d;
+  d.m = p.m, d.n = p.n;
+  const int depth = p.type == kDenseInt8 ? 128 : 64;
+  d.k_stages = (p.k + depth - 1) / depth;
+  const int parts = (p.m + kFewMaxTokens - 1) / kFewMaxTokens;
+  d.tokens = ((p.m + parts - 1) / parts + 15) & ~15;
+  const int width = p.kind == kGated ? kFewRows / 2 : kFewRows, tiles = (p.n + width - 1) / width;
+  const int stage_bytes = kFewRows * 128 + d.tokens * 128;
+  const bool two = d.tokens <= 128;
+  const int smem = two ? kFewSmemHalf : kFewSmemFull;
+  d.stages = std::min((smem - 2048) / stage_bytes, kFewMaxStages);
+  d.split = std::max(1, std::min({8, (two ? 2 : 1) * sms / (tiles * parts), d.k_stages / 4}));
+  d.idesc = product_idesc(p.type, p.b.k_rows, false, kFewRows, d.tokens);
+  d.tmem_cols = d.tokens <= 32 ? 32 : d.tokens <= 64 ? 64 : d.tokens <= 128 ? 128 : 256;
+  d.epi = p.epi;
+  d.status = p.status;
+  d.timeout_ns = (p.timeout_ms > 0 ? (int64_t)p.timeout_ms : 2000) * 1000000ll;
+  if (!encode(&d.map_w, p.b, p.type, p.kind == kGated ? 2 * (uint64_t)p.n : p.n, p.k, width) || !encode(&d.map_t, p.a, p.type, p.m, p.k, d.tokens))
+    return cudaErrorInvalidValue;
+  bool found = false;
+  const cudaError_t e = for_each_few_kernel([&](auto kernel, int type, bool w_mn, int kind) {
+    if ((type == kDenseInt8) != (p.type == kDenseInt8) || w_mn != p.b.k_rows || kind != p.kind) return cudaSuccess;
+    found = true;
+    return launch_clustered(kernel, dim3(tiles * d.split, parts), dim3(kFewThreads), smem, d.split, s, d);
+  });
+  return found ? e : cudaErrorInvalidValue;
+}
+
 cudaError_t launch_pairs(const DenseProduct& p, int sms, cudaStream_t s) {
   DenseParams d;
   d.m = p.m, d.n = p.n;
@@ -312,7 +553,7 @@ cudaError_t launch_pairs(const DenseProduct& p, int sms, cudaStream_t s) {
   d.m_tiles = (p.m + 2 * kPairRows - 1) / (2 * kPairRows);
   d.n_tiles = (p.n + width - 1) / width;
   if ((int64_t)d.m_tiles * d.n_tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
-  d.idesc = product_idesc(p, 2 * kPairRows, d.cols);
+  d.idesc = product_idesc(p.type, p.a.k_rows, p.b.k_rows, 2 * kPairRows, d.cols);
   d.epi = p.epi;
   d.status = p.status;
   d.timeout_ns = (p.timeout_ms > 0 ? (int64_t)p.timeout_ms : 2000) * 1000000ll;
@@ -422,6 +663,8 @@ cudaError_t prepare_dense() {
   e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess)
     e = for_each_pair_kernel([](auto kernel, int, bool, bool, int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem); });
+  if (e == cudaSuccess)
+    e = for_each_few_kernel([](auto kernel, int, bool, int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmemFull); });
   if (e == cudaSuccess) g_sms[dev].store(sms);
   return e;
 }
@@ -430,7 +673,7 @@ cudaError_t launch_dense(const DenseProduct& p, cudaStream_t s) {
   if (p.m <= 0 || p.n <= 0) return cudaSuccess;
   const int sms = prepared_sms();
   if (sms == 0) return cudaErrorNotReady;
-  return launch_pairs(p, sms, s);
+  return !p.a.k_rows && p.m <= kFewMaxTokens ? launch_few(p, sms, s) : launch_pairs(p, sms, s);
 }
 
 cudaError_t launch_quantize_int8(const void* x, int type, int64_t ld, int8_t* q, float* scales, int m, int k, cudaStream_t s) {

@@ -96,6 +96,11 @@ __device__ __forceinline__ void dense_finish8(const DenseEpilogue& e, int n, int
   const int valid = n - col;
   if (valid <= 0) return;
   const auto load8 = [&](const float* src, float (&v)[8]) {
+    if (valid >= 8 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
+      const float4 lo = __ldg(reinterpret_cast<const float4*>(src)), hi = __ldg(reinterpret_cast<const float4*>(src) + 1);
+      v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = j < valid ? __ldg(src + j) : 0.f;
   };
