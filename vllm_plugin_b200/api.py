@@ -12,6 +12,7 @@ from typing import Any, Optional, Tuple, Union
 
 # implementations of the per-step functions, looked up once (a function-local import costs about a microsecond per call)
 _mega_moe = _stage = _route_and_stage = None
+_feed_forward = _quantize_int8 = _int8_projection = _int8_gated_projection = None
 
 
 def get_symm_buffer_for_mega_moe(group, num_experts: int, num_max_tokens_per_rank: int, num_topk: int, hidden: int,
@@ -118,41 +119,40 @@ def gated_feed_forward(x, w13, w2, *, activation_clamp: Optional[float] = None):
     pass; g and u themselves are kept for it in FP32.  A value on the border of the clamp passes its gradient, one beyond it does not.
     First derivatives only.  A training step can be captured into a CUDA graph behind a first call, but not while the graph of an eager
     call with the same leaves is alive (``RuntimeError``)."""
-    from .backend.dense import gated_feed_forward as _impl
-
-    return _impl(x, w13, w2, activation_clamp=activation_clamp)
+    global _feed_forward
+    if _feed_forward is None:
+        from .backend.dense import gated_feed_forward as _feed_forward
+    return _feed_forward(x, w13, w2, activation_clamp=activation_clamp)
 
 
 def prepare_int8_inputs(hidden_states, out=None):
     """Per-token 8-bit quantiser of BF16 or FP16 hidden states ``(..., K)``; returns ``(int8 (..., K), float32 scales (...))``.
     ``scale = max|x| / 127`` (1 for a row of zeros), values ``x / scale`` rounded to the nearest, ties to even.  A row that holds an infinity or
     a NaN gets the scale NaN and zeros, so that what is computed from it is NaN.  ``out``: the two tensors, contiguous."""
-    from .backend.dense import prepare_int8_inputs as _impl
-
-    return _impl(hidden_states, out)
+    global _quantize_int8
+    if _quantize_int8 is None:
+        from .backend.dense import prepare_int8_inputs as _quantize_int8
+    return _quantize_int8(hidden_states, out)
 
 
 def int8_projection(x, x_scales, w, w_scales, *, bias=None, out_dtype=None):
     """``(x w^T) * x_scales[..., None] * w_scales + bias`` with exact integer sums: ``x`` int8 ``(..., K)`` with float32 scales ``(...)``, ``w`` int8
     ``(N, K)`` with ``(N,)``, optional ``bias`` float32 ``(N,)``; K a multiple of 16 below 131072.  ``out_dtype``: BF16 (default), FP16 or
     FP32.  No gradient."""
-    import torch
-
-    from .backend.dense import int8_projection as _impl
-
-    return _impl(x, x_scales, w, w_scales, bias=bias, out_dtype=torch.bfloat16 if out_dtype is None else out_dtype)
+    global _int8_projection
+    if _int8_projection is None:
+        from .backend.dense import int8_projection as _int8_projection
+    return _int8_projection(x, x_scales, w, w_scales, bias=bias, out_dtype=out_dtype)
 
 
 def int8_gated_projection(x, x_scales, w13, w13_scales, *, activation_clamp: Optional[float] = None, out_dtype=None):
     """The first half of a gated feed-forward block in 8-bit integers: both products (``w13`` int8 ``(2 I, K)``, the gate's rows first, scales
     ``(2 I,)``), the activation and their product in one kernel, ``silu(min(g, c)) * clip(u, -c, c)`` in ``(..., I)``.  Quantise it with
     :func:`prepare_int8_inputs` for :func:`int8_projection`.  Otherwise as there."""
-    import torch
-
-    from .backend.dense import int8_gated_projection as _impl
-
-    return _impl(x, x_scales, w13, w13_scales, activation_clamp=activation_clamp,
-                 out_dtype=torch.bfloat16 if out_dtype is None else out_dtype)
+    global _int8_gated_projection
+    if _int8_gated_projection is None:
+        from .backend.dense import int8_gated_projection as _int8_gated_projection
+    return _int8_gated_projection(x, x_scales, w13, w13_scales, activation_clamp=activation_clamp, out_dtype=out_dtype)
 
 
 def read_dense_status(device=None) -> None:

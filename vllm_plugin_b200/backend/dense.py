@@ -31,41 +31,65 @@ class _Device:
     def __init__(self, device: torch.device):
         self.status = torch.zeros(8, dtype=torch.int32, device=device)
         self.status_ptr = self.status.data_ptr()
-        self.poll = None
+        self.poll = _f._StatusPoll(self)
+        self.calls = self.due = 0            # launching calls so far, and the one at which to look at the words
 
 
 _devices: Dict[int, _Device] = {}
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+
+
+def _prepare(index: int) -> _Device:
+    _f.require_sm100()
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the dense operators must be called once on a device before CUDA-graph capture")
+    _native.check(_native.load().mmoe_dense_prepare(_native.raw_stream(index)))
+    state = _Device(torch.device("cuda", index))
+    torch.cuda.synchronize(index)                   # the words are zero before a call on another stream may look at them
+    return _devices.setdefault(index, state)
 
 
 def _on_device(index: int) -> _Device:
     """State of the current device ``index``, made at the first call."""
-    state = _devices.get(index)
-    if state is None:
-        _f.require_sm100()
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("the dense operators must be called once on a device before CUDA-graph capture")
-        device = torch.device("cuda", index)
-        _native.check(_native.load().mmoe_dense_prepare(_native.raw_stream(index)))
-        state = _Device(device)
-        torch.cuda.synchronize(device)              # the words are zero before a call on another stream may look at them
-        _devices[index] = state
-    return state
+    return _devices.get(index) or _prepare(index)
 
 
-def _watch(state: _Device):
-    """Non-blocking look at the status words, as the layer's calls do it: returns what to call behind the launch."""
+def _launch(name: str, index: int, arguments, *more) -> None:
+    """One call of the C library on the current stream of device ``index``: ``arguments`` is its structure but for the status words."""
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return _launch(name, index, arguments, *more)
+    state = _on_device(index)
+    arguments.status = state.status_ptr
+    arguments.timeout_ms = _f._kernel_options.timeout_ms
+    state.calls += 1
+    if state.calls >= state.due:
+        _watch(state)
+    code = getattr(_native.load(), name)(ctypes.byref(arguments), *more, _native.raw_stream(index))
+    if code:
+        _native.check(code)
+
+
+def _watch(state: _Device) -> None:
+    """Non-blocking look at the status words, as the layer's calls take it: every so many eager calls a copy of the words is queued, and a
+    later call that finds it complete raises what it says."""
     interval = _f._kernel_options.status_poll_interval
+    state.due = state.calls + 1
     if interval <= 0 or torch.cuda.is_current_stream_capturing():
-        return None
-    if state.poll is None:
-        state.poll = _f._StatusPoll(state)
+        return
     state.poll.before_call(state)
-    return state.poll
+    if not state.poll.pending:
+        if state.calls >= state.poll.calls + interval:
+            state.poll.calls = state.calls - 1
+            state.poll.after_call(state, 1)
+        else:
+            state.due = state.poll.calls + interval
 
 
 def read_dense_status(device=None) -> None:
     """Synchronise and raise ``RuntimeError`` if a device-side wait of a dense operator expired on ``device`` since the last
     read; clears the condition."""
+    _f.require_sm100()
     index = torch.device("cuda" if device is None else device).index
     index = torch.cuda.current_device() if index is None else index
     with torch.cuda.device(index):
@@ -77,234 +101,236 @@ def read_dense_status(device=None) -> None:
 # ---------------------------------------------------------------------------------------------------------------------
 # arguments
 # ---------------------------------------------------------------------------------------------------------------------
-def _need(condition: bool, message: str) -> None:
-    if not condition:
-        raise AssertionError(message)
-
-
 def _clamp_of(activation_clamp: Optional[float]) -> float:
     if activation_clamp is None:
         return math.inf
     value = float(activation_clamp)
-    _need(value > 0, "activation_clamp must be positive")
+    if not value > 0:
+        raise AssertionError("activation_clamp must be positive")
     return value
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` as ``(rows, width)`` whose rows are dense and start on 16 bytes: a view where there is one, else a copy."""
-    width = t.shape[-1]
-    r = t if t.dim() == 2 else t.reshape(-1, width)
-    unit = 16 // r.element_size()
-    if r.shape[0] <= 1:
-        dense = r.stride(1) == 1 or width == 1
-    else:
-        dense = (r.stride(1) == 1 or width == 1) and r.stride(0) >= width and r.stride(0) % unit == 0
-    if dense and r.data_ptr() % 16 == 0:
-        return r
-    return r.contiguous() if not r.is_contiguous() else r.clone(memory_format=torch.contiguous_format)
+    if t.is_contiguous():
+        r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+        return r if r.data_ptr() % 16 == 0 else r.clone()
+    r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    tokens, width = r.shape
+    dense = r.stride(1) == 1 or width == 1
+    if tokens > 1:
+        dense = dense and r.stride(0) >= width and r.stride(0) * r.element_size() % 16 == 0
+    return r if dense and r.data_ptr() % 16 == 0 else r.clone(memory_format=torch.contiguous_format)
 
 
 def _stride(r: torch.Tensor) -> int:
     return r.stride(0) if r.shape[0] > 1 else r.shape[1]
 
 
-def _check_weight(w: torch.Tensor, what: str, dtype: torch.dtype, device: torch.device) -> None:
-    _need(w.dim() == 2 and w.dtype == dtype, f"{what} must be 2-D {dtype}, got {tuple(w.shape)} {w.dtype}")
-    _need(w.device == device, f"{what} must be on {device}")
-    _need(w.is_contiguous() and w.data_ptr() % 16 == 0, f"{what} must be contiguous and 16-byte aligned")
+def _refuse_weight(w: torch.Tensor, what: str, dtype: torch.dtype, device: torch.device) -> None:
+    if w.dim() != 2 or w.dtype != dtype:
+        raise AssertionError(f"{what} must be 2-D {dtype}, got {tuple(w.shape)} {w.dtype}")
+    if w.device != device:
+        raise AssertionError(f"{what} must be on {device}, got {w.device}")
+    raise AssertionError(f"{what} must be contiguous and 16-byte aligned")
 
 
-def _needs_cuda(t: torch.Tensor, what: str) -> None:
-    if not t.is_cuda:
-        raise RuntimeError(f"{what} runs on the GPU only (there is no CPU path).")
+def _check_weight(w: torch.Tensor, what: str, dtype: torch.dtype, x: torch.Tensor) -> None:
+    if w.dtype != dtype or w.dim() != 2 or not w.is_contiguous() or w.data_ptr() % 16 != 0 or w.device != x.device:
+        _refuse_weight(w, what, dtype, x.device)
 
 
 # ---------------------------------------------------------------------------------------------------------------------
 # gated feed-forward block
 # ---------------------------------------------------------------------------------------------------------------------
-def _check_block(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> Tuple[int, int]:
-    _needs_cuda(x, "gated_feed_forward")
-    _need(x.dim() >= 1 and x.dtype in _FF_TYPES, f"x must be BF16 or FP16 (..., H), got {tuple(x.shape)} {x.dtype}")
-    _check_weight(w13, "w13", x.dtype, x.device)
-    _check_weight(w2, "w2", x.dtype, x.device)
+def _check_block(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> None:
+    if not x.is_cuda:
+        raise RuntimeError("gated_feed_forward runs on the GPU only (there is no CPU path).")
+    dtype = x.dtype
+    if dtype not in _FF_TYPES or x.dim() < 1:
+        raise AssertionError(f"x must be BF16 or FP16 (..., H), got {tuple(x.shape)} {dtype}")
+    _check_weight(w13, "w13", dtype, x)
+    _check_weight(w2, "w2", dtype, x)
     hidden, inter = w2.shape
-    _need(x.shape[-1] == hidden and tuple(w13.shape) == (2 * inter, hidden),
-          f"expected x (..., H), w13 (2 I, H) and w2 (H, I), got {tuple(x.shape)}, {tuple(w13.shape)} and {tuple(w2.shape)}")
-    _need(hidden > 0 and inter > 0 and hidden % 8 == 0 and inter % 8 == 0, f"H={hidden} and I={inter} must be positive multiples of 8")
-    return hidden, inter
+    if x.shape[-1] != hidden or w13.shape != (2 * inter, hidden):
+        raise AssertionError(f"expected x (..., H), w13 (2 I, H) and w2 (H, I), got {tuple(x.shape)}, {tuple(w13.shape)} and {tuple(w2.shape)}")
+    if hidden <= 0 or inter <= 0 or hidden % 8 != 0 or inter % 8 != 0:
+        raise AssertionError(f"H={hidden} and I={inter} must be positive multiples of 8")
 
 
 def _launch_block(x2: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, clamp: float, keep: bool):
     """``(y, h, preact or None)`` of rows ``x2``."""
     tokens, hidden = x2.shape
     inter = w2.shape[1]
-    y = torch.empty((tokens, hidden), dtype=x2.dtype, device=x2.device)
-    h = torch.empty((tokens, inter), dtype=x2.dtype, device=x2.device)
-    preact = torch.empty((tokens, 2 * inter), dtype=torch.float32, device=x2.device) if keep else None
+    y = x2.new_empty((tokens, hidden))
+    h = x2.new_empty((tokens, inter))
+    preact = x2.new_empty((tokens, 2 * inter), dtype=torch.float32) if keep else None
     if tokens > 0:
-        index = x2.get_device()
-        state = _on_device(index)
-        poll = _watch(state)
-        a = _native.MmoeFeedForward(_CODES[x2.dtype], hidden, inter, tokens, clamp, _f._kernel_options.timeout_ms, _stride(x2),
-                                    x2.data_ptr(), w13.data_ptr(), w2.data_ptr(), h.data_ptr(),
-                                    preact.data_ptr() if keep else None, y.data_ptr(), state.status_ptr)
-        _native.check(_native.load().mmoe_feed_forward(ctypes.byref(a), _native.raw_stream(index)))
-        if poll is not None:
-            poll.after_call(state, _f._kernel_options.status_poll_interval)
+        _launch("mmoe_feed_forward", x2.get_device(),
+                _native.MmoeFeedForward(_CODES[x2.dtype], hidden, inter, tokens, clamp, 0, _stride(x2), x2.data_ptr(), w13.data_ptr(),
+                                        w2.data_ptr(), h.data_ptr(), preact.data_ptr() if keep else None, y.data_ptr()))
     return y, h, preact
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def _launch_block_grad(x2, w13, w2, h, preact, dy2, clamp: float, wanted):
     tokens, hidden = x2.shape
     inter = w2.shape[1]
-    dx, dw13, dw2 = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((x2, w13, w2), wanted))
-    dpre = torch.empty((tokens, 2 * inter), dtype=x2.dtype, device=x2.device) if wanted[0] or wanted[1] else None
-    index = x2.get_device()
-    state = _on_device(index)
-    poll = _watch(state)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    a = _native.MmoeFeedForward(_CODES[x2.dtype], hidden, inter, tokens, clamp, _f._kernel_options.timeout_ms, _stride(x2),
-                                x2.data_ptr(), w13.data_ptr(), w2.data_ptr(), ptr(h), ptr(preact), None, state.status_ptr)
-    _native.check(_native.load().mmoe_feed_forward_grad(ctypes.byref(a), dy2.data_ptr(), ptr(dpre), ptr(dx), ptr(dw13), ptr(dw2),
-                                                        _native.raw_stream(index)))
-    if poll is not None:
-        poll.after_call(state, _f._kernel_options.status_poll_interval)
+    dx, dw13, dw2 = (x2.new_empty(t.shape) if w else None for t, w in zip((x2, w13, w2), wanted))
+    dpre = x2.new_empty((tokens, 2 * inter)) if wanted[0] or wanted[1] else None
+    _launch("mmoe_feed_forward_grad", x2.get_device(),
+            _native.MmoeFeedForward(_CODES[x2.dtype], hidden, inter, tokens, clamp, 0, _stride(x2), x2.data_ptr(), w13.data_ptr(),
+                                    w2.data_ptr(), _ptr(h), _ptr(preact), None),
+            dy2.data_ptr(), _ptr(dpre), _ptr(dx), _ptr(dw13), _ptr(dw2))
     return dx, dw13, dw2
-
-
-_EAGER = "mmoe_eager_graph"
-
-
-def _accumulators(leaves):
-    return [torch.autograd.graph.get_gradient_edge(t).node for t in leaves if t.requires_grad and t.is_leaf]
 
 
 class _Block(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w13, w2, clamp):
-        x2 = _rows(x.detach())
-        w13d, w2d = w13.detach(), w2.detach()
-        need_x, need_13, need_2 = ctx.needs_input_grad[:3]
-        with torch.cuda.device(x.device):
-            y, h, preact = _launch_block(x2, w13d, w2d, clamp, need_x or need_13)
-        ctx.clamp, ctx.x_shape = clamp, x.shape
-        # the rows as the products read them (x itself unless its rows had to be copied), so that a change of x is noticed
-        own_rows = x2.data_ptr() != x.data_ptr()
-        ctx.save_for_backward(x, w13, w2, h if need_2 else None, preact, x2 if own_rows else None)
-        return y.view(x.shape)
+        x2 = _rows(x)
+        need_x, need_13, need_2, _ = ctx.needs_input_grad
+        y, h, preact = _launch_block(x2, w13, w2, clamp, need_x or need_13)
+        ctx.clamp = clamp
+        # x is kept beside a copy of its rows, where there had to be one, so that a change of x is noticed
+        ctx.save_for_backward(x, w13, w2, h if need_2 else None, preact, x2 if x2.data_ptr() != x.data_ptr() else None)
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, w13, w2, h, preact, x2 = ctx.saved_tensors
-        x2 = _rows(x.detach()) if x2 is None else x2
-        with torch.cuda.device(x.device):
-            dy2 = dy.reshape(-1, dy.shape[-1]).contiguous()
-            if dy2.data_ptr() % 16 != 0:
-                dy2 = dy2.clone()
-            dx, dw13, dw2 = _launch_block_grad(x2, w13, w2, h, preact, dy2, ctx.clamp, ctx.needs_input_grad[:3])
-        return None if dx is None else dx.view(ctx.x_shape), dw13, dw2, None
+        dy2 = dy.reshape(-1, w2.shape[0]).contiguous()
+        if dy2.data_ptr() % 16 != 0:
+            dy2 = dy2.clone()
+        dx, dw13, dw2 = _launch_block_grad(_rows(x) if x2 is None else x2, w13, w2, h, preact, dy2, ctx.clamp, ctx.needs_input_grad[:3])
+        return dx.view(x.shape) if dx is not None and x.dim() != 2 else dx, dw13, dw2, None
+
+
+_EAGER = "mmoe_eager_graph"
+
+
+def _refuse_beside_eager_graph(leaves) -> None:
+    """The node that accumulates a leaf's gradient belongs to the stream on which the first live graph made it.  A captured backward
+    pass would wait for that stream, which is not being captured, and the process would end."""
+    for t in leaves:
+        if t.requires_grad and t.is_leaf and _EAGER in torch.autograd.graph.get_gradient_edge(t).node.metadata:
+            raise RuntimeError("a graph of an eager gated_feed_forward call with the same leaves is still alive: drop its output "
+                               "before the call is captured for training")
 
 
 def gated_feed_forward(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, *, activation_clamp: Optional[float] = None) -> torch.Tensor:
     """``y = h w2^T`` with ``h = silu(min(x wg^T, c)) * clip(x wu^T, -c, c)`` and ``w13 = [wg; wu]``.  See ``api.gated_feed_forward``."""
     _check_block(x, w13, w2)
     clamp = _clamp_of(activation_clamp)
-    if not (torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad or w2.requires_grad)):
-        with torch.cuda.device(x.device):
-            return _launch_block(_rows(x.detach()), w13.detach(), w2.detach(), clamp, False)[0].view(x.shape)
-    leaves = (x, w13, w2)
+    if not ((x.requires_grad or w13.requires_grad or w2.requires_grad) and torch.is_grad_enabled()):
+        y = _launch_block(_rows(x), w13, w2, clamp, False)[0]
+        return y if x.dim() == 2 else y.view(x.shape)
     if torch.cuda.is_current_stream_capturing():
-        # The node that accumulates a leaf's gradient belongs to the stream on which the first live graph made it.  A captured
-        # backward pass would wait for that stream, which is not being captured, and the process would end.
-        if any(_EAGER in node.metadata for node in _accumulators(leaves)):
-            raise RuntimeError("a graph of an eager gated_feed_forward call with the same leaves is still alive: drop its output "
-                               "before the call is captured for training")
+        _refuse_beside_eager_graph((x, w13, w2))
         return _Block.apply(x, w13, w2, clamp)
     y = _Block.apply(x, w13, w2, clamp)
-    for node in _accumulators(leaves):
-        node.metadata[_EAGER] = True
+    for node, _ in y.grad_fn.next_functions:
+        if node is not None:
+            node.metadata[_EAGER] = True
     return y
 
 
 # ---------------------------------------------------------------------------------------------------------------------
 # 8-bit integers
 # ---------------------------------------------------------------------------------------------------------------------
-def _no_gradient(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _refuse_gradient(what: str) -> None:
+    if torch.is_grad_enabled():
         raise NotImplementedError(f"{what} has no gradient: call it under torch.no_grad() or with tensors that need none")
 
 
 def prepare_int8_inputs(hidden_states: torch.Tensor, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
                         ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Per-token 8-bit quantiser.  See ``api.prepare_int8_inputs``."""
-    if hidden_states.dtype not in _FF_TYPES or not hidden_states.is_cuda or hidden_states.dim() < 1:
+    x = hidden_states
+    code = _CODES.get(x.dtype)
+    if code is None or code == _native.MMOE_FP32 or not x.is_cuda or x.dim() < 1:
         raise ValueError("INT8 staging requires BF16 or FP16 CUDA hidden states.")
-    _no_gradient("INT8 staging", hidden_states)
-    width = hidden_states.shape[-1]
+    if x.requires_grad:
+        _refuse_gradient("INT8 staging")
+    shape = x.shape
+    width, lead = shape[-1], shape[:-1]
     if width == 0:
         raise ValueError("INT8 staging requires a positive hidden_size.")
-    lead = hidden_states.shape[:-1]
-    x = hidden_states.detach() if hidden_states.dim() == 2 else hidden_states.detach().reshape(-1, width)
-    if width > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < width:
-        x = x.contiguous()
+    if len(shape) != 2:
+        x = x.reshape(-1, width)
     tokens = x.shape[0]
+    if not x.is_contiguous() and (width > 1 and x.stride(1) != 1 or tokens > 1 and x.stride(0) < width):
+        x = x.contiguous()
     if out is None:
-        q = torch.empty((*lead, width), dtype=torch.int8, device=x.device)
-        scales = torch.empty(lead, dtype=torch.float32, device=x.device)
+        q, scales = x.new_empty(shape, dtype=torch.int8), x.new_empty(lead, dtype=torch.float32)
     else:
         q, scales = out
-        if (q.shape != hidden_states.shape or scales.shape != lead or q.dtype != torch.int8 or scales.dtype != torch.float32
+        if (q.shape != shape or scales.shape != lead or q.dtype != torch.int8 or scales.dtype != torch.float32
                 or q.device != x.device or scales.device != x.device or not q.is_contiguous() or not scales.is_contiguous()):
             raise ValueError("INT8 staging requires out=(int8 of the shape of hidden_states, float32 of its leading shape), contiguous.")
     if tokens > 0:
-        index = x.get_device()
-        with torch.cuda.device(index):
-            _native.check(_native.load().mmoe_quantize_int8(x.data_ptr(), _CODES[x.dtype], _stride(x), q.data_ptr(), scales.data_ptr(),
-                                                            tokens, width, _native.raw_stream(index)))
+        _quantize(x, code, q, scales, tokens, width)
     return q, scales
 
 
-def _int8_product(what: str, x, x_scales, w, w_scales, bias, out_dtype, clamp: float, gated: bool) -> torch.Tensor:
-    _needs_cuda(x, what)
-    _no_gradient(what, x_scales, w_scales, bias)
-    _need(x.dtype == torch.int8 and x.dim() >= 1, f"x must be int8 (..., K), got {tuple(x.shape)} {x.dtype}")
-    _check_weight(w, "w13" if gated else "w", torch.int8, x.device)
-    rows, width = w.shape
-    lead = x.shape[:-1]
-    _need(x.shape[-1] == width and 16 <= width < 131072 and width % 16 == 0,
-          f"x (..., K) and the weights (N, K) must agree on K, a multiple of 16 below 131072, got {x.shape[-1]} and {width}")
-    _need(rows > 0 and (not gated or rows % 2 == 0), "the gated projection needs as many gate as up rows" if gated else "w has no rows")
-    _need(out_dtype in _CODES, f"out_dtype must be BF16, FP16 or FP32, got {out_dtype}")
-    for t, shape, name in ((x_scales, lead, "x_scales"), (w_scales, (rows,), "w_scales"), (bias, (rows,), "bias")):
-        if t is not None:
-            _need(t.dtype == torch.float32 and t.device == x.device and tuple(t.shape) in (tuple(shape), (*shape, 1)),
-                  f"{name} must be float32 {tuple(shape)} on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    channels = rows // 2 if gated else rows
-    out = torch.empty((*lead, channels), dtype=out_dtype, device=x.device)
+def _quantize(x, code, q, scales, tokens, width) -> None:
     index = x.get_device()
-    with torch.cuda.device(index):
-        x2 = _rows(x)
-        if x2.shape[0] > 0:
-            x_scales, w_scales = x_scales.detach().contiguous(), w_scales.detach().contiguous()
-            bias = bias.detach().contiguous() if bias is not None else None
-            state = _on_device(index)
-            poll = _watch(state)
-            a = _native.MmoeInt8Product(x2.shape[0], width, channels, _CODES[out_dtype], clamp, _f._kernel_options.timeout_ms,
-                                        _stride(x2), x2.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(),
-                                        bias.data_ptr() if bias is not None else None, out.data_ptr(), state.status_ptr)
-            lib = _native.load()
-            run = lib.mmoe_int8_gated_projection if gated else lib.mmoe_int8_projection
-            _native.check(run(ctypes.byref(a), _native.raw_stream(index)))
-            if poll is not None:
-                poll.after_call(state, _f._kernel_options.status_poll_interval)
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return _quantize(x, code, q, scales, tokens, width)
+    code = _native.load().mmoe_quantize_int8(x.data_ptr(), code, _stride(x), q.data_ptr(), scales.data_ptr(), tokens, width,
+                                             _native.raw_stream(index))
+    if code:
+        _native.check(code)
+
+
+def _float_vector(t: torch.Tensor, shape, what: str, x: torch.Tensor) -> torch.Tensor:
+    if t.dtype != torch.float32 or (t.shape != shape and t.shape != (*shape, 1)) or t.device != x.device:
+        raise AssertionError(f"{what} must be float32 {tuple(shape)} on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if t.requires_grad:
+        _refuse_gradient("a product of 8-bit integers")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _int8_product(x, x_scales, w, w_scales, bias, out_dtype, clamp: float, gated: bool) -> torch.Tensor:
+    if not x.is_cuda:
+        raise RuntimeError("products of 8-bit integers run on the GPU only (there is no CPU path).")
+    shape = x.shape
+    if x.dtype != torch.int8 or len(shape) < 1:
+        raise AssertionError(f"x must be int8 (..., K), got {tuple(shape)} {x.dtype}")
+    _check_weight(w, "w13" if gated else "w", torch.int8, x)
+    rows, width = w.shape
+    if shape[-1] != width or width < 16 or width >= 131072 or width % 16 != 0:
+        raise AssertionError(f"x (..., K) and the weights (N, K) must agree on K, a multiple of 16 below 131072, got {shape[-1]} and {width}")
+    if rows < 1 or (gated and rows % 2 != 0):
+        raise AssertionError(f"the weights have {rows} rows" + (": the gated projection needs as many gate as up rows" if gated else ""))
+    code = _CODES.get(out_dtype)
+    if code is None:
+        raise AssertionError(f"out_dtype must be BF16, FP16 or FP32, got {out_dtype}")
+    lead = shape[:-1]
+    x_scales = _float_vector(x_scales, lead, "x_scales", x)
+    w_scales = _float_vector(w_scales, (rows,), "w_scales", x)
+    if bias is not None:
+        bias = _float_vector(bias, (rows,), "bias", x)
+    channels = rows // 2 if gated else rows
+    out = x.new_empty((*lead, channels), dtype=out_dtype)
+    x2 = _rows(x)
+    tokens = x2.shape[0]
+    if tokens > 0:
+        _launch("mmoe_int8_gated_projection" if gated else "mmoe_int8_projection", x2.get_device(),
+                _native.MmoeInt8Product(tokens, width, channels, code, clamp, 0, _stride(x2), x2.data_ptr(), x_scales.data_ptr(), w.data_ptr(),
+                                        w_scales.data_ptr(), _ptr(bias), out.data_ptr()))
     return out
 
 
-def int8_projection(x, x_scales, w, w_scales, *, bias=None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    return _int8_product("int8_projection", x, x_scales, w, w_scales, bias, out_dtype, math.inf, False)
+def int8_projection(x, x_scales, w, w_scales, *, bias=None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    return _int8_product(x, x_scales, w, w_scales, bias, torch.bfloat16 if out_dtype is None else out_dtype, math.inf, False)
 
 
 def int8_gated_projection(x, x_scales, w13, w13_scales, *, activation_clamp: Optional[float] = None,
-                          out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    return _int8_product("int8_gated_projection", x, x_scales, w13, w13_scales, None, out_dtype, _clamp_of(activation_clamp), True)
+                          out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    return _int8_product(x, x_scales, w13, w13_scales, None, torch.bfloat16 if out_dtype is None else out_dtype, _clamp_of(activation_clamp), True)

@@ -466,7 +466,14 @@ std::atomic<int> g_sms[kMaxDevices];        // per device, 0: prepare_dense() ha
 
 int prepared_sms() {
   int dev = 0;
-  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? g_sms[dev].load() : 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+  // tensor maps are encoded by the driver, which wants the device's context on this thread; one that has launched nothing yet has none
+  thread_local int bound = -1;
+  if (bound != dev) {
+    if (cudaSetDevice(dev) != cudaSuccess) return 0;
+    bound = dev;
+  }
+  return g_sms[dev].load();
 }
 
 // `rows` x k matrix; boxes of 128 bytes of K by `box` rows, or (stored transposed) of 64 rows by 64 k's
