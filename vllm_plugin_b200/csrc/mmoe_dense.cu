@@ -23,8 +23,8 @@ constexpr int kPairCols = 256;                        // most rows of B per tile
 constexpr int kStageA = kPairRows * 128;              // bytes
 constexpr int kStageB = kPairCols / 2 * 128;
 constexpr int kStageBytes = kStageA + kStageB;
-constexpr int kStages = 6;
-constexpr int kEpiWarps = 4;
+constexpr int kStages = 5;
+constexpr int kEpiWarps = 8;                          // two per TMEM lane quadrant, each with every other block of columns
 constexpr int kEpiBlock = 32 * 64 * 4;                // a warp's 32 rows x 64 sums on their way from lanes to rows
 constexpr int kPairThreads = 32 * (2 + kEpiWarps);
 constexpr int kPairSmem = 1024 + 1024 + kStages * kStageBytes + kEpiWarps * kEpiBlock;
@@ -191,31 +191,34 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
     }
   } else {
     // --------------------------------------------------------------------------------------------- epilogue
-    const int q = warp & 3;                       // TMEM lane quadrant this warp may read
+    const int q = warp & 3, side = (warp - 2) >> 2;   // TMEM lane quadrant this warp may read
     const uint32_t leader_empty = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
     uint8_t* block = blocks + (warp - 2) * kEpiBlock;
+    constexpr int kChunk = kKind == kGated ? 32 : 64, kLanes = kChunk / 8, kRowsAtOnce = 32 / kLanes;
+    const int sub = lane / kLanes, piece = lane % kLanes;
     uint32_t it = 0;
     for (int t = blockIdx.x / 2; t < tiles; t += step, ++it) {
       const TilePlace at = place_tile(t, p.m_tiles, p.n_tiles);
       const uint32_t acc = it & 1u;
       const int row0 = at.m * 2 * kPairRows + static_cast<int>(cta) * kPairRows + q * 32, rows = min(32, p.m - row0);
-      const int width = kKind == kGated ? half : p.cols, col0 = at.n * width;
-      constexpr int kChunk = kKind == kGated ? 32 : 64;
+      const int width = kKind == kGated ? half : p.cols, col0 = at.n * width, last = min(p.n, col0 + width);
+      const float row_scale = kInt8 && lane < rows ? __ldg(p.epi.row_scale + row0 + lane) : 0.f;
       if (!waiter.wait_warp(smem_u32(&ctl->acc_full[acc]), (it >> 1) & 1u)) break;
       tc_fence_after();
       const uint32_t d = tmem_base + acc * kPairCols + (static_cast<uint32_t>(q * 32) << 16);
-      const int chunks = rows > 0 ? (min(width, p.n - col0) + kChunk - 1) / kChunk : 0;
+      const int chunks = rows > 0 ? (last - col0 + kChunk - 1) / kChunk : 0;
 #pragma unroll 1
-      for (int c = 0; c < chunks; ++c) {
+      for (int c = side; c < chunks; c += 2) {
         uint32_t v[64];
         tc_ld32(d + kChunk * c, v);
         tc_ld32(kKind == kGated ? d + half + 32 * c : d + 64 * c + 32, v + 32);
+        const DenseFinish<kKind, kInt8> finish(p.epi, last, col0 + kChunk * c + 8 * piece);
         tc_ld_wait();
         if (kInt8) {
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] = __float_as_uint(static_cast<float>(static_cast<int32_t>(v[j])));
         }
-        if (c + 1 == chunks) {
+        if (c + 2 >= chunks) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_pair(leader_empty + 8 * acc);
@@ -223,19 +226,17 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
         __syncwarp();                             // the previous block has been read
         block_write(block, lane, v);
         __syncwarp();
-        constexpr int kLanes = kChunk / 8, kRowsAtOnce = 32 / kLanes;
-        const int sub = lane / kLanes, piece = lane % kLanes;
-        const int col = col0 + kChunk * c + 8 * piece;
-        const int last = min(p.n, col0 + width);
-#pragma unroll 2
-        for (int r = sub; r < rows; r += kRowsAtOnce) {
+#pragma unroll 4
+        for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
+          const int r = i * kRowsAtOnce + sub;
           float a[8], b[8];
           block_read8(block, r, 2 * piece, kKind != kGated && piece >= 4, a);
           if (kKind == kGated) block_read8(block, r, 8 + 2 * piece, false, b);
-          dense_finish8<kKind>(p.epi, last, row0 + r, col, a, b);
+          const float rs = kInt8 ? __shfl_sync(0xffffffffu, row_scale, r) : 0.f;
+          if (r < rows) finish.row(row0 + r, rs, a, b);
         }
       }
-      if (chunks == 0) {
+      if (side >= chunks) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_pair(leader_empty + 8 * acc);
@@ -262,11 +263,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
 // in shared memory, added in the order of the CTAs: no atomics, no workspace, and the same bits in every call.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 128;                         // rows of B per tile
-constexpr int kFewThreads = 192;
+constexpr int kFewThreads = 256;
 constexpr int kFewMaxStages = 12;
-constexpr int kFewChunk = 64;                         // tokens whose partial sums are in shared memory at a time
-constexpr int kFewPartBytes = kFewChunk * kFewRows * 4;
 constexpr int kFewMaxTokens = 256;                    // per tile
+constexpr int kFewMaxSplit = 8;
+constexpr int kFewSmem = 227 * 1024;
 
 struct FewParams {
   CUtensorMap map_w, map_t;
@@ -286,8 +287,10 @@ struct FewControl {
   uint64_t acc_full;
   uint32_t tmem_base;
   volatile int32_t abort_flag;
+  float row_scale[kFewMaxTokens];
 };
-static_assert(sizeof(FewControl) <= 1024, "control block");
+static_assert(sizeof(FewControl) <= 2048, "control block");
+static_assert(2 * 1024 + 1024 + kFewMaxTokens * kFewRows * 4 <= kFewSmem, "partial sums of a tile fit where the stages were");
 
 template <bool kInt8>
 __device__ __forceinline__ void single_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -305,20 +308,31 @@ __device__ __forceinline__ float4 cluster_load(uint32_t addr) {
   return v;
 }
 
-// eight neighbouring sums of a token over the CTAs of the cluster
+// eight neighbouring sums of a token over the CTAs of the cluster; `swap`: second half first, so that eight lanes read all banks
 template <bool kInt8>
-__device__ __forceinline__ void add_parts(uint32_t addr, int split, float (&v)[8]) {
-  int32_t whole[8];
+__device__ __forceinline__ void add_parts(uint32_t addr, bool swap, int split, float (&v)[8]) {
+  float4 lo[4], hi[4];
+  int32_t whole[8] = {};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = 0.f, whole[j] = 0;
-  for (int r = 0; r < split; ++r) {
-    const uint32_t from = map_to_cta(addr, r);
-    const float4 lo = cluster_load(from), hi = cluster_load(from + 16);
-    const float part[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  for (int r0 = 0; r0 < split; r0 += 4) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (kInt8) whole[j] += __float_as_int(part[j]);
-      else v[j] += part[j];
+    for (int r = 0; r < 4; ++r) {
+      if (r0 + r >= split) break;
+      const uint32_t from = map_to_cta(addr, r0 + r);
+      lo[r] = cluster_load(from + (swap ? 16 : 0));
+      hi[r] = cluster_load(from + (swap ? 0 : 16));
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (r0 + r >= split) break;
+      const float4 p = swap ? hi[r] : lo[r], q = swap ? lo[r] : hi[r];
+      const float part[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (kInt8) whole[j] += __float_as_int(part[j]);
+        else v[j] += part[j];
+      }
     }
   }
   if (kInt8) {
@@ -328,11 +342,11 @@ __device__ __forceinline__ void add_parts(uint32_t addr, int split, float (&v)[8
 }
 
 template <bool kInt8, bool kWmn, int kKind>
-__global__ void __launch_bounds__(kFewThreads, 2) dense_few_kernel(const __grid_constant__ FewParams p) {
+__global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_constant__ FewParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the same offset in all CTAs
   FewControl* ctl = reinterpret_cast<FewControl*>(smem);
-  uint8_t* stages = smem + 1024;
+  uint8_t* stages = smem + 2048;
   constexpr int kDepth = kInt8 ? 128 : 64;
   constexpr int kWBytes = kFewRows * 128;
   const int t_bytes = p.tokens * 128, stage_bytes = kWBytes + t_bytes;
@@ -410,39 +424,40 @@ __global__ void __launch_bounds__(kFewThreads, 2) dense_few_kernel(const __grid_
   }
 
   // ------------------------------------------------------------------------------------------------- sums
-  // everything staged has been multiplied when the accumulator is complete, so the partial sums may take its place: [token][128 rows]
-  bool ok = true;
-  if (warp >= 2) {
-    ok = waiter.wait_warp(smem_u32(&ctl->acc_full), 0);
-    tc_fence_after();
-  }
+  // A thread finishes the same eight channels of every so many tokens; what belongs to the channels and tokens is fetched ahead.
   constexpr int kGroups = kKind == kGated ? kFewRows / 16 : kFewRows / 8;     // eight channels each
-  const int tokens = min(p.tokens, p.m - tok0);
-  for (int c0 = 0; c0 < tokens; c0 += kFewChunk) {
-    const int here = min(kFewChunk, tokens - c0);
-    if (warp >= 2 && ok) {
-      const int row = (warp & 3) * 32 + lane;
-      const uint32_t d = tmem_base + c0 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-      for (int j0 = 0; j0 < here; j0 += 16) {
-        uint32_t v[16];
-        tc_ld16(d + j0, v);
-        tc_ld_wait();
+  static_assert(kFewThreads % kGroups == 0, "a thread keeps its channels");
+  const int tokens = min(p.tokens, p.m - tok0), g = static_cast<int>(threadIdx.x) % kGroups;
+  const DenseFinish<kKind, kInt8> finish(p.epi, p.n, tile * 8 * kGroups + 8 * g);
+  if (kInt8)
+    for (int t = threadIdx.x; t < tokens; t += kFewThreads) ctl->row_scale[t] = __ldg(p.epi.row_scale + tok0 + t);
+  // Everything staged has been multiplied when the accumulator is complete, so the partial sums may take its place: [token][128 rows].
+  if (warp >= 2 && warp < 6 && waiter.wait_warp(smem_u32(&ctl->acc_full), 0)) {
+    tc_fence_after();
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t d = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    for (int j0 = 0; j0 < tokens; j0 += 16) {
+      uint32_t v[16];
+      tc_ld16(d + j0, v);
+      tc_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) reinterpret_cast<uint32_t*>(stages)[(j0 + j) * kFewRows + row] = v[j];
-      }
+      for (int j = 0; j < 16; ++j) reinterpret_cast<uint32_t*>(stages)[(j0 + j) * kFewRows + row] = v[j];
     }
-    __syncwarp();
-    cluster_sync_all();
-    for (int i = rank * kFewThreads + static_cast<int>(threadIdx.x); i < here * kGroups; i += p.split * kFewThreads) {
-      const int t = i / kGroups, g = i - t * kGroups;
-      float a[8], b[8];
-      add_parts<kInt8>(base + (t * kFewRows + 8 * g) * 4, p.split, a);
-      if (kKind == kGated) add_parts<kInt8>(base + (t * kFewRows + kFewRows / 2 + 8 * g) * 4, p.split, b);
-      dense_finish8<kKind>(p.epi, p.n, tok0 + c0 + t, tile * 8 * kGroups + 8 * g, a, b);
-    }
-    __syncwarp();
-    cluster_sync_all();                     // read by all, before the next sums or the end of this CTA
   }
+  __syncwarp();
+  cluster_sync_all();
+#pragma unroll 2
+  for (int i = rank * kFewThreads + static_cast<int>(threadIdx.x); i < tokens * kGroups; i += p.split * kFewThreads) {
+    const int t = i / kGroups;
+    const uint32_t at = base + (t * kFewRows + 8 * g) * 4;
+    const bool swap = (g & 4) != 0;
+    float a[8], b[8];
+    add_parts<kInt8>(at, swap, p.split, a);
+    if (kKind == kGated) add_parts<kInt8>(at + kFewRows / 2 * 4, swap, p.split, b);
+    finish.row(tok0 + t, kInt8 ? ctl->row_scale[t] : 0.f, a, b);
+  }
+  __syncwarp();
+  cluster_sync_all();                       // the sums are read by all before any CTA ends
 
   // ---------------------------------------------------------------------------------------------------- teardown
   if (ctl->abort_flag != 0) {
@@ -519,9 +534,9 @@ cudaError_t for_each_few_kernel(F f) {
   return e;
 }
 
-constexpr int kFewSmemHalf = 113 * 1024, kFewSmemFull = 227 * 1024;     // two CTAs to an SM, or one
+std::atomic<int> g_clusters[kMaxDevices][kFewMaxSplit + 1];     // clusters of so many CTAs that run at once
 
-cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
+cudaError_t launch_few(const DenseProduct& p, cudaStream_t s) {
   FewParams d;
   d.m = p.m, d.n = p.n;
   const int depth = p.type == kDenseInt8 ? 128 : 64;
@@ -529,11 +544,13 @@ cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   const int parts = (p.m + kFewMaxTokens - 1) / kFewMaxTokens;
   d.tokens = ((p.m + parts - 1) / parts + 15) & ~15;
   const int width = p.kind == kGated ? kFewRows / 2 : kFewRows, tiles = (p.n + width - 1) / width;
-  const int stage_bytes = kFewRows * 128 + d.tokens * 128;
-  const bool two = d.tokens <= 128;
-  const int smem = two ? kFewSmemHalf : kFewSmemFull;
-  d.stages = std::min((smem - 2048) / stage_bytes, kFewMaxStages);
-  d.split = std::max(1, std::min({8, (two ? 2 : 1) * sms / (tiles * parts), d.k_stages / 4}));
+  d.stages = std::min((kFewSmem - 3072) / (kFewRows * 128 + d.tokens * 128), kFewMaxStages);
+  // as many CTAs as run at once, with a few stages for each
+  int dev = 0;
+  cudaGetDevice(&dev);
+  d.split = 1;
+  for (int c = 2; c <= kFewMaxSplit; ++c)
+    if (tiles * parts <= g_clusters[dev][c].load() && d.k_stages >= 4 * c) d.split = c;
   d.idesc = product_idesc(p.type, p.b.k_rows, false, kFewRows, d.tokens);
   d.tmem_cols = d.tokens <= 32 ? 32 : d.tokens <= 64 ? 64 : d.tokens <= 128 ? 128 : 256;
   d.epi = p.epi;
@@ -545,7 +562,7 @@ cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   const cudaError_t e = for_each_few_kernel([&](auto kernel, int type, bool w_mn, int kind) {
     if ((type == kDenseInt8) != (p.type == kDenseInt8) || w_mn != p.b.k_rows || kind != p.kind) return cudaSuccess;
     found = true;
-    return launch_clustered(kernel, dim3(tiles * d.split, parts), dim3(kFewThreads), smem, d.split, s, d);
+    return launch_clustered(kernel, dim3(tiles * d.split, parts), dim3(kFewThreads), kFewSmem, d.split, s, d);
   });
   return found ? e : cudaErrorInvalidValue;
 }
@@ -671,7 +688,18 @@ cudaError_t prepare_dense() {
   if (e == cudaSuccess)
     e = for_each_pair_kernel([](auto kernel, int, bool, bool, int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem); });
   if (e == cudaSuccess)
-    e = for_each_few_kernel([](auto kernel, int, bool, int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmemFull); });
+    e = for_each_few_kernel([](auto kernel, int, bool, int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem); });
+  for (int c = 2; c <= kFewMaxSplit && e == cudaSuccess; ++c) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c), cfg.blockDim = dim3(kFewThreads), cfg.dynamicSmemBytes = kFewSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = c, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    int n = 0;
+    e = cudaOccupancyMaxActiveClusters(&n, dense_few_kernel<true, false, kLinear>, &cfg);
+    g_clusters[dev][c].store(n);
+  }
   if (e == cudaSuccess) g_sms[dev].store(sms);
   return e;
 }
@@ -680,7 +708,7 @@ cudaError_t launch_dense(const DenseProduct& p, cudaStream_t s) {
   if (p.m <= 0 || p.n <= 0) return cudaSuccess;
   const int sms = prepared_sms();
   if (sms == 0) return cudaErrorNotReady;
-  return !p.a.k_rows && p.m <= kFewMaxTokens ? launch_few(p, sms, s) : launch_pairs(p, sms, s);
+  return !p.a.k_rows && p.m <= kFewMaxTokens ? launch_few(p, s) : launch_pairs(p, sms, s);
 }
 
 cudaError_t launch_quantize_int8(const void* x, int type, int64_t ld, int8_t* q, float* scales, int m, int k, cudaStream_t s) {

@@ -90,12 +90,13 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8], int valid) {
     if (j < valid) dst[j] = from_float<T>(v[j]);
 }
 
-// What follows a product, for eight neighbouring columns of a row: `a` the sums (kGated: the gate's, and `b` the up row's).
-template <int kKind>
-__device__ __forceinline__ void dense_finish8(const DenseEpilogue& e, int n, int row, int col, float (&a)[8], float (&b)[8]) {
-  const int valid = n - col;
-  if (valid <= 0) return;
-  const auto load8 = [&](const float* src, float (&v)[8]) {
+// What follows a product, for eight neighbouring columns: made once for the columns, then called for the rows.  `n` ends the columns.
+template <int kKind, bool kScaled>
+struct DenseFinish {
+  const DenseEpilogue& e;
+  const int col, valid;
+  float cs[8], second[8];              // scales of the columns; kGated: those of the up columns, kLinear: bias
+  __device__ __forceinline__ void load8(const float* src, float (&v)[8]) const {
     if (valid >= 8 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
       const float4 lo = __ldg(reinterpret_cast<const float4*>(src)), hi = __ldg(reinterpret_cast<const float4*>(src) + 1);
       v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
@@ -103,53 +104,56 @@ __device__ __forceinline__ void dense_finish8(const DenseEpilogue& e, int n, int
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = j < valid ? __ldg(src + j) : 0.f;
-  };
-  const auto scale8 = [&](float (&v)[8], const float* col_scale) {
-    const float rs = __ldg(e.row_scale + row);
-    float cs[8];
-    load8(col_scale, cs);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = v[j] * rs * cs[j];
-  };
-  const auto put = [&](int64_t at, const float (&v)[8]) {
+  }
+  __device__ __forceinline__ DenseFinish(const DenseEpilogue& epi, int n, int column) : e(epi), col(column), valid(n - column) {
+    if (!kScaled) return;
+    load8(e.col_scale + col, cs);
+    if (kKind == kGated) load8(e.col_scale + e.inter + col, second);
+    else if (e.bias != nullptr) load8(e.bias + col, second);
+  }
+  __device__ __forceinline__ void put(int64_t at, const float (&v)[8]) const {
     if (e.out_type == kDenseBf16) store8(static_cast<__nv_bfloat16*>(e.out) + at, v, valid);
     else if (e.out_type == kDenseFp16) store8(static_cast<__half*>(e.out) + at, v, valid);
     else store8(static_cast<float*>(e.out) + at, v, valid);
-  };
-  const int64_t at = row * e.ld_out + col;
-  if (kKind == kLinear) {
-    if (e.col_scale != nullptr) scale8(a, e.col_scale + col);
-    if (e.bias != nullptr) {
-      float bias[8];
-      load8(e.bias + col, bias);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] += bias[j];
-    }
-    put(at, a);
-  } else if (kKind == kGated) {
-    if (e.col_scale != nullptr) {
-      scale8(a, e.col_scale + col);
-      scale8(b, e.col_scale + e.inter + col);
-    }
-    if (e.preact != nullptr) {
-      float* keep = e.preact + (int64_t)row * 2 * e.inter + col;
-      store8(keep, a, valid);
-      store8(keep + e.inter, b, valid);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = gated_value(a[j], b[j], e.clamp);
-    put(at, a);
-  } else {
-    const float* keep = e.preact + (int64_t)row * 2 * e.inter + col;
-    float g[8], u[8];
-    load8(keep, g);
-    load8(keep + e.inter, u);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) gated_grad(a[j], g[j], u[j], e.clamp, g[j], u[j]);
-    put(at, g);
-    put(at + e.inter, u);
   }
-}
+  // `a`: the sums (kGated: the gate's, `b` the up row's), `rs` the scale of the row
+  __device__ __forceinline__ void row(int row, float rs, float (&a)[8], float (&b)[8]) const {
+    if (valid <= 0) return;
+    const int64_t at = row * e.ld_out + col;
+    if (kKind == kLinear) {
+      if (kScaled) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] = a[j] * rs * cs[j];
+        if (e.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) a[j] += second[j];
+        }
+      }
+      put(at, a);
+    } else if (kKind == kGated) {
+      if (kScaled) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] = a[j] * rs * cs[j], b[j] = b[j] * rs * second[j];
+      } else if (e.preact != nullptr) {
+        float* keep = e.preact + (int64_t)row * 2 * e.inter + col;
+        store8(keep, a, valid);
+        store8(keep + e.inter, b, valid);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] = gated_value(a[j], b[j], e.clamp);
+      put(at, a);
+    } else {
+      const float* keep = e.preact + (int64_t)row * 2 * e.inter + col;
+      float g[8], u[8];
+      load8(keep, g);
+      load8(keep + e.inter, u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) gated_grad(a[j], g[j], u[j], e.clamp, g[j], u[j]);
+      put(at, g);
+      put(at + e.inter, u);
+    }
+  }
+};
 #endif
 
 }  // namespace mmoe
