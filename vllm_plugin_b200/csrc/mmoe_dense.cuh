@@ -116,8 +116,14 @@ struct DenseFinish {
     else if (e.out_type == kDenseFp16) store8(static_cast<__half*>(e.out) + at, v, valid);
     else store8(static_cast<float*>(e.out) + at, v, valid);
   }
-  // `a`: the sums (kGated: the gate's, `b` the up row's), `rs` the scale of the row
-  __device__ __forceinline__ void row(int row, float rs, float (&a)[8], float (&b)[8]) const {
+  // kGatedGrad: g and u of a row, to be fetched well ahead of row()
+  __device__ __forceinline__ void fetch(int row, float (&g)[8], float (&u)[8]) const {
+    const float* keep = e.preact + (int64_t)row * 2 * e.inter + col;
+    load8(keep, g);
+    load8(keep + e.inter, u);
+  }
+  // `a`: the sums (kGated: the gate's, `b` the up row's; kGatedGrad: `b` and `u` as fetched), `rs` the scale of the row
+  __device__ __forceinline__ void row(int row, float rs, float (&a)[8], float (&b)[8], float (&u)[8]) const {
     if (valid <= 0) return;
     const int64_t at = row * e.ld_out + col;
     if (kKind == kLinear) {
@@ -143,13 +149,9 @@ struct DenseFinish {
       for (int j = 0; j < 8; ++j) a[j] = gated_value(a[j], b[j], e.clamp);
       put(at, a);
     } else {
-      const float* keep = e.preact + (int64_t)row * 2 * e.inter + col;
-      float g[8], u[8];
-      load8(keep, g);
-      load8(keep + e.inter, u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) gated_grad(a[j], g[j], u[j], e.clamp, g[j], u[j]);
-      put(at, g);
+      for (int j = 0; j < 8; ++j) gated_grad(a[j], b[j], u[j], e.clamp, b[j], u[j]);
+      put(at, b);
       put(at + e.inter, u);
     }
   }
