@@ -635,76 +635,127 @@ cudaError_t launch_pairs(const DenseProduct& p, int sms, cudaStream_t s) {
 // Per-token quantiser: s = max|x| / 127, q = x / s rounded to the nearest whole number, ties to even.
 // A block per token; the row stays in registers between the two passes as far as it fits.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int kQuantThreads = 256, kQuantHeld = 4;      // vectors of eight values that a thread keeps
+constexpr int kQuantThreads = 512;
 
-// Exact: t = x / s is known to about an ulp, so rint(t) is the nearest whole number or, next to a border, its neighbour; the remainder
-// x - q s is exact in one fma (x has at most 11 bits and is above s / 2 in magnitude where it matters) and tells which.
-__device__ __forceinline__ int quantize_one(float x, float s, float inv) {
-  float q = rintf(inv > 0.f ? x * inv : __fdiv_rn(x, s));
-  const float r = fmaf(-q, s, x), twice = r + r;
-  if (fabsf(twice) >= s) {
-    const bool odd = (static_cast<int>(q) & 1) != 0;
-    if (fabsf(twice) > s || odd) q += copysignf(1.f, r);
+// x / s as whole numbers, exactly, in the low bytes.  Adding 1.5 * 2^23 rounds the product with the reciprocal to a whole number q, the nearest
+// one or, next to a border, its neighbour.  The remainder x - q s is exact in one fma (x has at most 11 bits and is above s / 2 in magnitude
+// where it matters) and tells which; that is looked at once for all n values.  kTiny: s is so small that its reciprocal overflows or half of
+// it is no number.
+template <bool kTiny, int n>
+__device__ __forceinline__ void quantize_some(const float (&x)[n], float s, float inv, uint32_t (&q)[n]) {
+  constexpr float kShift = 12582912.f;
+  float r[n], worst = 0.f;
+#pragma unroll
+  for (int j = 0; j < n; ++j) {
+    const float shifted = kTiny ? __fadd_rn(__fdiv_rn(x[j], s), kShift) : fmaf(x[j], inv, kShift);
+    q[j] = __float_as_uint(shifted);
+    r[j] = fmaf(-__fsub_rn(shifted, kShift), s, x[j]);
+    worst = fmaxf(worst, fabsf(r[j]));
   }
-  return static_cast<int>(q);
+  if (kTiny ? worst + worst < s : worst < 0.5f * s) return;
+#pragma unroll
+  for (int j = 0; j < n; ++j) {
+    const float twice = fabsf(r[j] + r[j]);
+    if (twice > s || (twice == s && (q[j] & 1u) != 0)) q[j] += r[j] > 0.f ? 1u : ~0u;
+  }
 }
 
-template <typename T, bool kVec>
+__device__ __forceinline__ __half2 pair_abs_max(__half2 top, __half2 v) { return __hmax2_nan(top, __habs2(v)); }
+__device__ __forceinline__ __nv_bfloat162 pair_abs_max(__nv_bfloat162 top, __nv_bfloat162 v) { return __hmax2_nan(top, __habs2(v)); }
+__device__ __forceinline__ float2 pair_floats(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 pair_floats(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+template <typename T> struct PairOf;
+template <> struct PairOf<__half> { using type = __half2; };
+template <> struct PairOf<__nv_bfloat16> { using type = __nv_bfloat162; };
+
+// kVec: eight values at a time, else (widths, strides or places that do not allow it) one.  kQuantHeld: vectors that a thread keeps.
+template <typename T, bool kVec, int kQuantHeld>
 __global__ void __launch_bounds__(kQuantThreads) quantize_int8_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q,
                                                                       float* __restrict__ scales, int k) {
   chain_begin();
+  using P = typename PairOf<T>::type;
   constexpr int kWide = kVec ? 8 : 1;
   struct alignas(sizeof(T) * kWide) Vec { T v[kWide]; };
-  struct alignas(kWide) Out { int8_t v[kWide]; };
   const int64_t row = blockIdx.x;
   const Vec* in = reinterpret_cast<const Vec*>(x + row * ld);
-  Out* out = reinterpret_cast<Out*>(q + row * k);
   const int n = k / kWide, step = blockDim.x;
   Vec held[kQuantHeld];
-  // magnitudes as bits: NaN is above infinity there, so neither is lost
-  uint32_t top = 0;
+  P top = {T(0.f), T(0.f)};
   const auto look = [&](const Vec& v) {
+    if (kVec) {
 #pragma unroll
-    for (int j = 0; j < kWide; ++j) top = max(top, __float_as_uint(fabsf(static_cast<float>(v.v[j]))));
+      for (int j = 0; j < kWide / 2; ++j) top = pair_abs_max(top, reinterpret_cast<const P*>(&v)[j]);
+    } else {
+      top = pair_abs_max(top, P{v.v[0], T(0.f)});
+    }
   };
 #pragma unroll
   for (int i = 0; i < kQuantHeld; ++i) {
     const int at = threadIdx.x + i * step;
-    if (at < n) look(held[i] = in[at]);
+    if (at < n) held[i] = in[at];
   }
+#pragma unroll
+  for (int i = 0; i < kQuantHeld; ++i)
+    if (threadIdx.x + i * step < n) look(held[i]);
   for (int at = threadIdx.x + kQuantHeld * step; at < n; at += step) look(in[at]);
+  // magnitudes as bits: NaN is above infinity there, so neither is lost
   __shared__ uint32_t tops[kQuantThreads / 32];
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  const float2 both = pair_floats(top);
+  uint32_t bits = __reduce_max_sync(0xffffffffu, max(__float_as_uint(both.x), __float_as_uint(both.y)));
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = bits;
   __syncthreads();
-  for (int w = 0; w < (step >> 5); ++w) top = max(top, tops[w]);
-  const float amax = __uint_as_float(top);
-  const bool finite = top < 0x7f800000u;
-  const float s = !finite ? __uint_as_float(0x7fffffffu) : (top == 0 ? 1.f : __fdiv_rn(amax, 127.f));
-  const float inv = s >= 0x1p-100f ? __fdiv_rn(1.f, s) : 0.f;       // of a tiny scale the reciprocal overflows
-  const auto put = [&](const Vec& v, int at) {
-    Out o;
-#pragma unroll
-    for (int j = 0; j < kWide; ++j) o.v[j] = finite ? static_cast<int8_t>(quantize_one(static_cast<float>(v.v[j]), s, inv)) : 0;
-    out[at] = o;
-  };
-#pragma unroll
-  for (int i = 0; i < kQuantHeld; ++i) {
-    const int at = threadIdx.x + i * step;
-    if (at < n) put(held[i], at);
-  }
-  for (int at = threadIdx.x + kQuantHeld * step; at < n; at += step) put(in[at], at);
+  for (int w = 0; w < (step >> 5); ++w) bits = max(bits, tops[w]);
+  const bool finite = bits < 0x7f800000u;
+  const float s = !finite ? __uint_as_float(0x7fffffffu) : (bits == 0 ? 1.f : __fdiv_rn(__uint_as_float(bits), 127.f));
   if (threadIdx.x == 0) scales[row] = s;
+  const auto finish = [&](auto some) {
+    const auto put = [&](const Vec& v, int at) {
+      float f[kWide];
+      uint32_t b[kWide];
+      if constexpr (kVec) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 two = pair_floats(reinterpret_cast<const P*>(&v)[j]);
+          f[2 * j] = two.x, f[2 * j + 1] = two.y;
+        }
+        some(f, b);
+        uint2 o;
+        o.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+        o.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+        reinterpret_cast<uint2*>(q + row * k)[at] = o;
+      } else {
+        f[0] = static_cast<float>(v.v[0]);
+        some(f, b);
+        q[row * k + at] = static_cast<int8_t>(b[0] & 0xffu);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kQuantHeld; ++i) {
+      const int at = threadIdx.x + i * step;
+      if (at < n) put(held[i], at);
+    }
+    for (int at = threadIdx.x + kQuantHeld * step; at < n; at += step) put(in[at], at);
+  };
+  const float inv = __fdiv_rn(1.f, s);
+  if (!finite) finish([](const float (&)[kWide], uint32_t (&b)[kWide]) { for (uint32_t& v : b) v = 0; });
+  else if (s >= 0x1p-100f) finish([&](const float (&f)[kWide], uint32_t (&b)[kWide]) { quantize_some<false>(f, s, inv, b); });
+  else finish([&](const float (&f)[kWide], uint32_t (&b)[kWide]) { quantize_some<true>(f, s, inv, b); });
 }
+
+// Many tokens: few threads to each, so that all tokens of an SM are on their way at once; few tokens: many, for a short way.
+constexpr int kQuantManyTokens = 512;
 
 template <typename T>
 cudaError_t launch_quantize(const void* x, int64_t ld, int8_t* q, float* scales, int m, int k, cudaStream_t s) {
   const T* in = static_cast<const T*>(x);
   const bool vec = k % 8 == 0 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0;
+  const bool many = vec && m >= kQuantManyTokens;
   // as few threads as keep the same number of vectors each
-  const int n = vec ? k / 8 : k, each = (n + kQuantThreads - 1) / kQuantThreads, threads = ((n + each - 1) / each + 31) & ~31;
-  return vec ? launch_chained(quantize_int8_kernel<T, true>, dim3(m), dim3(threads), 0, s, in, ld, q, scales, k)
-             : launch_chained(quantize_int8_kernel<T, false>, dim3(m), dim3(threads), 0, s, in, ld, q, scales, k);
+  const int n = vec ? k / 8 : k, most = many ? std::max(32, std::min(kQuantThreads, (n + 11) / 12)) : kQuantThreads;
+  const int each = (n + most - 1) / most, threads = std::min(kQuantThreads, ((n + each - 1) / each + 31) & ~31);
+  if (many) return launch_chained(quantize_int8_kernel<T, true, 12>, dim3(m), dim3(threads), 0, s, in, ld, q, scales, k);
+  return vec ? launch_chained(quantize_int8_kernel<T, true, 4>, dim3(m), dim3(threads), 0, s, in, ld, q, scales, k)
+             : launch_chained(quantize_int8_kernel<T, false, 12>, dim3(m), dim3(threads), 0, s, in, ld, q, scales, k);
 }
 
 }  // namespace
