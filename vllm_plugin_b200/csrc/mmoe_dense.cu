@@ -1,6 +1,7 @@
 // Products of the dense feed-forward operators for sm_100a (see mmoe_dense.cuh).
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "mmoe_dense.cuh"
 #include "mmoe_tc.cuh"
@@ -29,14 +30,22 @@ constexpr int kPairSmem = 227 * 1024;
 constexpr int kPairStageRoom = kPairSmem - 1024 - 1024 - kEpiWarps * kEpiBlock;
 constexpr int kStatusDense = 31;
 
-struct DenseParams {
+// One product of a launch
+struct DensePart {
   CUtensorMap map_a, map_b;
+  DenseEpilogue epi;
   int32_t m, n, k_stages;
   int32_t cols;              // rows of B per tile (kGated: half of them gate rows), a multiple of 32
-  int32_t stages, stage_bytes;
   int32_t m_tiles, n_tiles;
-  uint32_t idesc;
-  DenseEpilogue epi;
+  int32_t first_tile;        // of the launch
+  int32_t kind, a_mn, b_mn;
+  uint32_t idesc, tx_bytes;  // tx_bytes: a stage's copies into both CTAs
+};
+
+struct DenseParams {
+  DensePart part[kMaxParts];
+  int32_t parts, tiles;
+  int32_t stages, stage_bytes;
   int32_t* status;
   int64_t timeout_ns;
 };
@@ -56,6 +65,10 @@ __device__ __forceinline__ uint64_t operand_desc(bool mn_major, uint32_t block) 
   return desc_hi_sw128() | (mn_major ? static_cast<uint64_t>(block >> 4) << 16 : 0ull);
 }
 
+__device__ __forceinline__ void prefetch_bulk(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
 template <bool kInt8>
 __device__ __forceinline__ void pair_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   if (kInt8)
@@ -66,14 +79,19 @@ __device__ __forceinline__ void pair_product(uint32_t d, uint64_t a, uint64_t b,
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// The t-th tile: eight tiles of rows at a time, all columns of those before the next eight, so that what runs at once reads few
+// The t-th tile of a product: eight tiles of rows at a time, all columns of those before the next eight, so that what runs at once reads few
 // different rows of either operand.
 struct TilePlace {
   int m, n;
 };
-__device__ __forceinline__ TilePlace place_tile(int t, int m_tiles, int n_tiles) {
-  const int group = t / (8 * n_tiles), first = group * 8, rows = min(8, m_tiles - first), in = t - group * 8 * n_tiles;
+__device__ __forceinline__ TilePlace place_tile(const DensePart& q, int t) {
+  t -= q.first_tile;
+  const int group = t / (8 * q.n_tiles), first = group * 8, rows = min(8, q.m_tiles - first), in = t - group * 8 * q.n_tiles;
   return TilePlace{first + in % rows, in / rows};
+}
+template <int kParts>
+__device__ __forceinline__ const DensePart& part_of(const DenseParams& p, int t) {
+  return p.part[kParts > 1 && p.parts > 1 && t >= p.part[1].first_tile ? 1 : 0];
 }
 
 // A warp's 32 x 32 block of sums, turned from one row per lane to eight columns per lane.  16-byte piece g of row r lies at g ^ (r & 7).
@@ -88,7 +106,67 @@ __device__ __forceinline__ void block_read8(const uint8_t* block, int row, int p
   v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
 }
 
-template <bool kInt8, bool kAmn, bool kBmn, int kKind>
+// f(whether A, whether B is staged with its rows along the 128 bytes), known to the compiler
+template <bool kInt8, int kSet, typename F>
+__device__ __forceinline__ void by_order(const DensePart& q, F f) {
+  if (kInt8 || kSet == kGated || q.b_mn == 0) f(std::false_type(), std::false_type());
+  else if (q.a_mn == 0) f(std::false_type(), std::true_type());
+  else f(std::true_type(), std::true_type());
+}
+
+// What an epilogue warp does with its share of a tile: rows q * 32 ... of this CTA's 128, every other block of columns.
+struct EpiPlace {
+  uint32_t d;                // accumulator, this warp's lanes
+  int row0, rows, col0, last;
+  int side, lane;
+  uint8_t* block;
+};
+template <bool kInt8, int kKind, typename Release>
+__device__ __forceinline__ void pair_epilogue(const DenseEpilogue& epi, int cols, const EpiPlace& e, float row_scale, Release release) {
+  constexpr int kChunk = kKind == kGated ? 16 : 32, kLanes = kChunk / 8, kRowsAtOnce = 32 / kLanes, kTurns = kLanes;
+  const int sub = e.lane / kLanes, piece = e.lane % kLanes;
+  const int chunks = e.rows > 0 ? (e.last - e.col0 + kChunk - 1) / kChunk : 0;
+  if (e.side >= chunks) release();
+#pragma unroll 1
+  for (int c = e.side; c < chunks; c += 2) {
+    const DenseFinish<kKind, kInt8> finish(epi, e.last, e.col0 + kChunk * c + 8 * piece);
+    float g[kTurns][8], u[kTurns][8];
+    if (kKind == kGatedGrad) {
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i)
+        if (i * kRowsAtOnce + sub < e.rows) finish.fetch(e.row0 + i * kRowsAtOnce + sub, g[i], u[i]);
+    }
+    uint32_t v[32];
+    if (kKind == kGated) {
+      tc_ld16(e.d + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(v));
+      tc_ld16(e.d + cols / 2 + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
+    } else {
+      tc_ld32(e.d + 32 * c, v);
+    }
+    tc_ld_wait();
+    if (kInt8) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(static_cast<float>(static_cast<int32_t>(v[j])));
+    }
+    if (c + 2 >= chunks) release();
+    __syncwarp();                             // the previous block has been read
+    block_write(e.block, e.lane, v);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const int r = i * kRowsAtOnce + sub;
+      float a[8];
+      block_read8(e.block, r, 2 * piece, a);
+      if (kKind == kGated) block_read8(e.block, r, 4 + 2 * piece, g[i]);
+      const float rs = kInt8 ? __shfl_sync(0xffffffffu, row_scale, r) : 0.f;
+      if (r < e.rows) finish.row(e.row0 + r, rs, a, g[i], u[i]);
+    }
+  }
+}
+
+// kSet: the kind of every product of the launch; kGatedGrad: of the first or none, the others kLinear.  kParts: most products; with one, its
+// fields are at fixed places (two: 8-bit projection of 777 tokens 23.7 -> 24.7 us, 16-bit block of 1021 57.5 -> 58.5).
+template <bool kInt8, int kSet, int kParts>
 __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __grid_constant__ DenseParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the same offset in both CTAs
@@ -101,8 +179,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
   const uint32_t cta = cluster_ctarank();
   chain_release();
   if (threadIdx.x == 0) {
-    prefetch_map(&p.map_a);
-    prefetch_map(&p.map_b);
+    for (int i = 0; i < p.parts; ++i) {
+      prefetch_map(&p.part[i].map_a);
+      prefetch_map(&p.part[i].map_b);
+    }
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(smem_u32(&ctl->full[i]), 1);
       mbar_init(smem_u32(&ctl->empty[i]), 1);
@@ -124,7 +204,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
   tc_fence_after();
   chain_wait();                             // nothing above touches global memory
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
-  const int tiles = p.m_tiles * p.n_tiles, step = gridDim.x / 2, half = p.cols / 2;
+  const int tiles = p.tiles, step = gridDim.x / 2, n_stages = p.stages;
   Waiter waiter{&ctl->abort_flag, p.status, global_timer() + static_cast<uint64_t>(p.timeout_ns), kStatusDense, warp};
   const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
 
@@ -133,33 +213,38 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
     int stage = 0;
     uint32_t phase = 0;
     const uint32_t leader_full0 = map_to_cta(full0, 0), base = smem_u32(stages);
-    const int b_blocks = (half + 63) / 64;
-    const uint32_t tx = 2 * (kStageA + (kBmn ? b_blocks * 8192 : half * 128));
     bool ok = true;
     for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
-      const TilePlace at = place_tile(t, p.m_tiles, p.n_tiles);
+      const DensePart& q = part_of<kParts>(p, t);
+      const TilePlace at = place_tile(q, t);
+      const int half = q.cols / 2, k_stages = q.k_stages;
+      const uint32_t tx = q.tx_bytes;
       const int a_row = at.m * 2 * kPairRows + static_cast<int>(cta) * kPairRows;
-      const int b_row = kKind == kGated ? at.n * half + static_cast<int>(cta) * p.epi.inter : at.n * p.cols + static_cast<int>(cta) * half;
-      for (int kb = 0; kb < p.k_stages; ++kb) {
-        if (!waiter.wait_uniform(empty0 + 8 * stage, phase ^ 1u)) { ok = false; break; }
-        const uint32_t bar = leader_full0 + 8 * stage, a = base + stage * p.stage_bytes, b = a + kStageA;
-        if (elect_one()) {
-          if (cta == 0) mbar_expect_tx(full0 + 8 * stage, tx);
-          if (kAmn) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) pair_load_2d(a + j * 8192, &p.map_a, a_row + 64 * j, kb * kDepth, bar);
-          } else {
-            pair_load_2d(a, &p.map_a, kb * kDepth, a_row, bar);
+      const int b_row = kSet == kGated ? at.n * half + static_cast<int>(cta) * q.epi.inter : at.n * q.cols + static_cast<int>(cta) * half;
+      by_order<kInt8, kSet>(q, [&](auto a_order, auto b_order) {
+        constexpr bool a_mn = decltype(a_order)::value, b_mn = decltype(b_order)::value;
+        for (int kb = 0; kb < k_stages; ++kb) {
+          if (!waiter.wait_uniform(empty0 + 8 * stage, phase ^ 1u)) { ok = false; break; }
+          const uint32_t bar = leader_full0 + 8 * stage, a = base + stage * p.stage_bytes, b = a + kStageA;
+          if (elect_one()) {
+            if (cta == 0) mbar_expect_tx(full0 + 8 * stage, tx);
+            if (a_mn) {
+              pair_load_2d(a, &q.map_a, a_row, kb * kDepth, bar);
+              pair_load_2d(a + 8192, &q.map_a, a_row + 64, kb * kDepth, bar);
+            } else {
+              pair_load_2d(a, &q.map_a, kb * kDepth, a_row, bar);
+            }
+            if (b_mn) {
+              pair_load_2d(b, &q.map_b, b_row, kb * kDepth, bar);
+              if (half > 64) pair_load_2d(b + 8192, &q.map_b, b_row + 64, kb * kDepth, bar);
+            } else {
+              pair_load_2d(b, &q.map_b, kb * kDepth, b_row, bar);
+            }
           }
-          if (kBmn) {
-            for (int j = 0; j < b_blocks; ++j) pair_load_2d(b + j * 8192, &p.map_b, b_row + 64 * j, kb * kDepth, bar);
-          } else {
-            pair_load_2d(b, &p.map_b, kb * kDepth, b_row, bar);
-          }
+          __syncwarp();
+          if (++stage == n_stages) { stage = 0; phase ^= 1u; }
         }
-        __syncwarp();
-        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
-      }
+      });
     }
   } else if (warp == 1) {
     // --------------------------------------------------------------------------------------------- issuer
@@ -167,93 +252,69 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
       int stage = 0;
       uint32_t phase = 0, it = 0;
       bool ok = true;
-      const uint64_t a_hi = operand_desc(kAmn, 8192), b_hi = operand_desc(kBmn, 8192);
       const uint32_t lo0 = (smem_u32(stages) & 0x3FFFFu) >> 4, lo_step = p.stage_bytes >> 4;
-      // a K of 32 bytes further: along the 128 bytes, or 16 rows of them
-      constexpr uint32_t kStepA = kAmn ? 2048 >> 4 : 2, kStepB = kBmn ? 2048 >> 4 : 2;
       for (int t = blockIdx.x / 2; ok && t < tiles; t += step, ++it) {
+        const DensePart& q = part_of<kParts>(p, t);
+        const uint32_t idesc = q.idesc;
+        const int k_stages = q.k_stages;
         const uint32_t acc = it & 1u, d = tmem_base + acc * kPairCols;
         if (!waiter.wait_uniform(smem_u32(&ctl->acc_empty[acc]), ((it >> 1) & 1u) ^ 1u)) break;
         tc_fence_after();
-        for (int kb = 0; kb < p.k_stages; ++kb) {
-          if (!waiter.wait_uniform(full0 + 8 * stage, phase)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t a = lo0 + stage * lo_step, b = a + (kStageA >> 4);
-          if (elect_one()) {
+        by_order<kInt8, kSet>(q, [&](auto a_order, auto b_order) {
+          constexpr bool a_mn = decltype(a_order)::value, b_mn = decltype(b_order)::value;
+          const uint64_t a_hi = operand_desc(a_mn, 8192), b_hi = operand_desc(b_mn, 8192);
+          // a K of 32 bytes further: along the 128 bytes, or 16 rows of them
+          constexpr uint32_t kStepA = a_mn ? 2048 >> 4 : 2, kStepB = b_mn ? 2048 >> 4 : 2;
+          for (int kb = 0; kb < k_stages; ++kb) {
+            if (!waiter.wait_uniform(full0 + 8 * stage, phase)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t a = lo0 + stage * lo_step, b = a + (kStageA >> 4);
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              pair_product<kInt8>(d, a_hi | (a + kStepA * k), b_hi | (b + kStepB * k), p.idesc, (kb | k) != 0 ? 1u : 0u);
-            pair_commit(empty0 + 8 * stage);
+              for (int k = 0; k < 4; ++k)
+                pair_product<kInt8>(d, a_hi | (a + kStepA * k), b_hi | (b + kStepB * k), idesc, (kb | k) != 0 ? 1u : 0u);
+              pair_commit(empty0 + 8 * stage);
+            }
+            __syncwarp();
+            if (++stage == n_stages) { stage = 0; phase ^= 1u; }
           }
-          __syncwarp();
-          if (++stage == p.stages) { stage = 0; phase ^= 1u; }
-        }
+        });
         if (ok && elect_one()) pair_commit(smem_u32(&ctl->acc_full[acc]));
         __syncwarp();
       }
     }
   } else {
     // --------------------------------------------------------------------------------------------- epilogue
-    const int q = warp & 3, side = (warp - 2) >> 2;   // TMEM lane quadrant this warp may read
+    const int quadrant = warp & 3;                    // of the TMEM lanes: the one this warp may read
     const uint32_t leader_empty = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
-    uint8_t* block = blocks + (warp - 2) * kEpiBlock;
-    constexpr int kChunk = kKind == kGated ? 16 : 32, kLanes = kChunk / 8, kRowsAtOnce = 32 / kLanes, kTurns = kLanes;
-    const int sub = lane / kLanes, piece = lane % kLanes;
+    EpiPlace e;
+    e.side = (warp - 2) >> 2, e.lane = lane, e.block = blocks + (warp - 2) * kEpiBlock;
     uint32_t it = 0;
     for (int t = blockIdx.x / 2; t < tiles; t += step, ++it) {
-      const TilePlace at = place_tile(t, p.m_tiles, p.n_tiles);
+      const DensePart& q = part_of<kParts>(p, t);
+      const DenseEpilogue epi = q.epi;
+      const TilePlace at = place_tile(q, t);
       const uint32_t acc = it & 1u;
-      const int row0 = at.m * 2 * kPairRows + static_cast<int>(cta) * kPairRows + q * 32, rows = min(32, p.m - row0);
-      const int width = kKind == kGated ? half : p.cols, col0 = at.n * width, last = min(p.n, col0 + width);
-      const float row_scale = kInt8 && lane < rows ? __ldg(p.epi.row_scale + row0 + lane) : 0.f;
+      const int width = kSet == kGated ? q.cols / 2 : q.cols;
+      e.row0 = at.m * 2 * kPairRows + static_cast<int>(cta) * kPairRows + quadrant * 32, e.rows = min(32, q.m - e.row0);
+      e.col0 = at.n * width, e.last = min(q.n, e.col0 + width);
+      e.d = tmem_base + acc * kPairCols + (static_cast<uint32_t>(quadrant * 32) << 16);
+      const float row_scale = kInt8 && lane < e.rows ? __ldg(epi.row_scale + e.row0 + lane) : 0.f;
+      if (kSet == kGatedGrad && q.kind == kGatedGrad && e.side == 0 && lane < e.rows) {
+        // g and u come from HBM, a row's 1 KB each by now
+        const float* keep = epi.preact + (int64_t)(e.row0 + lane) * 2 * epi.inter + e.col0;
+        prefetch_bulk(keep, (e.last - e.col0) * 4);
+        prefetch_bulk(keep + epi.inter, (e.last - e.col0) * 4);
+      }
       if (!waiter.wait_warp(smem_u32(&ctl->acc_full[acc]), (it >> 1) & 1u)) break;
       tc_fence_after();
-      const uint32_t d = tmem_base + acc * kPairCols + (static_cast<uint32_t>(q * 32) << 16);
-      const int chunks = rows > 0 ? (last - col0 + kChunk - 1) / kChunk : 0;
-#pragma unroll 1
-      for (int c = side; c < chunks; c += 2) {
-        const DenseFinish<kKind, kInt8> finish(p.epi, last, col0 + kChunk * c + 8 * piece);
-        float g[kTurns][8], u[kTurns][8];
-        if (kKind == kGatedGrad) {
-#pragma unroll
-          for (int i = 0; i < kTurns; ++i)
-            if (i * kRowsAtOnce + sub < rows) finish.fetch(row0 + i * kRowsAtOnce + sub, g[i], u[i]);
-        }
-        uint32_t v[32];
-        if (kKind == kGated) {
-          tc_ld16(d + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(v));
-          tc_ld16(d + half + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
-        } else {
-          tc_ld32(d + 32 * c, v);
-        }
-        tc_ld_wait();
-        if (kInt8) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(static_cast<float>(static_cast<int32_t>(v[j])));
-        }
-        if (c + 2 >= chunks) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_pair(leader_empty + 8 * acc);
-        }
-        __syncwarp();                             // the previous block has been read
-        block_write(block, lane, v);
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kTurns; ++i) {
-          const int r = i * kRowsAtOnce + sub;
-          float a[8];
-          block_read8(block, r, 2 * piece, a);
-          if (kKind == kGated) block_read8(block, r, 4 + 2 * piece, g[i]);
-          const float rs = kInt8 ? __shfl_sync(0xffffffffu, row_scale, r) : 0.f;
-          if (r < rows) finish.row(row0 + r, rs, a, g[i], u[i]);
-        }
-      }
-      if (side >= chunks) {
+      const auto release = [&] {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_pair(leader_empty + 8 * acc);
-      }
+      };
+      if (kSet == kGatedGrad && q.kind == kLinear) pair_epilogue<kInt8, kLinear>(epi, q.cols, e, row_scale, release);
+      else pair_epilogue<kInt8, kSet>(epi, q.cols, e, row_scale, release);
     }
   }
 
@@ -529,15 +590,18 @@ uint32_t product_idesc(int type, bool a_mn, bool b_mn, int rows, int cols) {
          (static_cast<uint32_t>(cols >> 3) << 17) | (static_cast<uint32_t>(rows >> 4) << 24);
 }
 
+// bytes of B that a stage of a tile holds in each CTA
+int stage_b_bytes(const DenseProduct& p, int cols) { return p.b.k_rows ? (cols / 2 + 63) / 64 * 8192 : cols / 2 * 128; }
+
 template <typename F>
 cudaError_t for_each_pair_kernel(F f) {
-  cudaError_t e = f(dense_pair_kernel<false, false, false, kGated>, kDenseBf16, false, false, kGated);
-  if (e == cudaSuccess) e = f(dense_pair_kernel<false, false, false, kLinear>, kDenseBf16, false, false, kLinear);
-  if (e == cudaSuccess) e = f(dense_pair_kernel<false, false, true, kGatedGrad>, kDenseBf16, false, true, kGatedGrad);
-  if (e == cudaSuccess) e = f(dense_pair_kernel<false, false, true, kLinear>, kDenseBf16, false, true, kLinear);
-  if (e == cudaSuccess) e = f(dense_pair_kernel<false, true, true, kLinear>, kDenseBf16, true, true, kLinear);
-  if (e == cudaSuccess) e = f(dense_pair_kernel<true, false, false, kGated>, kDenseInt8, false, false, kGated);
-  if (e == cudaSuccess) e = f(dense_pair_kernel<true, false, false, kLinear>, kDenseInt8, false, false, kLinear);
+  cudaError_t e = f(dense_pair_kernel<false, kGated, 1>, false, kGated, 1);
+  if (e == cudaSuccess) e = f(dense_pair_kernel<false, kLinear, 1>, false, kLinear, 1);
+  if (e == cudaSuccess) e = f(dense_pair_kernel<false, kLinear, 2>, false, kLinear, 2);
+  if (e == cudaSuccess) e = f(dense_pair_kernel<false, kGatedGrad, 1>, false, kGatedGrad, 1);
+  if (e == cudaSuccess) e = f(dense_pair_kernel<false, kGatedGrad, 2>, false, kGatedGrad, 2);
+  if (e == cudaSuccess) e = f(dense_pair_kernel<true, kGated, 1>, true, kGated, 1);
+  if (e == cudaSuccess) e = f(dense_pair_kernel<true, kLinear, 1>, true, kLinear, 1);
   return e;
 }
 
@@ -585,50 +649,80 @@ cudaError_t launch_few(const DenseProduct& p, cudaStream_t s) {
   return found ? e : cudaErrorInvalidValue;
 }
 
-// Columns of a pair's tile: those whose tiles take the shortest time on the pairs there are.  In clocks: a stage costs 2.1 a column in the
-// tensor cores, or its bytes at 60 a clock into each SM; the epilogue 24 a column, beside the next tile's products or, of the last tile, behind
-// them.  Against 256 columns always: 8-bit projection of 777 tokens, 5120 x 5120, 33.4 -> 23.8 us (160 columns, two turns of 128 tiles
-// where 256 have two of 80), 16-bit block of 1021 tokens 60.5 -> 57.5, 8-bit gated product of 256 tokens 17.2 -> 11.9 (64 columns); 3840
-// tokens the same within 1 %.
-int pair_cols(int m_tiles, int n, int k_stages, bool gated, int pairs) {
-  int64_t least = INT64_MAX;
-  int best = kPairCols;
-  for (int cols = kPairCols; cols >= 64; cols -= 32) {
-    const int width = gated ? cols / 2 : cols;
-    const int64_t tiles = (int64_t)m_tiles * ((n + width - 1) / width), turns = (tiles + pairs - 1) / pairs;
-    const int64_t products = (int64_t)k_stages * std::max((kStageA + 64 * cols) / 60, 21 * cols / 10), epilogue = 24 * cols;
-    const int64_t cost = (turns - 1) * std::max(products, epilogue) + products + epilogue;
-    if (cost < least) least = cost, best = cols;
-  }
-  return best;
+// What a tile of a product costs on a pair, in clocks: a stage 2.1 a column in the tensor cores, or its bytes at 60 a clock into each SM; the
+// epilogue 24 a column, beside the next tile's products or, of the last tile, behind them.
+struct TileCost {
+  int64_t tiles, products, epilogue;
+};
+TileCost tile_cost(const DenseProduct& p, int cols) {
+  const int width = p.kind == kGated ? cols / 2 : cols, depth = p.type == kDenseInt8 ? 128 : 64;
+  const int64_t m_tiles = (p.m + 2 * kPairRows - 1) / (2 * kPairRows);
+  return TileCost{m_tiles * ((p.n + width - 1) / width),
+                  (int64_t)((p.k + depth - 1) / depth) * std::max((kStageA + stage_b_bytes(p, cols)) / 60, 21 * cols / 10), 24 * cols};
 }
 
-cudaError_t launch_pairs(const DenseProduct& p, int sms, cudaStream_t s) {
+// Columns of each product's tiles: those with which the pair that has most to do ends first.  Against 256 columns always: 8-bit projection of 777
+// tokens, 5120 x 5120, 33.4 -> 23.8 us (160 columns, two turns of 128 tiles where 256 have two of 80), 16-bit block of 1021 tokens 60.5 ->
+// 57.5, 8-bit gated product of 256 tokens 17.2 -> 11.9 (64 columns); 3840 tokens the same within 1 %.
+void choose_cols(const DenseProduct* p, int parts, int pairs, int (&best)[kMaxParts]) {
+  constexpr int kChoices = kPairCols / 32 - 1;          // 256, 224 ... 64
+  TileCost cost[kMaxParts][kChoices] = {};
+  for (int i = 0; i < parts; ++i)
+    for (int c = 0; c < kChoices; ++c) cost[i][c] = tile_cost(p[i], kPairCols - 32 * c);
+  int64_t least = INT64_MAX;
+  for (int c0 = 0; c0 < kChoices; ++c0)
+    for (int c1 = 0; c1 < (parts > 1 ? kChoices : 1); ++c1) {
+      const TileCost &x = cost[0][c0], &y = cost[1][c1];
+      // the pairs with most tiles of the first, and those with one less
+      const int64_t all = (x.tiles + y.tiles + pairs - 1) / pairs, most = (x.tiles + pairs - 1) / pairs;
+      int64_t longest = 0;
+      for (int64_t first = x.tiles / pairs; first <= most; ++first) {
+        const int64_t second = std::max<int64_t>(0, all - first);
+        longest = std::max(longest, first * std::max(x.products, x.epilogue) + second * std::max(y.products, y.epilogue) + (second > 0 ? y.epilogue : x.epilogue));
+      }
+      if (longest < least) least = longest, best[0] = kPairCols - 32 * c0, best[1] = kPairCols - 32 * c1;
+    }
+}
+
+cudaError_t launch_pairs(const DenseProduct* p, int parts, int sms, cudaStream_t s) {
   DenseParams d;
-  d.m = p.m, d.n = p.n;
-  const int depth = p.type == kDenseInt8 ? 128 : 64;
-  d.k_stages = (p.k + depth - 1) / depth;
-  d.m_tiles = (p.m + 2 * kPairRows - 1) / (2 * kPairRows);
-  d.cols = pair_cols(d.m_tiles, p.n, d.k_stages, p.kind == kGated, sms / 2);
-  d.stage_bytes = kStageA + (p.b.k_rows ? (d.cols / 2 + 63) / 64 * 8192 : d.cols / 2 * 128);
+  int cols[kMaxParts] = {};
+  choose_cols(p, parts, sms / 2, cols);
+  d.parts = parts;
+  d.status = p->status;
+  d.timeout_ns = (p->timeout_ms > 0 ? (int64_t)p->timeout_ms : 2000) * 1000000ll;
+  int64_t tiles = 0;
+  int set = p->kind;
+  d.stage_bytes = 0;
+  for (int i = 0; i < parts; ++i) {
+    const DenseProduct& f = p[i];
+    DensePart& q = d.part[i];
+    if (f.a.k_rows && !f.b.k_rows) return cudaErrorInvalidValue;       // no caller has that
+    if (i > 0 && (f.kind != kLinear || f.type == kDenseInt8 || f.type != p->type || set == kGated)) return cudaErrorInvalidValue;
+    const int depth = f.type == kDenseInt8 ? 128 : 64, width = f.kind == kGated ? cols[i] / 2 : cols[i];
+    q.epi = f.epi;
+    q.m = f.m, q.n = f.n, q.cols = cols[i], q.kind = f.kind;
+    q.a_mn = f.a.k_rows, q.b_mn = f.b.k_rows;
+    q.k_stages = (f.k + depth - 1) / depth;
+    q.m_tiles = (f.m + 2 * kPairRows - 1) / (2 * kPairRows);
+    q.n_tiles = (f.n + width - 1) / width;
+    q.first_tile = static_cast<int32_t>(tiles);
+    tiles += (int64_t)q.m_tiles * q.n_tiles;
+    if (tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
+    q.idesc = product_idesc(f.type, f.a.k_rows, f.b.k_rows, 2 * kPairRows, cols[i]);
+    const int bytes = kStageA + stage_b_bytes(f, cols[i]);
+    q.tx_bytes = 2 * bytes;
+    d.stage_bytes = std::max(d.stage_bytes, bytes);
+    if (!encode(&q.map_a, f.a, f.type, f.m, f.k, kPairRows) || !encode(&q.map_b, f.b, f.type, f.kind == kGated ? 2 * (uint64_t)f.n : f.n, f.k, cols[i] / 2))
+      return cudaErrorInvalidValue;
+  }
+  d.tiles = static_cast<int32_t>(tiles);
   d.stages = std::min(kPairStageRoom / d.stage_bytes, kMaxStages);
-  const int width = p.kind == kGated ? d.cols / 2 : d.cols;
-  d.n_tiles = (p.n + width - 1) / width;
-  if ((int64_t)d.m_tiles * d.n_tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
-  d.idesc = product_idesc(p.type, p.a.k_rows, p.b.k_rows, 2 * kPairRows, d.cols);
-  d.epi = p.epi;
-  d.status = p.status;
-  d.timeout_ns = (p.timeout_ms > 0 ? (int64_t)p.timeout_ms : 2000) * 1000000ll;
-  if (!encode(&d.map_a, p.a, p.type, p.m, p.k, kPairRows) || !encode(&d.map_b, p.b, p.type, p.kind == kGated ? 2 * (uint64_t)p.n : p.n, p.k, d.cols / 2))
-    return cudaErrorInvalidValue;
-  const int grid = 2 * std::min(sms / 2, d.m_tiles * d.n_tiles);
-  bool found = false;
-  const cudaError_t e = for_each_pair_kernel([&](auto kernel, int type, bool a_mn, bool b_mn, int kind) {
-    if ((type == kDenseInt8) != (p.type == kDenseInt8) || a_mn != p.a.k_rows || b_mn != p.b.k_rows || kind != p.kind) return cudaSuccess;
-    found = true;
+  const int grid = 2 * static_cast<int>(std::min<int64_t>(sms / 2, tiles));
+  return for_each_pair_kernel([&](auto kernel, bool int8, int kind, int most) {
+    if (int8 != (p->type == kDenseInt8) || kind != set || most != parts) return cudaSuccess;
     return launch_clustered(kernel, dim3(grid), dim3(kPairThreads), kPairSmem, 2, s, d);
   });
-  return found ? e : cudaErrorInvalidValue;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -776,7 +870,7 @@ cudaError_t prepare_dense() {
   }
   e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess)
-    e = for_each_pair_kernel([](auto kernel, int, bool, bool, int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem); });
+    e = for_each_pair_kernel([](auto kernel, bool, int, int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem); });
   if (e == cudaSuccess)
     e = for_each_few_kernel([](auto kernel, int, bool, int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem); });
   for (int c = 2; c <= kFewMaxSplit && e == cudaSuccess; ++c) {
@@ -794,15 +888,16 @@ cudaError_t prepare_dense() {
   return e;
 }
 
-cudaError_t launch_dense(const DenseProduct& p, cudaStream_t s) {
-  if (p.m <= 0 || p.n <= 0) return cudaSuccess;
+// Few tokens: up to 256 where the weights are read along their rows (MN-major), else up to 144.  Few -> pairs, 5120 x 2304: 16-bit block, 128
+// tokens 27.0 -> 28.9 us, 160 28.8 -> 29.0, 192 31.0 -> 29.1; 8-bit gated product, 128 11.6 -> 11.8, 160 12.3 -> 12.0; through the second product
+// and to dx, 192 46.5 -> 64.3, 256 57.6 -> 65.0, 128 40 -> 57.
+bool dense_few_tokens(const DenseProduct& p) { return !p.a.k_rows && p.m <= (p.b.k_rows ? 256 : 144); }
+
+cudaError_t launch_dense(const DenseProduct* p, int parts, cudaStream_t s) {
   const int sms = prepared_sms();
   if (sms == 0) return cudaErrorNotReady;
   const ChainScope chain(true);
-  // Few tokens: up to 256 where the weights are read along their rows (MN-major), else up to 144.  Few -> pairs, 5120 x 2304: 16-bit block, 128
-  // tokens 27.0 -> 28.9 us, 160 28.8 -> 29.0, 192 31.0 -> 29.1; 8-bit gated product, 128 11.6 -> 11.8, 160 12.3 -> 12.0; through the second product
-  // and to dx, 192 46.5 -> 64.3, 256 57.6 -> 65.0, 128 40 -> 57.
-  return !p.a.k_rows && p.m <= (p.b.k_rows ? 256 : 144) ? launch_few(p, s) : launch_pairs(p, sms, s);
+  return parts == 1 && dense_few_tokens(*p) ? launch_few(*p, s) : launch_pairs(p, parts, sms, s);
 }
 
 cudaError_t launch_quantize_int8(const void* x, int type, int64_t ld, int8_t* q, float* scales, int m, int k, cudaStream_t s) {

@@ -48,24 +48,43 @@ struct DenseProduct {
 
 cudaError_t prepare_dense();   // once per device, outside stream capture
 
-cudaError_t launch_dense(const DenseProduct& p, cudaStream_t s);
+// One product, or two 16-bit ones that need nothing of each other, at most the first of them kGatedGrad and the others kLinear, in one launch.
+constexpr int kMaxParts = 2;
+cudaError_t launch_dense(const DenseProduct* p, int parts, cudaStream_t s);
+bool dense_few_tokens(const DenseProduct& p);      // it goes by itself
 cudaError_t launch_quantize_int8(const void* x, int type, int64_t ld, int8_t* q, float* scales, int m, int k, cudaStream_t s);
 
 #ifdef __CUDACC__
-__device__ __forceinline__ float clip_above(float v, float c) { return v > c ? c : v; }                    // NaN stays NaN
-__device__ __forceinline__ float clip_both(float v, float c) { return v > c ? c : (v < -c ? -c : v); }
+// NaN stays NaN
+__device__ __forceinline__ float clip_above(float v, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float clip_both(float v, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(clip_above(v, c)), "f"(-c));
+  return r;
+}
+// 1 / (1 + exp(-v)): 0 where the exponential overflows
+__device__ __forceinline__ float sigmoid_of(float v) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return r;
+}
 
 // silu(min(g, c)) * clip(u, -c, c)
 __device__ __forceinline__ float gated_value(float g, float u, float c) {
   const float gc = clip_above(g, c);
-  return __fdividef(gc, 1.f + __expf(-gc)) * clip_both(u, c);
+  return gc * sigmoid_of(gc) * clip_both(u, c);
 }
 
 // Its derivatives, times the gradient dh of its value.  A clipped input has none; one on the border has.
 __device__ __forceinline__ void gated_grad(float dh, float g, float u, float c, float& dg, float& du) {
-  const float gc = clip_above(g, c), s = __fdividef(1.f, 1.f + __expf(-gc));
-  dg = g > c ? 0.f : dh * clip_both(u, c) * (s * (1.f + gc * (1.f - s)));
-  du = fabsf(u) > c ? 0.f : dh * (gc * s);
+  const float gc = clip_above(g, c), s = sigmoid_of(gc), silu = gc * s;
+  dg = g > c ? 0.f : dh * clip_both(u, c) * (s + silu * (1.f - s));
+  du = fabsf(u) > c ? 0.f : dh * silu;
 }
 
 template <typename T> __device__ __forceinline__ T from_float(float v);

@@ -38,8 +38,8 @@ int check_feed_forward(const MmoeFeedForward* f) {
   return MMOE_OK;
 }
 
-int run_dense(const mmoe::DenseProduct& p, const char* what, void* stream) {
-  const cudaError_t e = mmoe::launch_dense(p, static_cast<cudaStream_t>(stream));
+int run_dense(const mmoe::DenseProduct* p, int parts, const char* what, void* stream) {
+  const cudaError_t e = mmoe::launch_dense(p, parts, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MMOE_OK : e == cudaErrorNotReady ? fail(MMOE_ERR_NOT_PREPARED, "%s: mmoe_dense_prepare() has not run on this device", what) : cuda_fail(e, what);
 }
 
@@ -68,7 +68,7 @@ int int8_product(const MmoeInt8Product* a, bool gated, void* stream) {
   p.epi.row_scale = a->x_scales, p.epi.col_scale = a->w_scales;
   p.epi.bias = gated ? nullptr : a->bias;
   p.status = a->status, p.timeout_ms = a->timeout_ms;
-  return run_dense(p, what, stream);
+  return run_dense(&p, 1, what, stream);
 }
 
 }  // namespace
@@ -102,14 +102,14 @@ int mmoe_feed_forward(const MmoeFeedForward* f, void* stream) {
   p.n = f->intermediate, p.k = f->hidden, p.kind = mmoe::kGated;
   p.epi.out = f->h, p.epi.ld_out = f->intermediate, p.epi.out_type = f->type;
   p.epi.inter = f->intermediate, p.epi.clamp = f->clamp, p.epi.preact = f->preact;
-  rc = run_dense(p, "feed-forward, gated product", stream);
+  rc = run_dense(&p, 1, "feed-forward, gated product", stream);
   if (rc != MMOE_OK) return rc;
   p.a = {f->h, f->intermediate, false};
   p.b = {f->w2, f->intermediate, false};
   p.n = f->hidden, p.k = f->intermediate, p.kind = mmoe::kLinear;
   p.epi = {};
   p.epi.out = f->y, p.epi.ld_out = f->hidden, p.epi.out_type = f->type;
-  return run_dense(p, "feed-forward, second product", stream);
+  return run_dense(&p, 1, "feed-forward, second product", stream);
 }
 
 int mmoe_feed_forward_grad(const MmoeFeedForward* f, const void* dy, void* dpre, void* dx, void* dw13, void* dw2, void* stream) {
@@ -127,20 +127,49 @@ int mmoe_feed_forward_grad(const MmoeFeedForward* f, const void* dy, void* dpre,
   for (const void* q : {dy, static_cast<const void*>(dpre), static_cast<const void*>(dx), static_cast<const void*>(dw13), static_cast<const void*>(dw2)})
     if (!aligned16(q)) return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward gradient: pointers must be 16-byte aligned");
   const int h = f->hidden, i = f->intermediate, m = f->num_tokens;
-  mmoe::DenseProduct p = {};
-  p.type = f->type;
-  p.status = f->status, p.timeout_ms = f->timeout_ms;
-  const auto run = [&](mmoe::DenseOperand a, mmoe::DenseOperand b, int rows, int cols, int k, int kind, void* out, int64_t ld, const char* what) {
-    p.a = a, p.b = b, p.m = rows, p.n = cols, p.k = k, p.kind = kind;
-    p.epi = {};
+  const auto product = [&](mmoe::DenseOperand a, mmoe::DenseOperand b, int rows, int cols, int k, void* out, int64_t ld) {
+    mmoe::DenseProduct p = {};
+    p.a = a, p.b = b, p.m = rows, p.n = cols, p.k = k, p.type = f->type, p.kind = mmoe::kLinear;
+    p.status = f->status, p.timeout_ms = f->timeout_ms;
     p.epi.out = out, p.epi.ld_out = ld, p.epi.out_type = f->type;
-    if (kind == mmoe::kGatedGrad) p.epi.inter = i, p.epi.clamp = f->clamp, p.epi.preact = f->preact;
-    return run_dense(p, what, stream);
+    return p;
   };
-  if (inner) rc = run({dy, h, false}, {f->w2, i, true}, m, i, h, mmoe::kGatedGrad, dpre, 2 * (int64_t)i, "feed-forward gradient, through the second product");
-  if (rc == MMOE_OK && dx != nullptr) rc = run({dpre, 2 * (int64_t)i, false}, {f->w13, h, true}, m, h, 2 * i, mmoe::kLinear, dx, h, "feed-forward gradient, dx");
-  if (rc == MMOE_OK && dw13 != nullptr) rc = run({dpre, 2 * (int64_t)i, true}, {f->x, f->x_stride, true}, 2 * i, h, m, mmoe::kLinear, dw13, h, "feed-forward gradient, dw13");
-  if (rc == MMOE_OK && dw2 != nullptr) rc = run({dy, h, true}, {f->h, i, true}, h, i, m, mmoe::kLinear, dw2, i, "feed-forward gradient, dw2");
+  mmoe::DenseProduct through = product({dy, h, false}, {f->w2, i, true}, m, i, h, dpre, 2 * (int64_t)i);
+  through.kind = mmoe::kGatedGrad;
+  through.epi.inter = i, through.epi.clamp = f->clamp, through.epi.preact = f->preact;
+  const mmoe::DenseProduct to_x = product({dpre, 2 * (int64_t)i, false}, {f->w13, h, true}, m, h, 2 * i, dx, h);
+  const mmoe::DenseProduct to_w13 = product({dpre, 2 * (int64_t)i, true}, {f->x, f->x_stride, true}, 2 * i, h, m, dw13, h);
+  const mmoe::DenseProduct to_w2 = product({dy, h, true}, {f->h, i, true}, h, i, m, dw2, i);
+  // Launches of up to two products that need nothing of each other: what leads to g and u with dw2, then dx with dw13.  Few tokens: the
+  // products of few tokens by themselves, then both weights' gradients.
+  const char* what = "feed-forward gradient";
+  mmoe::DenseProduct group[mmoe::kMaxParts];
+  int n = 0;
+  const auto flush = [&] {
+    if (rc == MMOE_OK && n > 0) rc = run_dense(group, n, what, stream);
+    n = 0;
+  };
+  const auto add = [&](const mmoe::DenseProduct& p) {
+    const bool alone = mmoe::dense_few_tokens(p);
+    if (alone) {
+      if (rc == MMOE_OK) rc = run_dense(&p, 1, what, stream);
+      return;
+    }
+    group[n++] = p;
+    if (n == mmoe::kMaxParts) flush();
+  };
+  if (inner) add(through);
+  if (inner && mmoe::dense_few_tokens(through)) {
+    if (dx != nullptr) add(to_x);
+    if (dw13 != nullptr) add(to_w13);
+    if (dw2 != nullptr) add(to_w2);
+  } else {
+    if (dw2 != nullptr) add(to_w2);
+    flush();                                 // dx and dw13 read what the first has written
+    if (dx != nullptr) add(to_x);
+    if (dw13 != nullptr) add(to_w13);
+  }
+  flush();
   return rc;
 }
 
