@@ -177,7 +177,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t cta = cluster_ctarank();
-  chain_release();
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.parts; ++i) {
       prefetch_map(&p.part[i].map_a);
@@ -203,6 +202,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
   cluster_sync_all();                       // the peer's barriers are initialised before anything arrives on them
   tc_fence_after();
   chain_wait();                             // nothing above touches global memory
+  chain_release();                          // in this order: what precedes this launch is complete when the next one starts
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
   const int tiles = p.tiles, step = gridDim.x / 2, n_stages = p.stages;
   Waiter waiter{&ctl->abort_flag, p.status, global_timer() + static_cast<uint64_t>(p.timeout_ns), kStatusDense, warp};
@@ -342,6 +342,8 @@ constexpr int kFewMaxStages = 12;
 constexpr int kFewMaxTokens = 256;                    // per tile
 constexpr int kFewMaxSplit = 8;
 constexpr int kFewSmem = 227 * 1024;
+constexpr int kFewSmemHalf = 113 * 1024;              // up to so many tokens: room for a CTA of the next launch beside each one
+constexpr int kFewHalfTokens = 32;
 
 struct FewParams {
   CUtensorMap map_w, map_t;
@@ -428,7 +430,6 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const int tile = blockIdx.x / p.split, tok0 = blockIdx.y * p.tokens;
-  chain_release();
   const int k0 = static_cast<int>((int64_t)p.k_stages * rank / p.split), k1 = static_cast<int>((int64_t)p.k_stages * (rank + 1) / p.split);
   if (threadIdx.x == 0) {
     prefetch_map(&p.map_w);
@@ -448,11 +449,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  chain_wait();                             // nothing above touches global memory
-  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
-  Waiter waiter{&ctl->abort_flag, p.status, global_timer() + static_cast<uint64_t>(p.timeout_ns), kStatusDense + 1, warp};
   const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]), base = smem_u32(stages);
   const int n_stages = p.stages;
+  chain_wait();                             // nothing above touches global memory
+  chain_release();                          // in this order: what precedes this launch is complete when the next one starts
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+  Waiter waiter{&ctl->abort_flag, p.status, global_timer() + static_cast<uint64_t>(p.timeout_ns), kStatusDense + 1, warp};
 
   if (warp == 0) {
     // --------------------------------------------------------------------------------------------- producer
@@ -618,7 +620,7 @@ cudaError_t for_each_few_kernel(F f) {
 
 std::atomic<int> g_clusters[kMaxDevices][kFewMaxSplit + 1];     // clusters of so many CTAs that run at once
 
-cudaError_t launch_few(const DenseProduct& p, cudaStream_t s) {
+cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   FewParams d;
   d.m = p.m, d.n = p.n;
   const int depth = p.type == kDenseInt8 ? 128 : 64;
@@ -626,13 +628,23 @@ cudaError_t launch_few(const DenseProduct& p, cudaStream_t s) {
   const int parts = (p.m + kFewMaxTokens - 1) / kFewMaxTokens;
   d.tokens = ((p.m + parts - 1) / parts + 15) & ~15;
   const int width = p.kind == kGated ? kFewRows / 2 : kFewRows, tiles = (p.n + width - 1) / width;
-  d.stages = std::min((kFewSmem - 3072) / (kFewRows * 128 + d.tokens * 128), kFewMaxStages);
-  // as many CTAs as run at once, with a few stages for each
+  const bool halves = d.tokens <= kFewHalfTokens;
+  const int smem = halves ? kFewSmemHalf : kFewSmem;
+  d.stages = std::min((smem - 3072) / (kFewRows * 128 + d.tokens * 128), kFewMaxStages);
+  // CTAs that share a tile's K: what a stage costs each of them, or the weights' bytes all, against what meeting costs, in clocks.  Gated 8-bit
+  // product, 5120 x 4608, with 1, 2, 3, 4 of them: one token 10.5, 8.0, 7.5, 7.3 us, 16 tokens 10.6, 8.5, 8.2, 8.8, 64 tokens 11.8, 9.0, 9.8, 16.5;
+  // 4096 x 512 with 2, 4, 8: one token 5.4, 4.2, 3.9, 32 tokens 6.2, 5.3, 5.7.
   int dev = 0;
   cudaGetDevice(&dev);
+  const int64_t from_hbm = (int64_t)p.n * (p.kind == kGated ? 2 : 1) * d.k_stages * 128 / 4450;
+  int64_t least = INT64_MAX;
   d.split = 1;
-  for (int c = 2; c <= kFewMaxSplit; ++c)
-    if (tiles * parts <= g_clusters[dev][c].load() && d.k_stages >= 4 * c) d.split = c;
+  for (int c = 1; c <= kFewMaxSplit; ++c) {
+    const bool at_once = halves ? tiles * parts * c <= sms : tiles * parts <= g_clusters[dev][c].load();
+    if (c > 1 && (!at_once || d.k_stages < 2 * c)) continue;
+    const int64_t cost = std::max(from_hbm, (int64_t)(d.k_stages + c - 1) / c * (300 + d.tokens)) + (int64_t)c * 36 * std::min(p.m, d.tokens);
+    if (cost < least) least = cost, d.split = c;
+  }
   d.idesc = product_idesc(p.type, p.b.k_rows, false, kFewRows, d.tokens);
   d.tmem_cols = d.tokens <= 32 ? 32 : d.tokens <= 64 ? 64 : d.tokens <= 128 ? 128 : 256;
   d.epi = p.epi;
@@ -644,7 +656,7 @@ cudaError_t launch_few(const DenseProduct& p, cudaStream_t s) {
   const cudaError_t e = for_each_few_kernel([&](auto kernel, int type, bool w_mn, int kind) {
     if ((type == kDenseInt8) != (p.type == kDenseInt8) || w_mn != p.b.k_rows || kind != p.kind) return cudaSuccess;
     found = true;
-    return launch_clustered(kernel, dim3(tiles * d.split, parts), dim3(kFewThreads), kFewSmem, d.split, s, d);
+    return launch_clustered(kernel, dim3(tiles * d.split, parts), dim3(kFewThreads), smem, d.split, s, d);
   });
   return found ? e : cudaErrorInvalidValue;
 }
@@ -766,7 +778,8 @@ template <> struct PairOf<__nv_bfloat16> { using type = __nv_bfloat162; };
 template <typename T, bool kVec, int kQuantHeld>
 __global__ void __launch_bounds__(kQuantThreads) quantize_int8_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q,
                                                                       float* __restrict__ scales, int k) {
-  chain_begin();
+  chain_wait();
+  chain_release();
   using P = typename PairOf<T>::type;
   constexpr int kWide = kVec ? 8 : 1;
   struct alignas(sizeof(T) * kWide) Vec { T v[kWide]; };
@@ -897,7 +910,7 @@ cudaError_t launch_dense(const DenseProduct* p, int parts, cudaStream_t s) {
   const int sms = prepared_sms();
   if (sms == 0) return cudaErrorNotReady;
   const ChainScope chain(true);
-  return parts == 1 && dense_few_tokens(*p) ? launch_few(*p, s) : launch_pairs(p, parts, sms, s);
+  return parts == 1 && dense_few_tokens(*p) ? launch_few(*p, sms, s) : launch_pairs(p, parts, sms, s);
 }
 
 cudaError_t launch_quantize_int8(const void* x, int type, int64_t ld, int8_t* q, float* scales, int m, int k, cudaStream_t s) {
