@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import weakref
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -36,7 +37,8 @@ class _Device:
 
 
 _devices: Dict[int, _Device] = {}
-_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
 
 
 def _prepare(index: int) -> _Device:
@@ -75,7 +77,7 @@ def _watch(state: _Device) -> None:
     later call that finds it complete raises what it says."""
     interval = _f._kernel_options.status_poll_interval
     state.due = state.calls + 1
-    if interval <= 0 or torch.cuda.is_current_stream_capturing():
+    if interval <= 0 or _capturing():
         return
     state.poll.before_call(state)
     if not state.poll.pending:
@@ -159,65 +161,83 @@ def _check_block(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> None:
 
 
 def _launch_block(x2: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, clamp: float, keep: bool):
-    """``(y, h, preact or None)`` of rows ``x2``."""
+    """``(y, kept)`` of rows ``x2``: ``kept`` holds h, and behind it (``keep``) g and u for the backward pass, in bytes."""
     tokens, hidden = x2.shape
     inter = w2.shape[1]
     y = x2.new_empty((tokens, hidden))
-    h = x2.new_empty((tokens, inter))
-    preact = x2.new_empty((tokens, 2 * inter), dtype=torch.float32) if keep else None
+    kept = x2.new_empty(tokens * inter * (5 if keep else 1))       # 16-bit elements: 1 for h, 2 x 2 for g and u
     if tokens > 0:
+        h = kept.data_ptr()
         _launch("mmoe_feed_forward", x2.get_device(),
                 _native.MmoeFeedForward(_CODES[x2.dtype], hidden, inter, tokens, clamp, 0, _stride(x2), x2.data_ptr(), w13.data_ptr(),
-                                        w2.data_ptr(), h.data_ptr(), preact.data_ptr() if keep else None, y.data_ptr()))
-    return y, h, preact
+                                        w2.data_ptr(), h, h + 2 * tokens * inter if keep else None, y.data_ptr()))
+    return y, kept
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _launch_block_grad(x2, w13, w2, h, preact, dy2, clamp: float, wanted):
+def _launch_block_grad(x2, w13, w2, kept, dy2, clamp: float, wanted):
     tokens, hidden = x2.shape
     inter = w2.shape[1]
-    dx, dw13, dw2 = (x2.new_empty(t.shape) if w else None for t, w in zip((x2, w13, w2), wanted))
-    dpre = x2.new_empty((tokens, 2 * inter)) if wanted[0] or wanted[1] else None
+    inner = wanted[0] or wanted[1]
+    dx = x2.new_empty((tokens, hidden)) if wanted[0] else None
+    dw13 = w13.new_empty(w13.shape) if wanted[1] else None
+    dw2 = w2.new_empty(w2.shape) if wanted[2] else None
+    dpre = x2.new_empty((tokens, 2 * inter)) if inner else None
+    h = kept.data_ptr()
     _launch("mmoe_feed_forward_grad", x2.get_device(),
             _native.MmoeFeedForward(_CODES[x2.dtype], hidden, inter, tokens, clamp, 0, _stride(x2), x2.data_ptr(), w13.data_ptr(),
-                                    w2.data_ptr(), _ptr(h), _ptr(preact), None),
+                                    w2.data_ptr(), h, h + 2 * tokens * inter if inner else None, None),
             dy2.data_ptr(), _ptr(dpre), _ptr(dx), _ptr(dw13), _ptr(dw2))
     return dx, dw13, dw2
+
+
+# nodes of the calls outside of captures whose graphs are alive
+_eager_graphs = weakref.WeakSet()
 
 
 class _Block(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w13, w2, clamp):
         x2 = _rows(x)
-        need_x, need_13, need_2, _ = ctx.needs_input_grad
-        y, h, preact = _launch_block(x2, w13, w2, clamp, need_x or need_13)
+        need = ctx.needs_input_grad
+        y, kept = _launch_block(x2, w13, w2, clamp, need[0] or need[1])
         ctx.clamp = clamp
         # x is kept beside a copy of its rows, where there had to be one, so that a change of x is noticed
-        ctx.save_for_backward(x, w13, w2, h if need_2 else None, preact, x2 if x2.data_ptr() != x.data_ptr() else None)
+        if x2.data_ptr() == x.data_ptr():
+            ctx.save_for_backward(x, w13, w2, kept)
+        else:
+            ctx.save_for_backward(x, w13, w2, kept, x2)
+        if not _capturing():
+            _eager_graphs.add(ctx)
         return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, w13, w2, h, preact, x2 = ctx.saved_tensors
+        # (the wrapper that refuses second derivatives costs some microseconds, and only a graph of the gradients can have them)
+        return _Block._once(ctx, dy) if torch.is_grad_enabled() else _Block._gradients(ctx, dy)
+
+    @staticmethod
+    def _gradients(ctx, dy):
+        x, w13, w2, kept, *copy = ctx.saved_tensors
         dy2 = dy.reshape(-1, w2.shape[0]).contiguous()
         if dy2.data_ptr() % 16 != 0:
             dy2 = dy2.clone()
-        dx, dw13, dw2 = _launch_block_grad(_rows(x) if x2 is None else x2, w13, w2, h, preact, dy2, ctx.clamp, ctx.needs_input_grad[:3])
+        dx, dw13, dw2 = _launch_block_grad(copy[0] if copy else _rows(x), w13, w2, kept, dy2, ctx.clamp, ctx.needs_input_grad)
         return dx.view(x.shape) if dx is not None and x.dim() != 2 else dx, dw13, dw2, None
 
 
-_EAGER = "mmoe_eager_graph"
+_Block._once = staticmethod(once_differentiable(_Block._gradients))
 
 
 def _refuse_beside_eager_graph(leaves) -> None:
     """The node that accumulates a leaf's gradient belongs to the stream on which the first live graph made it.  A captured backward
     pass would wait for that stream, which is not being captured, and the process would end."""
-    for t in leaves:
-        if t.requires_grad and t.is_leaf and _EAGER in torch.autograd.graph.get_gradient_edge(t).node.metadata:
+    nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in leaves if t.requires_grad and t.is_leaf]
+    for graph in list(_eager_graphs):
+        if any(node is other for other, _ in graph.next_functions for node in nodes):
             raise RuntimeError("a graph of an eager gated_feed_forward call with the same leaves is still alive: drop its output "
                                "before the call is captured for training")
 
@@ -229,14 +249,9 @@ def gated_feed_forward(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, *, 
     if not ((x.requires_grad or w13.requires_grad or w2.requires_grad) and torch.is_grad_enabled()):
         y = _launch_block(_rows(x), w13, w2, clamp, False)[0]
         return y if x.dim() == 2 else y.view(x.shape)
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         _refuse_beside_eager_graph((x, w13, w2))
-        return _Block.apply(x, w13, w2, clamp)
-    y = _Block.apply(x, w13, w2, clamp)
-    for node, _ in y.grad_fn.next_functions:
-        if node is not None:
-            node.metadata[_EAGER] = True
-    return y
+    return _Block.apply(x, w13, w2, clamp)
 
 
 # ---------------------------------------------------------------------------------------------------------------------
