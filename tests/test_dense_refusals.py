@@ -44,6 +44,17 @@ def test_feed_forward_arguments(change):
     _refused(lib.mmoe_feed_forward_grad(ctypes.byref(a), FAKE, FAKE, FAKE, FAKE, FAKE, None))
 
 
+def test_sizes_past_32_bit_indexes():
+    lib = _native().load()
+    for change in (dict(num_tokens=2**30 + 1), dict(hidden=2**29 + 8, x_stride=2**29 + 8), dict(intermediate=2**29 + 8)):
+        a = _block(**change)
+        _refused(lib.mmoe_feed_forward(ctypes.byref(a), None))
+        _refused(lib.mmoe_feed_forward_grad(ctypes.byref(a), FAKE, FAKE, FAKE, FAKE, FAKE, None))
+    for change in (dict(num_tokens=2**31 - 1), dict(channels=2**29 + 1)):
+        _refused(lib.mmoe_int8_projection(ctypes.byref(_product(**change)), None))
+        _refused(lib.mmoe_int8_gated_projection(ctypes.byref(_product(**change)), None))
+
+
 def test_feed_forward_outputs():
     lib = _native().load()
     for change in (dict(h=None), dict(y=None)):

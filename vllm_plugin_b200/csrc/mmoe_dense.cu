@@ -11,13 +11,19 @@ namespace mmoe {
 namespace {
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Products on CTA pairs: a persistent pair takes tiles of 256 rows of A by up to 256 rows of B (tcgen05.mma.cta_group::2, M = 256), of
+// Products on CTA pairs: a persistent pair takes tiles of 256 rows of A by 64 to 256 rows of B (tcgen05.mma.cta_group::2, M = 256), of
 // which each CTA stages 128 rows of A and half of B, 128 bytes of K a stage.  One warp of the leader issues for both SMs; the
 // accumulators of two tiles alternate in tensor memory, so that a tile's epilogue runs beside the next one's products.
 // kGated: the leader stages gate rows and its peer the up rows of the same channels, so the two values of a channel are half a tile of
 // columns apart in one lane.
 // An operand whose rows run along K is staged as such; one that is stored transposed (k_rows) as 64 x 64 blocks with its own rows along the
 // 128 bytes, which the tensor core reads just as well (MN-major descriptors): no transposed copy is made.
+//
+// What bounds it: a tile of 256 x 256 costs each tensor core 512 clk a stage and its SM 32 KB from the L2, at 55-60 bytes a clock, so both ends
+// are near their limit there, and narrower tiles are bound by their copies (choose_cols).  Long calls sit at the power limit instead: 3840 tokens,
+// 5120 x 2304, one launch at a time, at 1.48-1.67 GHz: 16-bit gated product 129 us (1.41 PFLOP/s, g and u written too), second product 64 (1.40),
+// gradients 133 (dh with dw2, 1.37) and 226 (dx with dw13, 1.60; tensor pipe active 96 %); 8-bit gated product 60 (3.0), second 34 (2.6).
+// A launch of one turn has 1.3-1.6 us in front of its first products and 1.2-4 us of epilogue behind its last.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kPairRows = 128;                        // rows of A per CTA
 constexpr int kPairCols = 256;                        // most rows of B per tile
@@ -114,7 +120,9 @@ __device__ __forceinline__ void by_order(const DensePart& q, F f) {
   else f(std::true_type(), std::true_type());
 }
 
-// What an epilogue warp does with its share of a tile: rows q * 32 ... of this CTA's 128, every other block of columns.
+// An epilogue warp's share of a tile: 32 of this CTA's 128 rows, every other block of columns.  A lane has a row of sums in tensor memory; a block
+// of 32 x 32 of them is turned in shared memory, so that rows leave in 64 bytes and more.  Two warps to each quadrant instead of one:
+// 8-bit second product of 3840 tokens 61 -> 35 us.
 struct EpiPlace {
   uint32_t d;                // accumulator, this warp's lanes
   int row0, rows, col0, last;
@@ -335,11 +343,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
 // Products of few tokens, bound by the bytes of B (the weights): 128 of its rows are operand A of the tensor core and the tokens, padded to 16,
 // operand B, so that few tokens cost little.  kGated: 64 gate and 64 up rows.  K is split over the CTAs of a cluster, whose partial sums meet
 // in shared memory, added in the order of the CTAs: no atomics, no workspace, and the same bits in every call.
+// One token, weights from HBM, replayed back to back: 8-bit 5120 x 4608 (23.6 MB) 7.5 us, 2304 x 5120 (11.8 MB) 5.2, 16-bit block (71 MB, two
+// launches) 18.6; 64 tokens 9.0, 7.0 and 22.4.  Of the 7.5: 2.3 until the first stage has come, 3.6 at 6.5 TB/s, 1-2 for the sums and the last CTAs.
+// The second product's weights requested ahead of its wait, beside the first product: 18.1 -> 19.8, so it does not.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 128;                         // rows of B per tile
 constexpr int kFewThreads = 256;
 constexpr int kFewMaxStages = 12;
-constexpr int kFewMaxTokens = 256;                    // per tile
+constexpr int kFewMaxTokens = 256;
 constexpr int kFewMaxSplit = 8;
 constexpr int kFewSmem = 227 * 1024;
 constexpr int kFewSmemHalf = 113 * 1024;              // up to so many tokens: room for a CTA of the next launch beside each one
@@ -348,7 +359,7 @@ constexpr int kFewHalfTokens = 32;
 struct FewParams {
   CUtensorMap map_w, map_t;
   int32_t m, n, k_stages;
-  int32_t tokens;            // per tile, a multiple of 16
+  int32_t tokens;            // m, rounded up to 16
   int32_t split;             // CTAs of a cluster
   int32_t stages;
   uint32_t idesc;
@@ -429,7 +440,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
-  const int tile = blockIdx.x / p.split, tok0 = blockIdx.y * p.tokens;
+  const int tile = blockIdx.x / p.split;
   const int k0 = static_cast<int>((int64_t)p.k_stages * rank / p.split), k1 = static_cast<int>((int64_t)p.k_stages * (rank + 1) / p.split);
   if (threadIdx.x == 0) {
     prefetch_map(&p.map_w);
@@ -475,7 +486,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
         } else {
           tma_load_2d(w, &p.map_w, kb * kDepth, w_row, bar);
         }
-        tma_load_2d(w + kWBytes, &p.map_t, kb * kDepth, tok0, bar);
+        tma_load_2d(w + kWBytes, &p.map_t, kb * kDepth, 0, bar);
       }
       __syncwarp();
       if (++stage == n_stages) { stage = 0; phase ^= 1u; }
@@ -507,10 +518,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
   // A thread finishes the same eight channels of every so many tokens; what belongs to the channels and tokens is fetched ahead.
   constexpr int kGroups = kKind == kGated ? kFewRows / 16 : kFewRows / 8;     // eight channels each
   static_assert(kFewThreads % kGroups == 0, "a thread keeps its channels");
-  const int tokens = min(p.tokens, p.m - tok0), g = static_cast<int>(threadIdx.x) % kGroups;
+  const int tokens = p.m, g = static_cast<int>(threadIdx.x) % kGroups;
   const DenseFinish<kKind, kInt8> finish(p.epi, p.n, tile * 8 * kGroups + 8 * g);
   if (kInt8)
-    for (int t = threadIdx.x; t < tokens; t += kFewThreads) ctl->row_scale[t] = __ldg(p.epi.row_scale + tok0 + t);
+    for (int t = threadIdx.x; t < tokens; t += kFewThreads) ctl->row_scale[t] = __ldg(p.epi.row_scale + t);
   // Everything staged has been multiplied when the accumulator is complete, so the partial sums may take its place: [token][128 rows].
   if (warp >= 2 && warp < 6 && waiter.wait_warp(smem_u32(&ctl->acc_full), 0)) {
     tc_fence_after();
@@ -532,10 +543,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
     const uint32_t at = base + (t * kFewRows + 8 * g) * 4;
     const bool swap = (g & 4) != 0;
     float a[8], b[8], u[8];
-    if (kKind == kGatedGrad) finish.fetch(tok0 + t, b, u);
+    if (kKind == kGatedGrad) finish.fetch(t, b, u);
     add_parts<kInt8>(at, swap, p.split, a);
     if (kKind == kGated) add_parts<kInt8>(at + kFewRows / 2 * 4, swap, p.split, b);
-    finish.row(tok0 + t, kInt8 ? ctl->row_scale[t] : 0.f, a, b, u);
+    finish.row(t, kInt8 ? ctl->row_scale[t] : 0.f, a, b, u);
   }
   __syncwarp();
   cluster_sync_all();                       // the sums are read by all before any CTA ends
@@ -625,8 +636,7 @@ cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   d.m = p.m, d.n = p.n;
   const int depth = p.type == kDenseInt8 ? 128 : 64;
   d.k_stages = (p.k + depth - 1) / depth;
-  const int parts = (p.m + kFewMaxTokens - 1) / kFewMaxTokens;
-  d.tokens = ((p.m + parts - 1) / parts + 15) & ~15;
+  d.tokens = (p.m + 15) & ~15;
   const int width = p.kind == kGated ? kFewRows / 2 : kFewRows, tiles = (p.n + width - 1) / width;
   const bool halves = d.tokens <= kFewHalfTokens;
   const int smem = halves ? kFewSmemHalf : kFewSmem;
@@ -640,9 +650,9 @@ cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   int64_t least = INT64_MAX;
   d.split = 1;
   for (int c = 1; c <= kFewMaxSplit; ++c) {
-    const bool at_once = halves ? tiles * parts * c <= sms : tiles * parts <= g_clusters[dev][c].load();
+    const bool at_once = halves ? (int64_t)tiles * c <= sms : tiles <= g_clusters[dev][c].load();
     if (c > 1 && (!at_once || d.k_stages < 2 * c)) continue;
-    const int64_t cost = std::max(from_hbm, (int64_t)(d.k_stages + c - 1) / c * (300 + d.tokens)) + (int64_t)c * 36 * std::min(p.m, d.tokens);
+    const int64_t cost = std::max(from_hbm, (int64_t)(d.k_stages + c - 1) / c * (300 + d.tokens)) + (int64_t)c * 36 * p.m;
     if (cost < least) least = cost, d.split = c;
   }
   d.idesc = product_idesc(p.type, p.b.k_rows, false, kFewRows, d.tokens);
@@ -656,7 +666,7 @@ cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   const cudaError_t e = for_each_few_kernel([&](auto kernel, int type, bool w_mn, int kind) {
     if ((type == kDenseInt8) != (p.type == kDenseInt8) || w_mn != p.b.k_rows || kind != p.kind) return cudaSuccess;
     found = true;
-    return launch_clustered(kernel, dim3(tiles * d.split, parts), dim3(kFewThreads), smem, d.split, s, d);
+    return launch_clustered(kernel, dim3(tiles * d.split), dim3(kFewThreads), smem, d.split, s, d);
   });
   return found ? e : cudaErrorInvalidValue;
 }
@@ -739,7 +749,8 @@ cudaError_t launch_pairs(const DenseProduct* p, int parts, int sms, cudaStream_t
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Per-token quantiser: s = max|x| / 127, q = x / s rounded to the nearest whole number, ties to even.
-// A block per token; the row stays in registers between the two passes as far as it fits.
+// A block per token; the row stays in registers between the two passes as far as it fits, so a value is read once: 3840 x 2304 (26 MB) 9.5 us,
+// 3840 x 5120 (59 MB) 15.8, bound by the latency of the two passes; up to 64 rows 2.3, the launch.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kQuantThreads = 512;
 
@@ -904,7 +915,7 @@ cudaError_t prepare_dense() {
 // Few tokens: up to 256 where the weights are read along their rows (MN-major), else up to 144.  Few -> pairs, 5120 x 2304: 16-bit block, 128
 // tokens 27.0 -> 28.9 us, 160 28.8 -> 29.0, 192 31.0 -> 29.1; 8-bit gated product, 128 11.6 -> 11.8, 160 12.3 -> 12.0; through the second product
 // and to dx, 192 46.5 -> 64.3, 256 57.6 -> 65.0, 128 40 -> 57.
-bool dense_few_tokens(const DenseProduct& p) { return !p.a.k_rows && p.m <= (p.b.k_rows ? 256 : 144); }
+bool dense_few_tokens(const DenseProduct& p) { return !p.a.k_rows && p.m <= (p.b.k_rows ? kFewMaxTokens : 144); }
 
 cudaError_t launch_dense(const DenseProduct* p, int parts, cudaStream_t s) {
   const int sms = prepared_sms();

@@ -19,15 +19,20 @@ int fail(int code, const char* fmt, ...) {
 
 int cuda_fail(cudaError_t e, const char* what) { return fail(MMOE_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e)); }
 
+// row and column indexes, rounded up to a tile, are 32-bit numbers
+constexpr int32_t kMostTokens = 1 << 30, kMostChannels = 1 << 29;
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int check_feed_forward(const MmoeFeedForward* f) {
   if (f == nullptr) return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: arguments are NULL");
   if (f->type != MMOE_BF16 && f->type != MMOE_FP16) return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: type=%d (supported: BF16, FP16)", f->type);
-  if (f->hidden < 8 || f->hidden % 8 != 0) return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: hidden=%d must be a positive multiple of 8", f->hidden);
-  if (f->intermediate < 8 || f->intermediate % 8 != 0 || f->intermediate > (1 << 29))
-    return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: intermediate=%d must be a positive multiple of 8", f->intermediate);
-  if (f->num_tokens < 0) return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: num_tokens=%d must be >= 0", f->num_tokens);
+  if (f->hidden < 8 || f->hidden % 8 != 0 || f->hidden > kMostChannels)
+    return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: hidden=%d must be a positive multiple of 8, at most %d", f->hidden, kMostChannels);
+  if (f->intermediate < 8 || f->intermediate % 8 != 0 || f->intermediate > kMostChannels)
+    return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: intermediate=%d must be a positive multiple of 8, at most %d", f->intermediate, kMostChannels);
+  if (f->num_tokens < 0 || f->num_tokens > kMostTokens)
+    return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: num_tokens=%d outside [0, %d]", f->num_tokens, kMostTokens);
   if (!(f->clamp > 0.f)) return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: clamp must be positive");
   if (f->x_stride < f->hidden || f->x_stride % 8 != 0)
     return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: x_stride must be a multiple of 8 and at least hidden=%d", f->hidden);
@@ -46,10 +51,10 @@ int run_dense(const mmoe::DenseProduct* p, int parts, const char* what, void* st
 int int8_product(const MmoeInt8Product* a, bool gated, void* stream) {
   const char* what = gated ? "int8 gated projection" : "int8 projection";
   if (a == nullptr) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: arguments are NULL", what);
-  if (a->num_tokens < 0) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: num_tokens=%d must be >= 0", what, a->num_tokens);
+  if (a->num_tokens < 0 || a->num_tokens > kMostTokens) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: num_tokens=%d outside [0, %d]", what, a->num_tokens, kMostTokens);
   // 131072 products of magnitude up to 128 * 128 would reach 2^31; quantised values end at 127
   if (a->width < 16 || a->width % 16 != 0 || a->width >= 131072) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: width=%d must be a multiple of 16 in [16, 131072)", what, a->width);
-  if (a->channels < 1 || a->channels > (1 << 29)) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: channels=%d must be positive", what, a->channels);
+  if (a->channels < 1 || a->channels > kMostChannels) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: channels=%d outside [1, %d]", what, a->channels, kMostChannels);
   if (a->out_type != MMOE_BF16 && a->out_type != MMOE_FP16 && a->out_type != MMOE_FP32) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: out_type=%d", what, a->out_type);
   if (gated && !(a->clamp > 0.f)) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: clamp must be positive", what);
   if (a->x_stride < a->width || a->x_stride % 16 != 0) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: x_stride must be a multiple of 16 and at least width=%d", what, a->width);
