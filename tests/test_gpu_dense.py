@@ -503,6 +503,112 @@ def test_beside_the_layer():
     assert torch.equal(y, eager)
 
 
+@pytest.mark.parametrize("m", [144, 145, 256, 257, 520])
+def test_either_side_of_the_line_between_the_kernels(m):
+    """Few tokens and many take different kernels: 144 and 145 in products that read the weights as they are stored, 256 and 257 in those
+    that read them along their rows.  Values, all gradients and the 8-bit products, and rows that do not depend on how many others there are."""
+    api = _api()
+    x, w13, w2, dy = _block_inputs(m, 392, 200, torch.bfloat16, seed=m, grad=True)
+    y = api.gated_feed_forward(x, w13, w2, activation_clamp=1.5)
+    grads = torch.autograd.grad(y, (x, w13, w2), dy)
+    ref = R.Block(x, w13, w2, 1.5, dy)
+    R.check("y", y.detach(), ref.y, ref.off["y"])
+    for name, got in zip(("dx", "dw13", "dw2"), grads):
+        R.check(name, got, getattr(ref, name), ref.off[name])
+    gen = _gen(m)
+    (q, s), (w, sw) = _int8(gen, m, 336), _int8(gen, 222, 336)
+    out = api.int8_projection(q, s, w, sw, out_dtype=torch.float32)
+    R.check("y8", out, *R.projection(q, s, w, sw, None, torch.float32))
+    assert torch.equal(out[:3], api.int8_projection(q[:3], s[:3], w, sw, out_dtype=torch.float32))     # whole numbers: the same bits
+
+
+@pytest.mark.parametrize("mask", range(1, 8))
+def test_parts_of_the_gradients_of_many_tokens(mask):
+    """Each subset of the gradients by itself, rows of x in a wider tensor: the launches hold one product or two then."""
+    api = _api()
+    _, w13, w2, dy = _block_inputs(300, 136, 104, torch.float16, seed=mask)
+    wide = _randn(_gen(mask), 300, 400, dtype=torch.float16)
+    leaves = [t.detach().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate((wide[:, 64:200], w13, w2))]
+    y = api.gated_feed_forward(*leaves, activation_clamp=1.0)
+    ref = R.Block(*leaves, 1.0, dy)
+    R.check("y", y.detach(), ref.y, ref.off["y"])
+    got = torch.autograd.grad(y, [t for t in leaves if t.requires_grad], dy)
+    names = [n for i, n in enumerate(("dx", "dw13", "dw2")) if mask >> i & 1]
+    for name, g in zip(names, got):
+        R.check(name, g, getattr(ref, name), ref.off[name])
+
+
+def test_a_recorded_timeout_is_raised_once():
+    """What a kernel that gave up leaves in the status words reaches the caller: at the next read, and at a later call without one."""
+    from vllm_plugin_b200.backend import dense as D
+    api = _api()
+    gen = _gen(1)
+    (q, s), (w, sw) = _int8(gen, 4, 64), _int8(gen, 32, 64)
+    want = api.int8_projection(q, s, w, sw)
+    state = D._on_device(0)
+    state.status[:4] = torch.tensor([1, 31, 2, 5], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="kernel 31"):
+        api.read_dense_status()
+    api.read_dense_status()
+    try:
+        api.set_kernel_options(status_poll_interval=1)
+        for _ in range(3):                                     # whatever an earlier interval had queued is over
+            api.int8_projection(q, s, w, sw)
+            torch.cuda.synchronize()
+        state.status[:4] = torch.tensor([1, 32, 0, 7], dtype=torch.int32)
+        with pytest.raises(RuntimeError, match="kernel 32"):
+            for _ in range(3):
+                api.int8_projection(q, s, w, sw)
+                torch.cuda.synchronize()
+    finally:
+        api.set_kernel_options(status_poll_interval=32)
+    assert torch.equal(api.int8_projection(q, s, w, sw), want)
+    api.read_dense_status()
+
+
+def test_backward_twice_and_under_no_grad():
+    api = _api()
+    x, w13, w2, dy = _block_inputs(40, 64, 48, torch.bfloat16, seed=9, grad=True)
+    y = api.gated_feed_forward(x, w13, w2)
+    one = torch.autograd.grad(y, (x, w13, w2), dy, retain_graph=True)
+    two = torch.autograd.grad(y, (x, w13, w2), dy)
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
+    with torch.no_grad():
+        assert not api.gated_feed_forward(x, w13, w2).requires_grad
+    with torch.inference_mode():
+        assert torch.equal(api.gated_feed_forward(x, w13, w2), y)
+
+
+def test_a_first_call_from_another_thread():
+    """Threads that have not used the GPU yet, at once, each on a stream of its own; gradients too."""
+    import threading
+    api = _api()
+    x, w13, w2, dy = _block_inputs(200, 256, 136, torch.bfloat16, seed=12, grad=True)
+    want = [api.gated_feed_forward(x, w13, w2).detach()]
+    want += torch.autograd.grad(api.gated_feed_forward(x, w13, w2), (x, w13, w2), dy)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    y = api.gated_feed_forward(x, w13, w2)
+                    got = [y.detach(), *torch.autograd.grad(y, (x, w13, w2), dy)]
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                        wrong.append("other bits")
+        except Exception as e:  # noqa: BLE001 - reported below, in the test's own thread
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------------------------------------------------

@@ -33,7 +33,8 @@ class _Device:
         self.status = torch.zeros(8, dtype=torch.int32, device=device)
         self.status_ptr = self.status.data_ptr()
         self.poll = _f._StatusPoll(self)
-        self.calls = self.due = 0            # launching calls so far, and the one at which to look at the words
+        self.calls = self.due = 0            # launching calls so far, and the one at which to look at the words ...
+        self.options = None                  # ... by these options
 
 
 _devices: Dict[int, _Device] = {}
@@ -63,19 +64,21 @@ def _launch(name: str, index: int, arguments, *more) -> None:
             return _launch(name, index, arguments, *more)
     state = _on_device(index)
     arguments.status = state.status_ptr
-    arguments.timeout_ms = _f._kernel_options.timeout_ms
+    options = _f._kernel_options
+    arguments.timeout_ms = options.timeout_ms
     state.calls += 1
-    if state.calls >= state.due:
-        _watch(state)
+    if state.calls >= state.due or options is not state.options:
+        _watch(state, options)
     code = getattr(_native.load(), name)(ctypes.byref(arguments), *more, _native.raw_stream(index))
     if code:
         _native.check(code)
 
 
-def _watch(state: _Device) -> None:
+def _watch(state: _Device, options) -> None:
     """Non-blocking look at the status words, as the layer's calls take it: every so many eager calls a copy of the words is queued, and a
     later call that finds it complete raises what it says."""
-    interval = _f._kernel_options.status_poll_interval
+    interval = options.status_poll_interval
+    state.options = options
     state.due = state.calls + 1
     if interval <= 0 or _capturing():
         return
