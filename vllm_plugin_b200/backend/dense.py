@@ -38,6 +38,7 @@ class _Device:
 
 
 _devices: Dict[int, _Device] = {}
+_byref = ctypes.byref
 _current_device = getattr(torch._C, "_cuda_getDevice", None)
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
 
@@ -57,19 +58,30 @@ def _on_device(index: int) -> _Device:
     return _devices.get(index) or _prepare(index)
 
 
-def _launch(name: str, index: int, arguments, *more) -> None:
+def _library():
+    """The C library; what a call looks up is kept from here on."""
+    global _lib, _raw_stream
+    _lib = _native.load()
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+    return _lib
+
+
+_lib = _raw_stream = None
+
+
+def _launch(function, index: int, arguments, *more) -> None:
     """One call of the C library on the current stream of device ``index``: ``arguments`` is its structure but for the status words."""
     if _current_device() != index:
         with torch.cuda.device(index):
-            return _launch(name, index, arguments, *more)
-    state = _on_device(index)
-    arguments.status = state.status_ptr
+            return _launch(function, index, arguments, *more)
+    state = _devices.get(index) or _prepare(index)
     options = _f._kernel_options
+    arguments.status = state.status_ptr
     arguments.timeout_ms = options.timeout_ms
     state.calls += 1
     if state.calls >= state.due or options is not state.options:
         _watch(state, options)
-    code = getattr(_native.load(), name)(ctypes.byref(arguments), *more, _native.raw_stream(index))
+    code = function(_byref(arguments), *more, _raw_stream(index))
     if code:
         _native.check(code)
 
@@ -141,7 +153,7 @@ def _refuse_weight(w: torch.Tensor, what: str, dtype: torch.dtype, device: torch
 
 
 def _check_weight(w: torch.Tensor, what: str, dtype: torch.dtype, x: torch.Tensor) -> None:
-    if w.dtype != dtype or w.dim() != 2 or not w.is_contiguous() or w.data_ptr() % 16 != 0 or w.device != x.device:
+    if w.dtype is not dtype or w.dim() != 2 or not w.is_contiguous() or w.data_ptr() % 16 != 0 or w.get_device() != x.get_device():
         _refuse_weight(w, what, dtype, x.device)
 
 
@@ -171,7 +183,7 @@ def _launch_block(x2: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, clamp: 
     kept = x2.new_empty(tokens * inter * (5 if keep else 1))       # 16-bit elements: 1 for h, 2 x 2 for g and u
     if tokens > 0:
         h = kept.data_ptr()
-        _launch("mmoe_feed_forward", x2.get_device(),
+        _launch((_lib or _library()).mmoe_feed_forward, x2.get_device(),
                 _native.MmoeFeedForward(_CODES[x2.dtype], hidden, inter, tokens, clamp, 0, _stride(x2), x2.data_ptr(), w13.data_ptr(),
                                         w2.data_ptr(), h, h + 2 * tokens * inter if keep else None, y.data_ptr()))
     return y, kept
@@ -190,7 +202,7 @@ def _launch_block_grad(x2, w13, w2, kept, dy2, clamp: float, wanted):
     dw2 = w2.new_empty(w2.shape) if wanted[2] else None
     dpre = x2.new_empty((tokens, 2 * inter)) if inner else None
     h = kept.data_ptr()
-    _launch("mmoe_feed_forward_grad", x2.get_device(),
+    _launch((_lib or _library()).mmoe_feed_forward_grad, x2.get_device(),
             _native.MmoeFeedForward(_CODES[x2.dtype], hidden, inter, tokens, clamp, 0, _stride(x2), x2.data_ptr(), w13.data_ptr(),
                                     w2.data_ptr(), h, h + 2 * tokens * inter if inner else None, None),
             dy2.data_ptr(), _ptr(dpre), _ptr(dx), _ptr(dw13), _ptr(dw2))
@@ -300,25 +312,27 @@ def _quantize(x, code, q, scales, tokens, width) -> None:
     if _current_device() != index:
         with torch.cuda.device(index):
             return _quantize(x, code, q, scales, tokens, width)
-    code = _native.load().mmoe_quantize_int8(x.data_ptr(), code, _stride(x), q.data_ptr(), scales.data_ptr(), tokens, width,
-                                             _native.raw_stream(index))
+    code = (_lib or _library()).mmoe_quantize_int8(x.data_ptr(), code, _stride(x), q.data_ptr(), scales.data_ptr(), tokens, width,
+                                                   _raw_stream(index))
     if code:
         _native.check(code)
 
 
-def _float_vector(t: torch.Tensor, shape, what: str, x: torch.Tensor) -> torch.Tensor:
-    if t.dtype != torch.float32 or (t.shape != shape and t.shape != (*shape, 1)) or t.device != x.device:
-        raise AssertionError(f"{what} must be float32 {tuple(shape)} on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+def _float_vector(t: torch.Tensor, shape, what: str, index: int) -> torch.Tensor:
+    """A float32 tensor of ``shape`` (or with one more dimension of 1), dense; ``t`` itself where it is that."""
+    if t.dtype is not torch.float32 or t.get_device() != index or (t.shape != shape and t.shape != (*shape, 1)):
+        raise AssertionError(f"{what} must be float32 {tuple(shape)} on cuda:{index}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     if t.requires_grad:
         _refuse_gradient("a product of 8-bit integers")
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _int8_product(x, x_scales, w, w_scales, bias, out_dtype, clamp: float, gated: bool) -> torch.Tensor:
-    if not x.is_cuda:
+    index = x.get_device()
+    if index < 0:
         raise RuntimeError("products of 8-bit integers run on the GPU only (there is no CPU path).")
     shape = x.shape
-    if x.dtype != torch.int8 or len(shape) < 1:
+    if x.dtype is not torch.int8 or len(shape) < 1:
         raise AssertionError(f"x must be int8 (..., K), got {tuple(shape)} {x.dtype}")
     _check_weight(w, "w13" if gated else "w", torch.int8, x)
     rows, width = w.shape
@@ -330,18 +344,19 @@ def _int8_product(x, x_scales, w, w_scales, bias, out_dtype, clamp: float, gated
     if code is None:
         raise AssertionError(f"out_dtype must be BF16, FP16 or FP32, got {out_dtype}")
     lead = shape[:-1]
-    x_scales = _float_vector(x_scales, lead, "x_scales", x)
-    w_scales = _float_vector(w_scales, (rows,), "w_scales", x)
+    x_scales = _float_vector(x_scales, lead, "x_scales", index)
+    w_scales = _float_vector(w_scales, (rows,), "w_scales", index)
     if bias is not None:
-        bias = _float_vector(bias, (rows,), "bias", x)
+        bias = _float_vector(bias, (rows,), "bias", index)
     channels = rows // 2 if gated else rows
     out = x.new_empty((*lead, channels), dtype=out_dtype)
     x2 = _rows(x)
     tokens = x2.shape[0]
     if tokens > 0:
-        _launch("mmoe_int8_gated_projection" if gated else "mmoe_int8_projection", x2.get_device(),
+        lib = _lib or _library()
+        _launch(lib.mmoe_int8_gated_projection if gated else lib.mmoe_int8_projection, index,
                 _native.MmoeInt8Product(tokens, width, channels, code, clamp, 0, _stride(x2), x2.data_ptr(), x_scales.data_ptr(), w.data_ptr(),
-                                        w_scales.data_ptr(), _ptr(bias), out.data_ptr()))
+                                        w_scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr()))
     return out
 
 
