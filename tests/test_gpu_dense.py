@@ -57,6 +57,20 @@ def test_quantiser_is_exact(m, k, dtype):
     assert torch.equal(s, want_s) and torch.equal(q, want_q)
 
 
+@pytest.mark.parametrize("m,k", [(511, 264), (512, 8), (513, 264), (1001, 1280), (600, 1288), (520, 5120), (700, 24), (530, 33), (516, 21000)])
+def test_quantiser_of_many_tokens(m, k):
+    """From 512 tokens on fewer threads take a row, down to a warp of a block of eight rows; the last block has rows that are none."""
+    gen = _gen(m + k)
+    x = _randn(gen, m, k, dtype=torch.bfloat16)
+    x[m // 3, 1 % k] = math.inf
+    x[m // 2] = 0
+    room = torch.full((m + 9, k), 55, dtype=torch.int8, device=DEV), torch.full((m + 9,), 55.0, device=DEV)
+    _api().prepare_int8_inputs(x, out=(room[0][:m], room[1][:m]))
+    want_q, want_s = R.quantize(x)
+    assert torch.equal(room[0][:m], want_q) and torch.equal(room[1][:m].nan_to_num(-1), want_s.nan_to_num(-1))
+    assert bool((room[0][m:] == 55).all()) and bool((room[1][m:] == 55).all())
+
+
 def test_quantiser_borders():
     """Values halfway between two whole numbers go to the even one, neighbours of the border to their own side; rows of zeros, of
     the type's smallest and largest numbers, with infinities and NaN."""

@@ -749,10 +749,11 @@ cudaError_t launch_pairs(const DenseProduct* p, int parts, int sms, cudaStream_t
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Per-token quantiser: s = max|x| / 127, q = x / s rounded to the nearest whole number, ties to even.
-// A block per token; the row stays in registers between the two passes as far as it fits, so a value is read once: 3840 x 2304 (26 MB) 9.5 us,
-// 3840 x 5120 (59 MB) 15.8, bound by the latency of the two passes; up to 64 rows 2.3, the launch.
+// A block per token; the row stays in registers between the two passes as far as it fits, so a value is read once: 3840 x 2304 (26 MB) 7.1 us,
+// 3840 x 5120 (59 MB) 12.0, 20000 x 1024 12.9, 4.9 TB/s: the latency of the two passes; up to 64 rows 2.3, the launch.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int kQuantThreads = 512;
+constexpr int kQuantThreads = 512, kQuantManyTokens = 512;
+constexpr int kQuantHeld = 5;               // vectors that a thread keeps.  3840 x 5120 with 3, 5, 8, 12: 15.6, 11.5, 12.0, 14.5 us
 
 // x / s as whole numbers, exactly, in the low bytes.  Adding 1.5 * 2^23 rounds the product with the reciprocal to a whole number q, the nearest
 // one or, next to a border, its neighbour.  The remainder x - q s is exact in one fma (x has at most 11 bits and is above s / 2 in magnitude
@@ -785,16 +786,17 @@ template <typename T> struct PairOf;
 template <> struct PairOf<__half> { using type = __half2; };
 template <> struct PairOf<__nv_bfloat16> { using type = __nv_bfloat162; };
 
-// kVec: eight values at a time, else (widths, strides or places that do not allow it) one.  kQuantHeld: vectors that a thread keeps.
-template <typename T, bool kVec, int kQuantHeld>
+// kVec: eight values at a time, else (widths, strides or places that do not allow it) one.  kWarps: a warp per token, eight of them to a block.
+template <typename T, bool kVec, bool kWarps>
 __global__ void __launch_bounds__(kQuantThreads) quantize_int8_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q,
-                                                                      float* __restrict__ scales, int k) {
+                                                                      float* __restrict__ scales, int m, int k) {
   chain_wait();
   chain_release();
   using P = typename PairOf<T>::type;
   constexpr int kWide = kVec ? 8 : 1;
   struct alignas(sizeof(T) * kWide) Vec { T v[kWide]; };
-  const int64_t row = blockIdx.x;
+  const int64_t row = kWarps ? blockIdx.x * 8 + threadIdx.y : blockIdx.x;
+  if (row >= m) return;                     // a whole warp
   const Vec* in = reinterpret_cast<const Vec*>(x + row * ld);
   const int n = k / kWide, step = blockDim.x;
   Vec held[kQuantHeld];
@@ -820,9 +822,11 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_int8_kernel(const T* _
   __shared__ uint32_t tops[kQuantThreads / 32];
   const float2 both = pair_floats(top);
   uint32_t bits = __reduce_max_sync(0xffffffffu, max(__float_as_uint(both.x), __float_as_uint(both.y)));
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = bits;
-  __syncthreads();
-  for (int w = 0; w < (step >> 5); ++w) bits = max(bits, tops[w]);
+  if (!kWarps) {
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = bits;
+    __syncthreads();
+    for (int w = 0; w < (step >> 5); ++w) bits = max(bits, tops[w]);
+  }
   const bool finite = bits < 0x7f800000u;
   const float s = !finite ? __uint_as_float(0x7fffffffu) : (bits == 0 ? 1.f : __fdiv_rn(__uint_as_float(bits), 127.f));
   if (threadIdx.x == 0) scales[row] = s;
@@ -860,20 +864,16 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_int8_kernel(const T* _
   else finish([&](const float (&f)[kWide], uint32_t (&b)[kWide]) { quantize_some<true>(f, s, inv, b); });
 }
 
-// Many tokens: few threads to each, so that all tokens of an SM are on their way at once; few tokens: many, for a short way.
-constexpr int kQuantManyTokens = 512;
-
 template <typename T>
 cudaError_t launch_quantize(const void* x, int64_t ld, int8_t* q, float* scales, int m, int k, cudaStream_t s) {
   const T* in = static_cast<const T*>(x);
   const bool vec = k % 8 == 0 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0;
-  const bool many = vec && m >= kQuantManyTokens;
-  // as few threads as keep the same number of vectors each
-  const int n = vec ? k / 8 : k, most = many ? std::max(32, std::min(kQuantThreads, (n + 11) / 12)) : kQuantThreads;
+  // Many tokens: as few threads as keep a row, so that many rows are on their way at once; few tokens: many, for a short way.
+  const int n = vec ? k / 8 : k, most = m >= kQuantManyTokens ? std::max(32, std::min(kQuantThreads, (n + kQuantHeld - 1) / kQuantHeld)) : kQuantThreads;
   const int each = (n + most - 1) / most, threads = std::min(kQuantThreads, ((n + each - 1) / each + 31) & ~31);
-  if (many) return launch_chained(quantize_int8_kernel<T, true, 12>, dim3(m), dim3(threads), 0, s, in, ld, q, scales, k);
-  return vec ? launch_chained(quantize_int8_kernel<T, true, 4>, dim3(m), dim3(threads), 0, s, in, ld, q, scales, k)
-             : launch_chained(quantize_int8_kernel<T, false, 12>, dim3(m), dim3(threads), 0, s, in, ld, q, scales, k);
+  if (vec && threads == 32) return launch_chained(quantize_int8_kernel<T, true, true>, dim3((m + 7) / 8), dim3(32, 8), 0, s, in, ld, q, scales, m, k);
+  return vec ? launch_chained(quantize_int8_kernel<T, true, false>, dim3(m), dim3(threads), 0, s, in, ld, q, scales, m, k)
+             : launch_chained(quantize_int8_kernel<T, false, false>, dim3(m), dim3(threads), 0, s, in, ld, q, scales, m, k);
 }
 
 }  // namespace
