@@ -342,9 +342,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
 // ---------------------------------------------------------------------------------------------------------------------
 // Products of few tokens, bound by the bytes of B (the weights): 128 of its rows are operand A of the tensor core and the tokens, padded to 16,
 // operand B, so that few tokens cost little.  kGated: 64 gate and 64 up rows.  K is split over the CTAs of a cluster, whose partial sums meet
-// in shared memory, added in the order of the CTAs: no atomics, no workspace, and the same bits in every call.
-// One token, weights from HBM, replayed back to back: 8-bit 5120 x 4608 (23.6 MB) 7.5 us, 2304 x 5120 (11.8 MB) 5.2, 16-bit block (71 MB, two
-// launches) 18.6; 64 tokens 9.0, 7.0 and 22.4.  Of the 7.5: 2.3 until the first stage has come, 3.6 at 6.5 TB/s, 1-2 for the sums and the last CTAs.
+// in shared memory, added in the order of the CTAs: no atomics, no workspace, and the same bits in every call.  They are sent in one copy to each
+// CTA; read by every thread from the others' shared memory instead, 64 tokens of the block took 22.5 us, stored there value by value 23.7.
+// One token, weights from HBM, replayed back to back: 8-bit 5120 x 4608 (23.6 MB) 7.4 us, 2304 x 5120 (11.8 MB) 5.4, 16-bit block (71 MB, two
+// launches) 18.4; 64 tokens 9.0, 7.0 and 21.3.  Of the 7.4: 2.3 until the first stage has come, 3.6 at 6.5 TB/s, 1-2 for the sums and the last CTAs.
 // The second product's weights requested ahead of its wait, beside the first product: 18.1 -> 19.8, so it does not.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 128;                         // rows of B per tile
@@ -372,12 +373,15 @@ struct FewParams {
 struct FewControl {
   uint64_t full[kFewMaxStages], empty[kFewMaxStages];
   uint64_t acc_full;
+  uint64_t sums_in;             // what the other CTAs of the cluster send
   uint32_t tmem_base;
   volatile int32_t abort_flag;
   float row_scale[kFewMaxTokens];
 };
 static_assert(sizeof(FewControl) <= 2048, "control block");
-static_assert(2 * 1024 + 1024 + kFewMaxTokens * kFewRows * 4 <= kFewSmem, "partial sums of a tile fit where the stages were");
+// sums of m tokens, padded to 16, and what the other CTAs send of those that this one finishes
+constexpr int few_sum_bytes(int m, int split) { return ((m + 15) / 16 * 16 + (split - 1) * ((m + split - 1) / split)) * kFewRows * 4; }
+static_assert(few_sum_bytes(kFewMaxTokens, 1) <= kFewSmem - 3072, "partial sums of a tile fit where the stages were");
 
 template <bool kInt8>
 __device__ __forceinline__ void single_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -389,42 +393,22 @@ __device__ __forceinline__ void single_product(uint32_t d, uint64_t a, uint64_t 
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-__device__ __forceinline__ float4 cluster_load(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
+// shared memory of this CTA to that of another one of the cluster, counted on a barrier there
+__device__ __forceinline__ void cluster_send(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "r"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-// eight neighbouring sums of a token over the CTAs of the cluster; `swap`: second half first, so that eight lanes read all banks
+// adds eight neighbouring sums; `swap`: second half first, so that eight lanes read all banks
 template <bool kInt8>
-__device__ __forceinline__ void add_parts(uint32_t addr, bool swap, int split, float (&v)[8]) {
-  float4 lo[4], hi[4];
-  int32_t whole[8] = {};
+__device__ __forceinline__ void add_part(const uint8_t* at, bool swap, float (&v)[8], int32_t (&whole)[8]) {
+  const float4 p = *reinterpret_cast<const float4*>(at + (swap ? 16 : 0)), q = *reinterpret_cast<const float4*>(at + (swap ? 0 : 16));
+  const float4 lo = swap ? q : p, hi = swap ? p : q;
+  const float part[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = 0.f;
-  for (int r0 = 0; r0 < split; r0 += 4) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (r0 + r >= split) break;
-      const uint32_t from = map_to_cta(addr, r0 + r);
-      lo[r] = cluster_load(from + (swap ? 16 : 0));
-      hi[r] = cluster_load(from + (swap ? 0 : 16));
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (r0 + r >= split) break;
-      const float4 p = swap ? hi[r] : lo[r], q = swap ? lo[r] : hi[r];
-      const float part[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (kInt8) whole[j] += __float_as_int(part[j]);
-        else v[j] += part[j];
-      }
-    }
-  }
-  if (kInt8) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(whole[j]);
+  for (int j = 0; j < 8; ++j) {
+    if (kInt8) whole[j] += __float_as_int(part[j]);
+    else v[j] += part[j];
   }
 }
 
@@ -450,6 +434,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
       mbar_init(smem_u32(&ctl->empty[i]), 1);
     }
     mbar_init(smem_u32(&ctl->acc_full), 1);
+    mbar_init(smem_u32(&ctl->sums_in), 1);
     ctl->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -522,7 +507,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
   const DenseFinish<kKind, kInt8> finish(p.epi, p.n, tile * 8 * kGroups + 8 * g);
   if (kInt8)
     for (int t = threadIdx.x; t < tokens; t += kFewThreads) ctl->row_scale[t] = __ldg(p.epi.row_scale + t);
-  // Everything staged has been multiplied when the accumulator is complete, so the partial sums may take its place: [token][128 rows].
+  // The partial sums take the place of the stages, which this CTA needs no more when its accumulator is complete: [token][128 rows].  Each CTA
+  // of the cluster finishes some of the tokens; the others send it theirs, in one copy each, when no CTA needs its stages any more.
+  constexpr int kRowBytes = kFewRows * 4;
+  const int own = (tokens + p.split - 1) / p.split, first = rank * own, mine = max(0, min(own, tokens - first));
+  const uint32_t came = smem_u32(&ctl->sums_in);
+  uint8_t* sent = stages + p.tokens * kRowBytes;       // [CTA, this one left out][token][128 rows]
+  if (p.split > 1 && threadIdx.x == 0) mbar_expect_tx(came, (p.split - 1) * mine * kRowBytes);
   if (warp >= 2 && warp < 6 && waiter.wait_warp(smem_u32(&ctl->acc_full), 0)) {
     tc_fence_after();
     const int row = (warp & 3) * 32 + lane;
@@ -534,22 +525,43 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
 #pragma unroll
       for (int j = 0; j < 16; ++j) reinterpret_cast<uint32_t*>(stages)[(j0 + j) * kFewRows + row] = v[j];
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   __syncwarp();
   cluster_sync_all();
-#pragma unroll 2
-  for (int i = rank * kFewThreads + static_cast<int>(threadIdx.x); i < tokens * kGroups; i += p.split * kFewThreads) {
-    const int t = i / kGroups;
-    const uint32_t at = base + (t * kFewRows + 8 * g) * 4;
-    const bool swap = (g & 4) != 0;
-    float a[8], b[8], u[8];
-    if (kKind == kGatedGrad) finish.fetch(t, b, u);
-    add_parts<kInt8>(at, swap, p.split, a);
-    if (kKind == kGated) add_parts<kInt8>(at + kFewRows / 2 * 4, swap, p.split, b);
-    finish.row(t, kInt8 ? ctl->row_scale[t] : 0.f, a, b, u);
+  if (p.split > 1) {
+    if (threadIdx.x == 0)
+      for (int r = 0; r < p.split; ++r) {
+        const int theirs = min(own, tokens - r * own);
+        if (r != rank && theirs > 0)
+          cluster_send(map_to_cta(base + (p.tokens + (rank < r ? rank : rank - 1) * own) * kRowBytes, r), base + r * own * kRowBytes, theirs * kRowBytes, map_to_cta(came, r));
+      }
+    __syncwarp();
+    waiter.wait_warp(came, 0);
   }
-  __syncwarp();
-  cluster_sync_all();                       // the sums are read by all before any CTA ends
+#pragma unroll 2
+  for (int i = threadIdx.x; i < mine * kGroups; i += kFewThreads) {
+    const int t = i / kGroups, at = (t * kFewRows + 8 * g) * 4;
+    const bool swap = (g & 4) != 0;
+    float a[8] = {}, b[8] = {}, u[8];
+    int32_t wa[8] = {}, wb[8] = {};
+    if (kKind == kGatedGrad) finish.fetch(first + t, b, u);
+#pragma unroll 4
+    for (int r = 0; r < p.split; ++r) {                // in the order of the CTAs
+      const uint8_t* from = (r == rank ? stages + first * kRowBytes : sent + (r < rank ? r : r - 1) * own * kRowBytes) + at;
+      add_part<kInt8>(from, swap, a, wa);
+      if (kKind == kGated) add_part<kInt8>(from + kRowBytes / 2, swap, b, wb);
+    }
+    if (kInt8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] = static_cast<float>(wa[j]), b[j] = static_cast<float>(wb[j]);
+    }
+    finish.row(first + t, kInt8 ? ctl->row_scale[first + t] : 0.f, a, b, u);
+  }
+  if (p.split > 1) {
+    __syncwarp();
+    cluster_sync_all();                     // all that this CTA has sent has come
+  }
 
   // ---------------------------------------------------------------------------------------------------- teardown
   if (ctl->abort_flag != 0) {
@@ -641,9 +653,9 @@ cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   const bool halves = d.tokens <= kFewHalfTokens;
   const int smem = halves ? kFewSmemHalf : kFewSmem;
   d.stages = std::min((smem - 3072) / (kFewRows * 128 + d.tokens * 128), kFewMaxStages);
-  // CTAs that share a tile's K: what a stage costs each of them, or the weights' bytes all, against what meeting costs, in clocks.  Gated 8-bit
-  // product, 5120 x 4608, with 1, 2, 3, 4 of them: one token 10.5, 8.0, 7.5, 7.3 us, 16 tokens 10.6, 8.5, 8.2, 8.8, 64 tokens 11.8, 9.0, 9.8, 16.5;
-  // 4096 x 512 with 2, 4, 8: one token 5.4, 4.2, 3.9, 32 tokens 6.2, 5.3, 5.7.
+  // CTAs that share a tile's K: what a stage costs each of them, or the weights' bytes all, against what meeting costs, in clocks.  With 1, 2, 3, 4
+  // of them, 8-bit gated product 5120 x 4608: one token 10.2, 7.9, 7.4, 7.2 us, 16 tokens 10.4, 8.1, 7.7, 7.8, 64 tokens 11.4, 8.8, 9.1, - ; second
+  // product 2304 x 5120, 128 tokens: 8.8, 8.2, 8.7; 16-bit block, 144 tokens: 35.3, 27.0, 25.8.
   int dev = 0;
   cudaGetDevice(&dev);
   const int64_t from_hbm = (int64_t)p.n * (p.kind == kGated ? 2 : 1) * d.k_stages * 128 / 4450;
@@ -651,8 +663,8 @@ cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   d.split = 1;
   for (int c = 1; c <= kFewMaxSplit; ++c) {
     const bool at_once = halves ? (int64_t)tiles * c <= sms : tiles <= g_clusters[dev][c].load();
-    if (c > 1 && (!at_once || d.k_stages < 2 * c)) continue;
-    const int64_t cost = std::max(from_hbm, (int64_t)(d.k_stages + c - 1) / c * (300 + d.tokens)) + (int64_t)c * 36 * p.m;
+    if (c > 1 && (!at_once || d.k_stages < 2 * c || few_sum_bytes(p.m, c) > smem - 3072)) continue;
+    const int64_t cost = std::max(from_hbm, (int64_t)(d.k_stages + c - 1) / c * (300 + d.tokens)) + (int64_t)c * 20 * p.m;
     if (cost < least) least = cost, d.split = c;
   }
   d.idesc = product_idesc(p.type, p.b.k_rows, false, kFewRows, d.tokens);
