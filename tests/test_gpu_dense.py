@@ -517,10 +517,10 @@ def test_beside_the_layer():
     assert torch.equal(y, eager)
 
 
-@pytest.mark.parametrize("m", [144, 145, 256, 257, 520])
+@pytest.mark.parametrize("m", [144, 145, 160, 161, 256, 257, 520])
 def test_either_side_of_the_line_between_the_kernels(m):
-    """Few tokens and many take different kernels: 144 and 145 in products that read the weights as they are stored, 256 and 257 in those
-    that read them along their rows.  Values, all gradients and the 8-bit products, and rows that do not depend on how many others there are."""
+    """Few tokens and many take different kernels: up to 160 in products that read the weights as they are stored, up to 256 in those that read
+    them along their rows.  Values, all gradients and the 8-bit products, and rows that do not depend on how many others there are."""
     api = _api()
     x, w13, w2, dy = _block_inputs(m, 392, 200, torch.bfloat16, seed=m, grad=True)
     y = api.gated_feed_forward(x, w13, w2, activation_clamp=1.5)

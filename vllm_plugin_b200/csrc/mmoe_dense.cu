@@ -924,10 +924,10 @@ cudaError_t prepare_dense() {
   return e;
 }
 
-// Few tokens: up to 256 where the weights are read along their rows (MN-major), else up to 144.  Few -> pairs, 5120 x 2304: 16-bit block, 128
-// tokens 27.0 -> 28.9 us, 160 28.8 -> 29.0, 192 31.0 -> 29.1; 8-bit gated product, 128 11.6 -> 11.8, 160 12.3 -> 12.0; through the second product
-// and to dx, 192 46.5 -> 64.3, 256 57.6 -> 65.0, 128 40 -> 57.
-bool dense_few_tokens(const DenseProduct& p) { return !p.a.k_rows && p.m <= (p.b.k_rows ? kFewMaxTokens : 144); }
+// Few tokens: up to 256 where the weights are read along their rows (MN-major), else up to 160.  Few -> pairs, 5120 x 2304: 16-bit block, 128
+// tokens 25.3 -> 28.7 us, 160 27.0 -> 28.7, 176 29.1 -> 28.7, 256 36.0 -> 29.0; 8-bit gated product, 160 11.2 -> 11.7, 176 12.1 -> 11.7; through
+// the second product and to dx, before the sums were sent in one copy, 192 46.5 -> 64.3, 256 57.6 -> 65.0.
+bool dense_few_tokens(const DenseProduct& p) { return !p.a.k_rows && p.m <= (p.b.k_rows ? kFewMaxTokens : 160); }
 
 cudaError_t launch_dense(const DenseProduct* p, int parts, cudaStream_t s) {
   const int sms = prepared_sms();
