@@ -35,7 +35,7 @@ def _refused(code):
 
 @pytest.mark.parametrize("change", [dict(type=2), dict(type=3), dict(type=-1), dict(hidden=0), dict(hidden=60), dict(intermediate=4), dict(intermediate=-8),
                                     dict(num_tokens=-1), dict(clamp=0.0), dict(clamp=-3.0), dict(clamp=math.nan), dict(x_stride=56), dict(x_stride=68),
-                                    dict(x=None), dict(w13=None), dict(w2=None), dict(x=FAKE + 2), dict(w13=FAKE + 8), dict(w2=FAKE + 1),
+                                    dict(x=None), dict(w13=None), dict(w2=None), dict(status=None), dict(x=FAKE + 2), dict(w13=FAKE + 8), dict(w2=FAKE + 1),
                                     dict(h=FAKE + 4), dict(preact=FAKE + 4), dict(y=FAKE + 8)])
 def test_feed_forward_arguments(change):
     lib = _native().load()
@@ -75,7 +75,7 @@ def test_feed_forward_outputs():
 
 @pytest.mark.parametrize("change", [dict(num_tokens=-1), dict(width=0), dict(width=40), dict(width=131072), dict(channels=0), dict(out_type=2), dict(out_type=4),
                                     dict(x_stride=48), dict(x_stride=72), dict(x=None), dict(x_scales=None), dict(w=None), dict(w_scales=None),
-                                    dict(out=None), dict(x=FAKE + 8), dict(w=FAKE + 1), dict(out=FAKE + 4)])
+                                    dict(out=None), dict(status=None), dict(x=FAKE + 8), dict(w=FAKE + 1), dict(out=FAKE + 4)])
 def test_int8_arguments(change):
     lib = _native().load()
     a = _product(**change)

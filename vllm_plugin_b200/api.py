@@ -112,11 +112,11 @@ def gated_feed_forward(x, w13, w2, *, activation_clamp: Optional[float] = None):
     the reference): ``y = h w2^T`` with ``h = silu(min(g, c)) * clip(u, -c, c)``, ``g = x wg^T``, ``u = x wu^T``.
 
     ``x``: BF16 or FP16 ``(..., H)``, any strides (rows that are not dense or do not start on 16 bytes are copied).  ``w13``: ``(2 I, H)``
-    in checkpoint order, the gate's rows first; ``w2``: ``(H, I)``; both contiguous and of x's type; H and I multiples of 8.
+    in checkpoint order, the gate's rows first; ``w2``: ``(H, I)``; both contiguous, on 16 bytes and of x's type; H and I multiples of 8.
     ``activation_clamp``: ``c``, none by default.  Returns ``(..., H)`` of the same type.
 
     Sums are FP32.  ``h`` is rounded to the type, as the second product's operand, and so are the gradients of g and u in the backward
-    pass; g and u themselves are kept for it in FP32.  A value on the border of the clamp passes its gradient, one beyond it does not.
+    pass (in FP16 they overflow past 65504); g and u themselves are kept for it in FP32.  A value on the border of the clamp passes its gradient, one beyond it does not.
     First derivatives only.  A training step can be captured into a CUDA graph behind a first call, but not while the graph of an eager
     call with the same leaves is alive (``RuntimeError``)."""
     global _feed_forward
@@ -137,7 +137,7 @@ def prepare_int8_inputs(hidden_states, out=None):
 
 def int8_projection(x, x_scales, w, w_scales, *, bias=None, out_dtype=None):
     """``(x w^T) * x_scales[..., None] * w_scales + bias`` with exact integer sums: ``x`` int8 ``(..., K)`` with float32 scales ``(...)``, ``w`` int8
-    ``(N, K)`` with ``(N,)``, optional ``bias`` float32 ``(N,)``; K a multiple of 16 below 131072.  ``out_dtype``: BF16 (default), FP16 or
+    ``(N, K)`` with ``(N,)``, optional ``bias`` float32 ``(N,)``; ``w`` contiguous and on 16 bytes, K a multiple of 16 below 131072.  ``out_dtype``: BF16 (default), FP16 or
     FP32.  No gradient."""
     global _int8_projection
     if _int8_projection is None:

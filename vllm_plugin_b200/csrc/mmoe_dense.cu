@@ -115,7 +115,7 @@ __device__ __forceinline__ void block_read8(const uint8_t* block, int row, int p
 // f(whether A, whether B is staged with its rows along the 128 bytes), known to the compiler
 template <bool kInt8, int kSet, typename F>
 __device__ __forceinline__ void by_order(const DensePart& q, F f) {
-  if (kInt8 || kSet == kGated || q.b_mn == 0) f(std::false_type(), std::false_type());
+  if (kInt8 || kSet == kGated || (kSet == kLinear && q.b_mn == 0)) f(std::false_type(), std::false_type());
   else if (q.a_mn == 0) f(std::false_type(), std::true_type());
   else f(std::true_type(), std::true_type());
 }
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
   uint8_t* stages = smem + 2048;
   constexpr int kDepth = kInt8 ? 128 : 64;
   constexpr int kWBytes = kFewRows * 128;
-  const int t_bytes = p.tokens * 128, stage_bytes = kWBytes + t_bytes;
+  const int stage_bytes = kWBytes + p.tokens * 128;
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
@@ -538,6 +538,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
       }
     __syncwarp();
     waiter.wait_warp(came, 0);
+    __syncwarp();
   }
 #pragma unroll 2
   for (int i = threadIdx.x; i < mine * kGroups; i += kFewThreads) {
@@ -719,15 +720,14 @@ void choose_cols(const DenseProduct* p, int parts, int pairs, int (&best)[kMaxPa
 }
 
 cudaError_t launch_pairs(const DenseProduct* p, int parts, int sms, cudaStream_t s) {
-  DenseParams d;
+  DenseParams d = {};
   int cols[kMaxParts] = {};
   choose_cols(p, parts, sms / 2, cols);
   d.parts = parts;
   d.status = p->status;
   d.timeout_ns = (p->timeout_ms > 0 ? (int64_t)p->timeout_ms : 2000) * 1000000ll;
   int64_t tiles = 0;
-  int set = p->kind;
-  d.stage_bytes = 0;
+  const int set = p->kind;
   for (int i = 0; i < parts; ++i) {
     const DenseProduct& f = p[i];
     DensePart& q = d.part[i];

@@ -36,8 +36,8 @@ int check_feed_forward(const MmoeFeedForward* f) {
   if (!(f->clamp > 0.f)) return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: clamp must be positive");
   if (f->x_stride < f->hidden || f->x_stride % 8 != 0)
     return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: x_stride must be a multiple of 8 and at least hidden=%d", f->hidden);
-  if (f->w13 == nullptr || f->w2 == nullptr || (f->num_tokens > 0 && f->x == nullptr))
-    return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: x, w13 and w2 must not be NULL");
+  if (f->w13 == nullptr || f->w2 == nullptr || (f->num_tokens > 0 && (f->x == nullptr || f->status == nullptr)))
+    return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: x, w13, w2 and status must not be NULL");
   if (!aligned16(f->x) || !aligned16(f->w13) || !aligned16(f->w2) || !aligned16(f->h) || !aligned16(f->preact) || !aligned16(f->y))
     return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: pointers must be 16-byte aligned");
   return MMOE_OK;
@@ -59,7 +59,7 @@ int int8_product(const MmoeInt8Product* a, bool gated, void* stream) {
   if (gated && !(a->clamp > 0.f)) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: clamp must be positive", what);
   if (a->x_stride < a->width || a->x_stride % 16 != 0) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: x_stride must be a multiple of 16 and at least width=%d", what, a->width);
   if (a->num_tokens == 0) return MMOE_OK;
-  if (a->x == nullptr || a->x_scales == nullptr || a->w == nullptr || a->w_scales == nullptr || a->out == nullptr)
+  if (a->x == nullptr || a->x_scales == nullptr || a->w == nullptr || a->w_scales == nullptr || a->out == nullptr || a->status == nullptr)
     return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: pointers must not be NULL", what);
   if (!aligned16(a->x) || !aligned16(a->w) || !aligned16(a->out)) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: pointers must be 16-byte aligned", what);
   mmoe::DenseProduct p = {};
