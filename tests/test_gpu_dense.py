@@ -536,6 +536,21 @@ def test_either_side_of_the_line_between_the_kernels(m):
     assert torch.equal(out[:3], api.int8_projection(q[:3], s[:3], w, sw, out_dtype=torch.float32))     # whole numbers: the same bits
 
 
+@pytest.mark.parametrize("m", [1, 40, 150, 200, 256])
+def test_more_tiles_than_sms(m):
+    """Wide weights: few tokens then take half of an SM for each tile, if their sums fit there."""
+    api = _api()
+    gen = _gen(m)
+    (q, s), (w, sw) = _int8(gen, m, 112), _int8(gen, 20003, 112)
+    R.check("y8", api.int8_projection(q, s, w, sw), *R.projection(q, s, w, sw, None, torch.bfloat16))
+    x, w13, w2, dy = _block_inputs(m, 72, 19456, torch.bfloat16, seed=m, grad=True)
+    y = api.gated_feed_forward(x, w13, w2, activation_clamp=1.5)
+    dx, = torch.autograd.grad(y, (x,), dy)
+    ref = R.Block(x, w13, w2, 1.5, dy)
+    R.check("y", y.detach(), ref.y, ref.off["y"])
+    R.check("dx", dx, ref.dx, ref.off["dx"])
+
+
 @pytest.mark.parametrize("mask", range(1, 8))
 def test_parts_of_the_gradients_of_many_tokens(mask):
     """Each subset of the gradients by itself, rows of x in a wider tensor: the launches hold one product or two then."""

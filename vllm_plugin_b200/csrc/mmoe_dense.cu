@@ -354,7 +354,11 @@ constexpr int kFewMaxStages = 12;
 constexpr int kFewMaxTokens = 256;
 constexpr int kFewMaxSplit = 8;
 constexpr int kFewSmem = 227 * 1024;
-constexpr int kFewSmemHalf = 113 * 1024;              // up to so many tokens: room for a CTA of the next launch beside each one
+// Half of an SM for each CTA: up to so many tokens, which need no more, so that the next launch's CTAs find room; and where there are more tiles than
+// SMs, so that one CTA's start and sums run beside another's products: 8-bit projection, 2304 x 20000, one token 14.7 -> 10.2 us, 128
+// tokens 19.7 -> 14.8; 5120 x 25000 27.4 -> 23.1 and 34.1 -> 28.9; 5120 x 152064, 1, 64 and 128 tokens 117 -> 116, 133 -> 137, 168 -> 154.  With 128
+// tiles, 8192 x 16384, 64 tokens 26.2 -> 29.4, so not there.
+constexpr int kFewSmemHalf = 113 * 1024;
 constexpr int kFewHalfTokens = 32;
 
 struct FewParams {
@@ -651,7 +655,7 @@ cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   d.k_stages = (p.k + depth - 1) / depth;
   d.tokens = (p.m + 15) & ~15;
   const int width = p.kind == kGated ? kFewRows / 2 : kFewRows, tiles = (p.n + width - 1) / width;
-  const bool halves = d.tokens <= kFewHalfTokens;
+  const bool halves = d.tokens <= kFewHalfTokens || (tiles > sms && few_sum_bytes(p.m, 1) <= kFewSmemHalf - 3072);
   const int smem = halves ? kFewSmemHalf : kFewSmem;
   d.stages = std::min((smem - 3072) / (kFewRows * 128 + d.tokens * 128), kFewMaxStages);
   // CTAs that share a tile's K: what a stage costs each of them, or the weights' bytes all, against what meeting costs, in clocks.  With 1, 2, 3, 4
