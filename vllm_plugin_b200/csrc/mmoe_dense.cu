@@ -403,6 +403,9 @@ __device__ __forceinline__ void cluster_send(uint32_t dst, uint32_t src, uint32_
                ::"r"(dst), "r"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // adds eight neighbouring sums; `swap`: second half first, so that eight lanes read all banks
 template <bool kInt8>
 __device__ __forceinline__ void add_part(const uint8_t* at, bool swap, float (&v)[8], int32_t (&whole)[8]) {
@@ -543,6 +546,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
     __syncwarp();
     waiter.wait_warp(came, 0);
     __syncwarp();
+    cluster_arrive();                       // what this CTA waited for has come; behind the matching wait, all that it has sent has
   }
 #pragma unroll 2
   for (int i = threadIdx.x; i < mine * kGroups; i += kFewThreads) {
@@ -565,7 +569,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
   }
   if (p.split > 1) {
     __syncwarp();
-    cluster_sync_all();                     // all that this CTA has sent has come
+    cluster_wait();
   }
 
   // ---------------------------------------------------------------------------------------------------- teardown
