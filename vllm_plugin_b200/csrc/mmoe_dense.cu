@@ -354,6 +354,7 @@ constexpr int kFewMaxStages = 12;
 constexpr int kFewMaxTokens = 256;
 constexpr int kFewMaxSplit = 8;
 constexpr int kFewSmem = 227 * 1024;
+constexpr int kFewControl = 2048, kFewApart = kFewControl + 1024;      // beside the stages: control block, and the slack for aligning the base
 // Half of an SM for each CTA: up to so many tokens, which need no more, so that the next launch's CTAs find room; and where there are more tiles than
 // SMs, so that one CTA's start and sums run beside another's products: 8-bit projection, 2304 x 20000, one token 14.7 -> 10.2 us, 128
 // tokens 19.7 -> 14.8; 5120 x 25000 27.4 -> 23.1 and 34.1 -> 28.9; 5120 x 152064, 1, 64 and 128 tokens 117 -> 116, 133 -> 137, 168 -> 154.  With 128
@@ -382,10 +383,10 @@ struct FewControl {
   volatile int32_t abort_flag;
   float row_scale[kFewMaxTokens];
 };
-static_assert(sizeof(FewControl) <= 2048, "control block");
+static_assert(sizeof(FewControl) <= kFewControl, "control block");
 // sums of m tokens, padded to 16, and what the other CTAs send of those that this one finishes
 constexpr int few_sum_bytes(int m, int split) { return ((m + 15) / 16 * 16 + (split - 1) * ((m + split - 1) / split)) * kFewRows * 4; }
-static_assert(few_sum_bytes(kFewMaxTokens, 1) <= kFewSmem - 3072, "partial sums of a tile fit where the stages were");
+static_assert(few_sum_bytes(kFewMaxTokens, 1) <= kFewSmem - kFewApart, "partial sums of a tile fit where the stages were");
 
 template <bool kInt8>
 __device__ __forceinline__ void single_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the same offset in all CTAs
   FewControl* ctl = reinterpret_cast<FewControl*>(smem);
-  uint8_t* stages = smem + 2048;
+  uint8_t* stages = smem + kFewControl;
   constexpr int kDepth = kInt8 ? 128 : 64;
   constexpr int kWBytes = kFewRows * 128;
   const int stage_bytes = kWBytes + p.tokens * 128;
@@ -659,9 +660,9 @@ cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   d.k_stages = (p.k + depth - 1) / depth;
   d.tokens = (p.m + 15) & ~15;
   const int width = p.kind == kGated ? kFewRows / 2 : kFewRows, tiles = (p.n + width - 1) / width;
-  const bool halves = d.tokens <= kFewHalfTokens || (tiles > sms && few_sum_bytes(p.m, 1) <= kFewSmemHalf - 3072);
+  const bool halves = d.tokens <= kFewHalfTokens || (tiles > sms && few_sum_bytes(p.m, 1) <= kFewSmemHalf - kFewApart);
   const int smem = halves ? kFewSmemHalf : kFewSmem;
-  d.stages = std::min((smem - 3072) / (kFewRows * 128 + d.tokens * 128), kFewMaxStages);
+  d.stages = std::min((smem - kFewApart) / (kFewRows * 128 + d.tokens * 128), kFewMaxStages);
   // CTAs that share a tile's K: what a stage costs each of them, or the weights' bytes all, against what meeting costs, in clocks.  With 1, 2, 3, 4
   // of them, 8-bit gated product 5120 x 4608: one token 10.2, 7.9, 7.4, 7.2 us, 16 tokens 10.4, 8.1, 7.7, 7.8, 64 tokens 11.4, 8.8, 9.1, - ; second
   // product 2304 x 5120, 128 tokens: 8.8, 8.2, 8.7; 16-bit block, 144 tokens: 35.3, 27.0, 25.8.
@@ -672,7 +673,7 @@ cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   d.split = 1;
   for (int c = 1; c <= kFewMaxSplit; ++c) {
     const bool at_once = halves ? (int64_t)tiles * c <= sms : tiles <= g_clusters[dev][c].load();
-    if (c > 1 && (!at_once || d.k_stages < 2 * c || few_sum_bytes(p.m, c) > smem - 3072)) continue;
+    if (c > 1 && (!at_once || d.k_stages < 2 * c || few_sum_bytes(p.m, c) > smem - kFewApart)) continue;
     const int64_t cost = std::max(from_hbm, (int64_t)(d.k_stages + c - 1) / c * (300 + d.tokens)) + (int64_t)c * 20 * p.m;
     if (cost < least) least = cost, d.split = c;
   }
