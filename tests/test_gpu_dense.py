@@ -461,6 +461,52 @@ def test_a_training_step_in_a_graph():
         R.check(name, got, getattr(ref, name), ref.off[name])
 
 
+def test_a_module_made_graphed():
+    """A layer around the block through torch.cuda.make_graphed_callables: forward and backward replayed on new inputs."""
+    api = _api()
+
+    class Layer(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            _, w13, w2, _ = _block_inputs(1, 128, 72, torch.bfloat16, seed=5)
+            self.w13, self.w2 = torch.nn.Parameter(w13), torch.nn.Parameter(w2)
+
+        def forward(self, x):
+            return x + api.gated_feed_forward(x, self.w13, self.w2, activation_clamp=1.0)
+
+    layer = Layer()
+    w13, w2 = layer.w13.detach().clone(), layer.w2.detach().clone()
+    sample = torch.randn(2, 30, 128, device=DEV).bfloat16().requires_grad_(True)
+    graphed = torch.cuda.make_graphed_callables(layer, (sample,))
+    for seed in (1, 2):
+        x = _randn(_gen(seed), 2, 30, 128, dtype=torch.bfloat16).requires_grad_(True)
+        dy = _randn(_gen(seed + 9), 2, 30, 128, dtype=torch.bfloat16)
+        layer.zero_grad()
+        graphed(x).backward(dy)
+        ref = R.Block(x.reshape(60, 128), w13, w2, 1.0, dy.reshape(60, 128))
+        R.check("dw13", layer.w13.grad, ref.dw13, ref.off["dw13"])
+        R.check("dw2", layer.w2.grad, ref.dw2, ref.off["dw2"])
+        # the sum with dy is rounded once more
+        want = ref.dx + dy.reshape(60, 128).double()
+        R.check("dx", x.grad.reshape(60, 128), want, ref.off["dx"] + 2.0 ** -8 * want.abs())
+
+
+def test_capture_beside_a_graph_made_on_another_stream():
+    api = _api()
+    x, w13, w2, dy = _block_inputs(50, 128, 64, torch.bfloat16, seed=17, grad=True)
+    want = torch.autograd.grad(api.gated_feed_forward(x, w13, w2), (x, w13, w2), dy)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        alive = api.gated_feed_forward(x, w13, w2)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        api.gated_feed_forward(x, w13, w2).backward(dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(t.grad, g) for t, g in zip((x, w13, w2), want)) and alive.requires_grad
+
+
 def test_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
     api = _api()
     x, w13, w2, dy = _block_inputs(5, 64, 32, torch.bfloat16, seed=3, grad=True)
@@ -482,6 +528,22 @@ def test_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
     del alive
     with torch.cuda.graph(torch.cuda.CUDAGraph()):
         api.gated_feed_forward(x, w13, w2)
+    # weights in 32 bits behind the block's, which are no leaves themselves
+    master = w13.detach().float().requires_grad_(True)
+    alive = api.gated_feed_forward(x.detach(), master.bfloat16(), w2.detach()).sum()
+    graph = torch.cuda.CUDAGraph()
+    refused = False
+    with torch.cuda.graph(graph):
+        weights = master.bfloat16()
+        try:
+            api.gated_feed_forward(x.detach(), weights, w2.detach())
+        except RuntimeError:
+            refused = True
+    assert refused
+    other = w13.detach().float().requires_grad_(True)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        api.gated_feed_forward(x.detach(), other.bfloat16(), w2.detach())        # other leaves
+    alive.backward()
 
 
 def test_beside_the_layer():

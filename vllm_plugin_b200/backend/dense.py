@@ -209,7 +209,7 @@ def _launch_block_grad(x2, w13, w2, kept, dy2, clamp: float, wanted):
     return dx, dw13, dw2
 
 
-# nodes of the calls outside of captures whose graphs are alive
+# nodes of the calls on a default stream whose graphs are alive
 _eager_graphs = weakref.WeakSet()
 
 
@@ -225,7 +225,7 @@ class _Block(torch.autograd.Function):
             ctx.save_for_backward(x, w13, w2, kept)
         else:
             ctx.save_for_backward(x, w13, w2, kept, x2)
-        if not _capturing():
+        if (_raw_stream or _native.raw_stream)(x.get_device()) == 0:
             _eager_graphs.add(ctx)
         return y if x.dim() == 2 else y.view(x.shape)
 
@@ -247,14 +247,31 @@ class _Block(torch.autograd.Function):
 _Block._once = staticmethod(once_differentiable(_Block._gradients))
 
 
-def _refuse_beside_eager_graph(leaves) -> None:
+def _refuse_beside_eager_graph(inputs) -> None:
     """The node that accumulates a leaf's gradient belongs to the stream on which the first live graph made it.  A captured backward
-    pass would wait for that stream, which is not being captured, and the process would end."""
-    nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in leaves if t.requires_grad and t.is_leaf]
-    for graph in list(_eager_graphs):
-        if any(node is other for other, _ in graph.next_functions for node in nodes):
-            raise RuntimeError("a graph of an eager gated_feed_forward call with the same leaves is still alive: drop its output "
-                               "before the call is captured for training")
+    pass lets that stream wait for its own, which takes it into the capture; a default stream cannot be captured, and the process would
+    end.  Graphs made on other streams, as by a warm-up, are no obstacle."""
+    if not _eager_graphs:
+        return
+    mine = _accumulators([torch.autograd.graph.get_gradient_edge(t).node for t in inputs if t.requires_grad])
+    if mine & _accumulators(list(_eager_graphs)):
+        raise RuntimeError("a graph of an eager gated_feed_forward call with the same leaves on the default stream is still alive: "
+                           "drop its output before the call is captured for training")
+
+
+def _accumulators(nodes) -> set:
+    """The nodes behind ``nodes`` that accumulate the gradients of leaves."""
+    seen, found = set(nodes), set()
+    nodes = list(seen)
+    while nodes:
+        node = nodes.pop()
+        if hasattr(node, "variable"):
+            found.add(node)
+        for behind, _ in node.next_functions:
+            if behind is not None and behind not in seen:
+                seen.add(behind)
+                nodes.append(behind)
+    return found
 
 
 def gated_feed_forward(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, *, activation_clamp: Optional[float] = None) -> torch.Tensor:
