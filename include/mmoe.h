@@ -311,7 +311,7 @@ typedef struct MmoeFeedForward {
 int mmoe_feed_forward(const MmoeFeedForward* ff, void* stream);
 /* Gradients, from the h and preact that mmoe_feed_forward left and dy [M, H] (contiguous).  dpre [M, 2I]: scratch, the gradients of the
  * two products rounded to the type; needed where dx or dw13 are asked for.  dx [M, H], dw13 [2I, H], dw2 [H, I]: NULL where not
- * wanted (ff->preact may be NULL where only dw2 is, ff->h where it is not). */
+ * wanted (ff->preact may be NULL where only dw2 is, ff->h where it is not).  No tokens: dw13 and dw2 are set to zero. */
 int mmoe_feed_forward_grad(const MmoeFeedForward* ff, const void* dy, void* dpre, void* dx, void* dw13, void* dw2, void* stream);
 
 /* Per-token quantiser: scale = max|x| / 127 (1 for a row of zeros), q = x / scale to the nearest whole number, ties to even, by that scale

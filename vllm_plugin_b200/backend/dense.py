@@ -237,7 +237,7 @@ class _Block(torch.autograd.Function):
     @staticmethod
     def _gradients(ctx, dy):
         x, w13, w2, kept, *copy = ctx.saved_tensors
-        dy2 = dy.reshape(-1, w2.shape[0]).contiguous()
+        dy2 = dy if dy.dim() == 2 and dy.is_contiguous() else dy.reshape(-1, w2.shape[0]).contiguous()
         if dy2.data_ptr() % 16 != 0:
             dy2 = dy2.clone()
         dx, dw13, dw2 = _launch_block_grad(copy[0] if copy else _rows(x), w13, w2, kept, dy2, ctx.clamp, ctx.needs_input_grad)
