@@ -1,0 +1,62 @@
+"""Host side of the dense feed-forward operators on the CPU, launches and CUDA's own objects stubbed."""
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def stubbed(monkeypatch):
+    """Events that are always complete, and host memory that needs no pinning."""
+    class Event:
+        def record(self, *args):
+            pass
+
+        def query(self):
+            return True
+
+        def synchronize(self):
+            pass
+
+    monkeypatch.setattr(torch.cuda, "Event", Event)
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t, *a: t)
+
+
+@pytest.mark.parametrize("make_in_inference", [True, False])
+def test_status_words_work_in_any_mode(stubbed, make_in_inference):
+    """Whatever mode the first call ran in: polls, reports and the words' reset work outside inference mode and inside."""
+    from vllm_plugin_b200.backend import dense as D
+    with torch.inference_mode(make_in_inference):
+        state = D._Device(torch.device("cpu"))
+    assert not state.status.is_inference() and not state.poll.host.is_inference()
+    for inference in (False, True, False):
+        with torch.inference_mode(inference):
+            state.poll.before_call(state)
+            state.poll.after_call(state, 1)
+            state.poll.before_call(state)
+            state.status[:4] = torch.tensor([1, 31, 2, 5], dtype=torch.int32)
+            state.poll.after_call(state, 1)
+            with pytest.raises(RuntimeError, match="kernel 31"):
+                state.poll.before_call(state)
+            assert not state.status.any()
+
+
+def test_a_buffer_made_in_inference_mode_can_be_reset_outside(stubbed, monkeypatch):
+    """The layer's own words, which its poll resets as well."""
+    import types
+    from vllm_plugin_b200.backend import frontend as F, workspace as W
+    empty = torch.empty
+
+    def aligned(size, **kind):                       # on 1024 bytes, as CUDA's memory is
+        room = empty(size + 1024, **kind)
+        return room[-room.data_ptr() % 1024:][:size]
+
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    monkeypatch.setattr(torch, "empty", lambda size, **kind: aligned(size, **kind) if isinstance(size, int) else empty(size, **kind))
+    with torch.inference_mode():
+        buffer = W.SymmBuffer(types.SimpleNamespace(size=lambda: 1, rank=lambda: 0), 8, 64, 2, 512, 256, device=torch.device("cpu"))
+        poll = F._StatusPoll(buffer)
+    buffer.status[0] = 1
+    poll.after_call(buffer, 1)
+    with pytest.raises(RuntimeError, match="expired"):
+        poll.before_call(buffer)
+    assert not buffer.status.any()

@@ -30,7 +30,8 @@ _FF_TYPES = (torch.bfloat16, torch.float16)
 # ---------------------------------------------------------------------------------------------------------------------
 class _Device:
     def __init__(self, device: torch.device):
-        self.status = torch.zeros(8, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):    # kept for calls in any mode, whatever the first one runs in
+            self.status = torch.zeros(8, dtype=torch.int32, device=device)
         self.status_ptr = self.status.data_ptr()
         self.poll = _f._StatusPoll(self)
         self.calls = self.due = 0            # launching calls so far, and the one at which to look at the words ...

@@ -275,7 +275,8 @@ class _StatusPoll:
     to pinned host memory behind the call; a later call that finds the copy complete inspects it."""
 
     def __init__(self, sym_buffer):
-        self.host = torch.zeros(8, dtype=torch.int32).pin_memory()
+        with torch.inference_mode(False):              # kept for calls in any mode, whatever this one runs in
+            self.host = torch.zeros(8, dtype=torch.int32).pin_memory()
         self.event = torch.cuda.Event()
         self.pending = False
         self.calls = 0

@@ -72,19 +72,20 @@ class SymmBuffer:
         self.device = device
         self.peer_ptrs = None          # EP > 1: every rank's buffer mapped into this process (symmetric allocation)
         self.handle = None
-        if group.size() > 1 and device.type == "cuda":
-            self._allocate_symmetric(group, device)
-        if getattr(self, "buffer", None) is None:
-            self.buffer = torch.empty(self.layout.total_bytes, dtype=torch.int8, device=device)
-        assert self.buffer.data_ptr() % 1024 == 0
-        self.buffer.zero_()
-        torch.cuda.synchronize(device)
-        if group.size() > 1:
-            work = group.barrier()
-            if hasattr(work, "wait"):
-                work.wait()
-        torch.cuda.synchronize(device)
-        self._build_views()
+        with torch.inference_mode(False):      # its words are reset by calls in any mode, whatever this one runs in
+            if group.size() > 1 and device.type == "cuda":
+                self._allocate_symmetric(group, device)
+            if getattr(self, "buffer", None) is None:
+                self.buffer = torch.empty(self.layout.total_bytes, dtype=torch.int8, device=device)
+            assert self.buffer.data_ptr() % 1024 == 0
+            self.buffer.zero_()
+            torch.cuda.synchronize(device)
+            if group.size() > 1:
+                work = group.barrier()
+                if hasattr(work, "wait"):
+                    work.wait()
+            torch.cuda.synchronize(device)
+            self._build_views()
 
     def _allocate_symmetric(self, group, device) -> None:
         """Symmetric allocation + rendezvous; the outcome is agreed on by the whole group, so that no rank runs the peer
