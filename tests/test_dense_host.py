@@ -60,3 +60,37 @@ def test_a_buffer_made_in_inference_mode_can_be_reset_outside(stubbed, monkeypat
     with pytest.raises(RuntimeError, match="expired"):
         poll.before_call(buffer)
     assert not buffer.status.any()
+
+
+def test_a_read_forgets_the_copy_that_was_queued(stubbed, monkeypatch):
+    """A failure that a read has reported and cleared is not raised once more by a copy of the words queued in front of the read."""
+    import contextlib
+    import types
+    from vllm_plugin_b200.backend import _native, dense as D, frontend as F
+    state = D._Device(torch.device("cpu"))
+    raised = []
+
+    def read(*args):                                 # the C call: the words as they are, then cleared
+        raised.append(int(state.status[0]))
+        state.status.zero_()
+        return 0
+
+    monkeypatch.setattr(F, "require_sm100", lambda: None)
+    monkeypatch.setattr(_native, "load", lambda: types.SimpleNamespace(mmoe_dense_read_status=read, mmoe_read_status=read))
+    monkeypatch.setattr(_native, "raw_stream", lambda index: 0)
+    monkeypatch.setattr(torch.cuda, "device", lambda index: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=0))
+    monkeypatch.setitem(D._devices, 0, state)
+    buffer = types.SimpleNamespace(device=None, geo=_native.MmoeGeometry(), base_ptr=0, status=state.status, _status_poll=state.poll)
+    for reader in (lambda: D.read_dense_status("cuda:0"), lambda: F.read_status(buffer)):
+        state.status[:4] = torch.tensor([1, 31, 2, 5], dtype=torch.int32)
+        state.poll.after_call(state, 1)
+        assert state.poll.pending
+        reader()
+        assert raised.pop() == 1 and not state.status.any()
+        state.status[0] = 1                          # what a newer call leaves stays for the next look
+        state.poll.before_call(state)
+        assert state.status[0] == 1
+        state.status.zero_()
+    buffer._status_poll = None                       # no call has looked yet
+    F.read_status(buffer)

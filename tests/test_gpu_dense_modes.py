@@ -41,3 +41,28 @@ with torch.inference_mode():
 api.read_dense_status()
 print("ok")
 """)
+
+
+def test_a_timeout_read_beside_a_queued_copy_is_raised_once():
+    from vllm_plugin_b200 import api
+    from vllm_plugin_b200.backend import dense as D
+    x, w13, w2 = (torch.randn(s, device="cuda:0").bfloat16() for s in ((5, 64), (64, 64), (64, 32)))
+    want = api.gated_feed_forward(x, w13, w2)
+    state = D._on_device(0)
+    try:
+        api.set_kernel_options(status_poll_interval=1)
+        for _ in range(3):
+            api.gated_feed_forward(x, w13, w2)
+            torch.cuda.synchronize()
+        state.status[:4] = torch.tensor([1, 31, 2, 5], dtype=torch.int32)
+        torch.cuda.synchronize()
+        state.poll.pending = False
+        state.poll.after_call(state, 1)                          # the look that a call takes: queued, not yet inspected
+        with pytest.raises(RuntimeError, match="kernel 31"):
+            api.read_dense_status()
+        for _ in range(3):
+            assert torch.equal(api.gated_feed_forward(x, w13, w2), want)
+            torch.cuda.synchronize()
+    finally:
+        api.set_kernel_options(status_poll_interval=32)
+    api.read_dense_status()

@@ -113,7 +113,9 @@ def read_dense_status(device=None) -> None:
     with torch.cuda.device(index):
         state = _on_device(index)
         words = (ctypes.c_int32 * 8)()
-        _native.check(_native.load().mmoe_dense_read_status(state.status_ptr, words, _native.raw_stream(index)))
+        code = _native.load().mmoe_dense_read_status(state.status_ptr, words, _native.raw_stream(index))
+        state.poll.forget()
+        _native.check(code)
 
 
 # ---------------------------------------------------------------------------------------------------------------------

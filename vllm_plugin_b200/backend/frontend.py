@@ -299,6 +299,12 @@ class _StatusPoll:
             self.event.record()
             self.pending = True
 
+    def forget(self) -> None:
+        """Drop the queued copy: its words have been read and cleared."""
+        if self.pending:
+            self.event.synchronize()                           # the next copy may be on another stream
+            self.pending = False
+
 
 def _validate(y, l1_weights, l2_weights, sym_buffer, shared_l1_weights, shared_l2_weights, stats, recipe, activation,
               activation_clamp, fast_math, activation_alpha, activation_beta, tensors) -> _CallRecord:
@@ -418,4 +424,7 @@ def read_status(sym_buffer) -> None:
     ``KernelOptions.status_poll_interval``."""
     words = (ctypes.c_int32 * 8)()
     stream = torch.cuda.current_stream(sym_buffer.device).cuda_stream
-    _native.check(_native.load().mmoe_read_status(ctypes.byref(sym_buffer.geo), sym_buffer.base_ptr, words, stream))
+    code = _native.load().mmoe_read_status(ctypes.byref(sym_buffer.geo), sym_buffer.base_ptr, words, stream)
+    if sym_buffer._status_poll is not None:
+        sym_buffer._status_poll.forget()
+    _native.check(code)
