@@ -94,3 +94,13 @@ def test_a_read_forgets_the_copy_that_was_queued(stubbed, monkeypatch):
         state.status.zero_()
     buffer._status_poll = None                       # no call has looked yet
     F.read_status(buffer)
+
+
+def test_a_timeout_names_the_kind_of_call(stubbed):
+    from vllm_plugin_b200.backend import dense as D, frontend as F
+    state = D._Device(torch.device("cpu"))
+    for poll, name in ((state.poll, "dense operator's call"), (F._StatusPoll(state), "MegaMoE call")):
+        state.status[0] = 1
+        poll.after_call(state, 1)
+        with pytest.raises(RuntimeError, match=f"wait of an earlier {name} expired"):
+            poll.before_call(state)

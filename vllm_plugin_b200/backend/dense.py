@@ -33,7 +33,7 @@ class _Device:
         with torch.inference_mode(False):    # kept for calls in any mode, whatever the first one runs in
             self.status = torch.zeros(8, dtype=torch.int32, device=device)
         self.status_ptr = self.status.data_ptr()
-        self.poll = _f._StatusPoll(self)
+        self.poll = _f._StatusPoll(self, "dense operator's call")
         self.calls = self.due = 0            # launching calls so far, and the one at which to look at the words ...
         self.options = None                  # ... by these options
 

@@ -272,9 +272,11 @@ def _keep_record(records: Dict[Tuple[int, int], _CallRecord], key: Tuple[int, in
 
 class _StatusPoll:
     """Non-blocking watch on the device status words of one buffer: every ``interval`` eager calls the words are copied
-    to pinned host memory behind the call; a later call that finds the copy complete inspects it."""
+    to pinned host memory behind the call; a later call that finds the copy complete inspects it.  ``what`` names the calls
+    in its message."""
 
-    def __init__(self, sym_buffer):
+    def __init__(self, sym_buffer, what: str = "MegaMoE call"):
+        self.what = what
         with torch.inference_mode(False):              # kept for calls in any mode, whatever this one runs in
             self.host = torch.zeros(8, dtype=torch.int32).pin_memory()
         self.event = torch.cuda.Event()
@@ -288,7 +290,7 @@ class _StatusPoll:
             if words[0] != 0 or words[4] != 0:
                 sym_buffer.status.zero_()                      # re-arm: the next healthy call reports healthy
                 if words[0] != 0:
-                    raise RuntimeError(f"a device-side wait of an earlier MegaMoE call expired (kernel {words[1]}, role "
+                    raise RuntimeError(f"a device-side wait of an earlier {self.what} expired (kernel {words[1]}, role "
                                        f"{words[2]}, block {words[3]}): its output is not valid")
                 raise AssertionError(f"{words[4]} expert ids of an earlier MegaMoE call were >= num_experts")
 
