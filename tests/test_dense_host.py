@@ -104,3 +104,54 @@ def test_a_timeout_names_the_kind_of_call(stubbed):
         poll.after_call(state, 1)
         with pytest.raises(RuntimeError, match=f"wait of an earlier {name} expired"):
             poll.before_call(state)
+
+
+@pytest.fixture
+def launches(stubbed, monkeypatch):
+    """The operators on CPU tensors; the C library writes nothing.  The list of what was called."""
+    import types
+    from vllm_plugin_b200.backend import dense as D
+    calls = []
+    lib = types.SimpleNamespace(**{n: (lambda *a, n=n: calls.append(n) or 0) for n in (
+        "mmoe_feed_forward", "mmoe_feed_forward_grad", "mmoe_quantize_int8", "mmoe_int8_projection")})
+    monkeypatch.setattr(D, "_lib", lib)
+    monkeypatch.setattr(D, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(D, "_current_device", lambda: -1)
+    monkeypatch.setattr(D, "_capturing", lambda: False)
+    monkeypatch.setattr(D, "_check_block", lambda *a: None)
+    monkeypatch.setitem(D._devices, -1, D._Device(torch.device("cpu")))
+    return calls
+
+
+def _block():
+    return torch.randn(5, 64).bfloat16(), torch.randn(64, 64).bfloat16(), torch.randn(64, 32).bfloat16()
+
+
+def test_tangents_are_refused(launches):
+    """Forward-mode derivatives through any input, and through the gradient of the output, with and without a backward graph."""
+    import torch.autograd.forward_ad as fwd
+    from vllm_plugin_b200.backend import dense as D
+    args = _block()
+    with fwd.dual_level():
+        for grad in (False, True):
+            for i in range(3):
+                inputs = [t.detach().requires_grad_(grad) for t in args]
+                inputs[i] = fwd.make_dual(inputs[i], torch.ones_like(inputs[i]))
+                for run in (D.gated_feed_forward, torch.no_grad()(D.gated_feed_forward)):
+                    with pytest.raises((NotImplementedError, RuntimeError), match="forward"):
+                        run(*inputs)
+        assert not launches
+        scale = fwd.make_dual(torch.ones(5), torch.ones(5))
+        with pytest.raises(NotImplementedError, match="forward"):
+            D._float_vector(scale, (5,), "x_scales", -1)
+        D.gated_feed_forward(*args)                          # a level by itself is no obstacle
+        D._float_vector(torch.ones(5), (5,), "x_scales", -1)
+        assert launches == ["mmoe_feed_forward"]
+        inputs = [t.detach().requires_grad_(True) for t in args]
+        y = D.gated_feed_forward(*inputs)
+        torch.autograd.grad(y, inputs, torch.ones_like(y), retain_graph=True)
+        with pytest.raises(NotImplementedError, match="forward"):
+            torch.autograd.grad(y, inputs, fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        with fwd._set_fwd_grad_enabled(False):               # as inference mode has it: nobody asks for tangents
+            D.gated_feed_forward(fwd.make_dual(args[0], args[0]), *args[1:])
+    D.gated_feed_forward(*args)

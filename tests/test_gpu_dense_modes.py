@@ -66,3 +66,32 @@ def test_a_timeout_read_beside_a_queued_copy_is_raised_once():
     finally:
         api.set_kernel_options(status_poll_interval=32)
     api.read_dense_status()
+
+
+def test_tangents_are_refused():
+    """Forward mode, alone and through a backward pass; scales and bias of the 8-bit products and the quantiser's input too."""
+    import torch.autograd.forward_ad as fwd
+    from vllm_plugin_b200 import api
+    x, w13, w2 = (torch.randn(s, device="cuda:0").bfloat16() for s in ((5, 64), (64, 64), (64, 32)))
+    q, s = api.prepare_int8_inputs(x)
+    w, sw = api.prepare_int8_inputs(w13)
+    bias = torch.zeros(64, device="cuda:0")
+    want = x + api.gated_feed_forward(x, w13, w2)
+    with fwd.dual_level():
+        def dual(t):
+            return fwd.make_dual(t, torch.ones_like(t))
+        for args in ((dual(x), w13, w2), (x, dual(w13), w2), (x, w13, dual(w2))):
+            with pytest.raises(NotImplementedError):
+                api.gated_feed_forward(*args)
+        with pytest.raises(NotImplementedError):
+            api.prepare_int8_inputs(dual(x))
+        for args, b in (((q, dual(s), w, sw), bias), ((q, s, w, dual(sw)), bias), ((q, s, w, sw), dual(bias))):
+            with pytest.raises(NotImplementedError):
+                api.int8_projection(*args, bias=b)
+        with pytest.raises(NotImplementedError):
+            api.int8_gated_projection(q, s, w, dual(sw))
+        assert torch.equal(x + api.gated_feed_forward(x, w13, w2), want)      # a level by itself is no obstacle
+        leaf = x.detach().requires_grad_(True)
+        y = api.gated_feed_forward(leaf, w13, w2)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(y, leaf, dual(torch.ones_like(y)))

@@ -16,6 +16,7 @@ import weakref
 from typing import Dict, Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native
@@ -160,6 +161,15 @@ def _check_weight(w: torch.Tensor, what: str, dtype: torch.dtype, x: torch.Tenso
         _refuse_weight(w, what, dtype, x.device)
 
 
+def _refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """To be called inside a level of forward-mode differentiation only (``_forward_ad._current_level >= 0``).  Outputs are written where
+    PyTorch does not see it: they would come back without a tangent, and what is computed from them with a wrong one."""
+    if torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # gated feed-forward block
 # ---------------------------------------------------------------------------------------------------------------------
@@ -239,6 +249,8 @@ class _Block(torch.autograd.Function):
 
     @staticmethod
     def _gradients(ctx, dy):
+        if _forward_ad._current_level >= 0:
+            _refuse_tangents("the gradient of gated_feed_forward", dy)
         x, w13, w2, kept, *copy = ctx.saved_tensors
         dy2 = dy if dy.dim() == 2 and dy.is_contiguous() else dy.reshape(-1, w2.shape[0]).contiguous()
         if dy2.data_ptr() % 16 != 0:
@@ -281,6 +293,8 @@ def gated_feed_forward(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, *, 
     """``y = h w2^T`` with ``h = silu(min(x wg^T, c)) * clip(x wu^T, -c, c)`` and ``w13 = [wg; wu]``.  See ``api.gated_feed_forward``."""
     _check_block(x, w13, w2)
     clamp = _clamp_of(activation_clamp)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents("gated_feed_forward", x, w13, w2)
     if not ((x.requires_grad or w13.requires_grad or w2.requires_grad) and torch.is_grad_enabled()):
         y = _launch_block(_rows(x), w13, w2, clamp, False)[0]
         return y if x.dim() == 2 else y.view(x.shape)
@@ -306,6 +320,8 @@ def prepare_int8_inputs(hidden_states: torch.Tensor, out: Optional[Tuple[torch.T
         raise ValueError("INT8 staging requires BF16 or FP16 CUDA hidden states.")
     if x.requires_grad:
         _refuse_gradient("INT8 staging")
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents("INT8 staging", x)
     shape = x.shape
     width, lead = shape[-1], shape[:-1]
     if width == 0:
@@ -344,6 +360,8 @@ def _float_vector(t: torch.Tensor, shape, what: str, index: int) -> torch.Tensor
         raise AssertionError(f"{what} must be float32 {tuple(shape)} on cuda:{index}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     if t.requires_grad:
         _refuse_gradient("a product of 8-bit integers")
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents("a product of 8-bit integers", t)
     return t if t.is_contiguous() else t.contiguous()
 
 
