@@ -155,3 +155,44 @@ def test_tangents_are_refused(launches):
         with fwd._set_fwd_grad_enabled(False):               # as inference mode has it: nobody asks for tangents
             D.gated_feed_forward(fwd.make_dual(args[0], args[0]), *args[1:])
     D.gated_feed_forward(*args)
+
+
+def test_traces_are_refused(launches):
+    """torch.jit.trace and make_fx would record the allocation of the output and not what fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from vllm_plugin_b200.backend import dense as D
+    for tokens in (5, 0):
+        x, w13, w2 = _block()
+        x = x[:tokens]
+
+        def forward(a, b, c):
+            return D.gated_feed_forward(a, b, c)
+
+        def gradient(a, b, c):
+            return torch.autograd.grad(D.gated_feed_forward(a, b, c), (a, b, c), torch.ones_like(a))
+
+        for grad in (False, True):
+            args = tuple(t.clone().requires_grad_(grad) for t in (x, w13, w2))
+            with pytest.raises((NotImplementedError, TypeError)):           # TypeError: with gradients PyTorch's own, at the function's number argument
+                torch.jit.trace(forward, args, check_trace=False)
+            for early in (False, True):
+                with pytest.raises(NotImplementedError, match="trace"):
+                    make_fx(gradient if grad else forward, pre_dispatch=early)(*args)
+        args = tuple(t.clone().requires_grad_(True) for t in (x, w13, w2))
+        y = D.gated_feed_forward(*args)
+        with pytest.raises(NotImplementedError, match="trace"):                                  # the gradient alone
+            make_fx(lambda dy: torch.autograd.grad(y, args, dy))(torch.ones_like(y))
+
+    class Counts(TorchDispatchMode):                     # a mode that runs what it sees is no trace
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    launches.clear()
+    with Counts(), torch.device("cpu"):
+        D.gated_feed_forward(*_block())
+    assert launches == ["mmoe_feed_forward"]
+    with pytest.raises(NotImplementedError, match="trace"):
+        make_fx(lambda t: D._int8_product(t, None, None, None, None, torch.bfloat16, 1.0, False))(torch.zeros(5, 64, dtype=torch.int8))
+    with pytest.raises(NotImplementedError, match="trace"):
+        make_fx(D.prepare_int8_inputs)(_block()[0], None)

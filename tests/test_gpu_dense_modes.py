@@ -95,3 +95,27 @@ def test_tangents_are_refused():
         y = api.gated_feed_forward(leaf, w13, w2)
         with pytest.raises(NotImplementedError):
             torch.autograd.grad(y, leaf, dual(torch.ones_like(y)))
+
+
+def test_traces_are_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from vllm_plugin_b200 import api
+    x, w13, w2 = (torch.randn(s, device="cuda:0").bfloat16() for s in ((5, 64), (64, 64), (64, 32)))
+    q, s = api.prepare_int8_inputs(x)
+    w, sw = api.prepare_int8_inputs(w13)
+    for run, args in ((lambda a, b, c: api.gated_feed_forward(a, b, c), (x, w13, w2)), (lambda a: api.prepare_int8_inputs(a), (x,)),
+                      (lambda a, b, c, d: api.int8_projection(a, b, c, d), (q, s, w, sw)),
+                      (lambda a, b, c, d: api.int8_gated_projection(a, b, c, d), (q, s, w, sw))):
+        run(*args)
+        with pytest.raises(NotImplementedError):
+            make_fx(run)(*args)
+        with pytest.raises(NotImplementedError):
+            torch.jit.trace(run, args, check_trace=False)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w13, w2)]
+    y = api.gated_feed_forward(*leaves)
+    with pytest.raises(NotImplementedError):                     # the backward pass runs on a thread of its own
+        make_fx(lambda dy: torch.autograd.grad(y, leaves, dy, retain_graph=True))(x)
+    want = torch.autograd.grad(y, leaves, x)
+    with torch.utils.flop_counter.FlopCounterMode(display=False):        # a mode that runs what it sees
+        y = api.gated_feed_forward(*leaves)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, x), want))
