@@ -6,6 +6,7 @@ import sys
 
 import pytest
 import torch
+import torch.utils.flop_counter
 
 from helpers import ROOT
 
@@ -22,6 +23,7 @@ def test_a_first_call_in_inference_mode():
     """A serving warm-up, then more calls than lie between two looks at the status words, without a mode and training."""
     _fresh("""
 import torch
+import torch.utils.flop_counter
 from vllm_plugin_b200 import api
 x, w13, w2 = (torch.randn(s, device="cuda").bfloat16() for s in ((5, 64), (64, 64), (64, 32)))
 with torch.inference_mode():
