@@ -196,3 +196,15 @@ def test_traces_are_refused(launches):
         make_fx(lambda t: D._int8_product(t, None, None, None, None, torch.bfloat16, 1.0, False))(torch.zeros(5, 64, dtype=torch.int8))
     with pytest.raises(NotImplementedError, match="trace"):
         make_fx(D.prepare_int8_inputs)(_block()[0], None)
+
+
+def test_what_the_launch_in_front_writes_is_not_read_as_constant():
+    """The dense launches start beside the ones in front of them, which write their tokens, scales, weights and bias: behind the wait they
+    are read with ordinary loads, never through the read-only path, which is for memory that nobody writes while a kernel runs."""
+    import os
+    from helpers import ROOT
+    for name in ("mmoe_dense.cu", "mmoe_dense.cuh"):
+        with open(os.path.join(ROOT, "vllm_plugin_b200", "csrc", name)) as f:
+            text = f.read()
+        for form in ("__ldg(", "__restrict__", ".nc."):
+            assert form not in text, (name, form)

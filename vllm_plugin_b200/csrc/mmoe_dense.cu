@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
       e.row0 = at.m * 2 * kPairRows + static_cast<int>(cta) * kPairRows + quadrant * 32, e.rows = min(32, q.m - e.row0);
       e.col0 = at.n * width, e.last = min(q.n, e.col0 + width);
       e.d = tmem_base + acc * kPairCols + (static_cast<uint32_t>(quadrant * 32) << 16);
-      const float row_scale = kInt8 && lane < e.rows ? __ldg(epi.row_scale + e.row0 + lane) : 0.f;
+      const float row_scale = kInt8 && lane < e.rows ? epi.row_scale[e.row0 + lane] : 0.f;
       if (kSet == kGatedGrad && q.kind == kGatedGrad && e.side == 0 && lane < e.rows) {
         // g and u come from HBM, a row's 1 KB each by now
         const float* keep = epi.preact + (int64_t)(e.row0 + lane) * 2 * epi.inter + e.col0;
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
   const int tokens = p.m, g = static_cast<int>(threadIdx.x) % kGroups;
   const DenseFinish<kKind, kInt8> finish(p.epi, p.n, tile * 8 * kGroups + 8 * g);
   if (kInt8)
-    for (int t = threadIdx.x; t < tokens; t += kFewThreads) ctl->row_scale[t] = __ldg(p.epi.row_scale + t);
+    for (int t = threadIdx.x; t < tokens; t += kFewThreads) ctl->row_scale[t] = p.epi.row_scale[t];
   // The partial sums take the place of the stages, which this CTA needs no more when its accumulator is complete: [token][128 rows].  Each CTA
   // of the cluster finishes some of the tokens; the others send it theirs, in one copy each, when no CTA needs its stages any more.
   constexpr int kRowBytes = kFewRows * 4;
@@ -809,8 +809,7 @@ template <> struct PairOf<__nv_bfloat16> { using type = __nv_bfloat162; };
 
 // kVec: eight values at a time, else (widths, strides or places that do not allow it) one.  kWarps: a warp per token, eight of them to a block.
 template <typename T, bool kVec, bool kWarps>
-__global__ void __launch_bounds__(kQuantThreads) quantize_int8_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q,
-                                                                      float* __restrict__ scales, int m, int k) {
+__global__ void __launch_bounds__(kQuantThreads) quantize_int8_kernel(const T* x, int64_t ld, int8_t* q, float* scales, int m, int k) {
   chain_wait();
   chain_release();
   using P = typename PairOf<T>::type;

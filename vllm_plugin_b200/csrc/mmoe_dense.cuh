@@ -115,14 +115,15 @@ struct DenseFinish {
   const DenseEpilogue& e;
   const int col, valid;
   float cs[8], second[8];              // scales of the columns; kGated: those of the up columns, kLinear: bias
+  // by ordinary loads: what is read here may have been written by the launch in front, beside which this one has started
   __device__ __forceinline__ void load8(const float* src, float (&v)[8]) const {
     if (valid >= 8 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
-      const float4 lo = __ldg(reinterpret_cast<const float4*>(src)), hi = __ldg(reinterpret_cast<const float4*>(src) + 1);
+      const float4 lo = reinterpret_cast<const float4*>(src)[0], hi = reinterpret_cast<const float4*>(src)[1];
       v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
       return;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < valid ? __ldg(src + j) : 0.f;
+    for (int j = 0; j < 8; ++j) v[j] = j < valid ? src[j] : 0.f;
   }
   __device__ __forceinline__ DenseFinish(const DenseEpilogue& epi, int n, int column) : e(epi), col(column), valid(n - column) {
     if (!kScaled) return;
