@@ -159,7 +159,7 @@ typedef struct MmoeOptions {
   float activation_clamp;   /* SwiGLU clamp; +inf disables it */
   int32_t fast_math;        /* 1: ex2.approx / rcp.approx sigmoid, 0: IEEE expf and division */
   int32_t engine;           /* 0: tcgen05 tensor-core kernels; 1: scalar validation kernels (tests only) */
-  int32_t timeout_ms;       /* bound of every device-side wait; <= 0 selects the default (2000) */
+  int32_t timeout_ms;       /* from a kernel's start: after it, the kernel's waits give up; <= 0 selects the default (2000) */
   int32_t layer_mask;       /* 0 or 3: both grouped GEMMs; 1: GEMM1 (+SwiGLU) only; 2: GEMM2 only (per-kernel timing) */
   const void* residual;     /* mmoe_forward / mmoe_forward_ep: optional bf16 [num_tokens, H] added in the combine
                              * (see mmoe_combine_residual); NULL: none */
@@ -298,7 +298,8 @@ typedef struct MmoeFeedForward {
   int32_t intermediate;       /* I, a multiple of 8 */
   int32_t num_tokens;         /* M */
   float clamp;                /* +inf: none */
-  int32_t timeout_ms;         /* bound of every device-side wait; <= 0 selects the default (2000) */
+  int32_t timeout_ms;         /* bound of every device-side wait by itself, not of a launch (a wait for a whole sum: 10 us a step of 128 bytes of K more);
+                                 <= 0 selects the default (2000) */
   int64_t x_stride;           /* elements between the rows of x, >= H and a multiple of 8 */
   const void* x;              /* [M, H] */
   const void* w13;            /* [2I, H] */
@@ -326,7 +327,7 @@ typedef struct MmoeInt8Product {
   int32_t channels;           /* N: rows of w (projection), or half of them (gated) */
   int32_t out_type;           /* MMOE_BF16, MMOE_FP16 or MMOE_FP32 */
   float clamp;                /* gated only; +inf: none */
-  int32_t timeout_ms;
+  int32_t timeout_ms;         /* as above */
   int64_t x_stride;           /* bytes between the rows of x, >= K and a multiple of 16 */
   const void* x;              /* int8 [M, K] */
   const float* x_scales;      /* [M] */

@@ -121,3 +121,25 @@ def test_traces_are_refused():
     with torch.utils.flop_counter.FlopCounterMode(display=False):        # a mode that runs what it sees
         y = api.gated_feed_forward(*leaves)
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, x), want))
+
+
+def test_the_limit_is_that_of_a_wait_not_of_a_launch():
+    """Launches that take longer than the limit of a wait, none of whose waits does: the same results, and nothing recorded."""
+    from vllm_plugin_b200 import api
+    gen = torch.Generator(device="cuda:0").manual_seed(1)
+    m, n, k = 20000, 16384, 16384
+    x, w = (torch.randint(-127, 128, (r, k), generator=gen, device="cuda:0", dtype=torch.int32).to(torch.int8) for r in (m, n))
+    sx, sw = torch.rand(m, generator=gen, device="cuda:0"), torch.rand(n, generator=gen, device="cuda:0")
+    want = api.int8_projection(x, sx, w, sw)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    limit = api.get_kernel_options().timeout_ms
+    try:
+        api.set_kernel_options(timeout_ms=1)
+        start.record()
+        got = api.int8_projection(x, sx, w, sw)
+        end.record()
+        api.read_dense_status()
+    finally:
+        api.set_kernel_options(timeout_ms=limit)
+    assert start.elapsed_time(end) > 2                  # 1.1e13 operations in one launch
+    assert torch.equal(got, want)

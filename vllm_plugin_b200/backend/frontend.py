@@ -34,7 +34,7 @@ class KernelOptions:
     variable: ``backend/frontend.py:72-116``)."""
 
     block_m: int = 0          # > 0 forces the BLOCK_M variant
-    timeout_ms: int = 2000    # bound of every device-side wait
+    timeout_ms: int = 2000    # bound of device-side waits: of all in a launch of the layer, of each in a dense operator's
     ep_transport: str = "peer"  # EP > 1: "peer" = device-side exchange over NVLink peer memory (graph-capturable),
                                 # "nccl" = host-driven all-to-allv (also used when symmetric memory is unavailable)
     fuse_return: bool = True    # "peer" transport: GEMM2's epilogue stores its rows straight into the source rank's

@@ -57,6 +57,37 @@ struct PairControl {
   volatile int32_t abort_flag;
 };
 
+// Waits with a limit each, which counts from a wait's 64th probe on: a launch may take as long as its size asks for.  (The layer's limit is one for a
+// whole launch, which its buffers bound.)  What waits for a whole tile or for all of a CTA's K says how many stages that are: kStageNs, many times what
+// one takes, is added for each.
+constexpr int64_t kStageNs = 10000;
+struct DenseWaiter {
+  Waiter wait;               // its deadline is that of the wait under way
+  int64_t limit_ns;
+  __device__ __forceinline__ bool late(uint32_t spin, int stages) {
+    if (spin != 63u) return wait.abandoned();
+    wait.deadline = global_timer() + static_cast<uint64_t>(limit_ns + stages * kStageNs);
+    return *wait.abort_flag != 0;
+  }
+  // both by the whole warp; true when the phase has completed, false when the call is being abandoned (see Waiter for why two)
+  __device__ __forceinline__ bool wait_uniform(uint32_t bar, uint32_t parity) {
+    for (uint32_t spin = 0;; ++spin) {
+      if (__any_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+      if ((spin & 63u) == 63u && __any_sync(0xffffffffu, late(spin, 0))) return false;
+    }
+  }
+  __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int stages) {
+    if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+    bool ok = true;
+    if ((threadIdx.x & 31) == 0)
+      for (uint32_t spin = 0;; ++spin) {
+        if (mbar_try_wait(bar, parity)) break;
+        if ((spin & 63u) == 63u && late(spin, stages)) { ok = false; break; }
+      }
+    return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+  }
+};
+
 // descriptor without its address: 128-byte swizzle; K-major: eight-row groups 1024 bytes apart.  MN-major: groups of eight k's 1024 bytes
 // apart, blocks of 64 rows `block` bytes apart.
 __device__ __forceinline__ uint64_t operand_desc(bool mn_major, uint32_t block) {
@@ -205,7 +236,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
   chain_release();                          // in this order: what precedes this launch is complete when the next one starts
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
   const int tiles = p.tiles, step = gridDim.x / 2, n_stages = p.stages;
-  Waiter waiter{&ctl->abort_flag, p.status, global_timer() + static_cast<uint64_t>(p.timeout_ns), kStatusDense, warp};
+  DenseWaiter waiter{{&ctl->abort_flag, p.status, 0, kStatusDense, warp}, p.timeout_ns};
   const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
 
   if (warp == 0) {
@@ -306,7 +337,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
         prefetch_bulk(keep, (e.last - e.col0) * 4);
         prefetch_bulk(keep + epi.inter, (e.last - e.col0) * 4);
       }
-      if (!waiter.wait_warp(smem_u32(&ctl->acc_full[acc]), (it >> 1) & 1u)) break;
+      if (!waiter.wait_warp(smem_u32(&ctl->acc_full[acc]), (it >> 1) & 1u, q.k_stages)) break;
       tc_fence_after();
       const auto release = [&] {
         tc_fence_before();
@@ -450,7 +481,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
   chain_wait();                             // nothing above touches global memory
   chain_release();                          // in this order: what precedes this launch is complete when the next one starts
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
-  Waiter waiter{&ctl->abort_flag, p.status, global_timer() + static_cast<uint64_t>(p.timeout_ns), kStatusDense + 1, warp};
+  DenseWaiter waiter{{&ctl->abort_flag, p.status, 0, kStatusDense + 1, warp}, p.timeout_ns};
 
   if (warp == 0) {
     // --------------------------------------------------------------------------------------------- producer
@@ -514,7 +545,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
   const uint32_t came = smem_u32(&ctl->sums_in);
   uint8_t* sent = stages + p.tokens * kRowBytes;       // [CTA, this one left out][token][128 rows]
   if (p.split > 1 && threadIdx.x == 0) mbar_expect_tx(came, (p.split - 1) * mine * kRowBytes);
-  if (warp >= 2 && warp < 6 && waiter.wait_warp(smem_u32(&ctl->acc_full), 0)) {
+  if (warp >= 2 && warp < 6 && waiter.wait_warp(smem_u32(&ctl->acc_full), 0, k1 - k0)) {
     tc_fence_after();
     const int row = (warp & 3) * 32 + lane;
     const uint32_t d = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -537,7 +568,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
           cluster_send(map_to_cta(base + (p.tokens + (rank < r ? rank : rank - 1) * own) * kRowBytes, r), base + r * own * kRowBytes, theirs * kRowBytes, map_to_cta(came, r));
       }
     __syncwarp();
-    waiter.wait_warp(came, 0);
+    waiter.wait_warp(came, 0, 0);
     __syncwarp();
     cluster_arrive();                       // what this CTA waited for has come; behind the matching wait, all that it has sent has
   }

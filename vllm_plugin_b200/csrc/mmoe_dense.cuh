@@ -43,7 +43,7 @@ struct DenseProduct {
   int32_t kind;
   DenseEpilogue epi;
   int32_t* status;           // int32 [8], see kStatusTimeout
-  int32_t timeout_ms;        // of every wait; <= 0: the default
+  int32_t timeout_ms;        // of each wait; <= 0: the default
 };
 
 cudaError_t prepare_dense();   // once per device, outside stream capture
