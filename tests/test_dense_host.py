@@ -1,5 +1,7 @@
 """Host side of the dense feed-forward operators on the CPU, launches and CUDA's own objects stubbed."""
 
+import types
+
 import pytest
 import torch
 
@@ -42,7 +44,6 @@ def test_status_words_work_in_any_mode(stubbed, make_in_inference):
 
 def test_a_buffer_made_in_inference_mode_can_be_reset_outside(stubbed, monkeypatch):
     """The layer's own words, which its poll resets as well."""
-    import types
     from vllm_plugin_b200.backend import frontend as F, workspace as W
     empty = torch.empty
 
@@ -65,7 +66,6 @@ def test_a_buffer_made_in_inference_mode_can_be_reset_outside(stubbed, monkeypat
 def test_a_read_forgets_the_copy_that_was_queued(stubbed, monkeypatch):
     """A failure that a read has reported and cleared is not raised once more by a copy of the words queued in front of the read."""
     import contextlib
-    import types
     from vllm_plugin_b200.backend import _native, dense as D, frontend as F
     state = D._Device(torch.device("cpu"))
     raised = []
@@ -109,7 +109,6 @@ def test_a_timeout_names_the_kind_of_call(stubbed):
 @pytest.fixture
 def launches(stubbed, monkeypatch):
     """The operators on CPU tensors; the C library writes nothing.  The list of what was called."""
-    import types
     from vllm_plugin_b200.backend import dense as D
     calls = []
     lib = types.SimpleNamespace(**{n: (lambda *a, n=n: calls.append(n) or 0) for n in (
@@ -208,3 +207,22 @@ def test_what_the_launch_in_front_writes_is_not_read_as_constant():
             text = f.read()
         for form in ("__ldg(", "__restrict__", ".nc."):
             assert form not in text, (name, form)
+
+
+def test_sizes_past_32_bits_are_refused_before_anything_is_made(launches):
+    """The C interface takes 32-bit sizes; what does not fit is not cut to its low bits.  Broadcast tensors: nothing of that size exists."""
+    from vllm_plugin_b200.backend import dense as D
+    x, w13, w2 = _block()
+    for tokens in (2**32 + 5, 2**32, 2**31, 2**30 + 1):
+        many = x[:1].expand(tokens, 64)
+        for rows in (many, many.view(1, tokens, 64)):
+            with pytest.raises(AssertionError, match="tokens"):
+                D._rows(rows)
+        with pytest.raises(AssertionError, match="tokens"):
+            D.gated_feed_forward(many, w13, w2)
+        rows = types.SimpleNamespace(shape=(tokens, 64))                       # dense rows, of which no copy would be made
+        with pytest.raises(AssertionError, match="tokens"):
+            D._launch_block(rows, w13, w2, 1.0, False)
+    assert not launches
+    D.gated_feed_forward(x[:1].expand(7, 64), w13, w2)
+    assert launches

@@ -113,3 +113,9 @@ def test_there_is_no_cpu_path():
     if not torch.cuda.is_available():
         with pytest.raises(Exception):
             api.read_dense_status()
+
+
+def test_quantiser_sizes_past_32_bit_indexes():
+    lib = _native().load()
+    for tokens, width in ((2**31 - 1, 64), (2**31 - 4095, 8), (5, 2**31 - 1), (5, 2**31 - 4095)):
+        _refused(lib.mmoe_quantize_int8(FAKE, 0, max(width, 64), FAKE, FAKE, tokens, width, None))

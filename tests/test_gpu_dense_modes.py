@@ -143,3 +143,24 @@ def test_the_limit_is_that_of_a_wait_not_of_a_launch():
         api.set_kernel_options(timeout_ms=limit)
     assert start.elapsed_time(end) > 2                  # 1.1e13 operations in one launch
     assert torch.equal(got, want)
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Broadcast rows, so that nothing of that size exists: refused before a copy or an output is made."""
+    from vllm_plugin_b200 import api
+    x, w13, w2 = (torch.randn(s, device="cuda:0").bfloat16() for s in ((1, 64), (64, 64), (64, 32)))
+    q, s = api.prepare_int8_inputs(x)
+    w, sw = api.prepare_int8_inputs(w13)
+    held = torch.cuda.memory_allocated()
+    for tokens in (2**32 + 5, 2**32, 2**31):
+        with pytest.raises(AssertionError):
+            api.gated_feed_forward(x.expand(tokens, 64), w13, w2)
+        with pytest.raises(AssertionError):
+            api.int8_projection(q.expand(tokens, 64), s.expand(tokens), w, sw)
+        with pytest.raises(AssertionError):
+            api.int8_gated_projection(q.expand(tokens, 64), s.expand(tokens), w, sw)
+        with pytest.raises(ValueError):
+            api.prepare_int8_inputs(x.expand(tokens, 64))
+        with pytest.raises(ValueError):
+            api.prepare_int8_inputs(x[:, :1].expand(1, tokens))
+    assert torch.cuda.memory_allocated() == held

@@ -132,6 +132,14 @@ def _clamp_of(activation_clamp: Optional[float]) -> float:
     return value
 
 
+# the C interface's limits.  Its sizes have 32 bits, of which ctypes would take the low ones
+_MOST_TOKENS, _MOST_CHANNELS, _MOST_QUANTIZED = 1 << 30, 1 << 29, 2**31 - 4096
+
+
+def _too_many(tokens: int) -> AssertionError:
+    return AssertionError(f"{tokens} tokens: at most {_MOST_TOKENS}")
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` as ``(rows, width)`` whose rows are dense and start on 16 bytes: a view where there is one, else a copy."""
     if t.is_contiguous():
@@ -139,6 +147,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
         return r if r.data_ptr() % 16 == 0 else r.clone()
     r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     tokens, width = r.shape
+    if tokens > _MOST_TOKENS:                    # before a copy of them is made
+        raise _too_many(tokens)
     dense = r.stride(1) == 1 or width == 1
     if tokens > 1:
         dense = dense and r.stride(0) >= width and r.stride(0) * r.element_size() % 16 == 0
@@ -207,6 +217,8 @@ def _launch_block(x2: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, clamp: 
     """``(y, kept)`` of rows ``x2``: ``kept`` holds h, and behind it (``keep``) g and u for the backward pass, in bytes."""
     tokens, hidden = x2.shape
     inter = w2.shape[1]
+    if tokens > _MOST_TOKENS:
+        raise _too_many(tokens)
     y = x2.new_empty((tokens, hidden))
     kept = x2.new_empty(tokens * inter * (5 if keep else 1))       # 16-bit elements: 1 for h, 2 x 2 for g and u
     if tokens > 0:
@@ -347,6 +359,8 @@ def prepare_int8_inputs(hidden_states: torch.Tensor, out: Optional[Tuple[torch.T
     if len(shape) != 2:
         x = x.reshape(-1, width)
     tokens = x.shape[0]
+    if tokens > _MOST_QUANTIZED or width > _MOST_QUANTIZED:
+        raise ValueError(f"INT8 staging takes at most {_MOST_QUANTIZED} tokens and as many channels, got {tokens} and {width}.")
     if not x.is_contiguous() and (width > 1 and x.stride(1) != 1 or tokens > 1 and x.stride(0) < width):
         x = x.contiguous()
     if out is None:
@@ -395,20 +409,22 @@ def _int8_product(x, x_scales, w, w_scales, bias, out_dtype, clamp: float, gated
     rows, width = w.shape
     if shape[-1] != width or width < 16 or width >= 131072 or width % 16 != 0:
         raise AssertionError(f"x (..., K) and the weights (N, K) must agree on K, a multiple of 16 below 131072, got {shape[-1]} and {width}")
-    if rows < 1 or (gated and rows % 2 != 0):
+    if not 1 <= rows <= 2 * _MOST_CHANNELS or (gated and rows % 2 != 0):
         raise AssertionError(f"the weights have {rows} rows" + (": the gated projection needs as many gate as up rows" if gated else ""))
     code = _CODES.get(out_dtype)
     if code is None:
         raise AssertionError(f"out_dtype must be BF16, FP16 or FP32, got {out_dtype}")
     lead = shape[:-1]
+    x2 = _rows(x)
+    tokens = x2.shape[0]
+    if tokens > _MOST_TOKENS:
+        raise _too_many(tokens)
     x_scales = _float_vector(x_scales, lead, "x_scales", index)
     w_scales = _float_vector(w_scales, (rows,), "w_scales", index)
     if bias is not None:
         bias = _float_vector(bias, (rows,), "bias", index)
     channels = rows // 2 if gated else rows
     out = x.new_empty((*lead, channels), dtype=out_dtype)
-    x2 = _rows(x)
-    tokens = x2.shape[0]
     if tokens > 0:
         lib = _lib or _library()
         _launch(lib.mmoe_int8_gated_projection if gated else lib.mmoe_int8_projection, index,

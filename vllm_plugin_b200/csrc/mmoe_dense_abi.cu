@@ -181,6 +181,9 @@ int mmoe_feed_forward_grad(const MmoeFeedForward* f, const void* dy, void* dpre,
 int mmoe_quantize_int8(const void* x, int32_t type, int64_t x_stride, void* q, float* scales, int32_t num_tokens, int32_t width, void* stream) {
   if (num_tokens < 0 || width <= 0) return fail(MMOE_ERR_INVALID_ARGUMENT, "int8 quantiser: num_tokens=%d must be >= 0 and width=%d positive", num_tokens, width);
   if (type != MMOE_BF16 && type != MMOE_FP16) return fail(MMOE_ERR_INVALID_ARGUMENT, "int8 quantiser: type=%d (supported: BF16, FP16)", type);
+  constexpr int32_t kMost = INT32_MAX - 4095;          // the places of a block's threads in a row, a step past its end, are 32-bit numbers
+  if (num_tokens > kMost || width > kMost)
+    return fail(MMOE_ERR_INVALID_ARGUMENT, "int8 quantiser: num_tokens=%d and width=%d: at most %d", num_tokens, width, kMost);
   if (x_stride < width) return fail(MMOE_ERR_INVALID_ARGUMENT, "int8 quantiser: x_stride must be at least width=%d", width);
   if (num_tokens == 0) return MMOE_OK;
   if (x == nullptr || q == nullptr || scales == nullptr) return fail(MMOE_ERR_INVALID_ARGUMENT, "int8 quantiser: pointers must not be NULL");
