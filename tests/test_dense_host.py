@@ -226,3 +226,25 @@ def test_sizes_past_32_bits_are_refused_before_anything_is_made(launches):
     assert not launches
     D.gated_feed_forward(x[:1].expand(7, 64), w13, w2)
     assert launches
+
+
+def test_first_calls_at_once_find_all_of_the_library(monkeypatch):
+    """A thread that finds the library loaded by another one finds the look-up of streams as well, at every line in between."""
+    import sys
+    from vllm_plugin_b200.backend import _native, dense as D
+    monkeypatch.setattr(D, "_lib", None)
+    monkeypatch.setattr(D, "_raw_stream", None)
+    monkeypatch.setattr(_native, "load", lambda: object())
+    half = []
+
+    def watch(frame, event, arg):
+        if frame.f_code is D._library.__code__:
+            half.append(D._lib is not None and D._raw_stream is None)
+            return watch
+
+    sys.settrace(watch)
+    try:
+        D._library()
+    finally:
+        sys.settrace(None)
+    assert half and not any(half) and D._lib is not None and D._raw_stream is not None

@@ -64,8 +64,8 @@ def _on_device(index: int) -> _Device:
 def _library():
     """The C library; what a call looks up is kept from here on."""
     global _lib, _raw_stream
+    _raw_stream = torch._C._cuda_getCurrentRawStream    # first: a thread that finds the library takes this to be there
     _lib = _native.load()
-    _raw_stream = torch._C._cuda_getCurrentRawStream
     return _lib
 
 
