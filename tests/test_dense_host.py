@@ -248,3 +248,44 @@ def test_first_calls_at_once_find_all_of_the_library(monkeypatch):
     finally:
         sys.settrace(None)
     assert half and not any(half) and D._lib is not None and D._raw_stream is not None
+
+
+def test_live_graphs_are_listed_while_others_are_made(monkeypatch):
+    """Eager calls of other threads come and go while a captured call looks through the live graphs."""
+    import sys
+    import threading
+    from vllm_plugin_b200.backend import dense as D
+
+    class Node:
+        next_functions = ()
+
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    stop, wrong = threading.Event(), []
+
+    def make():
+        while not stop.is_set():
+            nodes = [Node() for _ in range(50)]
+            for n in nodes:
+                D._remember(n)
+
+    threads = [threading.Thread(target=make) for _ in range(3)]
+    try:
+        for t in threads:
+            t.start()
+        kept = Node()
+        D._remember(kept)
+        for _ in range(3000):
+            if kept not in D._live_graphs():
+                wrong.append("lost")
+    finally:
+        stop.set()
+        for t in threads:
+            t.join()
+        sys.setswitchinterval(interval)
+    assert not wrong
+    del kept, make
+    threads.clear()
+    import gc
+    gc.collect()
+    assert not D._live_graphs()

@@ -249,8 +249,17 @@ def _launch_block_grad(x2, w13, w2, kept, dy2, clamp: float, wanted):
     return dx, dw13, dw2
 
 
-# nodes of the calls on a default stream whose graphs are alive
-_eager_graphs = weakref.WeakSet()
+# Nodes of the calls on a default stream whose graphs are alive, by weak references that leave by themselves.  A plain set of them, which is listed and
+# changed in one step each: threads may make and drop graphs while another one captures.
+_eager_graphs = set()
+
+
+def _remember(node) -> None:
+    _eager_graphs.add(weakref.ref(node, _eager_graphs.discard))
+
+
+def _live_graphs() -> list:
+    return [node for node in [r() for r in list(_eager_graphs)] if node is not None]
 
 
 class _Block(torch.autograd.Function):
@@ -266,7 +275,7 @@ class _Block(torch.autograd.Function):
         else:
             ctx.save_for_backward(x, w13, w2, kept, x2)
         if (_raw_stream or _native.raw_stream)(x.get_device()) == 0:
-            _eager_graphs.add(ctx)
+            _remember(ctx)
         return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
@@ -297,7 +306,7 @@ def _refuse_beside_eager_graph(inputs) -> None:
     if not _eager_graphs:
         return
     mine = _accumulators([torch.autograd.graph.get_gradient_edge(t).node for t in inputs if t.requires_grad])
-    if mine & _accumulators(list(_eager_graphs)):
+    if mine & _accumulators(_live_graphs()):
         raise RuntimeError("a graph of an eager gated_feed_forward call with the same leaves on the default stream is still alive: "
                            "drop its output before the call is captured for training")
 
