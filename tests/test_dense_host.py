@@ -289,3 +289,16 @@ def test_live_graphs_are_listed_while_others_are_made(monkeypatch):
     import gc
     gc.collect()
     assert not D._live_graphs()
+
+
+def test_the_combine_does_not_read_its_inputs_as_constant():
+    """What it adds is written by launches in front of it, beside which it starts: the routed rows, and a residual that a dense operator left or that is
+    the output itself.  No restrict pointers, so that nothing tells the compiler that they stay as they are."""
+    import os
+    import re
+    from helpers import ROOT
+    with open(os.path.join(ROOT, "vllm_plugin_b200", "csrc", "mmoe_support.cu")) as f:
+        text = f.read()
+    for name in ("combine_narrow_kernel", "combine_kernel"):
+        (arguments,) = re.findall(rf"__launch_bounds__\(256\) {name}\((.*?)\) {{", text, re.S)
+        assert "residual" in arguments and "__restrict__" not in arguments, name

@@ -1125,8 +1125,8 @@ __device__ __forceinline__ __nv_bfloat162 add_residual(__nv_bfloat162 o, __nv_bf
 // each other: little hangs on where it lies.
 constexpr int kNarrowTokens = 16;
 __global__ void __launch_bounds__(256) combine_narrow_kernel(
-    const uint32_t* __restrict__ rows, const int32_t* __restrict__ route_pos, const uint32_t* __restrict__ shared_out,
-    const uint32_t* __restrict__ residual, uint32_t* __restrict__ y, int m, int h, int k, char* plan_base, int e_local) {
+    const uint32_t* rows, const int32_t* route_pos, const uint32_t* shared_out,
+    const uint32_t* residual, uint32_t* y, int m, int h, int k, char* plan_base, int e_local) {
   chain_wait();
   if (combine_zeroes(plan_base, e_local)) return;
   const uint32_t pairs = h / 2, i = blockIdx.x * blockDim.x + threadIdx.x, t = i / pairs;
@@ -1161,8 +1161,8 @@ __global__ void __launch_bounds__(256) combine_narrow_kernel(
 // once (with one dependent load after the other 3840 x 5120 top-6, 315 MB, took 63 us).
 constexpr int kCombineSegVec = 64;
 __global__ void __launch_bounds__(256) combine_kernel(
-    const uint4* __restrict__ rows, const int32_t* __restrict__ route_pos, const uint4* __restrict__ shared_out,
-    const uint4* __restrict__ residual, uint4* __restrict__ y, int m, int h, int k, char* plan_base, int e_local) {
+    const uint4* rows, const int32_t* route_pos, const uint4* shared_out,
+    const uint4* residual, uint4* y, int m, int h, int k, char* plan_base, int e_local) {
   chain_wait();
   if (combine_zeroes(plan_base, e_local)) return;
   const int blocks = plan_base != nullptr ? gridDim.x - 1 : gridDim.x;
