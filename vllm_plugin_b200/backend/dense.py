@@ -181,17 +181,14 @@ def _refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
                 raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
-_is_tracing = torch._C._is_tracing
-_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+# A trace, or a mode of PyTorch that may be one, is on when one of these is not zero.  Asked in place: a call of 11 us is 0.2 us longer for a function's sake.
+_tracing, _dispatch_modes, _function_modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
 
 
 def _refuse_traces(what: str) -> None:
     """A trace records the allocation of an output and not the launch that fills it.  Modes that run what they see are no obstacle."""
-    traced = _is_tracing()
-    if not traced and (_modes[0]() or _modes[1]()):
-        tracer = sys.modules.get("torch.fx.experimental.proxy_tensor")
-        traced = tracer is not None and tracer.get_proxy_mode() is not None
-    if traced:
+    tracer = sys.modules.get("torch.fx.experimental.proxy_tensor")
+    if _tracing() or (tracer is not None and tracer.get_proxy_mode() is not None):
         raise NotImplementedError(f"{what} cannot be traced (torch.jit.trace, make_fx)")
 
 
@@ -285,7 +282,8 @@ class _Block(torch.autograd.Function):
 
     @staticmethod
     def _gradients(ctx, dy):
-        _refuse_traces("the gradient of gated_feed_forward")
+        if _tracing() or _dispatch_modes() or _function_modes():
+            _refuse_traces("the gradient of gated_feed_forward")
         if _forward_ad._current_level >= 0:
             _refuse_tangents("the gradient of gated_feed_forward", dy)
         x, w13, w2, kept, *copy = ctx.saved_tensors
@@ -328,7 +326,8 @@ def _accumulators(nodes) -> set:
 
 def gated_feed_forward(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, *, activation_clamp: Optional[float] = None) -> torch.Tensor:
     """``y = h w2^T`` with ``h = silu(min(x wg^T, c)) * clip(x wu^T, -c, c)`` and ``w13 = [wg; wu]``.  See ``api.gated_feed_forward``."""
-    _refuse_traces("gated_feed_forward")
+    if _tracing() or _dispatch_modes() or _function_modes():
+        _refuse_traces("gated_feed_forward")
     _check_block(x, w13, w2)
     clamp = _clamp_of(activation_clamp)
     if _forward_ad._current_level >= 0:
@@ -352,7 +351,8 @@ def _refuse_gradient(what: str) -> None:
 def prepare_int8_inputs(hidden_states: torch.Tensor, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
                         ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Per-token 8-bit quantiser.  See ``api.prepare_int8_inputs``."""
-    _refuse_traces("INT8 staging")
+    if _tracing() or _dispatch_modes() or _function_modes():
+        _refuse_traces("INT8 staging")
     x = hidden_states
     code = _CODES.get(x.dtype)
     if code is None or code == _native.MMOE_FP32 or not x.is_cuda or x.dim() < 1:
@@ -407,7 +407,8 @@ def _float_vector(t: torch.Tensor, shape, what: str, index: int) -> torch.Tensor
 
 
 def _int8_product(x, x_scales, w, w_scales, bias, out_dtype, clamp: float, gated: bool) -> torch.Tensor:
-    _refuse_traces("a product of 8-bit integers")
+    if _tracing() or _dispatch_modes() or _function_modes():
+        _refuse_traces("a product of 8-bit integers")
     index = x.get_device()
     if index < 0:
         raise RuntimeError("products of 8-bit integers run on the GPU only (there is no CPU path).")
