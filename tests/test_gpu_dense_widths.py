@@ -67,3 +67,22 @@ def test_projection_of_8_bits(shape, out_dtype):
     for bias in (None, _randn(5, n)):
         y = api.int8_projection(x, sx, w, sw, bias=bias, out_dtype=out_dtype)
         R.check(f"{out_dtype}", y, *R.projection(x, sx, w, sw, bias, out_dtype))
+
+
+@pytest.mark.parametrize("shape", [(392, 200), (1032, 264), (520, 1288)], ids=_name)
+@pytest.mark.parametrize("m", [160, 161, 176, 191, 192, 193, 208, 224, 256])
+def test_gradients_on_either_side_of_the_lines(m, shape):
+    """From 161 tokens on the forward products run on pairs, from 193 on those of the gradients that read the weights along their rows."""
+    from vllm_plugin_b200 import api
+    hidden, inter = shape
+    x, w13 = _randn(1, m, hidden, dtype=torch.bfloat16), _randn(2, 2 * inter, hidden, dtype=torch.bfloat16, std=hidden ** -0.5)
+    w2, dy = _randn(3, hidden, inter, dtype=torch.bfloat16, std=inter ** -0.5), _randn(4, m, hidden, dtype=torch.bfloat16)
+    leaves = [t.requires_grad_(True) for t in (x, w13, w2)]
+    y = api.gated_feed_forward(*leaves, activation_clamp=1.25)
+    grads = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    ref = R.Block(*leaves, 1.25, dy)
+    R.check("y", y.detach(), ref.y, ref.off["y"])
+    for name, got in zip(("dx", "dw13", "dw2"), grads):
+        R.check(name, got, getattr(ref, name), ref.off[name])
+    dx, = torch.autograd.grad(y, leaves[:1], dy)
+    assert torch.equal(dx, grads[0])

@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
 constexpr int kFewRows = 128;                         // rows of B per tile
 constexpr int kFewThreads = 256;
 constexpr int kFewMaxStages = 12;
-constexpr int kFewMaxTokens = 256;
+constexpr int kFewTokens = 160, kFewMaxTokens = 192;  // with the weights as they are stored; read along their rows (dense_few_tokens)
 constexpr int kFewMaxSplit = 8;
 constexpr int kFewSmem = 227 * 1024;
 constexpr int kFewControl = 2048, kFewApart = kFewControl + 1024;      // beside the stages: control block, and the slack for aligning the base
@@ -917,10 +917,12 @@ cudaError_t prepare_dense() {
   return e;
 }
 
-// Few tokens: up to 256 where the weights are read along their rows (MN-major), else up to 160.  Few -> pairs, 5120 x 2304: 16-bit block, 128
-// tokens 25.3 -> 28.7 us, 160 27.0 -> 28.7, 176 29.1 -> 28.7, 256 36.0 -> 29.0; 8-bit gated product, 160 11.2 -> 11.7, 176 12.1 -> 11.7; through
-// the second product and to dx, before the sums were sent in one copy, 192 46.5 -> 64.3, 256 57.6 -> 65.0.
-bool dense_few_tokens(const DenseProduct& p) { return !p.a.k_rows && p.m <= (p.b.k_rows ? kFewMaxTokens : 160); }
+// Few tokens: up to 192 where the weights are read along their rows (MN-major), else up to 160.  Few -> pairs, 5120 x 2304: 16-bit block, 128
+// tokens 25.3 -> 28.7 us, 160 27.0 -> 28.7, 176 29.1 -> 28.7, 256 36.0 -> 29.0; 8-bit gated product, 160 11.2 -> 11.7, 176 12.1 -> 11.7.  Through the
+// second product and to dx, 161 tokens 30.7 -> 37.1, 192 34.2 -> 37.3, 224 37.3 -> 37.4, 256 42.8 -> 37.7; all gradients (three launches, or two), 161
+// 63.1 -> 76.2, 192 66.3 -> 76.2, 224 73.1 -> 74.8, 256 79.1 -> 75.2; of 8192 x 4096, 192 138 -> 185, 224 164 -> 162, 256 175 -> 164.  A small
+// block would have its lines lower: 2048 x 1408, all gradients, 96 28.0 -> 29.6, 128 31.5 -> 30.0, 192 38.9 -> 30.2.
+bool dense_few_tokens(const DenseProduct& p) { return !p.a.k_rows && p.m <= (p.b.k_rows ? kFewMaxTokens : kFewTokens); }
 
 cudaError_t launch_dense(const DenseProduct* p, int parts, cudaStream_t s) {
   const int sms = prepared_sms();
