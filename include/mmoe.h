@@ -323,7 +323,7 @@ int mmoe_quantize_int8(const void* x, int32_t type, int64_t x_stride, void* q, f
 /* Products of 8-bit integers with a scale per token and per channel; the sums are exact. */
 typedef struct MmoeInt8Product {
   int32_t num_tokens;         /* M */
-  int32_t width;              /* K, a multiple of 16, at most 131072 */
+  int32_t width;              /* K, a multiple of 16 below 131072 */
   int32_t channels;           /* N: rows of w (projection), or half of them (gated) */
   int32_t out_type;           /* MMOE_BF16, MMOE_FP16 or MMOE_FP32 */
   float clamp;                /* gated only; +inf: none */

@@ -88,6 +88,8 @@ struct DenseWaiter {
   }
 };
 
+static_assert(sizeof(PairControl) <= 1024, "control block");
+
 // descriptor without its address: 128-byte swizzle; K-major: eight-row groups 1024 bytes apart.  MN-major: groups of eight k's 1024 bytes
 // apart, blocks of 64 rows `block` bytes apart.
 __device__ __forceinline__ uint64_t operand_desc(bool mn_major, uint32_t block) {
@@ -367,21 +369,21 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
 // operand B, so that few tokens cost little.  kGated: 64 gate and 64 up rows.  K is split over the CTAs of a cluster, whose partial sums meet
 // in shared memory, added in the order of the CTAs: no atomics, no workspace, and the same bits in every call.  They are sent in one copy to each
 // CTA; read by every thread from the others' shared memory instead, 64 tokens of the block took 22.5 us, stored there value by value 23.7.
-// One token, weights from HBM, replayed back to back: 8-bit 5120 x 4608 (23.6 MB) 7.4 us, 2304 x 5120 (11.8 MB) 5.4, 16-bit block (71 MB, two
-// launches) 18.4; 64 tokens 9.0, 7.0 and 21.3.  Of the 7.4: 2.3 until the first stage has come, 3.6 at 6.5 TB/s, 1-2 for the sums and the last CTAs.
+// One token, weights from HBM, replayed back to back: 8-bit 5120 x 4608 (23.6 MB) 7.4 us, 2304 x 5120 (11.8 MB) 4.3, 16-bit block (71 MB, two
+// launches) 17.9; 64 tokens 9.0, 6.3 and 21.2.  Of the 7.4: 2.3 until the first stage has come, 3.6 at 6.5 TB/s, 1-2 for the sums and the last CTAs.
 // The second product's weights requested ahead of its wait, beside the first product: 18.1 -> 19.8, so it does not.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 128;                         // rows of B per tile
 constexpr int kFewThreads = 256;
-constexpr int kFewMaxStages = 12;
+constexpr int kFewMaxStages = 10;                      // what fits beside 48 tokens; fewer tokens have half of an SM
 constexpr int kFewTokens = 160, kFewMaxTokens = 192;  // with the weights as they are stored; read along their rows (dense_few_tokens)
 constexpr int kFewMaxSplit = 8;
 constexpr int kFewSmem = 227 * 1024;
 constexpr int kFewControl = 2048, kFewApart = kFewControl + 1024;      // beside the stages: control block, and the slack for aligning the base
 // Half of an SM for each CTA: up to so many tokens, which need no more, so that the next launch's CTAs find room; and where there are more tiles than
 // SMs, so that one CTA's start and sums run beside another's products: 8-bit projection, 2304 x 20000, one token 14.7 -> 10.2 us, 128
-// tokens 19.7 -> 14.8; 5120 x 25000 27.4 -> 23.1 and 34.1 -> 28.9; 5120 x 152064, 1, 64 and 128 tokens 117 -> 116, 133 -> 137, 168 -> 154.  With 128
-// tiles, 8192 x 16384, 64 tokens 26.2 -> 29.4, so not there.
+// tokens 19.7 -> 14.8; 5120 x 25000 27.4 -> 23.1 and 34.1 -> 28.9; 5120 x 152064, 1, 64 and 128 tokens 117 -> 116, 133 -> 137, 168 -> 154 (the
+// one there that loses, 3 %, between two that gain).  With 128 tiles, 8192 x 16384, 64 tokens 26.2 -> 29.4, so not there.
 constexpr int kFewSmemHalf = 113 * 1024;
 constexpr int kFewHalfTokens = 32;
 
@@ -409,6 +411,8 @@ struct FewControl {
 static_assert(sizeof(FewControl) <= kFewControl, "control block");
 // sums of m tokens, padded to 16, and what the other CTAs send of those that this one finishes
 constexpr int few_sum_bytes(int m, int split) { return ((m + 15) / 16 * 16 + (split - 1) * ((m + split - 1) / split)) * kFewRows * 4; }
+static_assert((kFewSmem - kFewApart) / (kFewRows * 128 + (kFewHalfTokens + 16) * 128) == kFewMaxStages &&
+              (kFewSmemHalf - kFewApart) / (kFewRows * 128 + 16 * 128) <= kFewMaxStages, "stages of few tokens");
 static_assert(few_sum_bytes(kFewMaxTokens, 1) <= kFewSmem - kFewApart, "partial sums of a tile fit where the stages were");
 
 template <bool kInt8>
@@ -684,8 +688,10 @@ cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   const int smem = halves ? kFewSmemHalf : kFewSmem;
   d.stages = std::min((smem - kFewApart) / (kFewRows * 128 + d.tokens * 128), kFewMaxStages);
   // CTAs that share a tile's K: what a stage costs each of them, or the weights' bytes all, against what meeting costs, in clocks.  With 1, 2, 3, 4
-  // of them, 8-bit gated product 5120 x 4608: one token 10.2, 7.9, 7.4, 7.2 us, 16 tokens 10.4, 8.1, 7.7, 7.8, 64 tokens 11.4, 8.8, 9.1, - ; second
-  // product 2304 x 5120, 128 tokens: 8.8, 8.2, 8.7; 16-bit block, 144 tokens: 35.3, 27.0, 25.8.
+  // of them (- : do not fit at once), 8-bit gated product 5120 x 4608: one token 10.3, 8.0, 7.5, 7.4 us, 16 tokens 10.5, 8.3, 7.8, 7.9, 64 tokens
+  // 11.6, 8.95, 8.98, - , 128 tokens 13.2, 10.6, 11.1, - ; second product 2304 x 5120, one token 5.5, 4.6, 4.3, - , 16 tokens 5.7, 4.8, 4.45, - , 128
+  // tokens 8.6, 7.6, 7.9, - ; 16-bit block, one token 27.7, 19.8, 17.9, 17.6, 64 tokens 29.7, 21.9, 21.1, - , 144 tokens 35.4, 27.3, 25.9, - .  It takes
+  // 3 where the weights' bytes are the cost, 2 in the second product from 16 tokens on; at most 0.5 us from the best (128 tokens, gated).
   int dev = 0;
   cudaGetDevice(&dev);
   const int64_t from_hbm = (int64_t)p.n * (p.kind == kGated ? 2 : 1) * d.k_stages * 128 / 4450;

@@ -10,12 +10,13 @@ namespace mmoe {
 constexpr int kPairRows = 128;                        // rows of A per CTA
 constexpr int kPairCols = 256;                        // most rows of B per tile
 constexpr int kStageA = kPairRows * 128;              // bytes
-constexpr int kMaxStages = 10;
+constexpr int kMaxStages = 9;                         // what fits of the narrowest tiles, 64 columns
 constexpr int kEpiWarps = 8;                          // two per TMEM lane quadrant, each with every other block of columns
 constexpr int kEpiBlock = 32 * 32 * 4;                // a warp's 32 rows x 32 sums on their way from lanes to rows
 constexpr int kPairThreads = 32 * (2 + kEpiWarps);
 constexpr int kPairSmem = 227 * 1024;
 constexpr int kPairStageRoom = kPairSmem - 1024 - 1024 - kEpiWarps * kEpiBlock;
+static_assert(kPairStageRoom / (kStageA + 32 * 128) == kMaxStages, "stages of the narrowest tiles");
 
 // bytes of B that a stage of a tile holds in each CTA
 inline int stage_b_bytes(const DenseProduct& p, int cols) { return p.b.k_rows ? (cols / 2 + 63) / 64 * 8192 : cols / 2 * 128; }
