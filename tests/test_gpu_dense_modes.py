@@ -164,3 +164,45 @@ def test_sizes_past_32_bits_are_refused():
         with pytest.raises(ValueError):
             api.prepare_int8_inputs(x[:, :1].expand(1, tokens))
     assert torch.cuda.memory_allocated() == held
+
+
+def test_a_first_call_of_the_quantiser_in_a_capture():
+    """The one operator that needs no preparation."""
+    _fresh("""
+import torch
+from vllm_plugin_b200 import api
+x = torch.randn(5, 64, device="cuda").bfloat16()
+many = torch.randn(600, 64, device="cuda").half()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    q, s = api.prepare_int8_inputs(x)
+    q2, s2 = api.prepare_int8_inputs(many)
+graph.replay()
+torch.cuda.synchronize()
+want, want2 = api.prepare_int8_inputs(x), api.prepare_int8_inputs(many)
+assert torch.equal(q, want[0]) and torch.equal(s, want[1]) and torch.equal(q2, want2[0]) and torch.equal(s2, want2[1])
+print("ok")
+""")
+
+
+def test_a_first_call_of_the_others_in_a_capture_is_refused():
+    _fresh("""
+import torch
+from vllm_plugin_b200 import api
+x, w13, w2 = (torch.randn(s, device="cuda").bfloat16() for s in ((5, 64), (64, 64), (64, 32)))
+refused = 0
+with torch.cuda.graph(torch.cuda.CUDAGraph()):
+    try:
+        api.gated_feed_forward(x, w13, w2)
+    except RuntimeError:
+        refused += 1
+y = api.gated_feed_forward(x, w13, w2)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    z = api.gated_feed_forward(x, w13, w2)
+graph.replay()
+torch.cuda.synchronize()
+assert refused == 1 and torch.equal(y, z)
+api.read_dense_status()
+print("ok")
+""")
