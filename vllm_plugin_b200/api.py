@@ -119,7 +119,8 @@ def gated_feed_forward(x, w13, w2, *, activation_clamp: Optional[float] = None):
     pass (in FP16 they overflow past 65504); g and u themselves are kept for it in FP32.  A value on the border of the clamp passes its gradient, one beyond it does not.
     First derivatives only, in backward mode.  Tangents and traces (``torch.jit.trace``, ``make_fx``) are refused by all dense operators,
     ``NotImplementedError``.  A training step can be captured into a CUDA graph behind a first call, but not while the graph of an eager
-    call with the same leaves on the default stream is alive (``RuntimeError``); warm up on another stream, as PyTorch asks for anyway."""
+    call with the same leaves on the default stream is alive (``RuntimeError``); warm up on another stream, as PyTorch asks for anyway
+    (graphs of other operators with the same leaves end a capture as they do in PyTorch; they are not looked for)."""
     global _feed_forward
     if _feed_forward is None:
         from .backend.dense import gated_feed_forward as _feed_forward

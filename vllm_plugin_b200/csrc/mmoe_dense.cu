@@ -369,8 +369,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) dense_pair_kernel(const __gri
 // operand B, so that few tokens cost little.  kGated: 64 gate and 64 up rows.  K is split over the CTAs of a cluster, whose partial sums meet
 // in shared memory, added in the order of the CTAs: no atomics, no workspace, and the same bits in every call.  They are sent in one copy to each
 // CTA; read by every thread from the others' shared memory instead, 64 tokens of the block took 22.5 us, stored there value by value 23.7.
-// One token, weights from HBM, replayed back to back: 8-bit 5120 x 4608 (23.6 MB) 7.4 us, 2304 x 5120 (11.8 MB) 4.3, 16-bit block (71 MB, two
-// launches) 17.9; 64 tokens 9.0, 6.3 and 21.2.  Of the 7.4: 2.3 until the first stage has come, 3.6 at 6.5 TB/s, 1-2 for the sums and the last CTAs.
+// One token, weights from HBM, replayed back to back: 8-bit 5120 x 4608 (23.6 MB) 7.4 us, 2304 x 5120 (11.8 MB) 5.4, 16-bit block (71 MB, two
+// launches) 17.9; 64 tokens 9.0, 7.0 and 21.2.  Of the 7.4: 2.3 until the first stage has come, 3.6 at 6.5 TB/s, 1-2 for the sums and the last CTAs.
 // The second product's weights requested ahead of its wait, beside the first product: 18.1 -> 19.8, so it does not.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 128;                         // rows of B per tile
@@ -689,8 +689,8 @@ cudaError_t launch_few(const DenseProduct& p, int sms, cudaStream_t s) {
   d.stages = std::min((smem - kFewApart) / (kFewRows * 128 + d.tokens * 128), kFewMaxStages);
   // CTAs that share a tile's K: what a stage costs each of them, or the weights' bytes all, against what meeting costs, in clocks.  With 1, 2, 3, 4
   // of them (- : do not fit at once), 8-bit gated product 5120 x 4608: one token 10.3, 8.0, 7.5, 7.4 us, 16 tokens 10.5, 8.3, 7.8, 7.9, 64 tokens
-  // 11.6, 8.95, 8.98, - , 128 tokens 13.2, 10.6, 11.1, - ; second product 2304 x 5120, one token 5.5, 4.6, 4.3, - , 16 tokens 5.7, 4.8, 4.45, - , 128
-  // tokens 8.6, 7.6, 7.9, - ; 16-bit block, one token 27.7, 19.8, 17.9, 17.6, 64 tokens 29.7, 21.9, 21.1, - , 144 tokens 35.4, 27.3, 25.9, - .  It takes
+  // 11.6, 8.95, 8.98, - , 128 tokens 13.2, 10.6, 11.1, - ; second product 2304 x 5120, one token 6.3, 5.55, 5.4, - , 32 tokens 7.2, 6.3, 5.9, - , 128
+  // tokens 9.15, 8.3, 9.0, - ; 16-bit block, one token 27.7, 19.8, 17.9, 17.6, 64 tokens 29.7, 21.9, 21.1, - , 144 tokens 35.4, 27.3, 25.9, - .  It takes
   // 3 where the weights' bytes are the cost, 2 in the second product from 16 tokens on; at most 0.5 us from the best (128 tokens, gated).
   int dev = 0;
   cudaGetDevice(&dev);
