@@ -345,6 +345,87 @@ int mmoe_int8_gated_projection(const MmoeInt8Product* p, void* stream);
 /* mmoe_read_status for the words of these calls. */
 int mmoe_dense_read_status(int32_t* status, int32_t* words8, void* stream);
 
+/* ---- Products of a layer's experts beside the MXFP8 x MXFP4 layer (no counterpart in the reference): rows that are grouped by expert, in 16 bits with
+ * their gradients, and products in 8-bit floating point with block scales, of such rows or of all rows by one weight.  As above: no workspace, no
+ * geometry, `status` words (kernels 33 and 34), mmoe_dense_prepare() first.
+ * `ends`: int32 [num_experts] device words; the rows of expert e end before row ends[e] and begin where those of e - 1 end, with row 0 for the first.
+ * An expert may have no rows.  Rows from the last end on belong to no expert: their outputs and gradients are zero.  Ends that fall, are
+ * negative or pass num_rows: no row is an expert's, and the launch is counted in word [4] of `status`. */
+enum { MMOE_E4M3 = 4 };
+
+/* y[t, n] = sum_k x[t, k] w[e][n, k] for the rows t of expert e */
+typedef struct MmoeGroupedProduct {
+  int32_t type;               /* MMOE_BF16 or MMOE_FP16: x, w, out and their gradients */
+  int32_t num_rows;           /* T */
+  int32_t num_experts;        /* E, 1 to 1024 */
+  int32_t width;              /* K, a multiple of 8, at most 2^20 */
+  int32_t channels;           /* N, a multiple of 8, at most 2^20 */
+  int32_t timeout_ms;         /* as above */
+  int64_t x_stride;           /* elements between the rows of x, >= K and a multiple of 8 */
+  const void* x;              /* [T, K] */
+  const void* w;              /* [E, N, K] */
+  const int32_t* ends;        /* [E] */
+  void* out;                  /* [T, N] */
+  int32_t* status;
+} MmoeGroupedProduct;
+int mmoe_grouped_projection(const MmoeGroupedProduct* p, void* stream);
+/* Gradients from dy [T, N] (contiguous): dx [T, K], dw [E, N, K] (zero for experts without rows); NULL where not wanted.  p->out is not used. */
+int mmoe_grouped_projection_grad(const MmoeGroupedProduct* p, const void* dy, void* dx, void* dw, void* stream);
+
+/* mmoe_feed_forward with the weights of each row's expert */
+typedef struct MmoeGroupedFeedForward {
+  int32_t type;               /* MMOE_BF16 or MMOE_FP16 */
+  int32_t num_rows;           /* T */
+  int32_t num_experts;        /* E, 1 to 1024 */
+  int32_t hidden;             /* H, a multiple of 8, at most 2^20 */
+  int32_t intermediate;       /* I, a multiple of 8, at most 2^20 */
+  float clamp;                /* +inf: none */
+  int32_t timeout_ms;         /* as above */
+  int32_t reserved;
+  int64_t x_stride;           /* elements between the rows of x, >= H and a multiple of 8 */
+  const void* x;              /* [T, H] */
+  const void* w13;            /* [E, 2I, H], the gate's rows first */
+  const void* w2;             /* [E, H, I] */
+  const int32_t* ends;        /* [E] */
+  void* h;                    /* [T, I], rounded to the type; rows of no expert are left as they were */
+  float* preact;              /* float [T, 2I] for the backward call, likewise; NULL: not kept */
+  void* y;                    /* [T, H] */
+  int32_t* status;
+} MmoeGroupedFeedForward;
+int mmoe_grouped_feed_forward(const MmoeGroupedFeedForward* ff, void* stream);
+/* As mmoe_feed_forward_grad: dpre [T, 2I] scratch, dx [T, H], dw13 [E, 2I, H], dw2 [E, H, I]. */
+int mmoe_grouped_feed_forward_grad(const MmoeGroupedFeedForward* ff, const void* dy, void* dpre, void* dx, void* dw13, void* dw2, void* stream);
+
+/* Quantiser: for each 128 values of a row (the last group may have fewer) scale = max|x| / 448 (1 for zeros), q = x / scale to the nearest E4M3 value,
+ * ties to even, by that scale as it is in FP32.  A group that holds an infinity or a NaN gets the scale NaN and zeros.  x: `type` BF16 or FP16,
+ * [M, K] with `x_stride` elements between rows, any K; q [M, K]; scales float [M, ceil(K / 128)]. */
+int mmoe_quantize_fp8(const void* x, int32_t type, int64_t x_stride, void* q, float* scales, int32_t num_rows, int32_t width, void* stream);
+
+/* Products of E4M3 values with FP32 scales; sums over 128 values in the tensor core, over those in FP32. */
+typedef struct MmoeFp8Product {
+  int32_t num_rows;           /* T */
+  int32_t num_experts;        /* E, 1 to 1024; 1 without ends */
+  int32_t width;              /* K, a multiple of 16, at most 2^20 */
+  int32_t channels;           /* N, at most 2^20: rows of w (projection), or half of them (gated: a multiple of 8) */
+  int32_t out_type;           /* MMOE_BF16, MMOE_FP16 or MMOE_FP32 */
+  float clamp;                /* gated only; +inf: none */
+  int32_t timeout_ms;         /* as above */
+  int32_t reserved;
+  int64_t x_stride;           /* bytes between the rows of x, >= K and a multiple of 16 */
+  const void* x;              /* E4M3 [T, K] */
+  const float* x_scales;      /* [T, ceil(K / 128)] */
+  const void* w;              /* E4M3 [E, N, K]; gated: [E, 2N, K], the gate's rows first */
+  const float* w_scales;      /* [E, ceil(N / 128), ceil(K / 128)], one for each block of 128 x 128; gated: [E, 2 ceil(N / 128), ...], the blocks of the
+                                 gate's rows first, those of the up rows begun anew */
+  const int32_t* ends;        /* [E]; NULL: all rows are expert 0's */
+  void* out;                  /* [T, N], contiguous */
+  int32_t* status;
+} MmoeFp8Product;
+/* out = sum over groups of 128 k's of (x w^T of the group) * x_scales * w_scales */
+int mmoe_fp8_projection(const MmoeFp8Product* p, void* stream);
+/* g and u as above; out = silu(min(g, clamp)) * clip(u, -clamp, clamp) */
+int mmoe_fp8_gated_projection(const MmoeFp8Product* p, void* stream);
+
 /* Process-wide tuning of the tensor-core kernels (the reference keeps such knobs in `KernelOptions`,
  * backend/frontend.py:72-116).  `max_stages`: cap on the shared-memory pipeline depth of the weights-as-A kernels (0: no
  * cap).  `orientation`: 0 = chosen per expert from the rows it received (weights-as-A kernels for few rows, tokens-as-A

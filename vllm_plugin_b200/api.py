@@ -13,6 +13,7 @@ from typing import Any, Optional, Tuple, Union
 # implementations of the per-step functions, looked up once (a function-local import costs about a microsecond per call)
 _mega_moe = _stage = _route_and_stage = None
 _feed_forward = _quantize_int8 = _int8_projection = _int8_gated_projection = None
+_grouped_projection = _grouped_feed_forward = _quantize_fp8 = _fp8_projection = _fp8_gated_projection = None
 
 
 def get_symm_buffer_for_mega_moe(group, num_experts: int, num_max_tokens_per_rank: int, num_topk: int, hidden: int,
@@ -158,8 +159,73 @@ def int8_gated_projection(x, x_scales, w13, w13_scales, *, activation_clamp: Opt
     return _int8_gated_projection(x, x_scales, w13, w13_scales, activation_clamp=activation_clamp, out_dtype=out_dtype)
 
 
+def grouped_projection(x, w, ends):
+    """Product of rows that are grouped by expert with their expert's weights, with its gradients (no counterpart in the reference):
+    ``y[t] = w[e] x[t]``.
+
+    ``x``: BF16 or FP16 ``(T, K)``, any strides (rows that are not dense or do not start on 16 bytes are copied), the rows of expert 0
+    first.  ``w``: ``(E, N, K)``, contiguous, on 16 bytes and of x's type; K and N multiples of 8, at most 2^20; at most 1024 experts.
+    ``ends``: int32 ``(E,)`` on the device, ``torch.cumsum(counts, 0, dtype=torch.int32)``: expert e's rows end before ``ends[e]`` and begin where those of
+    the one before end.  An expert may have no rows.  Rows behind the last expert's get zeros, in the output and in x's gradient, whatever they hold.
+    Returns ``(T, N)`` of x's type.
+
+    The kernels read ``ends``; nothing comes back to the host.  A call that is captured into a CUDA graph goes by what they hold at each
+    replay.  Where they fall, are negative or pass T, no row is taken to be an expert's (all results are zero), and a later call or :func:`read_dense_status`
+    raises ``AssertionError``.
+
+    Sums are FP32, rounded once.  Gradients, captures, tangents and traces as for :func:`gated_feed_forward`; the gradient of an expert without rows is
+    zero.  The same bits in every call."""
+    global _grouped_projection
+    if _grouped_projection is None:
+        from .backend.grouped import grouped_projection as _grouped_projection
+    return _grouped_projection(x, w, ends)
+
+
+def grouped_feed_forward(x, w13, w2, ends, *, activation_clamp: Optional[float] = None):
+    """:func:`gated_feed_forward` with the weights of each row's expert, with its gradients: ``x`` ``(T, H)``, ``w13`` ``(E, 2 I, H)`` in checkpoint order, the
+    gate's rows first, ``w2`` ``(E, H, I)``; rows and ``ends`` as in :func:`grouped_projection`.  Returns ``(T, H)``."""
+    global _grouped_feed_forward
+    if _grouped_feed_forward is None:
+        from .backend.grouped import grouped_feed_forward as _grouped_feed_forward
+    return _grouped_feed_forward(x, w13, w2, ends, activation_clamp=activation_clamp)
+
+
+def prepare_fp8_inputs(hidden_states, out=None):
+    """Quantiser of BF16 or FP16 hidden states ``(..., K)`` by groups of 128 values; returns ``(float8_e4m3fn (..., K), float32 scales (..., ceil(K / 128)))``.
+    ``scale = max|x| / 448`` (1 for a group of zeros), values ``x / scale`` rounded to the nearest, ties to even.  A group that holds an infinity or a
+    NaN gets the scale NaN and zeros, so that what is computed from it is NaN.  ``out``: the two tensors, contiguous."""
+    global _quantize_fp8
+    if _quantize_fp8 is None:
+        from .backend.grouped import prepare_fp8_inputs as _quantize_fp8
+    return _quantize_fp8(hidden_states, out)
+
+
+def fp8_projection(x, x_scales, w, w_scales, *, ends=None, out_dtype=None):
+    """Product in 8-bit floating point with a scale for each 128 values of a row and each block of 128 x 128 weights: ``y[t, n] = sum_k x[t, k] sx[t, k / 128]
+    w[n, k] sw[n / 128, k / 128]``.  ``x``: float8_e4m3fn ``(..., K)`` with float32 scales ``(..., ceil(K / 128))`` (:func:`prepare_fp8_inputs`); ``w``:
+    float8_e4m3fn ``(N, K)``, contiguous and on 16 bytes, with ``(ceil(N / 128), ceil(K / 128))``; K a multiple of 16, K and N at most 2^20.  With
+    ``ends`` rows are grouped by expert as in :func:`grouped_projection`: ``x`` ``(T, K)``, ``w`` ``(E, N, K)``, ``w_scales`` ``(E, ..., ...)``.  ``out_dtype``:
+    BF16 (default), FP16 or FP32.  Scales may be any numbers; each sum over 128 values is multiplied by their product and added in FP32.  No gradient."""
+    global _fp8_projection
+    if _fp8_projection is None:
+        from .backend.grouped import fp8_projection as _fp8_projection
+    return _fp8_projection(x, x_scales, w, w_scales, ends=ends, out_dtype=out_dtype)
+
+
+def fp8_gated_projection(x, x_scales, w13, w13_scales, *, ends=None, activation_clamp: Optional[float] = None, out_dtype=None):
+    """The first half of a gated feed-forward block in 8-bit floating point: both products (``w13`` ``(2 I, K)``, the gate's rows first, I a multiple of 8, scales
+    ``(2 ceil(I / 128), ceil(K / 128))``, the gate's blocks first and those of the up rows begun anew), the activation and their product in one
+    kernel, ``silu(min(g, c)) * clip(u, -c, c)`` in ``(..., I)``.  Quantise it with :func:`prepare_fp8_inputs` for :func:`fp8_projection`.  Otherwise as there; the
+    activation as in :func:`int8_gated_projection`."""
+    global _fp8_gated_projection
+    if _fp8_gated_projection is None:
+        from .backend.grouped import fp8_gated_projection as _fp8_gated_projection
+    return _fp8_gated_projection(x, x_scales, w13, w13_scales, ends=ends, activation_clamp=activation_clamp, out_dtype=out_dtype)
+
+
 def read_dense_status(device=None) -> None:
-    """:func:`read_status` of the dense operators' calls on ``device`` (default: the current one)."""
+    """:func:`read_status` of the dense and grouped operators' calls on ``device`` (default: the current one): ``RuntimeError`` for a wait that
+    expired, ``AssertionError`` for ``ends`` that were not in order."""
     from .backend.dense import read_dense_status as _impl
 
     return _impl(device)
@@ -240,4 +306,5 @@ __all__ = [
     "precompile_mega_moe_variants", "set_kernel_options", "get_kernel_options", "is_localization_available",
     "get_balanced_sm_locality_domains", "localize", "localize_mega_moe_weights", "read_status", "SymmBuffer",
     "gated_feed_forward", "prepare_int8_inputs", "int8_projection", "int8_gated_projection", "read_dense_status",
+    "grouped_projection", "grouped_feed_forward", "prepare_fp8_inputs", "fp8_projection", "fp8_gated_projection",
 ]

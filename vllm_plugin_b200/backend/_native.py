@@ -36,6 +36,8 @@ EXPORTED_SYMBOLS = (
     "mmoe_combine_residual", "mmoe_split_halves",
     "mmoe_dense_prepare", "mmoe_feed_forward", "mmoe_feed_forward_grad", "mmoe_quantize_int8", "mmoe_int8_projection",
     "mmoe_int8_gated_projection", "mmoe_dense_read_status",
+    "mmoe_grouped_projection", "mmoe_grouped_projection_grad", "mmoe_grouped_feed_forward", "mmoe_grouped_feed_forward_grad", "mmoe_quantize_fp8",
+    "mmoe_fp8_projection", "mmoe_fp8_gated_projection",
 )
 
 
@@ -80,7 +82,25 @@ class MmoeInt8Product(ctypes.Structure):
         (n, ctypes.c_void_p) for n in ("x", "x_scales", "w", "w_scales", "bias", "out", "status")]
 
 
-MMOE_BF16, MMOE_FP16, MMOE_INT8, MMOE_FP32 = range(4)
+class MmoeGroupedProduct(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("type", "num_rows", "num_experts", "width", "channels", "timeout_ms")] + [
+        ("x_stride", ctypes.c_int64)] + [(n, ctypes.c_void_p) for n in ("x", "w", "ends", "out", "status")]
+
+
+class MmoeGroupedFeedForward(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("type", "num_rows", "num_experts", "hidden", "intermediate")] + [
+        ("clamp", ctypes.c_float), ("timeout_ms", ctypes.c_int32), ("reserved", ctypes.c_int32), ("x_stride", ctypes.c_int64)] + [
+        (n, ctypes.c_void_p) for n in ("x", "w13", "w2", "ends", "h", "preact", "y", "status")]
+
+
+class MmoeFp8Product(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("num_rows", "num_experts", "width", "channels", "out_type")] + [
+        ("clamp", ctypes.c_float), ("timeout_ms", ctypes.c_int32), ("reserved", ctypes.c_int32), ("x_stride", ctypes.c_int64)] + [
+        (n, ctypes.c_void_p) for n in ("x", "x_scales", "w", "w_scales", "ends", "out", "status")]
+
+
+MMOE_BF16, MMOE_FP16, MMOE_INT8, MMOE_FP32, MMOE_E4M3 = range(5)
+MOST_EXPERTS, MOST_GROUPED_WIDTH = 1024, 1 << 20
 
 _lib: Optional[ctypes.CDLL] = None
 _raw_stream = None
@@ -145,6 +165,14 @@ def load() -> ctypes.CDLL:
     lib.mmoe_int8_projection.argtypes = [i8_p, vp]
     lib.mmoe_int8_gated_projection.argtypes = [i8_p, vp]
     lib.mmoe_dense_read_status.argtypes = [vp, ctypes.POINTER(i32), vp]
+    gp_p, gf_p, f8_p = ctypes.POINTER(MmoeGroupedProduct), ctypes.POINTER(MmoeGroupedFeedForward), ctypes.POINTER(MmoeFp8Product)
+    lib.mmoe_grouped_projection.argtypes = [gp_p, vp]
+    lib.mmoe_grouped_projection_grad.argtypes = [gp_p, vp, vp, vp, vp]
+    lib.mmoe_grouped_feed_forward.argtypes = [gf_p, vp]
+    lib.mmoe_grouped_feed_forward_grad.argtypes = [gf_p, vp, vp, vp, vp, vp, vp]
+    lib.mmoe_quantize_fp8.argtypes = [vp, i32, ctypes.c_int64, vp, vp, i32, i32, vp]
+    lib.mmoe_fp8_projection.argtypes = [f8_p, vp]
+    lib.mmoe_fp8_gated_projection.argtypes = [f8_p, vp]
     for name in EXPORTED_SYMBOLS:
         fn = getattr(lib, name)
         if fn.restype is not ctypes.c_char_p:

@@ -35,7 +35,8 @@ class _Device:
         with torch.inference_mode(False):    # kept for calls in any mode, whatever the first one runs in
             self.status = torch.zeros(8, dtype=torch.int32, device=device)
         self.status_ptr = self.status.data_ptr()
-        self.poll = _f._StatusPoll(self, "dense operator's call")
+        self.poll = _f._StatusPoll(self, "dense operator's call", "launches of earlier grouped operators had ends that fall or pass the last row: "
+                                                                  "no row was taken to be an expert's")
         self.calls = self.due = 0            # launching calls so far, and the one at which to look at the words ...
         self.options = None                  # ... by these options
 
@@ -107,8 +108,8 @@ def _watch(state: _Device, options) -> None:
 
 
 def read_dense_status(device=None) -> None:
-    """Synchronise and raise ``RuntimeError`` if a device-side wait of a dense operator expired on ``device`` since the last
-    read; clears the condition."""
+    """Synchronise and raise ``RuntimeError`` if a device-side wait of a dense or grouped operator expired on ``device`` since the last
+    read, ``AssertionError`` if the ``ends`` of a grouped one were not in order; clears the condition."""
     _f.require_sm100()
     index = torch.device("cuda" if device is None else device).index
     index = torch.cuda.current_device() if index is None else index
@@ -297,7 +298,7 @@ class _Block(torch.autograd.Function):
 _Block._once = staticmethod(once_differentiable(_Block._gradients))
 
 
-def _refuse_beside_eager_graph(inputs) -> None:
+def _refuse_beside_eager_graph(inputs, what: str = "gated_feed_forward") -> None:
     """The node that accumulates a leaf's gradient belongs to the stream on which the first live graph made it.  A captured backward
     pass lets that stream wait for its own, which takes it into the capture; a default stream cannot be captured, and the process would
     end.  Graphs made on other streams, as by a warm-up, are no obstacle."""
@@ -305,8 +306,8 @@ def _refuse_beside_eager_graph(inputs) -> None:
         return
     mine = _accumulators([torch.autograd.graph.get_gradient_edge(t).node for t in inputs if t.requires_grad])
     if mine & _accumulators(_live_graphs()):
-        raise RuntimeError("a graph of an eager gated_feed_forward call with the same leaves on the default stream is still alive: "
-                           "drop its output before the call is captured for training")
+        raise RuntimeError("a graph of an eager call of gated_feed_forward, grouped_feed_forward or grouped_projection with the same leaves on the "
+                           f"default stream is still alive: drop its output before the call of {what} is captured for training")
 
 
 def _accumulators(nodes) -> set:

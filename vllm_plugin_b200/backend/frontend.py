@@ -273,10 +273,10 @@ def _keep_record(records: Dict[Tuple[int, int], _CallRecord], key: Tuple[int, in
 class _StatusPoll:
     """Non-blocking watch on the device status words of one buffer: every ``interval`` eager calls the words are copied
     to pinned host memory behind the call; a later call that finds the copy complete inspects it.  ``what`` names the calls
-    in its message."""
+    in its message, ``bad`` what their word [4] counts."""
 
-    def __init__(self, sym_buffer, what: str = "MegaMoE call"):
-        self.what = what
+    def __init__(self, sym_buffer, what: str = "MegaMoE call", bad: str = "expert ids of an earlier MegaMoE call were >= num_experts"):
+        self.what, self.bad = what, bad
         with torch.inference_mode(False):              # kept for calls in any mode, whatever this one runs in
             self.host = torch.zeros(8, dtype=torch.int32).pin_memory()
         self.event = torch.cuda.Event()
@@ -292,7 +292,7 @@ class _StatusPoll:
                 if words[0] != 0:
                     raise RuntimeError(f"a device-side wait of an earlier {self.what} expired (kernel {words[1]}, role "
                                        f"{words[2]}, block {words[3]}): its output is not valid")
-                raise AssertionError(f"{words[4]} expert ids of an earlier MegaMoE call were >= num_experts")
+                raise AssertionError(f"{words[4]} {self.bad}")
 
     def after_call(self, sym_buffer, interval: int) -> None:
         self.calls += 1

@@ -3,9 +3,8 @@
 #include <atomic>
 #include <type_traits>
 
-#include "mmoe_dense.cuh"
+#include "mmoe_dense_device.cuh"
 #include "mmoe_dense_rules.h"
-#include "mmoe_tc.cuh"
 
 namespace mmoe {
 
@@ -26,8 +25,6 @@ namespace {
 // gradients 133 (dh with dw2, 1.37) and 226 (dx with dw13, 1.60; tensor pipe active 96 %); 8-bit gated product 60 (3.0), second 34 (2.6).
 // A launch of one turn has 1.3-1.6 us in front of its first products and 1.2-4 us of epilogue behind its last.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int kStatusDense = 31;
-
 // One product of a launch
 struct DensePart {
   CUtensorMap map_a, map_b;
@@ -57,58 +54,7 @@ struct PairControl {
   volatile int32_t abort_flag;
 };
 
-// Waits with a limit each, which counts from a wait's 64th probe on: a launch may take as long as its size asks for.  (The layer's limit is one for a
-// whole launch, which its buffers bound.)  What waits for a whole tile or for all of a CTA's K says how many stages that are: kStageNs, many times what
-// one takes, is added for each.
-constexpr int64_t kStageNs = 10000;
-struct DenseWaiter {
-  Waiter wait;               // its deadline is that of the wait under way
-  int64_t limit_ns;
-  __device__ __forceinline__ bool late(uint32_t spin, int stages) {
-    if (spin != 63u) return wait.abandoned();
-    wait.deadline = global_timer() + static_cast<uint64_t>(limit_ns + stages * kStageNs);
-    return *wait.abort_flag != 0;
-  }
-  // both by the whole warp; true when the phase has completed, false when the call is being abandoned (see Waiter for why two)
-  __device__ __forceinline__ bool wait_uniform(uint32_t bar, uint32_t parity) {
-    for (uint32_t spin = 0;; ++spin) {
-      if (__any_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-      if ((spin & 63u) == 63u && __any_sync(0xffffffffu, late(spin, 0))) return false;
-    }
-  }
-  __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int stages) {
-    if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
-    bool ok = true;
-    if ((threadIdx.x & 31) == 0)
-      for (uint32_t spin = 0;; ++spin) {
-        if (mbar_try_wait(bar, parity)) break;
-        if ((spin & 63u) == 63u && late(spin, stages)) { ok = false; break; }
-      }
-    return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-  }
-};
-
 static_assert(sizeof(PairControl) <= 1024, "control block");
-
-// descriptor without its address: 128-byte swizzle; K-major: eight-row groups 1024 bytes apart.  MN-major: groups of eight k's 1024 bytes
-// apart, blocks of 64 rows `block` bytes apart.
-__device__ __forceinline__ uint64_t operand_desc(bool mn_major, uint32_t block) {
-  return desc_hi_sw128() | (mn_major ? static_cast<uint64_t>(block >> 4) << 16 : 0ull);
-}
-
-__device__ __forceinline__ void prefetch_bulk(const void* p, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
-}
-
-template <bool kInt8>
-__device__ __forceinline__ void pair_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  if (kInt8)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-  else
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
 
 // The t-th tile of a product: eight tiles of rows at a time, all columns of those before the next eight, so that what runs at once reads few
 // different rows of either operand.
@@ -415,25 +361,6 @@ static_assert((kFewSmem - kFewApart) / (kFewRows * 128 + (kFewHalfTokens + 16) *
               (kFewSmemHalf - kFewApart) / (kFewRows * 128 + 16 * 128) <= kFewMaxStages, "stages of few tokens");
 static_assert(few_sum_bytes(kFewMaxTokens, 1) <= kFewSmem - kFewApart, "partial sums of a tile fit where the stages were");
 
-template <bool kInt8>
-__device__ __forceinline__ void single_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  if (kInt8)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-  else
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-
-// shared memory of this CTA to that of another one of the cluster, counted on a barrier there
-__device__ __forceinline__ void cluster_send(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "r"(src), "r"(bytes), "r"(bar) : "memory");
-}
-
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
 // adds eight neighbouring sums; `swap`: second half first, so that eight lanes read all banks
 template <bool kInt8>
 __device__ __forceinline__ void add_part(const uint8_t* at, bool swap, float (&v)[8], int32_t (&whole)[8]) {
@@ -614,23 +541,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) dense_few_kernel(const __grid_
 // ---------------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------------
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 std::atomic<EncodeFn> g_encode{nullptr};
-constexpr int kMaxDevices = 64;
 std::atomic<int> g_sms[kMaxDevices];        // per device, 0: prepare_dense() has not run there
-
-int prepared_sms() {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
-  // tensor maps are encoded by the driver, which wants the device's context on this thread; one that has launched nothing yet has none
-  thread_local int bound = -1;
-  if (bound != dev) {
-    if (cudaSetDevice(dev) != cudaSuccess) return 0;
-    bound = dev;
-  }
-  return g_sms[dev].load();
-}
 
 // `rows` x k matrix; boxes of 128 bytes of K by `box` rows, or (stored transposed) of 64 rows by 64 k's
 bool encode(CUtensorMap* map, const DenseOperand& o, int type, uint64_t rows, uint64_t k, uint32_t box) {
@@ -642,14 +554,6 @@ bool encode(CUtensorMap* map, const DenseOperand& o, int type, uint64_t rows, ui
   const CUtensorMapDataType t = type == kDenseInt8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type == kDenseBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   return g_encode.load()(map, t, 2, const_cast<void*>(o.p), dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// Instruction descriptor: [4,6) sums (1 FP32, 2 32-bit integers), [7,10) and [10,13) operands (16 bits: 0 FP16, 1 BF16; 8 bits: 1 signed),
-// [15], [16] MN-major operands, [17,23) N >> 3, [24,29) M >> 4.
-uint32_t product_idesc(int type, bool a_mn, bool b_mn, int rows, int cols) {
-  const uint32_t format = type == kDenseFp16 ? 0 : 1;
-  return ((type == kDenseInt8 ? 2u : 1u) << 4) | (format << 7) | (format << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
-         (static_cast<uint32_t>(cols >> 3) << 17) | (static_cast<uint32_t>(rows >> 4) << 24);
 }
 
 template <typename F>
@@ -889,6 +793,20 @@ cudaError_t launch_quantize(const void* x, int64_t ld, int8_t* q, float* scales,
 
 }  // namespace
 
+int dense_sms() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+  // tensor maps are encoded by the driver, which wants the device's context on this thread; one that has launched nothing yet has none
+  thread_local int bound = -1;
+  if (bound != dev) {
+    if (cudaSetDevice(dev) != cudaSuccess) return 0;
+    bound = dev;
+  }
+  return g_sms[dev].load();
+}
+
+EncodeFn dense_encoder() { return g_encode.load(); }
+
 cudaError_t prepare_dense() {
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -931,7 +849,7 @@ cudaError_t prepare_dense() {
 bool dense_few_tokens(const DenseProduct& p) { return !p.a.k_rows && p.m <= (p.b.k_rows ? kFewMaxTokens : kFewTokens); }
 
 cudaError_t launch_dense(const DenseProduct* p, int parts, cudaStream_t s) {
-  const int sms = prepared_sms();
+  const int sms = dense_sms();
   if (sms == 0) return cudaErrorNotReady;
   const ChainScope chain(true);
   return parts == 1 && dense_few_tokens(*p) ? launch_few(*p, sms, s) : launch_pairs(p, parts, sms, s);

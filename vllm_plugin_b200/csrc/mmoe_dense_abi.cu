@@ -1,28 +1,11 @@
 // extern "C" entry points of the dense feed-forward operators (declared in include/mmoe.h): argument checks and the products of a call.
 // Nothing here allocates device memory; only mmoe_dense_read_status synchronises.
-#include <stdarg.h>
-#include <stdio.h>
 #include <string.h>
 
-#include "mmoe_dense.cuh"
+#include "mmoe_dense_abi.h"
+#include "mmoe_grouped.cuh"
 
 namespace {
-
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  va_end(ap);
-  return mmoe::record_failure(code, buf);
-}
-
-int cuda_fail(cudaError_t e, const char* what) { return fail(MMOE_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e)); }
-
-// row and column indexes, rounded up to a tile, are 32-bit numbers
-constexpr int32_t kMostTokens = 1 << 30, kMostChannels = 1 << 29;
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int check_feed_forward(const MmoeFeedForward* f) {
   if (f == nullptr) return fail(MMOE_ERR_INVALID_ARGUMENT, "feed-forward: arguments are NULL");
@@ -92,6 +75,7 @@ int mmoe_dense_prepare(void* stream) {
   if (e != cudaSuccess) return cuda_fail(e, "dense_prepare");
   if (cap != cudaStreamCaptureStatusNone) return fail(MMOE_ERR_NOT_PREPARED, "mmoe_dense_prepare() must run before stream capture");
   e = mmoe::prepare_dense();
+  if (e == cudaSuccess) e = mmoe::prepare_grouped();
   return e == cudaSuccess ? MMOE_OK : cuda_fail(e, "dense_prepare");
 }
 
@@ -207,6 +191,9 @@ int mmoe_dense_read_status(int32_t* status, int32_t* words8, void* stream) {
   if (host[mmoe::kStatusTimeout] != 0)
     return fail(MMOE_ERR_DEVICE_TIMEOUT, "device wait expired: kernel %d role %d block %d", host[mmoe::kStatusKernel],
                 host[mmoe::kStatusRole], host[mmoe::kStatusBlock]);
+  if (host[mmoe::kStatusBadIndex] != 0)
+    return fail(MMOE_ERR_INVALID_ARGUMENT, "%d launches with ends of groups that fall or pass the last row: no row was taken to be an expert's",
+                host[mmoe::kStatusBadIndex]);
   return MMOE_OK;
 }
 
