@@ -76,6 +76,7 @@ int mmoe_dense_prepare(void* stream) {
   if (cap != cudaStreamCaptureStatusNone) return fail(MMOE_ERR_NOT_PREPARED, "mmoe_dense_prepare() must run before stream capture");
   e = mmoe::prepare_dense();
   if (e == cudaSuccess) e = mmoe::prepare_grouped();
+  if (e == cudaSuccess) e = mmoe::prepare_fp8();
   return e == cudaSuccess ? MMOE_OK : cuda_fail(e, "dense_prepare");
 }
 

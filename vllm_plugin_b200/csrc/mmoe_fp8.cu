@@ -1,0 +1,483 @@
+// Products in 8-bit floating point with block scales for sm_100a (see mmoe_grouped.cuh), and the quantiser in front of them.
+#include <algorithm>
+#include <type_traits>
+
+#include "mmoe_grouped_device.cuh"
+
+namespace mmoe {
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Products on CTA pairs: out[t, n] = sum over groups kb of 128 k's of (sum_k x[t, k] w[n, k]) sx[t, kb] sw[n / 128, kb].
+// Rows are operand A (256 a tile, 128 in each CTA), weights operand B (up to 256; gated: half of them gate rows, which the leader stages, the
+// up rows its peer).  The tensor core sums one group into one of two accumulators; the epilogue warps multiply that by the two scales and add
+// it to FP32 registers, 128 of them a thread, beside the next group's products.  A thread has one row of the tile, so that its scale is one number a
+// group; weights' scales are one for every 32 columns.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int kFp8Cols = 256;                         // most rows of B per tile
+constexpr int kFp8StageA = kGroupRows * 128;          // bytes
+constexpr int kFp8Stage = kFp8StageA + kFp8Cols / 2 * 128;
+constexpr int kFp8Stages = 5;
+constexpr int kFp8EpiWarps = 8;                       // two per TMEM lane quadrant, each with every other block of columns
+constexpr int kFp8Threads = 32 * (4 + kFp8EpiWarps);   // epilogue warps first, producer, issuer, two that only hand back registers
+constexpr int kFp8Registers = 224, kFp8FewRegisters = 56;
+static_assert(kFp8EpiWarps * 32 * kFp8Registers + 128 * kFp8FewRegisters <= kFp8Threads * 168, "registers that the block was launched with");
+constexpr int kFp8Batch = 8;                          // groups of k whose scales are fetched at a time
+constexpr int kFp8Turn = 32 * 144;                    // a warp's 32 rows x 128 bytes on their way from lanes to rows; before, its rows' scales
+constexpr int kFp8ScaleStride = 36;
+
+struct Fp8Control {
+  uint64_t full[kFp8Stages];      // leader only: every copy of the stage, in both CTAs, has landed
+  uint64_t empty[kFp8Stages];     // issuer -> producers of both CTAs
+  uint64_t acc_full[2];           // issuer -> epilogues of both CTAs
+  uint64_t acc_empty[2];          // leader only: epilogue warps of both CTAs -> issuer
+  uint32_t tmem_base;
+  volatile int32_t abort_flag;
+};
+
+struct Fp8Params {
+  CUtensorMap map_w;
+  CUtensorMap map_x[4];           // boxes of 128, 64, 32 and 16 rows
+  const int32_t* ends;
+  int32_t experts, rows;
+  int32_t n;                      // channels
+  int32_t cols, col_tiles;        // rows of B per tile (gated: both kinds), tiles of an expert's channels
+  int32_t groups;                 // of k: stages
+  int32_t blocks;                 // of channels (gated: of the gate's)
+  uint32_t idesc;
+  const float *x_scales, *w_scales;
+  DenseEpilogue epi;
+  int32_t* status;
+  int64_t timeout_ns;
+};
+
+constexpr int kFp8Smem = 227 * 1024;
+constexpr int kFp8Place = 1024;
+constexpr int kFp8PlanAt = kFp8Place + kFp8Stages * kFp8Stage;
+constexpr int kFp8TurnAt = kFp8PlanAt + (sizeof(GroupPlan) + 15) / 16 * 16;
+static_assert(sizeof(Fp8Control) <= kFp8Place, "control block");
+static_assert(kFp8TurnAt + kFp8EpiWarps * kFp8Turn + 1024 <= kFp8Smem, "shared memory of a CTA");
+
+struct Fp8Tile {
+  int expert, channel0;
+  int first, valid;               // rows, of the pair
+};
+template <bool kGate>
+__device__ __forceinline__ Fp8Tile fp8_tile_at(const Fp8Params& p, const GroupPlan& plan, int t) {
+  Fp8Tile g;
+  g.expert = expert_of(plan, p.experts, t);
+  const int start = plan.start[g.expert], count = plan.start[g.expert + 1] - start, parts = (count + 2 * kGroupRows - 1) / (2 * kGroupRows);
+  const int in = t - plan.tile[g.expert], at = in % parts * 2 * kGroupRows;
+  g.channel0 = in / parts * (kGate ? p.cols / 2 : p.cols);
+  g.first = start + at, g.valid = min(count - at, 2 * kGroupRows);
+  return g;
+}
+// of a CTA's 128 rows, rounded up to the smallest box
+__device__ __forceinline__ int fp8_rows_staged(int valid, int cta) { return min(max(valid - cta * kGroupRows + 15, 0), kGroupRows) & ~15; }
+
+__device__ __forceinline__ void fp8_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// a wait that ends as soon as it can: a thread that the hardware has put to sleep wakes up late, which is worth a tenth of a group's time here
+__device__ __forceinline__ bool poll(DenseWaiter& w, uint32_t bar, uint32_t parity) {
+  for (uint32_t spin = 0;; ++spin) {
+    if (__any_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+    // every 1024th probe as `late` wants it: the first sets the limit
+    if ((spin & 1023u) == 1023u && __any_sync(0xffffffffu, w.late(spin == 1023u ? 63u : 64u, 1))) return false;
+  }
+}
+
+template <bool kGate>
+__global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the same offset in both CTAs
+  Fp8Control* ctl = reinterpret_cast<Fp8Control*>(smem);
+  uint8_t* stages = smem + kFp8Place;
+  GroupPlan* plan = reinterpret_cast<GroupPlan*>(smem + kFp8PlanAt);
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int cta = static_cast<int>(cluster_ctarank());
+  if (threadIdx.x == 0) {
+    prefetch_map(&p.map_w);
+    for (int i = 0; i < 4; ++i) prefetch_map(&p.map_x[i]);
+    for (int i = 0; i < kFp8Stages; ++i) {
+      mbar_init(smem_u32(&ctl->full[i]), 1);
+      mbar_init(smem_u32(&ctl->empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&ctl->acc_full[i]), 1);
+      mbar_init(smem_u32(&ctl->acc_empty[i]), 2 * kFp8EpiWarps);
+    }
+    ctl->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kFp8EpiWarps + 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                       // the peer's barriers are initialised before anything arrives on them
+  tc_fence_after();
+  chain_wait();                             // nothing above touches global memory
+  chain_release();                          // in this order: what precedes this launch is complete when the next one starts
+  const int tiles = make_plan(plan, p.ends, p.experts, p.rows, 2 * kGroupRows, p.col_tiles, p.status);
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+  const int step = gridDim.x / 2, half = p.cols / 2;
+  DenseWaiter waiter{{&ctl->abort_flag, p.status, 0, kStatusGrouped + 1, warp}, p.timeout_ns};
+  const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
+  {
+    const int64_t row_bytes = p.epi.ld_out * (p.epi.out_type == kDenseFp32 ? 4 : 2), used = plan->start[p.experts];
+    clear_bytes(static_cast<char*>(p.epi.out) + used * row_bytes, (p.rows - used) * row_bytes);
+  }
+
+  if (warp < kFp8EpiWarps) {
+    // --------------------------------------------------------------------------------------------- epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFp8Registers));
+    const int quadrant = warp & 3;                    // of the TMEM lanes: the one this warp may read
+    const int side = warp >> 2;
+    const uint32_t leader_empty = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
+    const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
+    uint8_t* turn = smem + kFp8TurnAt + warp * kFp8Turn;
+    float* x_scale = reinterpret_cast<float*>(turn);
+    uint32_t it = 0;
+    bool ok = true;
+    // this warp's four blocks of 32 columns: the tile's column, and the channel behind the tile's first
+    const auto column = [&](int b) { return kGate ? (b >> 1) * 64 + side * 32 + (b & 1) * half : 64 * b + 32 * side; };
+    const auto channel = [&](int b) { return kGate ? (b >> 1) * 64 + side * 32 : 64 * b + 32 * side; };
+    const int width = kGate ? half : p.cols;          // channels of a tile
+    for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
+      const Fp8Tile g = fp8_tile_at<kGate>(p, *plan, t);
+      const int row0 = g.first + cta * kGroupRows + quadrant * 32, rows = g.valid - cta * kGroupRows - quadrant * 32;      // of this warp
+      const int channels = min(width, p.n - g.channel0);
+      const bool any = rows > 0 && channel(0) < channels;
+      float sum[4][32] = {};
+      // Scales of kFp8Batch groups, fetched a batch ahead: xs[i] that of row 4 i + lane / 8 in group lane % 8, ws that of block lane / 8 in it
+      float xs[kFp8Batch], ws = 0.f, w_now = 0.f;
+      const float* x_from = p.x_scales + (int64_t)(row0 + (lane >> 3)) * p.groups + (lane & 7);
+      const int block = min((g.channel0 + channel(lane >> 3)) / kScaleBlock, p.blocks - 1);
+      const float* w_from = p.w_scales + (((int64_t)g.expert * (kGate ? 2 : 1) + (kGate ? (lane >> 3) & 1 : 0)) * p.blocks + block) * p.groups + (lane & 7);
+      const auto fetch = [&](int kb) {
+        const bool there = kb + (lane & 7) < p.groups;
+#pragma unroll
+        for (int i = 0; i < kFp8Batch; ++i) xs[i] = there && 4 * i + (lane >> 3) < rows ? x_from[(int64_t)4 * i * p.groups + kb] : 0.f;
+        ws = there ? w_from[kb] : 0.f;
+      };
+      if (any) fetch(0);
+      for (int kb = 0; kb < p.groups; ++kb, ++it) {
+        const int in = kb % kFp8Batch;
+        if (any && in == 0) {
+          __syncwarp();                                 // the batch before has been read
+#pragma unroll
+          for (int i = 0; i < kFp8Batch; ++i) x_scale[(lane & 7) * kFp8ScaleStride + 4 * i + (lane >> 3)] = xs[i];
+          w_now = ws;
+          __syncwarp();
+          if (kb + kFp8Batch < p.groups) fetch(kb + kFp8Batch);
+        }
+        if (!poll(waiter, smem_u32(&ctl->acc_full[it & 1u]), (it >> 1) & 1u)) { ok = false; break; }
+        tc_fence_after();
+        const auto release = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_pair(leader_empty + 8 * (it & 1u));
+        };
+        if (!any) { release(); continue; }
+        const uint32_t d = tmem_base + (it & 1u) * kFp8Cols + lanes;
+        const float x_now = x_scale[in * kFp8ScaleStride + lane];
+        uint32_t v[2][32];
+        const auto add = [&](int b) {
+          const float s = x_now * __shfl_sync(0xffffffffu, w_now, 8 * b + in);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sum[b][j] = fmaf(__uint_as_float(v[b & 1][j]), s, sum[b][j]);
+        };
+        tc_ld32(d + column(0), v[0]);
+        tc_ld32(d + column(1), v[1]);
+        tc_ld_wait();
+        add(0);
+        tc_ld32(d + column(2), v[0]);
+        add(1);
+        tc_ld32(d + column(3), v[1]);
+        tc_ld_wait();
+        release();
+        add(2);
+        add(3);
+      }
+      if (!ok || !any) continue;
+      // ---- results
+      const bool dense_rows = p.epi.out_type == kDenseFp32 ? p.n % 4 == 0 : p.n % 8 == 0;
+#pragma unroll
+      for (int b = 0; b < 4; b += kGate ? 2 : 1) {
+        const int first = channel(b), count = min(32, channels - first);
+        if (count <= 0) continue;
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const float f = sum[b][j], u = sum[b + (kGate ? 1 : 0)][j];
+          v[j] = !kGate ? f : p.epi.out_type == kDenseFp32 ? gated_value_fp32(f, u, p.epi.clamp) : gated_value(f, u, p.epi.clamp);
+        }
+        const auto put = [&](auto* out) {
+          using T = std::remove_pointer_t<decltype(out)>;
+          constexpr int kPieces = 2 * sizeof(T), kStride = 16 * kPieces + 16;     // rows 16 bytes apart from a multiple of 64: no two of eight in one bank
+          static_assert(32 * kStride <= kFp8Turn, "results of a warp");
+          out += (int64_t)row0 * p.epi.ld_out + g.channel0 + first;
+          __syncwarp();                                 // the block before, or the scales, have been read
+#pragma unroll
+          for (int j = 0; j < kPieces; ++j) {
+            __align__(16) T piece[16 / sizeof(T)];
+#pragma unroll
+            for (int i = 0; i < 16 / sizeof(T); ++i) piece[i] = from_float<T>(v[j * (16 / sizeof(T)) + i]);
+            *reinterpret_cast<uint4*>(turn + lane * kStride + 16 * j) = *reinterpret_cast<const uint4*>(piece);
+          }
+          __syncwarp();
+          if (dense_rows) {
+            const int r0 = lane / kPieces, piece = lane % kPieces;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+              const int r = i * (32 / kPieces) + r0;
+              if (r < rows && piece * (16 / sizeof(T)) < count)
+                *reinterpret_cast<uint4*>(out + r * p.epi.ld_out + piece * (16 / sizeof(T))) = *reinterpret_cast<const uint4*>(turn + r * kStride + 16 * piece);
+            }
+          } else {                                      // rows that start anywhere: a lane per column
+            for (int r = 0; r < min(rows, 32); ++r)
+              if (lane < count) out[r * p.epi.ld_out + lane] = reinterpret_cast<const T*>(turn + r * kStride)[lane];
+          }
+        };
+        if (p.epi.out_type == kDenseBf16) put(static_cast<__nv_bfloat16*>(p.epi.out));
+        else if (p.epi.out_type == kDenseFp16) put(static_cast<__half*>(p.epi.out));
+        else put(static_cast<float*>(p.epi.out));
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp8FewRegisters));
+    if (warp == kFp8EpiWarps) {
+      // --------------------------------------------------------------------------------------------- producer
+      int stage = 0;
+      uint32_t phase = 0;
+      const uint32_t leader_full0 = map_to_cta(full0, 0), base = smem_u32(stages);
+      bool ok = true;
+      for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
+        const Fp8Tile g = fp8_tile_at<kGate>(p, *plan, t);
+        const int rows = fp8_rows_staged(g.valid, cta), x_row = g.first + cta * kGroupRows;
+        const uint32_t tx = (fp8_rows_staged(g.valid, 0) + fp8_rows_staged(g.valid, 1)) * 128 + 2 * half * 128;
+        const int w_row = kGate ? g.channel0 : g.channel0 + cta * half, part = kGate ? cta : 0;
+        for (int kb = 0; kb < p.groups; ++kb) {
+          if (!waiter.wait_uniform(empty0 + 8 * stage, phase ^ 1u)) { ok = false; break; }
+          const uint32_t bar = leader_full0 + 8 * stage, a = base + stage * kFp8Stage;
+          if (elect_one()) {
+            if (cta == 0) mbar_expect_tx(full0 + 8 * stage, tx);
+            pair_load_4d(a + kFp8StageA, &p.map_w, kb * 128, w_row, part, g.expert, bar);
+            int done = 0;
+  #pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (rows & (128 >> i)) {
+                pair_load_2d(a + done * 128, &p.map_x[i], kb * 128, x_row + done, bar);
+                done += 128 >> i;
+              }
+          }
+          __syncwarp();
+          if (++stage == kFp8Stages) { stage = 0; phase ^= 1u; }
+        }
+      }
+    } else if (warp == kFp8EpiWarps + 1) {
+      // --------------------------------------------------------------------------------------------- issuer
+      if (cta == 0) {
+        int stage = 0;
+        uint32_t phase = 0, it = 0;
+        bool ok = true;
+        const uint32_t lo0 = (smem_u32(stages) & 0x3FFFFu) >> 4;
+        const uint64_t hi = operand_desc(false, 0);
+        for (int t = blockIdx.x / 2; ok && t < tiles; t += step)
+          for (int kb = 0; kb < p.groups; ++kb, ++it) {
+            if (!poll(waiter, smem_u32(&ctl->acc_empty[it & 1u]), ((it >> 1) & 1u) ^ 1u) || !poll(waiter, full0 + 8 * stage, phase)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t a = lo0 + stage * (kFp8Stage >> 4), b = a + (kFp8StageA >> 4), d = tmem_base + (it & 1u) * kFp8Cols;
+            if (elect_one()) {
+  #pragma unroll
+              for (int k = 0; k < 4; ++k) fp8_product(d, hi | (a + 2 * k), hi | (b + 2 * k), p.idesc, k != 0 ? 1u : 0u);
+              pair_commit(empty0 + 8 * stage);
+              pair_commit(smem_u32(&ctl->acc_full[it & 1u]));
+            }
+            __syncwarp();
+            if (++stage == kFp8Stages) { stage = 0; phase ^= 1u; }
+          }
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------------------------------------------- teardown
+  __syncwarp();
+  if (ctl->abort_flag != 0) {               // copies still in flight land before this CTA's shared memory goes
+    const uint64_t t0 = global_timer();
+    while (global_timer() - t0 < 200000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                       // no CTA leaves while its peer may still arrive on its barriers
+  tc_fence_after();
+  if (warp == kFp8EpiWarps + 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------------
+// Columns of a tile: those with which the pair that has most to do ends first.  A group costs 2 clk a column in the tensor cores, or its bytes at 60 a clock
+// into each SM.  The rows of each expert are not known here; a tile of rows for all, and one for every expert beyond the first, is the most there can be.
+int fp8_cols(const GroupedProduct& p, int pairs) {
+  const int64_t row_tiles = (p.rows + 2 * kGroupRows - 1) / (2 * kGroupRows) + std::min(p.experts, p.rows) - 1;
+  int64_t least = INT64_MAX;
+  int best = kFp8Cols;
+  for (int cols = kFp8Cols; cols >= 64; cols -= p.kind == kGated ? 64 : 32) {
+    const int width = p.kind == kGated ? cols / 2 : cols;
+    const int64_t tiles = row_tiles * ((p.n + width - 1) / width), cost = (tiles + pairs - 1) / pairs * std::max(2 * cols, (kFp8StageA + cols / 2 * 128) / 60);
+    if (cost < least) least = cost, best = cols;
+  }
+  return best;
+}
+
+cudaError_t launch_fp8_pairs(const GroupedProduct& p, int sms, cudaStream_t s) {
+  Fp8Params d = {};
+  const bool gate = p.kind == kGated;
+  d.ends = p.ends, d.experts = p.experts, d.rows = p.rows, d.n = p.n;
+  d.cols = fp8_cols(p, sms / 2);
+  const int width = gate ? d.cols / 2 : d.cols;
+  d.col_tiles = (p.n + width - 1) / width;
+  d.groups = (p.k + kScaleBlock - 1) / kScaleBlock;
+  d.blocks = (p.n + kScaleBlock - 1) / kScaleBlock;
+  d.idesc = product_idesc(kDenseFp16, false, false, 2 * kGroupRows, d.cols);         // format 0: FP16, or in 8 bits E4M3
+  d.x_scales = p.x_scales, d.w_scales = p.w_scales;
+  d.epi = p.epi;
+  d.status = p.status;
+  d.timeout_ns = (p.timeout_ms > 0 ? (int64_t)p.timeout_ms : 2000) * 1000000ll;
+  const uint64_t n = p.n, k = p.k, parts = gate ? 2 : 1;
+  bool ok = encode_map(&d.map_w, kGroupedE4m3, p.w, 4, {k, n, parts, static_cast<uint64_t>(p.experts), 1}, {k, n * k, parts * n * k, 0},
+                       {128, static_cast<uint32_t>(d.cols / 2), 1, 1, 1});
+  for (int i = 0; ok && i < 4; ++i)
+    ok = encode_map(&d.map_x[i], kGroupedE4m3, p.x, 2, {k, static_cast<uint64_t>(p.rows), 1, 1, 1}, {static_cast<uint64_t>(p.x_ld), 0, 0, 0}, {128, 128u >> i, 1, 1, 1});
+  const int64_t most = ((int64_t)p.rows / (2 * kGroupRows) + std::min(p.experts, p.rows)) * d.col_tiles;
+  if (!ok || most > INT32_MAX / 2) return cudaErrorInvalidValue;
+  const int grid = 2 * static_cast<int>(std::min<int64_t>(sms / 2, most));
+  return gate ? launch_clustered(fp8_pair_kernel<true>, dim3(grid), dim3(kFp8Threads), kFp8Smem, 2, s, d)
+              : launch_clustered(fp8_pair_kernel<false>, dim3(grid), dim3(kFp8Threads), kFp8Smem, 2, s, d);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Quantiser: s = max|x| / 448 for each 128 values of a row, q = x / s rounded to the nearest E4M3 value, ties to even.
+// Sixteen lanes have a group, eight values each, which stay in registers between the maximum and the quotients.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int kQuantThreads = 256, kQuantLanes = 16;
+
+// x / s in E4M3, exactly, two values.  The product with the reciprocal is within 2^-22 of the quotient, which matters next to a border between two E4M3
+// values alone: there the 20 bits that E4M3 drops are near their middle (of a number below 2^-6, where the steps are those of [2^-6, 2^-5): when 2^-6 is
+// added).  Then the quotient is taken with its last bit set where it is not exact, which rounds as the exact one does.
+__device__ __forceinline__ bool near_border(float q) {
+  const float a = fabsf(q), z = a < 0x1p-6f ? a + 0x1p-6f : a;
+  return ((__float_as_uint(z) - 0x80000u + 8u) & 0xfffffu) < 16u;
+}
+__device__ __forceinline__ float odd_quotient(float x, float s) {
+  const float q = __fdiv_rn(x, s), rest = fmaf(-q, s, x);
+  uint32_t bits = __float_as_uint(q);
+  if (rest != 0.f) {
+    if ((rest < 0.f) != (q < 0.f)) --bits;       // towards zero ...
+    bits |= 1u;                                  // ... and marked
+  }
+  return __uint_as_float(bits);
+}
+__device__ __forceinline__ uint32_t two_e4m3(float a, float b) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
+// kVec: eight neighbouring values in one load; else (widths, strides or places that do not allow it) every sixteenth
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kQuantThreads) quantize_fp8_kernel(const T* x, int64_t ld, uint8_t* q, float* scales, uint32_t total, uint32_t groups, int k) {
+  chain_wait();
+  chain_release();
+  const uint64_t index = (uint64_t)blockIdx.x * (kQuantThreads / kQuantLanes) + threadIdx.x / kQuantLanes;
+  const bool there = index < total;            // sixteen lanes alike
+  const uint32_t row = static_cast<uint32_t>(index) / groups, group = static_cast<uint32_t>(index) - row * groups;
+  const int lane = threadIdx.x % kQuantLanes, first = static_cast<int>(group) * kScaleBlock, count = there ? min(kScaleBlock, k - first) : 0;
+  const T* in = x + row * ld + first;
+  float v[8];
+  if constexpr (kVec) {
+    struct alignas(16) Vec { T v[8]; };
+    Vec f = {};
+    if (8 * lane < count) f = *reinterpret_cast<const Vec*>(in + 8 * lane);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(f.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = lane + 16 * j < count ? static_cast<float>(in[lane + 16 * j]) : 0.f;
+  }
+  // magnitudes as bits: NaN is above infinity there, so neither is lost
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+  for (int d = kQuantLanes / 2; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+  const bool finite = top < 0x7f800000u;
+  float s = !finite ? __uint_as_float(0x7fffffffu) : top == 0 ? 1.f : __fdiv_rn(__uint_as_float(top), 448.f);
+  if (there && lane == 0) scales[(int64_t)row * groups + group] = s;
+  if (s < 0x1p-60f) {                          // remainders of quotients by so small a scale would be no numbers
+    s *= 0x1p80f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= 0x1p80f;
+  }
+  const float inv = __fdiv_rn(1.f, s);
+  float r[8];
+  bool near = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    r[j] = finite ? v[j] * inv : 0.f;
+    near |= near_border(r[j]);
+  }
+  if (near) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = odd_quotient(v[j], s);
+  }
+  uint8_t* out = q + (int64_t)row * k + first;
+  const uint32_t b[4] = {two_e4m3(r[0], r[1]), two_e4m3(r[2], r[3]), two_e4m3(r[4], r[5]), two_e4m3(r[6], r[7])};
+  if constexpr (kVec) {
+    if (8 * lane < count) *reinterpret_cast<uint2*>(out + 8 * lane) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (lane + 16 * j < count) out[lane + 16 * j] = static_cast<uint8_t>(b[j / 2] >> (j & 1) * 8);
+  }
+}
+
+template <typename T>
+cudaError_t launch_quantize(const void* x, int64_t ld, uint8_t* q, float* scales, int m, int k, cudaStream_t s) {
+  const T* in = static_cast<const T*>(x);
+  const bool vec = k % 8 == 0 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0;
+  const uint32_t groups = (static_cast<uint32_t>(k) + kScaleBlock - 1) / kScaleBlock;
+  const uint64_t total = (uint64_t)m * groups, blocks = (total + kQuantThreads / kQuantLanes - 1) / (kQuantThreads / kQuantLanes);
+  if (total > UINT32_MAX || blocks > INT32_MAX) return cudaErrorInvalidValue;
+  const uint32_t n = static_cast<uint32_t>(total);
+  return vec ? launch_chained(quantize_fp8_kernel<T, true>, dim3(static_cast<uint32_t>(blocks)), dim3(kQuantThreads), 0, s, in, ld, q, scales, n, groups, k)
+             : launch_chained(quantize_fp8_kernel<T, false>, dim3(static_cast<uint32_t>(blocks)), dim3(kQuantThreads), 0, s, in, ld, q, scales, n, groups, k);
+}
+
+}  // namespace
+
+cudaError_t prepare_fp8() {
+  cudaError_t e = cudaFuncSetAttribute(fp8_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8Smem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8Smem);
+  return e;
+}
+
+cudaError_t launch_fp8(const GroupedProduct& p, cudaStream_t s) {
+  const int sms = dense_sms();
+  if (sms == 0) return cudaErrorNotReady;
+  const ChainScope chain(true);
+  return launch_fp8_pairs(p, sms, s);
+}
+
+cudaError_t launch_quantize_fp8(const void* x, int type, int64_t ld, uint8_t* q, float* scales, int m, int k, cudaStream_t s) {
+  if (m <= 0) return cudaSuccess;
+  const ChainScope chain(true);
+  return type == kDenseBf16 ? launch_quantize<__nv_bfloat16>(x, ld, q, scales, m, k, s) : launch_quantize<__half>(x, ld, q, scales, m, k, s);
+}
+
+}  // namespace mmoe

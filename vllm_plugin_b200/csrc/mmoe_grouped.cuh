@@ -35,7 +35,9 @@ struct GroupedProduct {
 };
 
 cudaError_t prepare_grouped();          // behind prepare_dense()
-cudaError_t launch_grouped(const GroupedProduct& p, cudaStream_t s);
+cudaError_t prepare_fp8();
+cudaError_t launch_grouped(const GroupedProduct& p, cudaStream_t s);      // 16 bits
+cudaError_t launch_fp8(const GroupedProduct& p, cudaStream_t s);          // E4M3; rows behind the last expert's are set to zero
 cudaError_t launch_quantize_fp8(const void* x, int type, int64_t ld, uint8_t* q, float* scales, int m, int k, cudaStream_t s);
 
 }  // namespace mmoe

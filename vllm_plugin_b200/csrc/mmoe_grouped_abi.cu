@@ -33,7 +33,8 @@ int check_rows(const char* what, const void* x, int64_t stride, int32_t width, i
 }
 
 int run_grouped(const mmoe::GroupedProduct& p, const char* what, void* stream) {
-  const cudaError_t e = mmoe::launch_grouped(p, static_cast<cudaStream_t>(stream));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = p.type == mmoe::kGroupedE4m3 ? mmoe::launch_fp8(p, s) : mmoe::launch_grouped(p, s);
   return e == cudaSuccess ? MMOE_OK : e == cudaErrorNotReady ? fail(MMOE_ERR_NOT_PREPARED, "%s: mmoe_dense_prepare() has not run on this device", what) : cuda_fail(e, what);
 }
 
@@ -111,7 +112,6 @@ int fp8_product(const MmoeFp8Product* a, bool gated, void* stream) {
   p.kind = gated ? mmoe::kGated : mmoe::kLinear;
   p.n = a->channels, p.k = a->width, p.w = a->w, p.x = a->x, p.x_ld = a->x_stride, p.x_scales = a->x_scales, p.w_scales = a->w_scales;
   p.epi.out = a->out, p.epi.ld_out = a->channels, p.epi.out_type = a->out_type, p.epi.inter = a->channels, p.epi.clamp = a->clamp;
-  p.zero_behind = true;
   return run_grouped(p, what, stream);
 }
 
