@@ -347,7 +347,7 @@ int mmoe_dense_read_status(int32_t* status, int32_t* words8, void* stream);
 
 /* ---- Products of a layer's experts beside the MXFP8 x MXFP4 layer (no counterpart in the reference): rows that are grouped by expert, in 16 bits with
  * their gradients, and products in 8-bit floating point with block scales, of such rows or of all rows by one weight.  As above: no workspace, no
- * geometry, `status` words (kernels 33 and 34), mmoe_dense_prepare() first.
+ * geometry, `status` words (kernels 33: 16 bits on pairs, 34: 8 bits on pairs, 35: few rows), mmoe_dense_prepare() first.
  * `ends`: int32 [num_experts] device words; the rows of expert e end before row ends[e] and begin where those of e - 1 end, with row 0 for the first.
  * An expert may have no rows.  Rows from the last end on belong to no expert: their outputs and gradients are zero.  Ends that fall, are
  * negative or pass num_rows: no row is an expert's, and the launch is counted in word [4] of `status`. */

@@ -14,7 +14,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 OUT_DIR = os.path.join(os.path.dirname(HERE), "_lib")
 SOURCES = ("mmoe_abi.cu", "mmoe_support.cu", "mmoe_umma.cu", "mmoe_umma_tm.cu", "mmoe_ep.cu", "mmoe_weights.cu", "mmoe_dense.cu",
-           "mmoe_dense_abi.cu", "mmoe_grouped.cu", "mmoe_fp8.cu", "mmoe_grouped_abi.cu")
+           "mmoe_dense_abi.cu", "mmoe_grouped.cu", "mmoe_fp8.cu", "mmoe_grouped_few.cu",
+           "mmoe_grouped_abi.cu")
 LIB_NAME = "libmmoe_b200.so"
 
 

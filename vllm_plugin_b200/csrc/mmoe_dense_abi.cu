@@ -77,6 +77,7 @@ int mmoe_dense_prepare(void* stream) {
   e = mmoe::prepare_dense();
   if (e == cudaSuccess) e = mmoe::prepare_grouped();
   if (e == cudaSuccess) e = mmoe::prepare_fp8();
+  if (e == cudaSuccess) e = mmoe::prepare_grouped_few();
   return e == cudaSuccess ? MMOE_OK : cuda_fail(e, "dense_prepare");
 }
 

@@ -7,7 +7,7 @@
 
 namespace mmoe {
 
-// kernels in the status words: products on pairs, of few tokens; grouped products on pairs, of few rows
+// kernels in the status words: products on pairs, of few tokens; grouped products on pairs (16 and 8 bits), of few rows
 constexpr int kStatusDense = 31, kStatusGrouped = 33;
 
 #ifdef __CUDACC__

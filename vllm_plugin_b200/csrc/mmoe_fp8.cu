@@ -10,28 +10,41 @@ namespace {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Products on CTA pairs: out[t, n] = sum over groups kb of 128 k's of (sum_k x[t, k] w[n, k]) sx[t, kb] sw[n / 128, kb].
-// Rows are operand A (256 a tile, 128 in each CTA), weights operand B (up to 256; gated: half of them gate rows, which the leader stages, the
-// up rows its peer).  The tensor core sums one group into one of two accumulators; the epilogue warps multiply that by the two scales and add
-// it to FP32 registers, 128 of them a thread, beside the next group's products.  A thread has one row of the tile, so that its scale is one number a
-// group; weights' scales are one for every 32 columns.
+// Rows are operand A (256 a tile, 128 in each CTA), weights operand B (256 a tile; gated: half of them gate rows, which the leader stages, the
+// up rows its peer).  The tensor core sums one group into one of two accumulators, in two halves of 128 columns each; the epilogue warps multiply
+// a half by the two scales and add it to FP32 registers, 128 of them a thread, beside the next one's products.  A thread has one row of the tile, so
+// that its scale is one number a group; weights' scales are one for every 32 columns.  (Weights along the lanes instead: a scale for every
+// column and thread, 109 us where this takes 55.)  One warp brings the scales, word by word and up to three batches ahead.
+//
+// What bounds it, 3840 rows: 2304 -> 5120 55 us (1.65 PFLOP/s), gated 5120 -> 2 x 2304 94-103 us (1.8-1.9).  Without the multiplications 39 and 69:
+// the 256 of them that a scheduler has for each group, at most half of it beside the loads from tensor memory, are 250-300 clk of a group's 1000.
+// Without loads and multiplications 38 and 66, of which 32 KB a group into each SM are 700 clk.  Tried: tiles of 192 columns whose sums are
+// all fetched before the accumulator is released, 88; sixteen epilogue warps with 64 columns each, 63; the next group's columns fetched ahead of this
+// one's last multiplications, 59; packed pairs (fma.rn.f32x2), 66, as a move goes with each of them; whole accumulators instead of halves, 60.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFp8Cols = 256;                         // most rows of B per tile
 constexpr int kFp8StageA = kGroupRows * 128;          // bytes
 constexpr int kFp8Stage = kFp8StageA + kFp8Cols / 2 * 128;
-constexpr int kFp8Stages = 5;
+constexpr int kFp8Stages = 4;
 constexpr int kFp8EpiWarps = 8;                       // two per TMEM lane quadrant, each with every other block of columns
-constexpr int kFp8Threads = 32 * (4 + kFp8EpiWarps);   // epilogue warps first, producer, issuer, two that only hand back registers
-constexpr int kFp8Registers = 224, kFp8FewRegisters = 56;
+constexpr int kFp8Threads = 32 * (4 + kFp8EpiWarps);   // epilogue warps first, producer, issuer, one that fetches scales, one that only hands back registers
+constexpr int kFp8Registers = 216, kFp8FewRegisters = 72;
 static_assert(kFp8EpiWarps * 32 * kFp8Registers + 128 * kFp8FewRegisters <= kFp8Threads * 168, "registers that the block was launched with");
 constexpr int kFp8Batch = 8;                          // groups of k whose scales are fetched at a time
-constexpr int kFp8Turn = 32 * 144;                    // a warp's 32 rows x 128 bytes on their way from lanes to rows; before, its rows' scales
-constexpr int kFp8ScaleStride = 36;
+constexpr int kFp8Turn = 32 * 144;                    // a warp's 32 rows x 128 bytes on their way from lanes to rows
+constexpr int kFp8ScaleSlots = 4;
+// scales of a batch
+struct Fp8Scales {
+  float x[kFp8Batch][kGroupRows + 4];                 // of the CTA's rows; padded so that four rows x eight groups are written to 32 banks
+  float w[kFp8Batch][8];                              // of the blocks of 32 columns, by warp side
+};
 
 struct Fp8Control {
   uint64_t full[kFp8Stages];      // leader only: every copy of the stage, in both CTAs, has landed
   uint64_t empty[kFp8Stages];     // issuer -> producers of both CTAs
-  uint64_t acc_full[2];           // issuer -> epilogues of both CTAs
-  uint64_t acc_empty[2];          // leader only: epilogue warps of both CTAs -> issuer
+  uint64_t acc_full[4];           // issuer -> epilogues of both CTAs; by accumulator and half
+  uint64_t acc_empty[4];          // leader only: epilogue warps of both CTAs -> issuer
+  uint64_t scale_full[kFp8ScaleSlots], scale_empty[kFp8ScaleSlots];
   uint32_t tmem_base;
   volatile int32_t abort_flag;
 };
@@ -57,7 +70,8 @@ constexpr int kFp8Place = 1024;
 constexpr int kFp8PlanAt = kFp8Place + kFp8Stages * kFp8Stage;
 constexpr int kFp8TurnAt = kFp8PlanAt + (sizeof(GroupPlan) + 15) / 16 * 16;
 static_assert(sizeof(Fp8Control) <= kFp8Place, "control block");
-static_assert(kFp8TurnAt + kFp8EpiWarps * kFp8Turn + 1024 <= kFp8Smem, "shared memory of a CTA");
+constexpr int kFp8ScalesAt = kFp8TurnAt + kFp8EpiWarps * kFp8Turn;
+static_assert(kFp8ScalesAt + kFp8ScaleSlots * sizeof(Fp8Scales) + 1024 <= kFp8Smem, "shared memory of a CTA");
 
 struct Fp8Tile {
   int expert, channel0;
@@ -90,6 +104,13 @@ __device__ __forceinline__ bool poll(DenseWaiter& w, uint32_t bar, uint32_t pari
   }
 }
 
+// the same where the phase has mostly completed: two probes, then as everybody waits
+__device__ __forceinline__ bool wait_here(DenseWaiter& w, uint32_t bar, uint32_t parity) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) ok = mbar_try_wait(bar, parity);
+  return __all_sync(0xffffffffu, ok) || w.wait_uniform(bar, parity);
+}
+
 template <bool kGate>
 __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -97,6 +118,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
   Fp8Control* ctl = reinterpret_cast<Fp8Control*>(smem);
   uint8_t* stages = smem + kFp8Place;
   GroupPlan* plan = reinterpret_cast<GroupPlan*>(smem + kFp8PlanAt);
+  Fp8Scales* scales = reinterpret_cast<Fp8Scales*>(smem + kFp8ScalesAt);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int cta = static_cast<int>(cluster_ctarank());
@@ -107,9 +129,13 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
       mbar_init(smem_u32(&ctl->full[i]), 1);
       mbar_init(smem_u32(&ctl->empty[i]), 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&ctl->acc_full[i]), 1);
-      mbar_init(smem_u32(&ctl->acc_empty[i]), 2 * kFp8EpiWarps);
+      mbar_init(smem_u32(&ctl->acc_empty[i]), kFp8EpiWarps);
+    }
+    for (int i = 0; i < kFp8ScaleSlots; ++i) {
+      mbar_init(smem_u32(&ctl->scale_full[i]), 32);
+      mbar_init(smem_u32(&ctl->scale_empty[i]), kFp8EpiWarps);
     }
     ctl->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -142,12 +168,14 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
     const uint32_t leader_empty = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
     const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
     uint8_t* turn = smem + kFp8TurnAt + warp * kFp8Turn;
-    float* x_scale = reinterpret_cast<float*>(turn);
-    uint32_t it = 0;
+    uint32_t batch = 0, phase = 0, second = 0;
+    uint32_t full_at = smem_u32(&ctl->acc_full[side]), empty_at = leader_empty + 8 * side, d = tmem_base + side * (kFp8Cols / 2) + lanes;
+    const uint32_t full_flip = full_at ^ (full_at + 16), full_flip2 = empty_at ^ (empty_at + 16);
     bool ok = true;
     // this warp's four blocks of 32 columns: the tile's column, and the channel behind the tile's first
-    const auto column = [&](int b) { return kGate ? (b >> 1) * 64 + side * 32 + (b & 1) * half : 64 * b + 32 * side; };
-    const auto channel = [&](int b) { return kGate ? (b >> 1) * 64 + side * 32 : 64 * b + 32 * side; };
+    const int quarter = half / 2;                     // of the tile's columns: a half has those of the leader's weights and its peer's
+    const auto column = [&](int b) { return (b >> 1) * quarter + 32 * (b & 1); };
+    const auto channel = [&](int b) { return side * quarter + 32 * (b & 1) + (kGate ? 0 : (b >> 1) * half); };
     const int width = kGate ? half : p.cols;          // channels of a tile
     for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
       const Fp8Tile g = fp8_tile_at<kGate>(p, *plan, t);
@@ -155,94 +183,90 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
       const int channels = min(width, p.n - g.channel0);
       const bool any = rows > 0 && channel(0) < channels;
       float sum[4][32] = {};
-      // Scales of kFp8Batch groups, fetched a batch ahead: xs[i] that of row 4 i + lane / 8 in group lane % 8, ws that of block lane / 8 in it
-      float xs[kFp8Batch], ws = 0.f, w_now = 0.f;
-      const float* x_from = p.x_scales + (int64_t)(row0 + (lane >> 3)) * p.groups + (lane & 7);
-      const int block = min((g.channel0 + channel(lane >> 3)) / kScaleBlock, p.blocks - 1);
-      const float* w_from = p.w_scales + (((int64_t)g.expert * (kGate ? 2 : 1) + (kGate ? (lane >> 3) & 1 : 0)) * p.blocks + block) * p.groups + (lane & 7);
-      const auto fetch = [&](int kb) {
-        const bool there = kb + (lane & 7) < p.groups;
+      for (int kb = 0; ok && kb < p.groups; kb += kFp8Batch, ++batch) {
+        if (!wait_here(waiter, smem_u32(&ctl->scale_full[batch % kFp8ScaleSlots]), (batch / kFp8ScaleSlots) & 1u)) { ok = false; break; }
+        const Fp8Scales& now = scales[batch % kFp8ScaleSlots];
+        uint32_t x_at = smem_u32(&now.x[0][quadrant * 32 + lane]), w_at = smem_u32(&now.w[0][4 * side]);
+        const int count = min(kFp8Batch, p.groups - kb);
+        for (int j = 0; j < count; ++j) {
+          if (!wait_here(waiter, full_at, phase)) { ok = false; break; }
+          tc_fence_after();
+          if (any) {
+            uint32_t v[2][32];
+            tc_ld32(d, v[0]);
+            tc_ld32(d + 32, v[1]);
+            float x_now, w0, w1, w2, w3;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x_now) : "r"(x_at));
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w0), "=f"(w1), "=f"(w2), "=f"(w3) : "r"(w_at));
+            const auto add = [&](int b, float w) {
+              const float s = x_now * w;
 #pragma unroll
-        for (int i = 0; i < kFp8Batch; ++i) xs[i] = there && 4 * i + (lane >> 3) < rows ? x_from[(int64_t)4 * i * p.groups + kb] : 0.f;
-        ws = there ? w_from[kb] : 0.f;
-      };
-      if (any) fetch(0);
-      for (int kb = 0; kb < p.groups; ++kb, ++it) {
-        const int in = kb % kFp8Batch;
-        if (any && in == 0) {
-          __syncwarp();                                 // the batch before has been read
-#pragma unroll
-          for (int i = 0; i < kFp8Batch; ++i) x_scale[(lane & 7) * kFp8ScaleStride + 4 * i + (lane >> 3)] = xs[i];
-          w_now = ws;
-          __syncwarp();
-          if (kb + kFp8Batch < p.groups) fetch(kb + kFp8Batch);
+              for (int i = 0; i < 32; ++i) sum[b][i] = fmaf(__uint_as_float(v[b & 1][i]), s, sum[b][i]);
+            };
+            tc_ld_wait();
+            add(0, w0);
+            tc_ld32(d + column(2), v[0]);
+            add(1, w1);
+            tc_ld32(d + column(2) + 32, v[1]);
+            tc_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_pair(empty_at);
+            add(2, w2);
+            add(3, w3);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_pair(empty_at);
+          }
+          x_at += sizeof(now.x[0]), w_at += sizeof(now.w[0]);
+          phase ^= second;                       // a phase has both accumulators
+          full_at ^= full_flip, empty_at ^= full_flip2, d ^= kFp8Cols, second ^= 1u;
         }
-        if (!poll(waiter, smem_u32(&ctl->acc_full[it & 1u]), (it >> 1) & 1u)) { ok = false; break; }
-        tc_fence_after();
-        const auto release = [&] {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_pair(leader_empty + 8 * (it & 1u));
-        };
-        if (!any) { release(); continue; }
-        const uint32_t d = tmem_base + (it & 1u) * kFp8Cols + lanes;
-        const float x_now = x_scale[in * kFp8ScaleStride + lane];
-        uint32_t v[2][32];
-        const auto add = [&](int b) {
-          const float s = x_now * __shfl_sync(0xffffffffu, w_now, 8 * b + in);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) sum[b][j] = fmaf(__uint_as_float(v[b & 1][j]), s, sum[b][j]);
-        };
-        tc_ld32(d + column(0), v[0]);
-        tc_ld32(d + column(1), v[1]);
-        tc_ld_wait();
-        add(0);
-        tc_ld32(d + column(2), v[0]);
-        add(1);
-        tc_ld32(d + column(3), v[1]);
-        tc_ld_wait();
-        release();
-        add(2);
-        add(3);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl->scale_empty[batch % kFp8ScaleSlots]));
       }
       if (!ok || !any) continue;
-      // ---- results
+      // ---- results: rows of two neighbouring blocks, 64 channels
       const bool dense_rows = p.epi.out_type == kDenseFp32 ? p.n % 4 == 0 : p.n % 8 == 0;
 #pragma unroll
-      for (int b = 0; b < 4; b += kGate ? 2 : 1) {
-        const int first = channel(b), count = min(32, channels - first);
+      for (int pair = 0; pair < (kGate ? 1 : 2); ++pair) {
+        const int first = channel(2 * pair), count = min(quarter, channels - first);
         if (count <= 0) continue;
-        float v[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float f = sum[b][j], u = sum[b + (kGate ? 1 : 0)][j];
-          v[j] = !kGate ? f : p.epi.out_type == kDenseFp32 ? gated_value_fp32(f, u, p.epi.clamp) : gated_value(f, u, p.epi.clamp);
-        }
+        const auto value = [&](int j) {                  // of channel first + j
+          const float f = sum[2 * pair + (j >> 5)][j & 31];
+          if (!kGate) return f;
+          const float u = sum[2 + (j >> 5)][j & 31];
+          return p.epi.out_type == kDenseFp32 ? gated_value_fp32(f, u, p.epi.clamp) : gated_value(f, u, p.epi.clamp);
+        };
         const auto put = [&](auto* out) {
           using T = std::remove_pointer_t<decltype(out)>;
-          constexpr int kPieces = 2 * sizeof(T), kStride = 16 * kPieces + 16;     // rows 16 bytes apart from a multiple of 64: no two of eight in one bank
-          static_assert(32 * kStride <= kFp8Turn, "results of a warp");
+          constexpr int kEach = 16 / sizeof(T), kPart = 128 / sizeof(T), kStride = 144;       // 144: no two of eight rows in one bank
           out += (int64_t)row0 * p.epi.ld_out + g.channel0 + first;
-          __syncwarp();                                 // the block before, or the scales, have been read
 #pragma unroll
-          for (int j = 0; j < kPieces; ++j) {
-            __align__(16) T piece[16 / sizeof(T)];
+          for (int part = 0; part < 64 / kPart; ++part) {     // 128 bytes of every row
+            __syncwarp();                                 // what was there has been read
 #pragma unroll
-            for (int i = 0; i < 16 / sizeof(T); ++i) piece[i] = from_float<T>(v[j * (16 / sizeof(T)) + i]);
-            *reinterpret_cast<uint4*>(turn + lane * kStride + 16 * j) = *reinterpret_cast<const uint4*>(piece);
-          }
-          __syncwarp();
-          if (dense_rows) {
-            const int r0 = lane / kPieces, piece = lane % kPieces;
+            for (int j = 0; j < 8; ++j) {
+              __align__(16) T piece[kEach];
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-              const int r = i * (32 / kPieces) + r0;
-              if (r < rows && piece * (16 / sizeof(T)) < count)
-                *reinterpret_cast<uint4*>(out + r * p.epi.ld_out + piece * (16 / sizeof(T))) = *reinterpret_cast<const uint4*>(turn + r * kStride + 16 * piece);
+              for (int i = 0; i < kEach; ++i) piece[i] = from_float<T>(value(part * kPart + j * kEach + i));
+              *reinterpret_cast<uint4*>(turn + lane * kStride + 16 * j) = *reinterpret_cast<const uint4*>(piece);
             }
-          } else {                                      // rows that start anywhere: a lane per column
-            for (int r = 0; r < min(rows, 32); ++r)
-              if (lane < count) out[r * p.epi.ld_out + lane] = reinterpret_cast<const T*>(turn + r * kStride)[lane];
+            __syncwarp();
+            T* to = out + part * kPart;
+            const int left = count - part * kPart;
+            if (dense_rows) {
+              const int at = (lane & 7) * kEach;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = 4 * i + (lane >> 3);
+                if (r < rows && at < left) *reinterpret_cast<uint4*>(to + r * p.epi.ld_out + at) = *reinterpret_cast<const uint4*>(turn + r * kStride + 16 * (lane & 7));
+              }
+            } else {                                      // rows that start anywhere: a lane per column
+              for (int r = 0; r < min(rows, 32); ++r)
+                for (int at = lane; at < min(left, kPart); at += 32) to[r * p.epi.ld_out + at] = reinterpret_cast<const T*>(turn + r * kStride)[at];
+            }
           }
         };
         if (p.epi.out_type == kDenseBf16) put(static_cast<__nv_bfloat16*>(p.epi.out));
@@ -291,18 +315,52 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
         const uint64_t hi = operand_desc(false, 0);
         for (int t = blockIdx.x / 2; ok && t < tiles; t += step)
           for (int kb = 0; kb < p.groups; ++kb, ++it) {
-            if (!poll(waiter, smem_u32(&ctl->acc_empty[it & 1u]), ((it >> 1) & 1u) ^ 1u) || !poll(waiter, full0 + 8 * stage, phase)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t a = lo0 + stage * (kFp8Stage >> 4), b = a + (kFp8StageA >> 4), d = tmem_base + (it & 1u) * kFp8Cols;
-            if (elect_one()) {
-  #pragma unroll
-              for (int k = 0; k < 4; ++k) fp8_product(d, hi | (a + 2 * k), hi | (b + 2 * k), p.idesc, k != 0 ? 1u : 0u);
-              pair_commit(empty0 + 8 * stage);
-              pair_commit(smem_u32(&ctl->acc_full[it & 1u]));
+            if (!poll(waiter, full0 + 8 * stage, phase)) { ok = false; break; }
+#pragma unroll
+            for (int h = 0; ok && h < 2; ++h) {
+              const uint32_t acc = (it & 1u) * 2 + h;
+              if (!poll(waiter, smem_u32(&ctl->acc_empty[acc]), ((it >> 1) & 1u) ^ 1u)) { ok = false; break; }
+              tc_fence_after();
+              const uint32_t a = lo0 + stage * (kFp8Stage >> 4), b = a + (kFp8StageA >> 4) + h * (half / 2 * 8), d = tmem_base + acc * (kFp8Cols / 2);
+              if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) fp8_product(d, hi | (a + 2 * k), hi | (b + 2 * k), p.idesc, k != 0 ? 1u : 0u);
+                if (h == 1) pair_commit(empty0 + 8 * stage);
+                pair_commit(smem_u32(&ctl->acc_full[acc]));
+              }
             }
+            if (!ok) break;
             __syncwarp();
             if (++stage == kFp8Stages) { stage = 0; phase ^= 1u; }
           }
+      }
+    } else if (warp == kFp8EpiWarps + 2) {
+      // ------------------------------------------------------------------------------------------- scales
+      uint32_t batch = 0;
+      bool ok = true;
+      const int group = lane & 7, row0 = lane >> 3;      // a lane's group of a batch, and the first of its rows: eight lanes read 32 bytes of a row
+      for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
+        const Fp8Tile g = fp8_tile_at<kGate>(p, *plan, t);
+        const int rows = g.valid - cta * kGroupRows;
+        const float* x = p.x_scales + (int64_t)(g.first + cta * kGroupRows + row0) * p.groups + group;
+        // blocks row0 and row0 + 4 of the eight: those of either side
+        const float* w[2];
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+          const int channel = g.channel0 + side * (half / 2) + 32 * (row0 & 1) + (kGate ? 0 : (row0 >> 1) * half);
+          w[side] = p.w_scales + (((int64_t)g.expert * (kGate ? 2 : 1) + (kGate ? row0 >> 1 : 0)) * p.blocks + min(channel / kScaleBlock, p.blocks - 1)) * p.groups + group;
+        }
+        for (int kb = 0; kb < p.groups; kb += kFp8Batch, ++batch) {
+          if (!poll(waiter, smem_u32(&ctl->scale_empty[batch % kFp8ScaleSlots]), ((batch / kFp8ScaleSlots) & 1u) ^ 1u)) { ok = false; break; }
+          Fp8Scales& to = scales[batch % kFp8ScaleSlots];
+          const bool there = kb + group < p.groups;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) copy_word(smem_u32(&to.w[group][4 * i + row0]), there ? w[i] + kb : p.w_scales, there);
+          const int last = there ? rows - row0 : 0;
+#pragma unroll 8
+          for (int r = 0; r < kGroupRows; r += 4) copy_word(smem_u32(&to.x[group][r + row0]), r < last ? x + (int64_t)r * p.groups + kb : p.x_scales, r < last);
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl->scale_full[batch % kFp8ScaleSlots])) : "memory");
+        }
       }
     }
   }
@@ -323,18 +381,15 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
 // ---------------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------------
-// Columns of a tile: those with which the pair that has most to do ends first.  A group costs 2 clk a column in the tensor cores, or its bytes at 60 a clock
-// into each SM.  The rows of each expert are not known here; a tile of rows for all, and one for every expert beyond the first, is the most there can be.
+// Columns of a tile: 128 where the pair that has most to do ends sooner, at 950 clk a group instead of 1000.  The rows of each expert are not known here; a
+// tile of rows for all, and one for every expert beyond the first, is the most there can be.
 int fp8_cols(const GroupedProduct& p, int pairs) {
   const int64_t row_tiles = (p.rows + 2 * kGroupRows - 1) / (2 * kGroupRows) + std::min(p.experts, p.rows) - 1;
-  int64_t least = INT64_MAX;
-  int best = kFp8Cols;
-  for (int cols = kFp8Cols; cols >= 64; cols -= p.kind == kGated ? 64 : 32) {
+  const auto turns = [&](int cols) {
     const int width = p.kind == kGated ? cols / 2 : cols;
-    const int64_t tiles = row_tiles * ((p.n + width - 1) / width), cost = (tiles + pairs - 1) / pairs * std::max(2 * cols, (kFp8StageA + cols / 2 * 128) / 60);
-    if (cost < least) least = cost, best = cols;
-  }
-  return best;
+    return (row_tiles * ((p.n + width - 1) / width) + pairs - 1) / pairs;
+  };
+  return 950 * turns(kFp8Cols / 2) < 1000 * turns(kFp8Cols) ? kFp8Cols / 2 : kFp8Cols;
 }
 
 cudaError_t launch_fp8_pairs(const GroupedProduct& p, int sms, cudaStream_t s) {
@@ -346,7 +401,7 @@ cudaError_t launch_fp8_pairs(const GroupedProduct& p, int sms, cudaStream_t s) {
   d.col_tiles = (p.n + width - 1) / width;
   d.groups = (p.k + kScaleBlock - 1) / kScaleBlock;
   d.blocks = (p.n + kScaleBlock - 1) / kScaleBlock;
-  d.idesc = product_idesc(kDenseFp16, false, false, 2 * kGroupRows, d.cols);         // format 0: FP16, or in 8 bits E4M3
+  d.idesc = product_idesc(kDenseFp16, false, false, 2 * kGroupRows, d.cols / 2);         // format 0: FP16, or in 8 bits E4M3
   d.x_scales = p.x_scales, d.w_scales = p.w_scales;
   d.epi = p.epi;
   d.status = p.status;
@@ -471,7 +526,7 @@ cudaError_t launch_fp8(const GroupedProduct& p, cudaStream_t s) {
   const int sms = dense_sms();
   if (sms == 0) return cudaErrorNotReady;
   const ChainScope chain(true);
-  return launch_fp8_pairs(p, sms, s);
+  return grouped_few_rows(p) ? launch_grouped_few(p, sms, s) : launch_fp8_pairs(p, sms, s);
 }
 
 cudaError_t launch_quantize_fp8(const void* x, int type, int64_t ld, uint8_t* q, float* scales, int m, int k, cudaStream_t s) {

@@ -112,6 +112,7 @@ int fp8_product(const MmoeFp8Product* a, bool gated, void* stream) {
   p.kind = gated ? mmoe::kGated : mmoe::kLinear;
   p.n = a->channels, p.k = a->width, p.w = a->w, p.x = a->x, p.x_ld = a->x_stride, p.x_scales = a->x_scales, p.w_scales = a->w_scales;
   p.epi.out = a->out, p.epi.ld_out = a->channels, p.epi.out_type = a->out_type, p.epi.inter = a->channels, p.epi.clamp = a->clamp;
+  p.zero_behind = true;
   return run_grouped(p, what, stream);
 }
 

@@ -59,6 +59,11 @@ __device__ __forceinline__ int expert_of(const GroupPlan& plan, int experts, int
   return low;
 }
 
+// Four bytes into shared memory, or zeros
+__device__ __forceinline__ void copy_word(uint32_t dst, const float* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+
 // Zeros from p on, by all threads of the grid
 __device__ __forceinline__ void clear_bytes(char* p, int64_t bytes) {
   const int64_t thread = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, threads = (int64_t)gridDim.x * blockDim.x;
