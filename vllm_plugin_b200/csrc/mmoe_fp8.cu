@@ -10,23 +10,29 @@ namespace {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Products on CTA pairs: out[t, n] = sum over groups kb of 128 k's of (sum_k x[t, k] w[n, k]) sx[t, kb] sw[n / 128, kb].
-// Rows are operand A (256 a tile, 128 in each CTA), weights operand B (256 a tile; gated: half of them gate rows, which the leader stages, the
-// up rows its peer).  The tensor core sums one group into one of two accumulators, in two halves of 128 columns each; the epilogue warps multiply
-// a half by the two scales and add it to FP32 registers, 128 of them a thread, beside the next one's products.  A thread has one row of the tile, so
-// that its scale is one number a group; weights' scales are one for every 32 columns.  (Weights along the lanes instead: a scale for every
-// column and thread, 109 us where this takes 55.)  One warp brings the scales, word by word and up to three batches ahead.
+// Rows are operand A (256 a tile, 128 in each CTA), weights operand B (256 or 128 a tile; gated: half of them gate rows, which the leader stages, the
+// up rows its peer).  The tensor core sums one group into an accumulator of 128 columns, one of four (wide tiles: into two of them, one
+// after the other); the epilogue warps multiply it by the two scales and add it to FP32 registers, beside the next products.  A thread has one row of
+// the tile, so that its scale is one number a group; weights' scales are one for every 32 columns.  (Weights along the lanes instead: a scale for
+// every column and thread, 109 us where this takes 55.)  One warp brings the scales, word by word and up to three batches ahead.
 //
-// What bounds it, 3840 rows: 2304 -> 5120 55 us (1.65 PFLOP/s), gated 5120 -> 2 x 2304 94-103 us (1.8-1.9).  Without the multiplications 39 and 69:
-// the 256 of them that a scheduler has for each group, at most half of it beside the loads from tensor memory, are 250-300 clk of a group's 1000.
-// Without loads and multiplications 38 and 66, of which 32 KB a group into each SM are 700 clk.  Tried: tiles of 192 columns whose sums are
-// all fetched before the accumulator is released, 88; sixteen epilogue warps with 64 columns each, 63; the next group's columns fetched ahead of this
-// one's last multiplications, 59; packed pairs (fma.rn.f32x2), 66, as a move goes with each of them; whole accumulators instead of halves, 60.
+// What bounds it: the power limit, in calls that last.  3840 rows, wide: 2304 -> 5120 55 us in bursts and 59 repeated (1.54-1.65 PFLOP/s, at 1.83 GHz), gated 5120 ->
+// 2 x 2304 92 and 103 us (1.76-1.97, at 1.73 GHz).  With nothing done by the epilogue warps, 38 and 66 us in bursts and 46 and 83 repeated (at 1.55 GHz): that
+// is what products and copies alone would take.  The multiplications are what is left, 256 of a scheduler for each group of 256 columns; loads from
+// tensor memory are hidden.  A group of 256 columns costs 1150 clk, one of 128 columns 700.  Tried, project and gated (54.5, 93): the next group's
+// columns fetched ahead of this one's last multiplications 59, 104; packed pairs (fma.rn.f32x2), with each of which a move goes, 66, 107; sixteen epilogue
+// warps with 64 columns each 63, 97, or with 64 of 128 columns and every other group 74, 116; tiles of 192 columns 88, 160; whole accumulators of
+// 256 columns 60, 101; eight groups' scales by the epilogue warps themselves 60, 102.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int kFp8Cols = 256;                         // most rows of B per tile
+constexpr int kFp8Unit = 128;                         // columns of an accumulator
+constexpr int kFp8Units = kTmemCols / kFp8Unit;
 constexpr int kFp8StageA = kGroupRows * 128;          // bytes
-constexpr int kFp8Stage = kFp8StageA + kFp8Cols / 2 * 128;
-constexpr int kFp8Stages = 4;
-constexpr int kFp8EpiWarps = 8;                       // two per TMEM lane quadrant, each with every other block of columns
+template <bool kWide> constexpr int kFp8Cols = kWide ? 256 : 128;                        // rows of B per tile
+template <bool kWide> constexpr int kFp8Stage = kFp8StageA + kFp8Cols<kWide> / 2 * 128;
+constexpr int kFp8MaxStages = 6;
+template <bool kWide> constexpr int kFp8Stages = kWide ? 5 : kFp8MaxStages;
+constexpr int kFp8RowsApart = 64;
+constexpr int kFp8EpiWarps = 8;                       // two per TMEM lane quadrant: wide, one for either accumulator of a group, else for half of its columns
 constexpr int kFp8Threads = 32 * (4 + kFp8EpiWarps);   // epilogue warps first, producer, issuer, one that fetches scales, one that only hands back registers
 constexpr int kFp8Registers = 216, kFp8FewRegisters = 72;
 static_assert(kFp8EpiWarps * 32 * kFp8Registers + 128 * kFp8FewRegisters <= kFp8Threads * 168, "registers that the block was launched with");
@@ -40,10 +46,10 @@ struct Fp8Scales {
 };
 
 struct Fp8Control {
-  uint64_t full[kFp8Stages];      // leader only: every copy of the stage, in both CTAs, has landed
-  uint64_t empty[kFp8Stages];     // issuer -> producers of both CTAs
-  uint64_t acc_full[4];           // issuer -> epilogues of both CTAs; by accumulator and half
-  uint64_t acc_empty[4];          // leader only: epilogue warps of both CTAs -> issuer
+  uint64_t full[kFp8MaxStages];      // leader only: every copy of the stage, in both CTAs, has landed
+  uint64_t empty[kFp8MaxStages];     // issuer -> producers of both CTAs
+  uint64_t acc_full[kFp8Units];           // issuer -> epilogues of both CTAs
+  uint64_t acc_empty[kFp8Units];          // leader only: epilogue warps of both CTAs -> issuer
   uint64_t scale_full[kFp8ScaleSlots], scale_empty[kFp8ScaleSlots];
   uint32_t tmem_base;
   volatile int32_t abort_flag;
@@ -55,7 +61,7 @@ struct Fp8Params {
   const int32_t* ends;
   int32_t experts, rows;
   int32_t n;                      // channels
-  int32_t cols, col_tiles;        // rows of B per tile (gated: both kinds), tiles of an expert's channels
+  int32_t col_tiles;              // of an expert's channels
   int32_t groups;                 // of k: stages
   int32_t blocks;                 // of channels (gated: of the gate's)
   uint32_t idesc;
@@ -67,7 +73,8 @@ struct Fp8Params {
 
 constexpr int kFp8Smem = 227 * 1024;
 constexpr int kFp8Place = 1024;
-constexpr int kFp8PlanAt = kFp8Place + kFp8Stages * kFp8Stage;
+constexpr int kFp8StageRoom = std::max(kFp8Stages<true> * kFp8Stage<true>, kFp8Stages<false> * kFp8Stage<false>);
+constexpr int kFp8PlanAt = kFp8Place + kFp8StageRoom;
 constexpr int kFp8TurnAt = kFp8PlanAt + (sizeof(GroupPlan) + 15) / 16 * 16;
 static_assert(sizeof(Fp8Control) <= kFp8Place, "control block");
 constexpr int kFp8ScalesAt = kFp8TurnAt + kFp8EpiWarps * kFp8Turn;
@@ -77,13 +84,13 @@ struct Fp8Tile {
   int expert, channel0;
   int first, valid;               // rows, of the pair
 };
-template <bool kGate>
+template <bool kGate, bool kWide>
 __device__ __forceinline__ Fp8Tile fp8_tile_at(const Fp8Params& p, const GroupPlan& plan, int t) {
   Fp8Tile g;
   g.expert = expert_of(plan, p.experts, t);
   const int start = plan.start[g.expert], count = plan.start[g.expert + 1] - start, parts = (count + 2 * kGroupRows - 1) / (2 * kGroupRows);
   const int in = t - plan.tile[g.expert], at = in % parts * 2 * kGroupRows;
-  g.channel0 = in / parts * (kGate ? p.cols / 2 : p.cols);
+  g.channel0 = in / parts * (kGate ? kFp8Cols<kWide> / 2 : kFp8Cols<kWide>);
   g.first = start + at, g.valid = min(count - at, 2 * kGroupRows);
   return g;
 }
@@ -111,7 +118,7 @@ __device__ __forceinline__ bool wait_here(DenseWaiter& w, uint32_t bar, uint32_t
   return __all_sync(0xffffffffu, ok) || w.wait_uniform(bar, parity);
 }
 
-template <bool kGate>
+template <bool kGate, bool kWide>
 __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the same offset in both CTAs
@@ -120,18 +127,21 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
   GroupPlan* plan = reinterpret_cast<GroupPlan*>(smem + kFp8PlanAt);
   Fp8Scales* scales = reinterpret_cast<Fp8Scales*>(smem + kFp8ScalesAt);
 
+  constexpr int kStages = kFp8Stages<kWide>, kStage = kFp8Stage<kWide>, half = kFp8Cols<kWide> / 2;
+  constexpr int kBlocks = kWide ? 4 : 2;                // of 32 columns, that an epilogue warp has
+
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int cta = static_cast<int>(cluster_ctarank());
   if (threadIdx.x == 0) {
     prefetch_map(&p.map_w);
     for (int i = 0; i < 4; ++i) prefetch_map(&p.map_x[i]);
-    for (int i = 0; i < kFp8Stages; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(&ctl->full[i]), 1);
       mbar_init(smem_u32(&ctl->empty[i]), 1);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kFp8Units; ++i) {
       mbar_init(smem_u32(&ctl->acc_full[i]), 1);
-      mbar_init(smem_u32(&ctl->acc_empty[i]), kFp8EpiWarps);
+      mbar_init(smem_u32(&ctl->acc_empty[i]), kWide ? kFp8EpiWarps : 2 * kFp8EpiWarps);
     }
     for (int i = 0; i < kFp8ScaleSlots; ++i) {
       mbar_init(smem_u32(&ctl->scale_full[i]), 32);
@@ -152,7 +162,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
   chain_release();                          // in this order: what precedes this launch is complete when the next one starts
   const int tiles = make_plan(plan, p.ends, p.experts, p.rows, 2 * kGroupRows, p.col_tiles, p.status);
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
-  const int step = gridDim.x / 2, half = p.cols / 2;
+  const int step = gridDim.x / 2;
   DenseWaiter waiter{{&ctl->abort_flag, p.status, 0, kStatusGrouped + 1, warp}, p.timeout_ns};
   const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
   {
@@ -168,33 +178,31 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
     const uint32_t leader_empty = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
     const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
     uint8_t* turn = smem + kFp8TurnAt + warp * kFp8Turn;
-    uint32_t batch = 0, phase = 0, second = 0;
-    uint32_t full_at = smem_u32(&ctl->acc_full[side]), empty_at = leader_empty + 8 * side, d = tmem_base + side * (kFp8Cols / 2) + lanes;
-    const uint32_t full_flip = full_at ^ (full_at + 16), full_flip2 = empty_at ^ (empty_at + 16);
+    const uint32_t full = smem_u32(&ctl->acc_full[0]), sums = tmem_base + lanes;
+    uint32_t batch = 0, phase = 0, unit = kWide ? side : 0;        // the accumulator whose turn it is; wide: those of this warp's half of the columns
     bool ok = true;
-    // this warp's four blocks of 32 columns: the tile's column, and the channel behind the tile's first
-    const int quarter = half / 2;                     // of the tile's columns: a half has those of the leader's weights and its peer's
-    const auto column = [&](int b) { return (b >> 1) * quarter + 32 * (b & 1); };
-    const auto channel = [&](int b) { return side * quarter + 32 * (b & 1) + (kGate ? 0 : (b >> 1) * half); };
-    const int width = kGate ? half : p.cols;          // channels of a tile
+    // this warp's blocks of 32 columns: the accumulator's column, and the channel behind the tile's first
+    const auto column = [&](int b) { return kWide ? 32 * b : kGate ? kFp8Unit / 2 * b + 32 * side : 64 * side + 32 * b; };
+    const auto channel = [&](int b) { return kWide ? 64 * side + 32 * (b & 1) + (kGate ? 0 : (b >> 1) * half) : kGate ? 32 * side : 64 * side + 32 * b; };
     for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
-      const Fp8Tile g = fp8_tile_at<kGate>(p, *plan, t);
+      const Fp8Tile g = fp8_tile_at<kGate, kWide>(p, *plan, t);
       const int row0 = g.first + cta * kGroupRows + quadrant * 32, rows = g.valid - cta * kGroupRows - quadrant * 32;      // of this warp
-      const int channels = min(width, p.n - g.channel0);
+      const int channels = p.n - g.channel0;
       const bool any = rows > 0 && channel(0) < channels;
-      float sum[4][32] = {};
+      float sum[kBlocks][32] = {};
       for (int kb = 0; ok && kb < p.groups; kb += kFp8Batch, ++batch) {
         if (!wait_here(waiter, smem_u32(&ctl->scale_full[batch % kFp8ScaleSlots]), (batch / kFp8ScaleSlots) & 1u)) { ok = false; break; }
         const Fp8Scales& now = scales[batch % kFp8ScaleSlots];
         uint32_t x_at = smem_u32(&now.x[0][quadrant * 32 + lane]), w_at = smem_u32(&now.w[0][4 * side]);
         const int count = min(kFp8Batch, p.groups - kb);
         for (int j = 0; j < count; ++j) {
-          if (!wait_here(waiter, full_at, phase)) { ok = false; break; }
+          if (!wait_here(waiter, full + 8 * unit, phase)) { ok = false; break; }
           tc_fence_after();
           if (any) {
+            const uint32_t d = sums + kFp8Unit * unit;
             uint32_t v[2][32];
-            tc_ld32(d, v[0]);
-            tc_ld32(d + 32, v[1]);
+            tc_ld32(d + column(0), v[0]);
+            tc_ld32(d + column(1), v[1]);
             float x_now, w0, w1, w2, w3;
             asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x_now) : "r"(x_at));
             asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w0), "=f"(w1), "=f"(w2), "=f"(w3) : "r"(w_at));
@@ -203,25 +211,34 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
 #pragma unroll
               for (int i = 0; i < 32; ++i) sum[b][i] = fmaf(__uint_as_float(v[b & 1][i]), s, sum[b][i]);
             };
+            const auto release = [&] {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_pair(leader_empty + 8 * unit);
+            };
             tc_ld_wait();
-            add(0, w0);
-            tc_ld32(d + column(2), v[0]);
-            add(1, w1);
-            tc_ld32(d + column(2) + 32, v[1]);
-            tc_ld_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_pair(empty_at);
-            add(2, w2);
-            add(3, w3);
+            if constexpr (kWide) {
+              add(0, w0);
+              tc_ld32(d + column(2), v[0]);
+              add(1, w1);
+              tc_ld32(d + column(3), v[1]);
+              tc_ld_wait();
+              release();
+              add(2, w2);
+              add(3, w3);
+            } else {
+              release();
+              add(0, w0);
+              add(1, w1);
+            }
           } else {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_pair(empty_at);
+            if (lane == 0) mbar_arrive_pair(leader_empty + 8 * unit);
           }
           x_at += sizeof(now.x[0]), w_at += sizeof(now.w[0]);
-          phase ^= second;                       // a phase has both accumulators
-          full_at ^= full_flip, empty_at ^= full_flip2, d ^= kFp8Cols, second ^= 1u;
+          unit = kWide ? unit ^ 2u : (unit + 1) % kFp8Units;
+          phase ^= (kWide ? unit < 2 : unit == 0) ? 1u : 0u;         // a phase has all accumulators
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&ctl->scale_empty[batch % kFp8ScaleSlots]));
@@ -230,13 +247,14 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
       // ---- results: rows of two neighbouring blocks, 64 channels
       const bool dense_rows = p.epi.out_type == kDenseFp32 ? p.n % 4 == 0 : p.n % 8 == 0;
 #pragma unroll
-      for (int pair = 0; pair < (kGate ? 1 : 2); ++pair) {
-        const int first = channel(2 * pair), count = min(quarter, channels - first);
+      for (int run = 0; run < (kGate ? 1 : kBlocks / 2); ++run) {
+        constexpr int kRun = kGate ? 16 * kBlocks : 64;    // neighbouring channels
+        const int first = channel(2 * run), count = min(kRun, channels - first);
         if (count <= 0) continue;
         const auto value = [&](int j) {                  // of channel first + j
-          const float f = sum[2 * pair + (j >> 5)][j & 31];
+          const float f = sum[2 * run + (j >> 5)][j & 31];
           if (!kGate) return f;
-          const float u = sum[2 + (j >> 5)][j & 31];
+          const float u = sum[kBlocks / 2 + (j >> 5)][j & 31];
           return p.epi.out_type == kDenseFp32 ? gated_value_fp32(f, u, p.epi.clamp) : gated_value(f, u, p.epi.clamp);
         };
         const auto put = [&](auto* out) {
@@ -244,10 +262,11 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
           constexpr int kEach = 16 / sizeof(T), kPart = 128 / sizeof(T), kStride = 144;       // 144: no two of eight rows in one bank
           out += (int64_t)row0 * p.epi.ld_out + g.channel0 + first;
 #pragma unroll
-          for (int part = 0; part < 64 / kPart; ++part) {     // 128 bytes of every row
+          for (int part = 0; part < (kRun + kPart - 1) / kPart; ++part) {     // 128 bytes of every row
             __syncwarp();                                 // what was there has been read
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
+              if (part * kPart + j * kEach >= kRun) break;
               __align__(16) T piece[kEach];
 #pragma unroll
               for (int i = 0; i < kEach; ++i) piece[i] = from_float<T>(value(part * kPart + j * kEach + i));
@@ -283,13 +302,13 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
       const uint32_t leader_full0 = map_to_cta(full0, 0), base = smem_u32(stages);
       bool ok = true;
       for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
-        const Fp8Tile g = fp8_tile_at<kGate>(p, *plan, t);
+        const Fp8Tile g = fp8_tile_at<kGate, kWide>(p, *plan, t);
         const int rows = fp8_rows_staged(g.valid, cta), x_row = g.first + cta * kGroupRows;
         const uint32_t tx = (fp8_rows_staged(g.valid, 0) + fp8_rows_staged(g.valid, 1)) * 128 + 2 * half * 128;
         const int w_row = kGate ? g.channel0 : g.channel0 + cta * half, part = kGate ? cta : 0;
         for (int kb = 0; kb < p.groups; ++kb) {
           if (!waiter.wait_uniform(empty0 + 8 * stage, phase ^ 1u)) { ok = false; break; }
-          const uint32_t bar = leader_full0 + 8 * stage, a = base + stage * kFp8Stage;
+          const uint32_t bar = leader_full0 + 8 * stage, a = base + stage * kStage;
           if (elect_one()) {
             if (cta == 0) mbar_expect_tx(full0 + 8 * stage, tx);
             pair_load_4d(a + kFp8StageA, &p.map_w, kb * 128, w_row, part, g.expert, bar);
@@ -302,7 +321,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
               }
           }
           __syncwarp();
-          if (++stage == kFp8Stages) { stage = 0; phase ^= 1u; }
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
       }
     } else if (warp == kFp8EpiWarps + 1) {
@@ -317,21 +336,21 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
           for (int kb = 0; kb < p.groups; ++kb, ++it) {
             if (!poll(waiter, full0 + 8 * stage, phase)) { ok = false; break; }
 #pragma unroll
-            for (int h = 0; ok && h < 2; ++h) {
-              const uint32_t acc = (it & 1u) * 2 + h;
-              if (!poll(waiter, smem_u32(&ctl->acc_empty[acc]), ((it >> 1) & 1u) ^ 1u)) { ok = false; break; }
+            for (int h = 0; ok && h < (kWide ? 2 : 1); ++h) {
+              const uint32_t acc = kWide ? (it & 1u) * 2 + h : it % kFp8Units;
+              if (!poll(waiter, smem_u32(&ctl->acc_empty[acc]), ((kWide ? it >> 1 : it / kFp8Units) & 1u) ^ 1u)) { ok = false; break; }
               tc_fence_after();
-              const uint32_t a = lo0 + stage * (kFp8Stage >> 4), b = a + (kFp8StageA >> 4) + h * (half / 2 * 8), d = tmem_base + acc * (kFp8Cols / 2);
+              const uint32_t a = lo0 + stage * (kStage >> 4), b = a + (kFp8StageA >> 4) + h * (kFp8Unit / 2 * 8), d = tmem_base + acc * kFp8Unit;
               if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) fp8_product(d, hi | (a + 2 * k), hi | (b + 2 * k), p.idesc, k != 0 ? 1u : 0u);
-                if (h == 1) pair_commit(empty0 + 8 * stage);
+                if (h == (kWide ? 1 : 0)) pair_commit(empty0 + 8 * stage);
                 pair_commit(smem_u32(&ctl->acc_full[acc]));
               }
             }
             if (!ok) break;
             __syncwarp();
-            if (++stage == kFp8Stages) { stage = 0; phase ^= 1u; }
+            if (++stage == kStages) { stage = 0; phase ^= 1u; }
           }
       }
     } else if (warp == kFp8EpiWarps + 2) {
@@ -340,15 +359,16 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
       bool ok = true;
       const int group = lane & 7, row0 = lane >> 3;      // a lane's group of a batch, and the first of its rows: eight lanes read 32 bytes of a row
       for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
-        const Fp8Tile g = fp8_tile_at<kGate>(p, *plan, t);
+        const Fp8Tile g = fp8_tile_at<kGate, kWide>(p, *plan, t);
         const int rows = g.valid - cta * kGroupRows;
         const float* x = p.x_scales + (int64_t)(g.first + cta * kGroupRows + row0) * p.groups + group;
         // blocks row0 and row0 + 4 of the eight: those of either side
         const float* w[2];
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
-          const int channel = g.channel0 + side * (half / 2) + 32 * (row0 & 1) + (kGate ? 0 : (row0 >> 1) * half);
-          w[side] = p.w_scales + (((int64_t)g.expert * (kGate ? 2 : 1) + (kGate ? row0 >> 1 : 0)) * p.blocks + min(channel / kScaleBlock, p.blocks - 1)) * p.groups + group;
+          const int up = !kGate ? 0 : kWide ? row0 >> 1 : row0 & 1;
+          const int channel = g.channel0 + (kWide ? 64 * side + 32 * (row0 & 1) + (kGate ? 0 : (row0 >> 1) * half) : kGate ? 32 * side : 64 * side + 32 * (row0 & 1));
+          w[side] = p.w_scales + (((int64_t)g.expert * (kGate ? 2 : 1) + up) * p.blocks + min(channel / kScaleBlock, p.blocks - 1)) * p.groups + group;
         }
         for (int kb = 0; kb < p.groups; kb += kFp8Batch, ++batch) {
           if (!poll(waiter, smem_u32(&ctl->scale_empty[batch % kFp8ScaleSlots]), ((batch / kFp8ScaleSlots) & 1u) ^ 1u)) { ok = false; break; }
@@ -381,41 +401,64 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
 // ---------------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------------
-// Columns of a tile: 128 where the pair that has most to do ends sooner, at 950 clk a group instead of 1000.  The rows of each expert are not known here; a
-// tile of rows for all, and one for every expert beyond the first, is the most there can be.
-int fp8_cols(const GroupedProduct& p, int pairs) {
-  const int64_t row_tiles = (p.rows + 2 * kGroupRows - 1) / (2 * kGroupRows) + std::min(p.experts, p.rows) - 1;
-  const auto turns = [&](int cols) {
-    const int width = p.kind == kGated ? cols / 2 : cols;
-    return (row_tiles * ((p.n + width - 1) / width) + pairs - 1) / pairs;
-  };
-  return 950 * turns(kFp8Cols / 2) < 1000 * turns(kFp8Cols) ? kFp8Cols / 2 : kFp8Cols;
+// What the pair that has most to do costs, in clocks a group of k.  The rows of each expert are not known here; a tile of rows for all, and one for every
+// expert beyond the first, is the most there can be.
+int64_t fp8_cost(const GroupedProduct& p, int rows, int pairs, bool wide) {
+  const int64_t row_tiles = (rows + 2 * kGroupRows - 1) / (2 * kGroupRows) + std::min(p.experts, rows) - 1;
+  const int cols = wide ? kFp8Cols<true> : kFp8Cols<false>, width = p.kind == kGated ? cols / 2 : cols;
+  return (row_tiles * ((p.n + width - 1) / width) + pairs - 1) / pairs * (wide ? 1150 : 700);
+}
+// 777 rows, 5120 -> 5003: 48.1 us wide (80 tiles, two turns of 74 pairs), 44.5 narrow (160, three)
+bool fp8_wide(const GroupedProduct& p, int pairs) { return fp8_cost(p, p.rows, pairs, true) <= fp8_cost(p, p.rows, pairs, false); }
+
+// Rows of one weight beyond the last tile of 256 that are better off in a launch of few rows: what that costs is the weights' bytes and its start.
+// 0: none.
+int fp8_rows_apart(const GroupedProduct& p, int pairs) {
+  const int last = p.rows % (2 * kGroupRows);
+  if (p.ends != nullptr || last == 0 || last == p.rows || last > kFp8RowsApart) return 0;
+  const int64_t groups = (p.k + kScaleBlock - 1) / kScaleBlock, apart = (int64_t)p.n * (p.kind == kGated ? 2 : 1) * p.k / 4450 + 6000;
+  const auto best = [&](int rows) { return groups * std::min(fp8_cost(p, rows, pairs, true), fp8_cost(p, rows, pairs, false)); };
+  return best(p.rows - last) + apart < best(p.rows) ? last : 0;
+}
+
+template <typename F>
+cudaError_t for_each_fp8_kernel(F f) {
+  cudaError_t e = f(fp8_pair_kernel<false, false>, false, false);
+  if (e == cudaSuccess) e = f(fp8_pair_kernel<false, true>, false, true);
+  if (e == cudaSuccess) e = f(fp8_pair_kernel<true, false>, true, false);
+  if (e == cudaSuccess) e = f(fp8_pair_kernel<true, true>, true, true);
+  return e;
 }
 
 cudaError_t launch_fp8_pairs(const GroupedProduct& p, int sms, cudaStream_t s) {
   Fp8Params d = {};
   const bool gate = p.kind == kGated;
   d.ends = p.ends, d.experts = p.experts, d.rows = p.rows, d.n = p.n;
-  d.cols = fp8_cols(p, sms / 2);
-  const int width = gate ? d.cols / 2 : d.cols;
+  const bool wide = fp8_wide(p, sms / 2);
+  const int width = gate ? (wide ? kFp8Cols<true> : kFp8Cols<false>) / 2 : (wide ? kFp8Cols<true> : kFp8Cols<false>);
   d.col_tiles = (p.n + width - 1) / width;
   d.groups = (p.k + kScaleBlock - 1) / kScaleBlock;
   d.blocks = (p.n + kScaleBlock - 1) / kScaleBlock;
-  d.idesc = product_idesc(kDenseFp16, false, false, 2 * kGroupRows, d.cols / 2);         // format 0: FP16, or in 8 bits E4M3
+  d.idesc = product_idesc(kDenseFp16, false, false, 2 * kGroupRows, kFp8Unit);         // format 0: FP16, or in 8 bits E4M3
   d.x_scales = p.x_scales, d.w_scales = p.w_scales;
   d.epi = p.epi;
   d.status = p.status;
   d.timeout_ns = (p.timeout_ms > 0 ? (int64_t)p.timeout_ms : 2000) * 1000000ll;
   const uint64_t n = p.n, k = p.k, parts = gate ? 2 : 1;
   bool ok = encode_map(&d.map_w, kGroupedE4m3, p.w, 4, {k, n, parts, static_cast<uint64_t>(p.experts), 1}, {k, n * k, parts * n * k, 0},
-                       {128, static_cast<uint32_t>(d.cols / 2), 1, 1, 1});
+                       {128, static_cast<uint32_t>((wide ? kFp8Cols<true> : kFp8Cols<false>) / 2), 1, 1, 1});
   for (int i = 0; ok && i < 4; ++i)
     ok = encode_map(&d.map_x[i], kGroupedE4m3, p.x, 2, {k, static_cast<uint64_t>(p.rows), 1, 1, 1}, {static_cast<uint64_t>(p.x_ld), 0, 0, 0}, {128, 128u >> i, 1, 1, 1});
   const int64_t most = ((int64_t)p.rows / (2 * kGroupRows) + std::min(p.experts, p.rows)) * d.col_tiles;
   if (!ok || most > INT32_MAX / 2) return cudaErrorInvalidValue;
   const int grid = 2 * static_cast<int>(std::min<int64_t>(sms / 2, most));
-  return gate ? launch_clustered(fp8_pair_kernel<true>, dim3(grid), dim3(kFp8Threads), kFp8Smem, 2, s, d)
-              : launch_clustered(fp8_pair_kernel<false>, dim3(grid), dim3(kFp8Threads), kFp8Smem, 2, s, d);
+  bool found = false;
+  const cudaError_t e = for_each_fp8_kernel([&](auto kernel, bool k_gate, bool k_wide) {
+    if (k_gate != gate || k_wide != wide) return cudaSuccess;
+    found = true;
+    return launch_clustered(kernel, dim3(grid), dim3(kFp8Threads), kFp8Smem, 2, s, d);
+  });
+  return found ? e : cudaErrorInvalidValue;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -517,16 +560,23 @@ cudaError_t launch_quantize(const void* x, int64_t ld, uint8_t* q, float* scales
 }  // namespace
 
 cudaError_t prepare_fp8() {
-  cudaError_t e = cudaFuncSetAttribute(fp8_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8Smem);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8Smem);
-  return e;
+  return for_each_fp8_kernel([](auto kernel, bool, bool) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8Smem); });
 }
 
 cudaError_t launch_fp8(const GroupedProduct& p, cudaStream_t s) {
   const int sms = dense_sms();
   if (sms == 0) return cudaErrorNotReady;
   const ChainScope chain(true);
-  return grouped_few_rows(p) ? launch_grouped_few(p, sms, s) : launch_fp8_pairs(p, sms, s);
+  if (grouped_few_rows(p)) return launch_grouped_few(p, sms, s);
+  const int apart = fp8_rows_apart(p, sms / 2);
+  if (apart == 0) return launch_fp8_pairs(p, sms, s);
+  GroupedProduct first = p, last = p;
+  first.rows = p.rows - apart, last.rows = apart;
+  last.x = static_cast<const uint8_t*>(p.x) + first.rows * p.x_ld;
+  last.x_scales = p.x_scales + (int64_t)first.rows * ((p.k + kScaleBlock - 1) / kScaleBlock);
+  last.epi.out = static_cast<uint8_t*>(p.epi.out) + first.rows * p.epi.ld_out * (p.epi.out_type == kDenseFp32 ? 4 : 2);
+  const cudaError_t e = launch_fp8_pairs(first, sms, s);
+  return e == cudaSuccess ? launch_grouped_few(last, sms, s) : e;
 }
 
 cudaError_t launch_quantize_fp8(const void* x, int type, int64_t ld, uint8_t* q, float* scales, int m, int k, cudaStream_t s) {
