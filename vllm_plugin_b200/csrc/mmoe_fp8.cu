@@ -31,7 +31,7 @@ template <bool kWide> constexpr int kFp8Cols = kWide ? 256 : 128;               
 template <bool kWide> constexpr int kFp8Stage = kFp8StageA + kFp8Cols<kWide> / 2 * 128;
 constexpr int kFp8MaxStages = 6;
 template <bool kWide> constexpr int kFp8Stages = kWide ? 5 : kFp8MaxStages;
-constexpr int kFp8RowsApart = 64;
+constexpr int kFp8RowsApart = 48;
 constexpr int kFp8EpiWarps = 8;                       // two per TMEM lane quadrant: wide, one for either accumulator of a group, else for half of its columns
 constexpr int kFp8Threads = 32 * (4 + kFp8EpiWarps);   // epilogue warps first, producer, issuer, one that fetches scales, one that only hands back registers
 constexpr int kFp8Registers = 216, kFp8FewRegisters = 72;
@@ -567,7 +567,7 @@ cudaError_t launch_fp8(const GroupedProduct& p, cudaStream_t s) {
   const int sms = dense_sms();
   if (sms == 0) return cudaErrorNotReady;
   const ChainScope chain(true);
-  if (grouped_few_rows(p)) return launch_grouped_few(p, sms, s);
+  if (grouped_few_rows(p, sms)) return launch_grouped_few(p, sms, s);
   const int apart = fp8_rows_apart(p, sms / 2);
   if (apart == 0) return launch_fp8_pairs(p, sms, s);
   GroupedProduct first = p, last = p;

@@ -501,7 +501,7 @@ cudaError_t launch_grouped(const GroupedProduct& p, cudaStream_t s) {
   const int sms = dense_sms();
   if (sms == 0) return cudaErrorNotReady;
   const ChainScope chain(true);
-  return grouped_few_rows(p) ? launch_grouped_few(p, sms, s) : launch_group_pairs(p, sms, s);
+  return grouped_few_rows(p, sms) ? launch_grouped_few(p, sms, s) : launch_group_pairs(p, sms, s);
 }
 
 }  // namespace mmoe

@@ -39,7 +39,7 @@ cudaError_t prepare_fp8();
 cudaError_t prepare_grouped_few();
 cudaError_t launch_grouped(const GroupedProduct& p, cudaStream_t s);      // 16 bits
 cudaError_t launch_fp8(const GroupedProduct& p, cudaStream_t s);          // E4M3; rows behind the last expert's are set to zero
-bool grouped_few_rows(const GroupedProduct& p);         // it goes to launch_grouped_few by itself
+bool grouped_few_rows(const GroupedProduct& p, int sms);       // it goes to launch_grouped_few
 cudaError_t launch_grouped_few(const GroupedProduct& p, int sms, cudaStream_t s);
 cudaError_t launch_quantize_fp8(const void* x, int type, int64_t ld, uint8_t* q, float* scales, int m, int k, cudaStream_t s);
 

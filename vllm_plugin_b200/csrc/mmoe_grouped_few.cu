@@ -382,8 +382,15 @@ cudaError_t for_each_few_kernel(F f) {
 
 }  // namespace
 
-bool grouped_few_rows(const GroupedProduct& p) {
-  return !p.w_k_rows && (p.kind == kLinear || p.kind == kGated) && p.rows <= 16 * p.experts + 48;
+// Against pairs, 5120 x 5120 of one expert: 16 bits, 16 rows 17.6 -> 11.1 us, 64 18.2 -> 13.9, 96 19.9 -> 20.7; 8 bits, 16 rows 15.8 -> 8.8, 48 16.1 -> 12.3, 96
+// 16.6 -> 20.5, gated 5120 -> 2 x 2304, 48 rows 16.8 -> 17.0.  More experts, 8 bits, gated: 8 experts, 256 rows 50.8 -> 36.0, 384 52.4 -> 55.7; 48 experts, 384
+// rows 257 -> 183, 1536 276 -> 202.  16 bits, 2304 -> 5120, where the tiles are more than run at once: 8 experts, 64 rows 38.5 -> 41.6; 48 experts, 384 rows
+// 176 -> 184; six of them, 240 tiles, 29.1 -> 28.0.
+bool grouped_few_rows(const GroupedProduct& p, int sms) {
+  if (p.w_k_rows || (p.kind != kLinear && p.kind != kGated)) return false;
+  if (p.type == kGroupedE4m3) return p.rows <= 40 * (int64_t)p.experts + 8;
+  const int width = p.kind == kGated ? kFewRows / 2 : kFewRows;
+  return p.rows <= kFewCols * (int64_t)p.experts && (int64_t)std::min(p.experts, p.rows) * ((p.n + width - 1) / width) <= 2 * sms;
 }
 
 cudaError_t prepare_grouped_few() {
