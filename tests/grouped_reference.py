@@ -65,7 +65,7 @@ def quantize(x):
     """E4M3 values and FP32 scales, exactly: the nearest of the type's 253 finite numbers, on a border the one whose last bit is 0."""
     x = x.double()
     lead, width = x.shape[:-1], x.shape[-1]
-    groups = torch.nn.functional.pad(x, (0, -width % BLOCK)).reshape(*lead, -1, BLOCK)
+    groups = torch.nn.functional.pad(x, (0, -width % BLOCK)).reshape(*lead, -(-width // BLOCK), BLOCK)
     amax = groups.abs().amax(-1)
     scale = torch.where(amax == 0, 1.0, (amax / 448).float().double())
     bad = ~torch.isfinite(amax)
@@ -75,7 +75,7 @@ def quantize(x):
     ratio = torch.where(bad[..., None], 0.0, groups / scale[..., None])
     low, high = torch.bucketize(ratio.abs(), borders), torch.bucketize(ratio.abs(), borders, right=True)
     q = codes[torch.where(low % 2 == 0, low, high)] * torch.where(ratio.signbit(), -1.0, 1.0)
-    return q.reshape(*lead, -1)[..., :width], scale.float()
+    return q.flatten(-2)[..., :width], scale.float()
 
 
 def spread(scales, rows, cols, parts=0):
