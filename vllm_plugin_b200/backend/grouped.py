@@ -29,7 +29,26 @@ _tracing, _dispatch_modes, _function_modes = _d._tracing, _d._dispatch_modes, _d
 # ---------------------------------------------------------------------------------------------------------------------
 # arguments
 # ---------------------------------------------------------------------------------------------------------------------
-def _refuse_weights(w, what, dtype, index):
+# A call that is right is told by one condition; what is wrong with any other is looked for afterwards.
+_INT32 = torch.int32
+
+
+def _refuse_rows(x: torch.Tensor, what: str) -> None:
+    if not x.is_cuda:
+        raise RuntimeError(f"{what} runs on the GPU only (there is no CPU path).")
+    if x.dtype not in _d._FF_TYPES or x.dim() != 2:
+        raise AssertionError(f"x must be BF16 or FP16 (T, width), got {tuple(x.shape)} {x.dtype}")
+    if x.shape[0] > _d._MOST_TOKENS:
+        raise _d._too_many(x.shape[0])
+
+
+def _weights_fit(w: torch.Tensor, dtype: torch.dtype, index: int) -> bool:
+    return w.dtype is dtype and w.dim() == 3 and w.is_contiguous() and w.data_ptr() % 16 == 0 and w.get_device() == index
+
+
+def _check_weights(w: torch.Tensor, what: str, dtype: torch.dtype, index: int) -> None:
+    if _weights_fit(w, dtype, index):
+        return
     if w.dim() != 3 or w.dtype != dtype:
         raise AssertionError(f"{what} must be 3-D {dtype} (experts first), got {tuple(w.shape)} {w.dtype}")
     if w.get_device() != index:
@@ -37,14 +56,8 @@ def _refuse_weights(w, what, dtype, index):
     raise AssertionError(f"{what} must be contiguous and 16-byte aligned")
 
 
-def _check_weights(w: torch.Tensor, what: str, dtype: torch.dtype, index: int) -> None:
-    if w.dtype is not dtype or w.dim() != 3 or not w.is_contiguous() or w.data_ptr() % 16 != 0 or w.get_device() != index:
-        _refuse_weights(w, what, dtype, index)
-
-
-def _check_ends(ends: torch.Tensor, experts: int, index: int) -> torch.Tensor:
-    """``ends``, dense."""
-    if not isinstance(ends, torch.Tensor) or ends.dtype is not torch.int32 or ends.get_device() != index or ends.shape != (experts,):
+def _dense_ends(ends: torch.Tensor, experts: int, index: int) -> torch.Tensor:
+    if not isinstance(ends, torch.Tensor) or ends.dtype is not _INT32 or ends.get_device() != index or ends.shape != (experts,):
         got = f"{tuple(ends.shape)} {ends.dtype} on {ends.device}" if isinstance(ends, torch.Tensor) else repr(type(ends))
         raise AssertionError(f"ends must be int32 ({experts},) on cuda:{index}, got {got}")
     if not 1 <= experts <= _MOST_EXPERTS:
@@ -52,19 +65,24 @@ def _check_ends(ends: torch.Tensor, experts: int, index: int) -> torch.Tensor:
     return ends if ends.is_contiguous() else ends.contiguous()
 
 
-def _check_sizes(step: int, **sizes: int) -> None:
-    for name, size in sizes.items():
-        if size <= 0 or size % step != 0 or size > _MOST_WIDTH:
-            raise AssertionError(f"{name}={size} must be a positive multiple of {step}, at most {_MOST_WIDTH}")
+def _size_fits(size: int, step: int) -> bool:
+    return 0 < size <= _MOST_WIDTH and size % step == 0
+
+
+def _refuse_size(name: str, size: int, step: int) -> None:
+    raise AssertionError(f"{name}={size} must be a positive multiple of {step}, at most {_MOST_WIDTH}")
+
+
+def _check_sizes(step: int, a: str, first: int, b: str, second: int) -> None:
+    if not _size_fits(first, step):
+        _refuse_size(a, first, step)
+    if not _size_fits(second, step):
+        _refuse_size(b, second, step)
 
 
 def _check_rows(x: torch.Tensor, what: str) -> None:
-    if not x.is_cuda:
-        raise RuntimeError(f"{what} runs on the GPU only (there is no CPU path).")
-    if x.dtype not in _d._FF_TYPES or x.dim() != 2:
-        raise AssertionError(f"x must be BF16 or FP16 (T, width), got {tuple(x.shape)} {x.dtype}")
-    if x.shape[0] > _d._MOST_TOKENS:
-        raise _d._too_many(x.shape[0])
+    if x.dtype not in _d._FF_TYPES or x.dim() != 2 or not x.is_cuda or x.shape[0] > _d._MOST_TOKENS:
+        _refuse_rows(x, what)
 
 
 def _dense_gradient(dy: torch.Tensor) -> torch.Tensor:
@@ -90,14 +108,16 @@ def _keep(ctx, x, x2, *more) -> None:
 # ---------------------------------------------------------------------------------------------------------------------
 def _projection_of(x2, w, ends, out):
     experts, channels, width = w.shape
-    return _native.MmoeGroupedProduct(_d._CODES[x2.dtype], x2.shape[0], experts, width, channels, 0, _d._stride(x2), x2.data_ptr(), w.data_ptr(),
-                                      ends.data_ptr(), _ptr(out))
+    rows = x2.shape[0]
+    return _native.MmoeGroupedProduct(_d._CODES[x2.dtype], rows, experts, width, channels, 0, x2.stride(0) if rows > 1 else width, x2.data_ptr(), w.data_ptr(),
+                                      ends.data_ptr(), out)
 
 
 def _launch_projection(x2, w, ends):
-    out = x2.new_empty((x2.shape[0], w.shape[1]))
-    if x2.shape[0] > 0:
-        _d._launch((_d._lib or _d._library()).mmoe_grouped_projection, x2.get_device(), _projection_of(x2, w, ends, out))
+    rows = x2.shape[0]
+    out = x2.new_empty((rows, w.shape[1]))
+    if rows > 0:
+        _d._launch((_d._lib or _d._library()).mmoe_grouped_projection, x2.get_device(), _projection_of(x2, w, ends, out.data_ptr()))
     return out
 
 
@@ -143,8 +163,8 @@ def grouped_projection(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor) -> 
     experts, channels, width = w.shape
     if x.shape[1] != width:
         raise AssertionError(f"expected x (T, K) and w (E, N, K), got {tuple(x.shape)} and {tuple(w.shape)}")
-    _check_sizes(8, K=width, N=channels)
-    ends = _check_ends(ends, experts, index)
+    _check_sizes(8, "K", width, "N", channels)
+    ends = _dense_ends(ends, experts, index)
     if _forward_ad._current_level >= 0:
         _d._refuse_tangents("grouped_projection", x, w)
     if not ((x.requires_grad or w.requires_grad) and torch.is_grad_enabled()):
@@ -228,8 +248,8 @@ def grouped_feed_forward(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, e
     experts, hidden, inter = w2.shape
     if x.shape[1] != hidden or w13.shape != (experts, 2 * inter, hidden):
         raise AssertionError(f"expected x (T, H), w13 (E, 2 I, H) and w2 (E, H, I), got {tuple(x.shape)}, {tuple(w13.shape)} and {tuple(w2.shape)}")
-    _check_sizes(8, H=hidden, I=inter)
-    ends = _check_ends(ends, experts, index)
+    _check_sizes(8, "H", hidden, "I", inter)
+    ends = _dense_ends(ends, experts, index)
     clamp = _d._clamp_of(activation_clamp)
     if _forward_ad._current_level >= 0:
         _d._refuse_tangents("grouped_feed_forward", x, w13, w2)
@@ -318,7 +338,7 @@ def _fp8_product(x, x_scales, w, w_scales, ends, out_dtype, clamp: float, gated:
     else:
         _check_weights(w, what, _E4M3, index)
         experts, rows, width = w.shape
-        ends = _check_ends(ends, experts, index)
+        ends = _dense_ends(ends, experts, index)
     if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         _d._refuse_gradient("a product in 8-bit floating point")
     if _forward_ad._current_level >= 0:
@@ -328,8 +348,10 @@ def _fp8_product(x, x_scales, w, w_scales, ends, out_dtype, clamp: float, gated:
     if gated and rows % 2 != 0:
         raise AssertionError(f"the weights have {rows} rows: the gated projection needs as many gate as up rows")
     channels = rows // 2 if gated else rows
-    _check_sizes(16, K=width)
-    _check_sizes(8 if gated else 1, N=channels)
+    if not _size_fits(width, 16):
+        _refuse_size("K", width, 16)
+    if not _size_fits(channels, 8 if gated else 1):
+        _refuse_size("N", channels, 8 if gated else 1)
     code = _d._CODES.get(out_dtype)
     if code is None:
         raise AssertionError(f"out_dtype must be BF16, FP16 or FP32, got {out_dtype}")
