@@ -27,7 +27,7 @@ constexpr int kGroupStage = kGroupStageA + kGroupCols / 2 * 128;
 constexpr int kGroupStages = 6;
 constexpr int kGroupEpiWarps = 8;                     // two per TMEM lane quadrant, each with every other block of columns
 constexpr int kGroupThreads = 32 * (2 + kGroupEpiWarps);
-constexpr int kTurnBytes = 16 * 80;                   // a warp's 16 rows x 64 bytes, rows 80 bytes apart so that stmatrix meets no bank twice
+constexpr int kTurnBytes = 16 * 144;                  // a warp's 16 rows x 64 or 128 bytes, rows 80 or 144 bytes apart so that stmatrix meets no bank twice
 
 struct GroupControl {
   uint64_t full[kGroupStages];    // leader only: every copy of the stage, in both CTAs, has landed
@@ -207,42 +207,44 @@ __device__ __forceinline__ void finish_columns_as(const DenseEpilogue& epi, cons
   }
 }
 
-// 32 columns x 32 rows of an expert's weights' gradient
+// 64 columns x 32 rows of an expert's weights' gradient, which leave in 128 bytes of a row.  v[h][g][r] with g = 0 .. 7
 template <typename T>
-__device__ __forceinline__ void put_weights(const Share& s, T* out, int64_t ld, int column, int columns, const float (&v)[2][4][4]) {
+__device__ __forceinline__ void put_weights(const Share& s, T* out, int64_t ld, int column, int columns, const float (&v)[2][8][4]) {
   const int l = s.lane;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     __syncwarp();
 #pragma unroll
     for (int p = 0; p < 2; ++p)
-      store_matrices<false>(smem_u32(s.turn) + (8 * p + (l & 7)) * 80 + (l >> 3) * 16, pack_two<T>(v[h][0][2 * p], v[h][0][2 * p + 1]),
-                            pack_two<T>(v[h][1][2 * p], v[h][1][2 * p + 1]), pack_two<T>(v[h][2][2 * p], v[h][2][2 * p + 1]),
-                            pack_two<T>(v[h][3][2 * p], v[h][3][2 * p + 1]));
+#pragma unroll
+      for (int g = 0; g < 8; g += 4)
+        store_matrices<false>(smem_u32(s.turn) + (8 * p + (l & 7)) * 144 + g * 16 + (l >> 3) * 16, pack_two<T>(v[h][g][2 * p], v[h][g][2 * p + 1]),
+                              pack_two<T>(v[h][g + 1][2 * p], v[h][g + 1][2 * p + 1]), pack_two<T>(v[h][g + 2][2 * p], v[h][g + 2][2 * p + 1]),
+                              pack_two<T>(v[h][g + 3][2 * p], v[h][g + 3][2 * p + 1]));
     __syncwarp();
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int row = s.channel0 + 16 * h + 8 * p + (l >> 2), at = column + 8 * (l & 3);
-      if (row < s.channels && at < columns)
-        *reinterpret_cast<uint4*>(out + row * ld + at) = *reinterpret_cast<const uint4*>(s.turn + (8 * p + (l >> 2)) * 80 + (l & 3) * 16);
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * i + (l >> 3), row = s.channel0 + 16 * h + r, at = column + 8 * (l & 7);
+      if (row < s.channels && at < columns) *reinterpret_cast<uint4*>(out + row * ld + at) = *reinterpret_cast<const uint4*>(s.turn + r * 144 + (l & 7) * 16);
     }
+  }
+}
+// ... of an expert without rows
+template <typename T>
+__device__ __forceinline__ void clear_weights(const Share& s, T* out, int64_t ld, int column, int columns) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = s.channel0 + 4 * i + (s.lane >> 3), at = column + 8 * (s.lane & 7);
+    if (row < s.channels && at < columns) *reinterpret_cast<uint4*>(out + row * ld + at) = make_uint4(0, 0, 0, 0);
   }
 }
 
 template <int kKind>
 __device__ __forceinline__ void finish_columns(const GroupedParams& p, const GroupTile& g, const Share& s, int column, const float (&v)[2][4][4]) {
   const DenseEpilogue& epi = p.epi;
-  if (kKind == kGroupedWeights) {
-    const int64_t at = (int64_t)g.expert * p.n * epi.ld_out;
-    if (epi.out_type == kDenseBf16) put_weights(s, static_cast<__nv_bfloat16*>(epi.out) + at, epi.ld_out, g.first + column, p.k, v);
-    else put_weights(s, static_cast<__half*>(epi.out) + at, epi.ld_out, g.first + column, p.k, v);
-    return;
-  }
   const int first = g.first + column, valid = g.valid - column;
-  if constexpr (kKind != kGroupedWeights) {
-    if (epi.out_type == kDenseBf16) finish_columns_as<kKind, __nv_bfloat16>(epi, s, first, valid, v);
-    else finish_columns_as<kKind, __half>(epi, s, first, valid, v);
-  }
+  if (epi.out_type == kDenseBf16) finish_columns_as<kKind, __nv_bfloat16>(epi, s, first, valid, v);
+  else finish_columns_as<kKind, __half>(epi, s, first, valid, v);
 }
 
 // kTurnedA, kTurnedB: the operand is staged with its rows along the 128 bytes (weights stored as [k, n]; both for the gradient of the weights)
@@ -390,18 +392,46 @@ __global__ void __launch_bounds__(kGroupThreads, 1) grouped_pair_kernel(const __
       if (!waiter.wait_warp(smem_u32(&ctl->acc_full[it & 1u]), (it >> 1) & 1u, g.k_stages)) break;
       tc_fence_after();
       const uint32_t d = tmem_base + (it & 1u) * kGroupCols + lanes;
-      if (side >= blocks) release(it & 1u);
+      if constexpr (kKind == kGroupedWeights) {
+        // two blocks at a time
+        const int chunks = g.cols / 64;
+        const int64_t at = (int64_t)g.expert * p.n * p.epi.ld_out;
+        const auto each = [&](auto* out) {
+          out += at;
 #pragma unroll 1
-      for (int block = side; block < blocks; block += 2) {
-        float v[2][4][4];
-        uint32_t raw[32];
-        tc_ld_fragments(d + 32 * block, raw);
-        tc_ld_fragments(d + 32 * block + (16u << 16), raw + 16);
-        tc_ld_wait();
-        if (block + 2 >= blocks) release(it & 1u);
+          for (int chunk = side; chunk < chunks; chunk += 2) {
+            if (g.k_stages == 0) {
+              if (chunk + 2 >= chunks) release(it & 1u);
+              clear_weights(s, out, p.epi.ld_out, g.first + 64 * chunk, p.k);
+              continue;
+            }
+            float v[2][8][4];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i >> 4][(i >> 2) & 3][i & 3] = kKind == kGroupedWeights && g.k_stages == 0 ? 0.f : __uint_as_float(raw[i]);
-        finish_columns<kKind>(p, g, s, 32 * block, v);
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int b = 0; b < 2; ++b)
+                tc_ld_fragments(d + 64 * chunk + 32 * b + (static_cast<uint32_t>(16 * h) << 16), reinterpret_cast<uint32_t*>(&v[h][4 * b][0]));
+            tc_ld_wait();
+            if (chunk + 2 >= chunks) release(it & 1u);
+            put_weights(s, out, p.epi.ld_out, g.first + 64 * chunk, p.k, v);
+          }
+        };
+        if (p.epi.out_type == kDenseBf16) each(static_cast<__nv_bfloat16*>(p.epi.out));
+        else each(static_cast<__half*>(p.epi.out));
+      } else {
+        if (side >= blocks) release(it & 1u);
+#pragma unroll 1
+        for (int block = side; block < blocks; block += 2) {
+          float v[2][4][4];
+          uint32_t raw[32];
+          tc_ld_fragments(d + 32 * block, raw);
+          tc_ld_fragments(d + 32 * block + (16u << 16), raw + 16);
+          tc_ld_wait();
+          if (block + 2 >= blocks) release(it & 1u);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i >> 4][(i >> 2) & 3][i & 3] = __uint_as_float(raw[i]);
+          finish_columns<kKind>(p, g, s, 32 * block, v);
+        }
       }
       ++it;
     }
