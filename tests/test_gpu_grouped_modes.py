@@ -216,7 +216,7 @@ def test_fp8_rows_that_start_anywhere(rows, channels):
 
 
 @pytest.mark.parametrize("gated", [False, True])
-@pytest.mark.parametrize("rows", [257, 256 + 48, 256 + 49, 777])
+@pytest.mark.parametrize("rows", [257, 256 + 64, 256 + 65, 777, 1030])
 def test_fp8_rows_beyond_the_last_tile(rows, gated):
     """5120 wide: a few rows beyond a tile of 256 go by themselves where that saves a turn, and the results are the same rows."""
     api = _api()

@@ -31,7 +31,7 @@ template <bool kWide> constexpr int kFp8Cols = kWide ? 256 : 128;               
 template <bool kWide> constexpr int kFp8Stage = kFp8StageA + kFp8Cols<kWide> / 2 * 128;
 constexpr int kFp8MaxStages = 6;
 template <bool kWide> constexpr int kFp8Stages = kWide ? 5 : kFp8MaxStages;
-constexpr int kFp8RowsApart = 48;
+constexpr int kFp8RowsApart = 64;
 constexpr int kFp8EpiWarps = 8;                       // two per TMEM lane quadrant: wide, one for either accumulator of a group, else for half of its columns
 constexpr int kFp8Threads = 32 * (4 + kFp8EpiWarps);   // epilogue warps first, producer, issuer, one that fetches scales, one that only hands back registers
 constexpr int kFp8Registers = 216, kFp8FewRegisters = 72;
@@ -411,12 +411,12 @@ int64_t fp8_cost(const GroupedProduct& p, int rows, int pairs, bool wide) {
 // 777 rows, 5120 -> 5003: 48.1 us wide (80 tiles, two turns of 74 pairs), 44.5 narrow (160, three)
 bool fp8_wide(const GroupedProduct& p, int pairs) { return fp8_cost(p, p.rows, pairs, true) <= fp8_cost(p, p.rows, pairs, false); }
 
-// Rows of one weight beyond the last tile of 256 that are better off in a launch of few rows: what that costs is the weights' bytes and its start.
-// 0: none.
+// Rows of one weight beyond the last tile of 256 that are better off in a launch of few rows: what that costs is the weights' bytes, its start, and
+// something for each row.  0: none.  777 rows, 5120 -> 5120: 41.2 -> 35.2 us, 1030 rows, gated 5120 -> 2 x 2304: 43.8 -> 39.1; 76 rows more would be 44.0 -> 46.1.
 int fp8_rows_apart(const GroupedProduct& p, int pairs) {
   const int last = p.rows % (2 * kGroupRows);
   if (p.ends != nullptr || last == 0 || last == p.rows || last > kFp8RowsApart) return 0;
-  const int64_t groups = (p.k + kScaleBlock - 1) / kScaleBlock, apart = (int64_t)p.n * (p.kind == kGated ? 2 : 1) * p.k / 4450 + 6000;
+  const int64_t groups = (p.k + kScaleBlock - 1) / kScaleBlock, apart = (int64_t)p.n * (p.kind == kGated ? 2 : 1) * p.k / 4450 + 12000 + 130 * last;
   const auto best = [&](int rows) { return groups * std::min(fp8_cost(p, rows, pairs, true), fp8_cost(p, rows, pairs, false)); };
   return best(p.rows - last) + apart < best(p.rows) ? last : 0;
 }

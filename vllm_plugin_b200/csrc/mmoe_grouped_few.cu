@@ -23,7 +23,7 @@ constexpr int kFewCols = 64;                          // most rows of B
 constexpr int kFewStageA = kFewRows * 128, kFewStage = kFewStageA + kFewCols * 128;
 constexpr int kFewStages = 4;
 constexpr int kFewThreads = 256;                      // producer, issuer, four warps that read the sums, one that fetches scales; all finish
-constexpr int kFewMaxSplit = 8;
+constexpr int kFewMaxSplit = 6;
 constexpr int kFewSmem = 113 * 1024;
 constexpr int kFewBatch = 8, kFewSlots = 4, kFewAccumulators = 4;
 
@@ -45,10 +45,8 @@ struct FewControl {
 constexpr int kFewPlace = 10 * 1024;
 static_assert(sizeof(FewControl) <= kFewPlace, "control block");
 static_assert(kFewPlace + kFewStages * kFewStage + 1024 <= kFewSmem, "shared memory of a CTA");
-// sums of all rows of a tile, and what the other CTAs send of those that this one finishes
-constexpr int few_sum_bytes(int split) { return (kFewCols + (split - 1) * ((kFewCols + split - 1) / split)) * kFewRows * 4; }
-static_assert(few_sum_bytes(2) <= kFewStages * kFewStage && few_sum_bytes(4) <= kFewStages * kFewStage && few_sum_bytes(8) <= kFewStages * kFewStage,
-              "partial sums fit where the stages were");
+// sums of all rows of a tile, and what the other CTAs send of those that this one finishes: of `split` CTAs each at most 1 / split, rounded up
+static_assert((kFewCols + kFewCols + kFewMaxSplit) * kFewRows * 4 <= kFewStages * kFewStage, "partial sums fit where the stages were");
 
 struct FewParams {
   CUtensorMap map_w;
@@ -371,6 +369,28 @@ __global__ void __launch_bounds__(kFewThreads, 2) grouped_few_kernel(const __gri
 // ---------------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------------
+// the most tiles that there can be
+int64_t few_tiles(const GroupedProduct& p) {
+  const int width = p.kind == kGated ? kFewRows / 2 : kFewRows;
+  return (std::min(p.experts, p.rows) + (int64_t)(p.rows - 1) / kFewCols) * ((p.n + width - 1) / width);
+}
+
+// CTAs that share a tile's K, by what their stages cost (twice that where two share an SM) and what meeting costs, in clocks.  With 1, 2, 3, 4, 6 of them,
+// 8 bits, 5120 -> 5120 (40 tiles): one row 15.0, 10.0, 8.4, 8.4, 8.0 us, 64 rows 24.0, 14.9, 12.7, 13.9, 13.3; 128 rows (80 tiles) 24.2, 18.8, 16.0, 23.1, -; gated
+// 5120 -> 2 x 2304 (72) 24.4, 15.4, 16.0, 22.9, -; 2304 -> 1024 (8), one row 8.4, 6.6, 5.7, 5.3, 5.1, 64 rows 13.3, 9.6, 8.4, 7.8, 7.2.  Clusters of 7 and 8 take longer.
+int few_split(const GroupedProduct& p, int64_t tiles, int k_stages, int sms) {
+  const int cols = std::min((p.rows + 15) & ~15, kFewCols);
+  const int64_t stage = p.type == kGroupedE4m3 ? 475 + 6 * cols : 340 + cols;
+  int64_t least = INT64_MAX;
+  int best = 1;
+  for (int c : {1, 2, 3, 4, kFewMaxSplit}) {
+    if (c > 1 && (tiles * c > 2 * sms || c > k_stages)) break;
+    const int64_t cost = (k_stages + c - 1) / c * stage * (tiles * c <= sms ? 1 : 2) + 8 * cols * c;
+    if (cost < least) least = cost, best = c;
+  }
+  return best;
+}
+
 template <typename F>
 cudaError_t for_each_few_kernel(F f) {
   cudaError_t e = f(grouped_few_kernel<false, false>, false, false);
@@ -382,15 +402,14 @@ cudaError_t for_each_few_kernel(F f) {
 
 }  // namespace
 
-// Against pairs, 5120 x 5120 of one expert: 16 bits, 16 rows 17.6 -> 11.1 us, 64 18.2 -> 13.9, 96 19.9 -> 20.7; 8 bits, 16 rows 15.8 -> 8.8, 48 16.1 -> 12.3, 96
-// 16.6 -> 20.5, gated 5120 -> 2 x 2304, 48 rows 16.8 -> 17.0.  More experts, 8 bits, gated: 8 experts, 256 rows 50.8 -> 36.0, 384 52.4 -> 55.7; 48 experts, 384
-// rows 257 -> 183, 1536 276 -> 202.  16 bits, 2304 -> 5120, where the tiles are more than run at once: 8 experts, 64 rows 38.5 -> 41.6; 48 experts, 384 rows
-// 176 -> 184; six of them, 240 tiles, 29.1 -> 28.0.
+// Against pairs, 5120 x 5120 of one expert: 16 bits, 16 rows 17.6 -> 10.4 us, 64 18.2 -> 12.3, 128 19.3 -> 16.0, 192 23.3 -> 18.4, 256 28.9 -> 27.6; 8 bits, 16 rows
+// 15.6 -> 8.8, 64 16.2 -> 12.7, 128 16.8 -> 16.0, 192 16.8 -> 19.2.  More experts, 8 bits, gated 5120 -> 2 x 2304: 8 experts, 256 rows 50.8 -> 36.0, 384 52.4 -> 55.7;
+// 48 experts, 384 rows 257 -> 183, 1536 276 -> 202.  16 bits, 2304 -> 5120, where the tiles are more than run at once: 8 experts, 64 rows 38.5 -> 41.6; 48
+// experts, 384 rows 176 -> 184; six of them, 240 tiles, 29.1 -> 28.0.
 bool grouped_few_rows(const GroupedProduct& p, int sms) {
   if (p.w_k_rows || (p.kind != kLinear && p.kind != kGated)) return false;
-  if (p.type == kGroupedE4m3) return p.rows <= 40 * (int64_t)p.experts + 8;
-  const int width = p.kind == kGated ? kFewRows / 2 : kFewRows;
-  return p.rows <= kFewCols * (int64_t)p.experts && (int64_t)std::min(p.experts, p.rows) * ((p.n + width - 1) / width) <= 2 * sms;
+  if (p.type == kGroupedE4m3) return p.rows <= std::max<int64_t>(128, 40 * (int64_t)p.experts);
+  return few_tiles(p) <= (p.rows <= kFewCols ? 2 * sms : sms);
 }
 
 cudaError_t prepare_grouped_few() {
@@ -412,10 +431,7 @@ cudaError_t launch_grouped_few(const GroupedProduct& p, int sms, cudaStream_t s)
   d.zero_behind = p.zero_behind && p.ends != nullptr;
   d.status = p.status;
   d.timeout_ns = (p.timeout_ms > 0 ? (int64_t)p.timeout_ms : 2000) * 1000000ll;
-  // CTAs that share a tile's K: as many as there are places for, two to an SM, while each has two stages
-  const int64_t likely = (int64_t)std::min(p.experts, p.rows) * d.row_tiles;
-  d.split = 1;
-  while (d.split < kFewMaxSplit && likely * 2 * d.split <= 2 * sms && d.k_stages >= 4 * d.split) d.split *= 2;
+  d.split = few_split(p, few_tiles(p), d.k_stages, sms);
   const uint64_t size = fp8 ? 1 : 2, n = p.n, k = p.k, parts = gate ? 2 : 1;
   const uint32_t depth = static_cast<uint32_t>(128 / size);
   bool ok = encode_map(&d.map_w, p.type, p.w, 4, {k, n, parts, static_cast<uint64_t>(p.experts), 1}, {k * size, n * k * size, parts * n * k * size, 0},
