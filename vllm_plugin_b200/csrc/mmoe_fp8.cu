@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
             if (cta == 0) mbar_expect_tx(full0 + 8 * stage, tx);
             pair_load_4d(a + kFp8StageA, &p.map_w, kb * 128, w_row, part, g.expert, bar);
             int done = 0;
-  #pragma unroll
+#pragma unroll
             for (int i = 0; i < 4; ++i)
               if (rows & (128 >> i)) {
                 pair_load_2d(a + done * 128, &p.map_x[i], kb * 128, x_row + done, bar);

@@ -20,6 +20,14 @@ namespace {
 // The gradient of the weights sums over an expert's rows.  Its last stage must not see the next expert's, whose values may be anything: the rows
 // are copied through a 3-D view [rows][64 of them][columns] whose second extent ends the copy.  It starts as many rows early as are missing, and
 // those are filled with zeros; the sum does not mind that they come first.
+//
+// What bounds it: the tensor cores, and in calls that last the power limit.  8 experts of 512 rows, gated 5120 -> 2 x 2304: 111 us (1.74 PFLOP/s; tensor
+// cores 90 % busy, 435 MB of memory where 420 are the least) alone, 158 at 1.24 GHz of one call after another; a dense product of as many operations by the
+// library 143.  46 experts with 23040 uneven rows, block 5120 -> 2304 -> 5120: 1.27 to 1.43 ms (1.14 to 1.28 PFLOP/s), all their weights read beside it.  3840 rows of
+// 8 experts with gradients: 720 to 740 us (1.1 PFLOP/s); through the second product 66 % and the gradients of the weights 68 to 73 % of the tensor cores' cycles,
+// the rest goes into tiles that do not come out even and sums that leave (dw13 writes 378 MB).
+// Tried: the widest tile of an expert's rows chosen from 256, 224 ... 128 by the turns of the pairs: 1021 rows of one expert, block with gradients 208 -> 186 us,
+// but 48 experts with 6000 rows 593 -> 602, 300 rows of one 122 -> 127, 8 with 3840 741 -> 752.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kGroupCols = 256;                       // most rows of B per tile
 constexpr int kGroupStageA = kGroupRows * 128;        // bytes
