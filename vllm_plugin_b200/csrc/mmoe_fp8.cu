@@ -26,15 +26,14 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFp8Unit = 128;                         // columns of an accumulator
 constexpr int kFp8Units = kTmemCols / kFp8Unit;
+constexpr int kFp8Cols = 2 * kFp8Unit;                // rows of B per tile
 constexpr int kFp8StageA = kGroupRows * 128;          // bytes
-template <bool kWide> constexpr int kFp8Cols = kWide ? 256 : 128;                        // rows of B per tile
-template <bool kWide> constexpr int kFp8Stage = kFp8StageA + kFp8Cols<kWide> / 2 * 128;
-constexpr int kFp8MaxStages = 6;
-template <bool kWide> constexpr int kFp8Stages = kWide ? 5 : kFp8MaxStages;
-constexpr int kFp8RowsApart = 64;
-constexpr int kFp8EpiWarps = 8;                       // two per TMEM lane quadrant: wide, one for either accumulator of a group, else for half of its columns
+constexpr int kFp8StageHalf = kFp8Unit / 2 * 128;     // of B, for one of the tile's accumulators
+constexpr int kFp8Stage = kFp8StageA + 2 * kFp8StageHalf;
+constexpr int kFp8Stages = 5;
+constexpr int kFp8EpiWarps = 8;                       // two per TMEM lane quadrant, each with half of an accumulator's columns
 constexpr int kFp8Threads = 32 * (4 + kFp8EpiWarps);   // epilogue warps first, producer, issuer, one that fetches scales, one that only hands back registers
-constexpr int kFp8Registers = 216, kFp8FewRegisters = 72;
+constexpr int kFp8Registers = 208, kFp8FewRegisters = 88;
 static_assert(kFp8EpiWarps * 32 * kFp8Registers + 128 * kFp8FewRegisters <= kFp8Threads * 168, "registers that the block was launched with");
 constexpr int kFp8Batch = 8;                          // groups of k whose scales are fetched at a time
 constexpr int kFp8Turn = 32 * 144;                    // a warp's 32 rows x 128 bytes on their way from lanes to rows
@@ -46,8 +45,8 @@ struct Fp8Scales {
 };
 
 struct Fp8Control {
-  uint64_t full[kFp8MaxStages];      // leader only: every copy of the stage, in both CTAs, has landed
-  uint64_t empty[kFp8MaxStages];     // issuer -> producers of both CTAs
+  uint64_t full[kFp8Stages];         // leader only: every copy of the stage, in both CTAs, has landed
+  uint64_t empty[kFp8Stages];        // issuer -> producers of both CTAs
   uint64_t acc_full[kFp8Units];           // issuer -> epilogues of both CTAs
   uint64_t acc_empty[kFp8Units];          // leader only: epilogue warps of both CTAs -> issuer
   uint64_t scale_full[kFp8ScaleSlots], scale_empty[kFp8ScaleSlots];
@@ -56,7 +55,7 @@ struct Fp8Control {
 };
 
 struct Fp8Params {
-  CUtensorMap map_w;
+  CUtensorMap map_w[2];           // boxes of 128 and 64 rows
   CUtensorMap map_x[4];           // boxes of 128, 64, 32 and 16 rows
   const int32_t* ends;
   int32_t experts, rows;
@@ -73,8 +72,7 @@ struct Fp8Params {
 
 constexpr int kFp8Smem = 227 * 1024;
 constexpr int kFp8Place = 1024;
-constexpr int kFp8StageRoom = std::max(kFp8Stages<true> * kFp8Stage<true>, kFp8Stages<false> * kFp8Stage<false>);
-constexpr int kFp8PlanAt = kFp8Place + kFp8StageRoom;
+constexpr int kFp8PlanAt = kFp8Place + kFp8Stages * kFp8Stage;
 constexpr int kFp8TurnAt = kFp8PlanAt + (sizeof(GroupPlan) + 15) / 16 * 16;
 static_assert(sizeof(Fp8Control) <= kFp8Place, "control block");
 constexpr int kFp8ScalesAt = kFp8TurnAt + kFp8EpiWarps * kFp8Turn;
@@ -84,16 +82,32 @@ struct Fp8Tile {
   int expert, channel0;
   int first, valid;               // rows, of the pair
 };
-template <bool kGate, bool kWide>
-__device__ __forceinline__ Fp8Tile fp8_tile_at(const Fp8Params& p, const GroupPlan& plan, int t) {
+// The first `whole` tiles, then the two halves of each of the others
+template <bool kGate>
+__device__ __forceinline__ Fp8Tile fp8_tile_at(const Fp8Params& p, const GroupPlan& plan, int t, int whole) {
   Fp8Tile g;
+  if (t >= whole) t = whole + (t - whole) / 2;
   g.expert = expert_of(plan, p.experts, t);
   const int start = plan.start[g.expert], count = plan.start[g.expert + 1] - start, parts = (count + 2 * kGroupRows - 1) / (2 * kGroupRows);
   const int in = t - plan.tile[g.expert], at = in % parts * 2 * kGroupRows;
-  g.channel0 = in / parts * (kGate ? kFp8Cols<kWide> / 2 : kFp8Cols<kWide>);
+  g.channel0 = in / parts * (kGate ? kFp8Cols / 2 : kFp8Cols);
   g.first = start + at, g.valid = min(count - at, 2 * kGroupRows);
   return g;
 }
+// Which accumulator's columns the warps of a side have: of a whole tile all of their own one, of half a tile 64 of the only one (gated: 32 of the gate's and
+// 32 of the up rows').  Blocks of 32 columns, two or four; the channel behind the tile's first that the b-th begins with.
+template <bool kGate, bool kWhole>
+__device__ __forceinline__ int fp8_column(int side, int b) { return kWhole ? 32 * b : kGate ? 64 * b + 32 * side : 64 * side + 32 * b; }
+template <bool kGate>
+__device__ __forceinline__ int fp8_channel(int side, int b) { return 64 * side + 32 * (b & 1) + (kGate ? 0 : (b >> 1) * kFp8Unit); }
+template <bool kGate>
+__device__ __forceinline__ int fp8_half_channel(int side, int b, int h) { return 64 * h + (kGate ? 32 * side : kFp8Unit * side + 32 * b); }
+
+// as mbar_arrive_pair, for two
+__device__ __forceinline__ void arrive_twice(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0], 2;" ::"r"(bar) : "memory");
+}
+
 // of a CTA's 128 rows, rounded up to the smallest box
 __device__ __forceinline__ int fp8_rows_staged(int valid, int cta) { return min(max(valid - cta * kGroupRows + 15, 0), kGroupRows) & ~15; }
 
@@ -111,14 +125,7 @@ __device__ __forceinline__ bool poll(DenseWaiter& w, uint32_t bar, uint32_t pari
   }
 }
 
-// the same where the phase has mostly completed: two probes, then as everybody waits
-__device__ __forceinline__ bool wait_here(DenseWaiter& w, uint32_t bar, uint32_t parity) {
-  bool ok = mbar_try_wait(bar, parity);
-  if (!ok) ok = mbar_try_wait(bar, parity);
-  return __all_sync(0xffffffffu, ok) || w.wait_uniform(bar, parity);
-}
-
-template <bool kGate, bool kWide>
+template <bool kGate>
 __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the same offset in both CTAs
@@ -127,21 +134,18 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
   GroupPlan* plan = reinterpret_cast<GroupPlan*>(smem + kFp8PlanAt);
   Fp8Scales* scales = reinterpret_cast<Fp8Scales*>(smem + kFp8ScalesAt);
 
-  constexpr int kStages = kFp8Stages<kWide>, kStage = kFp8Stage<kWide>, half = kFp8Cols<kWide> / 2;
-  constexpr int kBlocks = kWide ? 4 : 2;                // of 32 columns, that an epilogue warp has
-
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int cta = static_cast<int>(cluster_ctarank());
   if (threadIdx.x == 0) {
-    prefetch_map(&p.map_w);
+    for (int i = 0; i < 2; ++i) prefetch_map(&p.map_w[i]);
     for (int i = 0; i < 4; ++i) prefetch_map(&p.map_x[i]);
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kFp8Stages; ++i) {
       mbar_init(smem_u32(&ctl->full[i]), 1);
       mbar_init(smem_u32(&ctl->empty[i]), 1);
     }
     for (int i = 0; i < kFp8Units; ++i) {
       mbar_init(smem_u32(&ctl->acc_full[i]), 1);
-      mbar_init(smem_u32(&ctl->acc_empty[i]), kWide ? kFp8EpiWarps : 2 * kFp8EpiWarps);
+      mbar_init(smem_u32(&ctl->acc_empty[i]), 2 * kFp8EpiWarps);
     }
     for (int i = 0; i < kFp8ScaleSlots; ++i) {
       mbar_init(smem_u32(&ctl->scale_full[i]), 32);
@@ -160,9 +164,10 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
   tc_fence_after();
   chain_wait();                             // nothing above touches global memory
   chain_release();                          // in this order: what precedes this launch is complete when the next one starts
-  const int tiles = make_plan(plan, p.ends, p.experts, p.rows, 2 * kGroupRows, p.col_tiles, p.status);
+  int tiles = make_plan(plan, p.ends, p.experts, p.rows, 2 * kGroupRows, p.col_tiles, p.status), whole = tiles;
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
   const int step = gridDim.x / 2;
+  if (2 * (tiles % step) <= step) whole = tiles / step * step, tiles += tiles - whole;      // the last turn by halves
   DenseWaiter waiter{{&ctl->abort_flag, p.status, 0, kStatusGrouped + 1, warp}, p.timeout_ns};
   const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
   {
@@ -179,77 +184,76 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
     const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
     uint8_t* turn = smem + kFp8TurnAt + warp * kFp8Turn;
     const uint32_t full = smem_u32(&ctl->acc_full[0]), sums = tmem_base + lanes;
-    uint32_t batch = 0, phase = 0, unit = kWide ? side : 0;        // the accumulator whose turn it is; wide: those of this warp's half of the columns
-    bool ok = true;
-    // this warp's blocks of 32 columns: the accumulator's column, and the channel behind the tile's first
-    const auto column = [&](int b) { return kWide ? 32 * b : kGate ? kFp8Unit / 2 * b + 32 * side : 64 * side + 32 * b; };
-    const auto channel = [&](int b) { return kWide ? 64 * side + 32 * (b & 1) + (kGate ? 0 : (b >> 1) * half) : kGate ? 32 * side : 64 * side + 32 * b; };
-    for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
-      const Fp8Tile g = fp8_tile_at<kGate, kWide>(p, *plan, t);
-      const int row0 = g.first + cta * kGroupRows + quadrant * 32, rows = g.valid - cta * kGroupRows - quadrant * 32;      // of this warp
-      const int channels = p.n - g.channel0;
-      const bool any = rows > 0 && channel(0) < channels;
+    uint32_t batch = 0, phase = 0, unit = side;       // the accumulator whose turn it is
+    // Where the phase has mostly completed: two probes, then as everybody waits, by a waiter of its own, which takes no registers meanwhile
+    const auto wait = [&](uint32_t bar, uint32_t parity) {
+      bool there = mbar_try_wait(bar, parity);
+      if (!there) there = mbar_try_wait(bar, parity);
+      if (__all_sync(0xffffffffu, there)) return true;
+      DenseWaiter slow{{&ctl->abort_flag, p.status, 0, kStatusGrouped + 1, static_cast<int>(threadIdx.x >> 5)}, p.timeout_ns};
+      return slow.wait_uniform(bar, parity);
+    };
+    const auto tile = [&](auto all, int t) {           // a whole one, or half of one
+      constexpr bool kWhole = all.value;
+      constexpr int kBlocks = kWhole ? 4 : 2;            // of 32 columns; gated: the gate's, then the up rows'
       float sum[kBlocks][32] = {};
-      for (int kb = 0; ok && kb < p.groups; kb += kFp8Batch, ++batch) {
-        if (!wait_here(waiter, smem_u32(&ctl->scale_full[batch % kFp8ScaleSlots]), (batch / kFp8ScaleSlots) & 1u)) { ok = false; break; }
-        const Fp8Scales& now = scales[batch % kFp8ScaleSlots];
-        uint32_t x_at = smem_u32(&now.x[0][quadrant * 32 + lane]), w_at = smem_u32(&now.w[0][4 * side]);
-        const int count = min(kFp8Batch, p.groups - kb);
-        for (int j = 0; j < count; ++j) {
-          if (!wait_here(waiter, full + 8 * unit, phase)) { ok = false; break; }
-          tc_fence_after();
-          if (any) {
-            const uint32_t d = sums + kFp8Unit * unit;
-            uint32_t v[2][32];
-            tc_ld32(d + column(0), v[0]);
-            tc_ld32(d + column(1), v[1]);
-            float x_now, w0, w1, w2, w3;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x_now) : "r"(x_at));
-            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w0), "=f"(w1), "=f"(w2), "=f"(w3) : "r"(w_at));
-            const auto add = [&](int b, float w) {
-              const float s = x_now * w;
+      uint32_t v[2][16];                                // 16 columns on their way while 16 are added
+      const auto fetch = [&](int c) { tc_ld16(sums + kFp8Unit * unit + fp8_column<kGate, kWhole>(side, c >> 1) + 16 * (c & 1), v[c & 1]); };
+      if (!wait(full + 8 * unit, phase)) return false;
+      tc_fence_after();
+      fetch(0);
+      for (int left = p.groups; left > 0; ++batch) {
+        if (!wait(smem_u32(&ctl->scale_full[batch % kFp8ScaleSlots]), (batch / kFp8ScaleSlots) & 1u)) return false;
+        uint32_t x_at = smem_u32(&scales[batch % kFp8ScaleSlots].x[0][quadrant * 32 + lane]), w_at = smem_u32(&scales[batch % kFp8ScaleSlots].w[0][4 * side]);
+        const int behind = max(left - kFp8Batch, 0);
+        do {
+          float x_now, w0, w1, w2, w3;
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x_now) : "r"(x_at));
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w0), "=f"(w1), "=f"(w2), "=f"(w3) : "r"(w_at));
+          const float scale[4] = {x_now * w0, x_now * w1, x_now * w2, x_now * w3};
+          const auto add = [&](int c) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) sum[b][i] = fmaf(__uint_as_float(v[b & 1][i]), s, sum[b][i]);
-            };
-            const auto release = [&] {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_pair(leader_empty + 8 * unit);
-            };
-            tc_ld_wait();
-            if constexpr (kWide) {
-              add(0, w0);
-              tc_ld32(d + column(2), v[0]);
-              add(1, w1);
-              tc_ld32(d + column(3), v[1]);
-              tc_ld_wait();
-              release();
-              add(2, w2);
-              add(3, w3);
-            } else {
-              release();
-              add(0, w0);
-              add(1, w1);
+            for (int i = 0; i < 16; ++i) {
+              float& to = sum[c >> 1][16 * (c & 1) + i];
+              to = fmaf(__uint_as_float(v[c & 1][i]), scale[c >> 1], to);
             }
-          } else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_pair(leader_empty + 8 * unit);
+          };
+          tc_ld_wait();
+#pragma unroll
+          for (int c = 1; c < 2 * kBlocks; ++c) {
+            fetch(c);
+            add(c - 1);
+            tc_ld_wait();
           }
-          x_at += sizeof(now.x[0]), w_at += sizeof(now.w[0]);
-          unit = kWide ? unit ^ 2u : (unit + 1) % kFp8Units;
-          phase ^= (kWide ? unit < 2 : unit == 0) ? 1u : 0u;         // a phase has all accumulators
-        }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (kWhole) arrive_twice(leader_empty + 8 * unit);
+            else mbar_arrive_pair(leader_empty + 8 * unit);
+          }
+          unit = kWhole ? unit ^ 2u : (unit + 1) % kFp8Units;
+          phase ^= (kWhole ? unit < 2 : unit == 0) ? 1u : 0u;          // a phase has all accumulators
+          if (--left > 0) {                              // the next group's first columns
+            if (!wait(full + 8 * unit, phase)) return false;
+            tc_fence_after();
+            fetch(0);
+          }
+          add(2 * kBlocks - 1);
+          x_at += sizeof(scales->x[0]), w_at += sizeof(scales->w[0]);
+        } while (left > behind);
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&ctl->scale_empty[batch % kFp8ScaleSlots]));
       }
-      if (!ok || !any) continue;
-      // ---- results: rows of two neighbouring blocks, 64 channels
+      // ---- results: 64 neighbouring channels of every row, or (half a gated tile) 32
+      const Fp8Tile g = fp8_tile_at<kGate>(p, *plan, t, whole);
+      const int row0 = g.first + cta * kGroupRows + quadrant * 32, rows = g.valid - cta * kGroupRows - quadrant * 32;      // of this warp
+      if (rows <= 0) return true;
       const bool dense_rows = p.epi.out_type == kDenseFp32 ? p.n % 4 == 0 : p.n % 8 == 0;
 #pragma unroll
       for (int run = 0; run < (kGate ? 1 : kBlocks / 2); ++run) {
-        constexpr int kRun = kGate ? 16 * kBlocks : 64;    // neighbouring channels
-        const int first = channel(2 * run), count = min(kRun, channels - first);
+        constexpr int kRun = kGate ? 16 * kBlocks : 64;
+        const int first = g.channel0 + (kWhole ? fp8_channel<kGate>(side, 2 * run) : fp8_half_channel<kGate>(side, 0, (t - whole) & 1));
+        const int count = min(kRun, p.n - first);
         if (count <= 0) continue;
         const auto value = [&](int j) {                  // of channel first + j
           const float f = sum[2 * run + (j >> 5)][j & 31];
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
         const auto put = [&](auto* out) {
           using T = std::remove_pointer_t<decltype(out)>;
           constexpr int kEach = 16 / sizeof(T), kPart = 128 / sizeof(T), kStride = 144;       // 144: no two of eight rows in one bank
-          out += (int64_t)row0 * p.epi.ld_out + g.channel0 + first;
+          out += (int64_t)row0 * p.epi.ld_out + first;
 #pragma unroll
           for (int part = 0; part < (kRun + kPart - 1) / kPart; ++part) {     // 128 bytes of every row
             __syncwarp();                                 // what was there has been read
@@ -292,7 +296,16 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
         else if (p.epi.out_type == kDenseFp16) put(static_cast<__half*>(p.epi.out));
         else put(static_cast<float*>(p.epi.out));
       }
+      return true;
+    };
+    bool ok = true;
+    int t = blockIdx.x / 2;
+    for (; ok && t < whole; t += step) ok = tile(std::true_type(), t);
+    if (ok && t < tiles) {
+      unit &= 2u;                                      // both sides go on with the first of the two whose turn it is
+      tile(std::false_type(), t);
     }
+    tc_ld_wait();                                       // one that was abandoned may have columns on their way
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp8FewRegisters));
     if (warp == kFp8EpiWarps) {
@@ -302,16 +315,17 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
       const uint32_t leader_full0 = map_to_cta(full0, 0), base = smem_u32(stages);
       bool ok = true;
       for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
-        const Fp8Tile g = fp8_tile_at<kGate, kWide>(p, *plan, t);
+        const Fp8Tile g = fp8_tile_at<kGate>(p, *plan, t, whole);
         const int rows = fp8_rows_staged(g.valid, cta), x_row = g.first + cta * kGroupRows;
-        const uint32_t tx = (fp8_rows_staged(g.valid, 0) + fp8_rows_staged(g.valid, 1)) * 128 + 2 * half * 128;
-        const int w_row = kGate ? g.channel0 : g.channel0 + cta * half, part = kGate ? cta : 0;
+        const bool all = t < whole;
+        const uint32_t tx = (fp8_rows_staged(g.valid, 0) + fp8_rows_staged(g.valid, 1)) * 128 + 2 * (all ? 2 * kFp8StageHalf : kFp8StageHalf);
+        const int w_row = g.channel0 + (kGate ? 0 : cta * kFp8Unit) + (all ? 0 : (t - whole & 1) * (kFp8Unit / 2)), part = kGate ? cta : 0;
         for (int kb = 0; kb < p.groups; ++kb) {
           if (!waiter.wait_uniform(empty0 + 8 * stage, phase ^ 1u)) { ok = false; break; }
-          const uint32_t bar = leader_full0 + 8 * stage, a = base + stage * kStage;
+          const uint32_t bar = leader_full0 + 8 * stage, a = base + stage * kFp8Stage;
           if (elect_one()) {
             if (cta == 0) mbar_expect_tx(full0 + 8 * stage, tx);
-            pair_load_4d(a + kFp8StageA, &p.map_w, kb * 128, w_row, part, g.expert, bar);
+            pair_load_4d(a + kFp8StageA, &p.map_w[all ? 0 : 1], kb * 128, w_row, part, g.expert, bar);
             int done = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -321,7 +335,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
               }
           }
           __syncwarp();
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          if (++stage == kFp8Stages) { stage = 0; phase ^= 1u; }
         }
       }
     } else if (warp == kFp8EpiWarps + 1) {
@@ -329,29 +343,33 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
       if (cta == 0) {
         int stage = 0;
         uint32_t phase = 0, it = 0;
-        bool ok = true;
         const uint32_t lo0 = (smem_u32(stages) & 0x3FFFFu) >> 4;
         const uint64_t hi = operand_desc(false, 0);
-        for (int t = blockIdx.x / 2; ok && t < tiles; t += step)
-          for (int kb = 0; kb < p.groups; ++kb, ++it) {
-            if (!poll(waiter, full0 + 8 * stage, phase)) { ok = false; break; }
+        const auto issue = [&](auto halves) {              // one tile, or half of one
+          for (int kb = 0; kb < p.groups; ++kb) {
+            if (!poll(waiter, full0 + 8 * stage, phase)) return false;
 #pragma unroll
-            for (int h = 0; ok && h < (kWide ? 2 : 1); ++h) {
-              const uint32_t acc = kWide ? (it & 1u) * 2 + h : it % kFp8Units;
-              if (!poll(waiter, smem_u32(&ctl->acc_empty[acc]), ((kWide ? it >> 1 : it / kFp8Units) & 1u) ^ 1u)) { ok = false; break; }
+            for (int h = 0; h < halves.value; ++h, ++it) {
+              const uint32_t acc = it % kFp8Units;
+              if (!poll(waiter, smem_u32(&ctl->acc_empty[acc]), ((it / kFp8Units) & 1u) ^ 1u)) return false;
               tc_fence_after();
-              const uint32_t a = lo0 + stage * (kStage >> 4), b = a + (kFp8StageA >> 4) + h * (kFp8Unit / 2 * 8), d = tmem_base + acc * kFp8Unit;
+              const uint32_t a = lo0 + stage * (kFp8Stage >> 4), b = a + ((kFp8StageA + h * kFp8StageHalf) >> 4), d = tmem_base + acc * kFp8Unit;
               if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) fp8_product(d, hi | (a + 2 * k), hi | (b + 2 * k), p.idesc, k != 0 ? 1u : 0u);
-                if (h == (kWide ? 1 : 0)) pair_commit(empty0 + 8 * stage);
+                if (h == halves.value - 1) pair_commit(empty0 + 8 * stage);
                 pair_commit(smem_u32(&ctl->acc_full[acc]));
               }
             }
-            if (!ok) break;
             __syncwarp();
-            if (++stage == kStages) { stage = 0; phase ^= 1u; }
+            if (++stage == kFp8Stages) { stage = 0; phase ^= 1u; }
           }
+          return true;
+        };
+        bool ok = true;
+        int t = blockIdx.x / 2;
+        for (; ok && t < whole; t += step) ok = issue(std::integral_constant<int, 2>());
+        if (ok && t < tiles) issue(std::integral_constant<int, 1>());
       }
     } else if (warp == kFp8EpiWarps + 2) {
       // ------------------------------------------------------------------------------------------- scales
@@ -359,15 +377,15 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
       bool ok = true;
       const int group = lane & 7, row0 = lane >> 3;      // a lane's group of a batch, and the first of its rows: eight lanes read 32 bytes of a row
       for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
-        const Fp8Tile g = fp8_tile_at<kGate, kWide>(p, *plan, t);
+        const Fp8Tile g = fp8_tile_at<kGate>(p, *plan, t, whole);
         const int rows = g.valid - cta * kGroupRows;
         const float* x = p.x_scales + (int64_t)(g.first + cta * kGroupRows + row0) * p.groups + group;
         // blocks row0 and row0 + 4 of the eight: those of either side
         const float* w[2];
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
-          const int up = !kGate ? 0 : kWide ? row0 >> 1 : row0 & 1;
-          const int channel = g.channel0 + (kWide ? 64 * side + 32 * (row0 & 1) + (kGate ? 0 : (row0 >> 1) * half) : kGate ? 32 * side : 64 * side + 32 * (row0 & 1));
+          const int up = !kGate ? 0 : t < whole ? row0 >> 1 : row0 & 1;
+          const int channel = g.channel0 + (t < whole ? fp8_channel<kGate>(side, row0) : fp8_half_channel<kGate>(side, row0 & 1, (t - whole) & 1));
           w[side] = p.w_scales + (((int64_t)g.expert * (kGate ? 2 : 1) + up) * p.blocks + min(channel / kScaleBlock, p.blocks - 1)) * p.groups + group;
         }
         for (int kb = 0; kb < p.groups; kb += kFp8Batch, ++batch) {
@@ -401,41 +419,17 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
 // ---------------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------------
-// What the pair that has most to do costs, in clocks a group of k.  The rows of each expert are not known here; a tile of rows for all, and one for every
-// expert beyond the first, is the most there can be.
-int64_t fp8_cost(const GroupedProduct& p, int rows, int pairs, bool wide) {
-  const int64_t row_tiles = (rows + 2 * kGroupRows - 1) / (2 * kGroupRows) + std::min(p.experts, rows) - 1;
-  const int cols = wide ? kFp8Cols<true> : kFp8Cols<false>, width = p.kind == kGated ? cols / 2 : cols;
-  return (row_tiles * ((p.n + width - 1) / width) + pairs - 1) / pairs * (wide ? 1150 : 700);
-}
-// 777 rows, 5120 -> 5003: 48.1 us wide (80 tiles, two turns of 74 pairs), 44.5 narrow (160, three)
-bool fp8_wide(const GroupedProduct& p, int pairs) { return fp8_cost(p, p.rows, pairs, true) <= fp8_cost(p, p.rows, pairs, false); }
-
-// Rows of one weight beyond the last tile of 256 that are better off in a launch of few rows: what that costs is the weights' bytes, its start, and
-// something for each row.  0: none.  777 rows, 5120 -> 5120: 41.2 -> 35.2 us, 1030 rows, gated 5120 -> 2 x 2304: 43.8 -> 39.1; 76 rows more would be 44.0 -> 46.1.
-int fp8_rows_apart(const GroupedProduct& p, int pairs) {
-  const int last = p.rows % (2 * kGroupRows);
-  if (p.ends != nullptr || last == 0 || last == p.rows || last > kFp8RowsApart) return 0;
-  const int64_t groups = (p.k + kScaleBlock - 1) / kScaleBlock, apart = (int64_t)p.n * (p.kind == kGated ? 2 : 1) * p.k / 4450 + 12000 + 130 * last;
-  const auto best = [&](int rows) { return groups * std::min(fp8_cost(p, rows, pairs, true), fp8_cost(p, rows, pairs, false)); };
-  return best(p.rows - last) + apart < best(p.rows) ? last : 0;
-}
-
 template <typename F>
 cudaError_t for_each_fp8_kernel(F f) {
-  cudaError_t e = f(fp8_pair_kernel<false, false>, false, false);
-  if (e == cudaSuccess) e = f(fp8_pair_kernel<false, true>, false, true);
-  if (e == cudaSuccess) e = f(fp8_pair_kernel<true, false>, true, false);
-  if (e == cudaSuccess) e = f(fp8_pair_kernel<true, true>, true, true);
-  return e;
+  const cudaError_t e = f(fp8_pair_kernel<false>, false);
+  return e == cudaSuccess ? f(fp8_pair_kernel<true>, true) : e;
 }
 
 cudaError_t launch_fp8_pairs(const GroupedProduct& p, int sms, cudaStream_t s) {
   Fp8Params d = {};
   const bool gate = p.kind == kGated;
   d.ends = p.ends, d.experts = p.experts, d.rows = p.rows, d.n = p.n;
-  const bool wide = fp8_wide(p, sms / 2);
-  const int width = gate ? (wide ? kFp8Cols<true> : kFp8Cols<false>) / 2 : (wide ? kFp8Cols<true> : kFp8Cols<false>);
+  const int width = gate ? kFp8Cols / 2 : kFp8Cols;
   d.col_tiles = (p.n + width - 1) / width;
   d.groups = (p.k + kScaleBlock - 1) / kScaleBlock;
   d.blocks = (p.n + kScaleBlock - 1) / kScaleBlock;
@@ -445,20 +439,15 @@ cudaError_t launch_fp8_pairs(const GroupedProduct& p, int sms, cudaStream_t s) {
   d.status = p.status;
   d.timeout_ns = (p.timeout_ms > 0 ? (int64_t)p.timeout_ms : 2000) * 1000000ll;
   const uint64_t n = p.n, k = p.k, parts = gate ? 2 : 1;
-  bool ok = encode_map(&d.map_w, kGroupedE4m3, p.w, 4, {k, n, parts, static_cast<uint64_t>(p.experts), 1}, {k, n * k, parts * n * k, 0},
-                       {128, static_cast<uint32_t>((wide ? kFp8Cols<true> : kFp8Cols<false>) / 2), 1, 1, 1});
+  bool ok = true;
+  for (int i = 0; ok && i < 2; ++i)
+    ok = encode_map(&d.map_w[i], kGroupedE4m3, p.w, 4, {k, n, parts, static_cast<uint64_t>(p.experts), 1}, {k, n * k, parts * n * k, 0}, {128, 128u >> i, 1, 1, 1});
   for (int i = 0; ok && i < 4; ++i)
     ok = encode_map(&d.map_x[i], kGroupedE4m3, p.x, 2, {k, static_cast<uint64_t>(p.rows), 1, 1, 1}, {static_cast<uint64_t>(p.x_ld), 0, 0, 0}, {128, 128u >> i, 1, 1, 1});
   const int64_t most = ((int64_t)p.rows / (2 * kGroupRows) + std::min(p.experts, p.rows)) * d.col_tiles;
   if (!ok || most > INT32_MAX / 2) return cudaErrorInvalidValue;
-  const int grid = 2 * static_cast<int>(std::min<int64_t>(sms / 2, most));
-  bool found = false;
-  const cudaError_t e = for_each_fp8_kernel([&](auto kernel, bool k_gate, bool k_wide) {
-    if (k_gate != gate || k_wide != wide) return cudaSuccess;
-    found = true;
-    return launch_clustered(kernel, dim3(grid), dim3(kFp8Threads), kFp8Smem, 2, s, d);
-  });
-  return found ? e : cudaErrorInvalidValue;
+  const int grid = 2 * static_cast<int>(std::min<int64_t>(sms / 2, 2 * most));       // every tile could come in halves
+  return for_each_fp8_kernel([&](auto kernel, bool k_gate) { return k_gate != gate ? cudaSuccess : launch_clustered(kernel, dim3(grid), dim3(kFp8Threads), kFp8Smem, 2, s, d); });
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -600,23 +589,14 @@ cudaError_t launch_quantize(const void* x, int64_t ld, uint8_t* q, float* scales
 }  // namespace
 
 cudaError_t prepare_fp8() {
-  return for_each_fp8_kernel([](auto kernel, bool, bool) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8Smem); });
+  return for_each_fp8_kernel([](auto kernel, bool) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8Smem); });
 }
 
 cudaError_t launch_fp8(const GroupedProduct& p, cudaStream_t s) {
   const int sms = dense_sms();
   if (sms == 0) return cudaErrorNotReady;
   const ChainScope chain(true);
-  if (grouped_few_rows(p, sms)) return launch_grouped_few(p, sms, s);
-  const int apart = fp8_rows_apart(p, sms / 2);
-  if (apart == 0) return launch_fp8_pairs(p, sms, s);
-  GroupedProduct first = p, last = p;
-  first.rows = p.rows - apart, last.rows = apart;
-  last.x = static_cast<const uint8_t*>(p.x) + first.rows * p.x_ld;
-  last.x_scales = p.x_scales + (int64_t)first.rows * ((p.k + kScaleBlock - 1) / kScaleBlock);
-  last.epi.out = static_cast<uint8_t*>(p.epi.out) + first.rows * p.epi.ld_out * (p.epi.out_type == kDenseFp32 ? 4 : 2);
-  const cudaError_t e = launch_fp8_pairs(first, sms, s);
-  return e == cudaSuccess ? launch_grouped_few(last, sms, s) : e;
+  return grouped_few_rows(p, sms) ? launch_grouped_few(p, sms, s) : launch_fp8_pairs(p, sms, s);
 }
 
 cudaError_t launch_quantize_fp8(const void* x, int type, int64_t ld, uint8_t* q, float* scales, int m, int k, cudaStream_t s) {
