@@ -10,19 +10,23 @@ namespace {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Products on CTA pairs: out[t, n] = sum over groups kb of 128 k's of (sum_k x[t, k] w[n, k]) sx[t, kb] sw[n / 128, kb].
-// Rows are operand A (256 a tile, 128 in each CTA), weights operand B (256 or 128 a tile; gated: half of them gate rows, which the leader stages, the
-// up rows its peer).  The tensor core sums one group into an accumulator of 128 columns, one of four (wide tiles: into two of them, one
-// after the other); the epilogue warps multiply it by the two scales and add it to FP32 registers, beside the next products.  A thread has one row of
-// the tile, so that its scale is one number a group; weights' scales are one for every 32 columns.  (Weights along the lanes instead: a scale for
-// every column and thread, 109 us where this takes 55.)  One warp brings the scales, word by word and up to three batches ahead.
+// Rows are operand A (256 a tile, 128 in each CTA), weights operand B (256 a tile; gated: half of them gate rows, which the leader stages, the up rows its
+// peer).  The tensor core sums one group into two accumulators of 128 columns, one after the other, of four; the epilogue warps multiply them by the two scales
+// and add them to FP32 registers, beside the next products.  Four warps have one accumulator of a group, four the other.  A thread has one row of the tile,
+// so that its scale is one number a group; weights' scales are one for every 32 columns.  (Weights along the lanes instead: a scale for every column and
+// thread, 109 us where this form began with 55.)  Columns come by sixteens beside the multiplications of the sixteen before, the next group's first ones too: 54.5
+// -> 50.7 us of a linear and 96 -> 90 of a gated product below.  One warp brings the scales, word by word and up to three batches ahead.
 //
-// What bounds it: the power limit, in calls that last.  3840 rows, wide: 2304 -> 5120 55 us in bursts and 59 repeated (1.54-1.65 PFLOP/s, at 1.83 GHz), gated 5120 ->
-// 2 x 2304 92 and 103 us (1.76-1.97, at 1.73 GHz).  With nothing done by the epilogue warps, 38 and 66 us in bursts and 46 and 83 repeated (at 1.55 GHz): that
-// is what products and copies alone would take.  The multiplications are what is left, 256 of a scheduler for each group of 256 columns; loads from
-// tensor memory are hidden.  A group of 256 columns costs 1150 clk, one of 128 columns 700.  Tried, project and gated (54.5, 93): the next group's
-// columns fetched ahead of this one's last multiplications 59, 104; packed pairs (fma.rn.f32x2), with each of which a move goes, 66, 107; sixteen epilogue
-// warps with 64 columns each 63, 97, or with 64 of 128 columns and every other group 74, 116; tiles of 192 columns 88, 160; whole accumulators of
-// 256 columns 60, 101; eight groups' scales by the epilogue warps themselves 60, 102.
+// Where at most half of the pairs had a tile in the last turn, its tiles come in two halves of their columns: one accumulator a group, which all
+// warps share.  50.7 -> 49.2 us (300 tiles for 74 pairs); 1021 rows, 5120 -> 5003 (80) 52.8 -> 46.1.
+//
+// What bounds it: the power limit, in calls that last.  3840 rows, 2304 -> 5120 49 us in bursts and 54.5 repeated (1.66-1.85 PFLOP/s), gated 5120 -> 2 x 2304 90
+// and 103.5 us (1.75-2.01).  With nothing done by the epilogue warps, 38.5 and 70 us in bursts and 46 and 83 repeated (at 1.55 GHz): that is what
+// products and copies alone would take; with loads from tensor memory alone 45 and 79 in bursts.  Tried, linear and gated (49, 90): all warps with 64 columns of
+// each accumulator 56, 102; 24 columns at a time 51.6, 90.9, and 32, for which registers are short, 53.8, 94; waits of the issuing warp that put it to
+// sleep 53, 96; one thread that issues 66, 128.  Before columns came by sixteens (54.5, 93): packed pairs (fma.rn.f32x2), with each of which a
+// move goes, 66, 107; sixteen epilogue warps with 64 columns each 63, 97; tiles of 192 columns 88, 160; whole accumulators of 256 columns 60, 101; eight groups'
+// scales by the epilogue warps themselves 60, 102.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFp8Unit = 128;                         // columns of an accumulator
 constexpr int kFp8Units = kTmemCols / kFp8Unit;
@@ -319,7 +323,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
         const int rows = fp8_rows_staged(g.valid, cta), x_row = g.first + cta * kGroupRows;
         const bool all = t < whole;
         const uint32_t tx = (fp8_rows_staged(g.valid, 0) + fp8_rows_staged(g.valid, 1)) * 128 + 2 * (all ? 2 * kFp8StageHalf : kFp8StageHalf);
-        const int w_row = g.channel0 + (kGate ? 0 : cta * kFp8Unit) + (all ? 0 : (t - whole & 1) * (kFp8Unit / 2)), part = kGate ? cta : 0;
+        const int w_row = g.channel0 + (kGate ? 0 : cta * kFp8Unit) + (all ? 0 : ((t - whole) & 1) * (kFp8Unit / 2)), part = kGate ? cta : 0;
         for (int kb = 0; kb < p.groups; ++kb) {
           if (!waiter.wait_uniform(empty0 + 8 * stage, phase ^ 1u)) { ok = false; break; }
           const uint32_t bar = leader_full0 + 8 * stage, a = base + stage * kFp8Stage;
@@ -389,7 +393,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
           w[side] = p.w_scales + (((int64_t)g.expert * (kGate ? 2 : 1) + up) * p.blocks + min(channel / kScaleBlock, p.blocks - 1)) * p.groups + group;
         }
         for (int kb = 0; kb < p.groups; kb += kFp8Batch, ++batch) {
-          if (!poll(waiter, smem_u32(&ctl->scale_empty[batch % kFp8ScaleSlots]), ((batch / kFp8ScaleSlots) & 1u) ^ 1u)) { ok = false; break; }
+          if (!waiter.wait_uniform(smem_u32(&ctl->scale_empty[batch % kFp8ScaleSlots]), ((batch / kFp8ScaleSlots) & 1u) ^ 1u)) { ok = false; break; }
           Fp8Scales& to = scales[batch % kFp8ScaleSlots];
           const bool there = kb + group < p.groups;
 #pragma unroll
