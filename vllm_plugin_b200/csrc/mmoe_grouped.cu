@@ -24,10 +24,11 @@ namespace {
 // What bounds it: the tensor cores, and in calls that last the power limit.  8 experts of 512 rows, gated 5120 -> 2 x 2304: 111 us (1.74 PFLOP/s; tensor
 // cores 90 % busy, 435 MB of memory where 420 are the least) alone, 158 at 1.24 GHz of one call after another; a dense product of as many operations by the
 // library 143.  46 experts with 23040 uneven rows, block 5120 -> 2304 -> 5120: 1.27 to 1.43 ms (1.14 to 1.28 PFLOP/s), all their weights read beside it.  3840 rows of
-// 8 experts with gradients: 720 to 740 us (1.1 PFLOP/s); through the second product 66 % and the gradients of the weights 68 to 73 % of the tensor cores' cycles,
+// 8 experts with gradients: 710 to 740 us (1.1 PFLOP/s); through the second product 66 % and the gradients of the weights 68 to 73 % of the tensor cores' cycles,
 // the rest goes into tiles that do not come out even and sums that leave (dw13 writes 378 MB).
-// Tried: the widest tile of an expert's rows chosen from 256, 224 ... 128 by the turns of the pairs: 1021 rows of one expert, block with gradients 208 -> 186 us,
-// but 48 experts with 6000 rows 593 -> 602, 300 rows of one 122 -> 127, 8 with 3840 741 -> 752.
+// Where at most half of the pairs had a tile in the last turn, its tiles come in two halves of their columns (those of more than 128; fewer cost what the
+// weights' bytes cost): 1021 rows of one expert, block with gradients 207 -> 184 us, 300 rows 122 -> 117, 3840 576 -> 567; not so the gradients of the
+// weights, whose tiles are many.  Tried: the widest tile chosen from 256, 224 ... 128 by the turns of the pairs, 186 us, but 48 experts with 6000 rows 593 -> 602.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kGroupCols = 256;                       // most rows of B per tile
 constexpr int kGroupStageA = kGroupRows * 128;        // bytes
@@ -75,9 +76,12 @@ struct GroupTile {
   int k_stages, k_first, k_rows;  // kGroupedWeights: the expert's rows
 };
 
+// The first `whole` tiles, then two parts of each of the others: halves of its columns, where it has more than 128, else all and none
 template <int kKind>
-__device__ __forceinline__ GroupTile tile_at(const GroupedParams& p, const GroupPlan* plan, int t) {
+__device__ __forceinline__ GroupTile tile_at(const GroupedParams& p, const GroupPlan* plan, int t, int whole) {
   GroupTile g;
+  const int part = kKind != kGroupedWeights && t >= whole ? (t - whole) & 1 : -1;
+  if (part >= 0) t = whole + (t - whole) / 2;
   if (kKind == kGroupedWeights) {
     const int each = p.row_tiles * p.col_tiles, in = t % each;
     g.expert = t / each;
@@ -86,16 +90,21 @@ __device__ __forceinline__ GroupTile tile_at(const GroupedParams& p, const Group
     g.valid = min(p.k - g.first, p.cols), g.cols = p.cols;
     g.k_first = plan->start[g.expert], g.k_rows = plan->start[g.expert + 1] - g.k_first;
     g.k_stages = (g.k_rows + 63) / 64;
-    return g;
+  } else {
+    const int low = expert_of(*plan, p.experts, t);
+    const int start = plan->start[low], count = plan->start[low + 1] - start, parts = (count + kGroupCols - 1) / kGroupCols;
+    const int in = t - plan->tile[low], width = ((count + parts - 1) / parts + 31) & ~31, at = in % parts * width;
+    g.expert = low;
+    g.row0 = in / parts * (kKind == kGated ? kGroupRows : 2 * kGroupRows);
+    g.first = start + at;
+    g.valid = min(count - at, width), g.cols = (g.valid + 31) & ~31;
+    g.k_stages = p.k_stages, g.k_first = g.k_rows = 0;
   }
-  const int low = expert_of(*plan, p.experts, t);
-  const int start = plan->start[low], count = plan->start[low + 1] - start, parts = (count + kGroupCols - 1) / kGroupCols;
-  const int in = t - plan->tile[low], width = ((count + parts - 1) / parts + 31) & ~31, at = in % parts * width;
-  g.expert = low;
-  g.row0 = in / parts * (kKind == kGated ? kGroupRows : 2 * kGroupRows);
-  g.first = start + at;
-  g.valid = min(count - at, width), g.cols = (g.valid + 31) & ~31;
-  g.k_stages = p.k_stages, g.k_first = g.k_rows = 0;
+  if (part >= 0) {
+    const int cut = g.cols > 128 ? (g.cols / 2 + 31) & ~31 : g.cols;
+    if (part == 0) g.valid = min(g.valid, cut), g.cols = cut;
+    else g.first += cut, g.valid -= cut, g.cols -= cut;
+  }
   return g;
 }
 
@@ -294,8 +303,10 @@ __global__ void __launch_bounds__(kGroupThreads, 1) grouped_pair_kernel(const __
   chain_release();                          // in this order: what precedes this launch is complete when the next one starts
   int tiles = make_plan(plan, p.ends, p.experts, p.rows, kGroupCols, p.row_tiles, p.status);
   if (kKind == kGroupedWeights) tiles = p.experts * p.row_tiles * p.col_tiles;
+  int whole = tiles;
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
   const int step = gridDim.x / 2;
+  if (kKind != kGroupedWeights && 2 * (tiles % step) <= step) whole = tiles / step * step, tiles += tiles - whole;        // the last turn in parts
   DenseWaiter waiter{{&ctl->abort_flag, p.status, 0, kStatusGrouped, warp}, p.timeout_ns};
   const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
   if (p.zero_behind) {
@@ -310,7 +321,8 @@ __global__ void __launch_bounds__(kGroupThreads, 1) grouped_pair_kernel(const __
     const uint32_t leader_full0 = map_to_cta(full0, 0), base = smem_u32(stages);
     bool ok = true;
     for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
-      const GroupTile g = tile_at<kKind>(p, plan, t);
+      const GroupTile g = tile_at<kKind>(p, plan, t, whole);
+      if (kKind != kGroupedWeights && g.valid <= 0) break;
       const int half = g.cols / 2;
       const uint32_t tx = 2 * (kGroupStageA + half * 128);
       const int a_row = g.row0 + static_cast<int>(cta) * (kKind == kGated ? kGroupRows / 2 : kGroupRows);
@@ -358,7 +370,8 @@ __global__ void __launch_bounds__(kGroupThreads, 1) grouped_pair_kernel(const __
       const uint64_t a_hi = operand_desc(kTurnedA, 8192), b_hi = operand_desc(kTurnedB, 8192);
       constexpr uint32_t kStepA = kTurnedA ? 2048 >> 4 : 2, kStepB = kTurnedB ? 2048 >> 4 : 2;
       for (int t = blockIdx.x / 2; ok && t < tiles; t += step) {
-        const GroupTile g = tile_at<kKind>(p, plan, t);
+        const GroupTile g = tile_at<kKind>(p, plan, t, whole);
+        if (kKind != kGroupedWeights && g.valid <= 0) break;
         const uint32_t idesc = p.idesc | (static_cast<uint32_t>(g.cols >> 3) << 17);
         if (!waiter.wait_uniform(smem_u32(&ctl->acc_empty[it & 1u]), ((it >> 1) & 1u) ^ 1u)) break;
         tc_fence_after();
@@ -389,7 +402,8 @@ __global__ void __launch_bounds__(kGroupThreads, 1) grouped_pair_kernel(const __
     s.turn = smem + kGroupTurnAt + (warp - 2) * kTurnBytes, s.lane = lane, s.channels = p.n;
     uint32_t it = 0;
     for (int t = blockIdx.x / 2; t < tiles; t += step) {
-      const GroupTile g = tile_at<kKind>(p, plan, t);
+      const GroupTile g = tile_at<kKind>(p, plan, t, whole);
+      if (kKind != kGroupedWeights && g.valid <= 0) break;
       s.channel0 = g.row0 + (static_cast<int>(cta) * 4 + quadrant) * (kKind == kGated ? 16 : 32);
       const int blocks = (g.cols + 31) / 32;
       const auto release = [&](uint32_t acc) {
@@ -519,7 +533,7 @@ cudaError_t launch_group_pairs(const GroupedProduct& p, int sms, cudaStream_t s)
     most = ((int64_t)p.rows / kGroupCols + std::min(p.experts, p.rows)) * d.row_tiles;
   }
   if (!ok || most > INT32_MAX / 2) return cudaErrorInvalidValue;
-  const int grid = 2 * static_cast<int>(std::min<int64_t>(sms / 2, most));
+  const int grid = 2 * static_cast<int>(std::min<int64_t>(sms / 2, 2 * most));       // every tile could come in two
   bool found = false;
   const cudaError_t e = for_each_group_kernel([&](auto kernel, int kind, bool k_turned) {
     if (kind != p.kind || k_turned != turned) return cudaSuccess;
