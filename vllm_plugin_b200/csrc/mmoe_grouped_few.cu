@@ -407,14 +407,16 @@ cudaError_t for_each_few_kernel(F f) {
 
 }  // namespace
 
-// Against pairs, 5120 x 5120 of one expert: 16 bits, 16 rows 17.6 -> 10.4 us, 64 18.2 -> 12.3, 128 19.3 -> 16.0, 192 23.3 -> 18.4, 256 28.9 -> 27.6; 8 bits, 16 rows
-// 15.8 -> 8.6, 64 16.2 -> 12.7, 128 16.6 -> 16.2, 192 16.8 -> 24.6.  More experts, 8 bits, gated 5120 -> 2 x 2304: 8 experts, 256 rows 50.2 -> 35.8, 500 62.5 -> 56.5, 600
-// 62.7 -> 62.5; 48 experts, 384 rows 266 -> 186, 2304 280 -> 218, 3600 292 -> 266, 5000 315 -> 371.  16 bits, 2304 -> 5120, where the tiles are more than run at
-// once: 8 experts, 64 rows 38.5 -> 41.6; 48 experts, 384 rows 176 -> 184; six of them, 240 tiles, 29.1 -> 28.0.
+// Against pairs.  16 bits, 5120 x 5120 of one expert: 16 rows 17.6 -> 10.4 us, 64 18.4 -> 12.1, 128 19.3 -> 16.0, 192 (120 tiles) 21.3 -> 22.1, 256 21.1 -> 28.5;
+// both products of a block of one, 5120 -> 2304 -> 5120: 64 rows 29.3 -> 21.3, 128 31.3 -> 29.1, 160 (108 and 120 tiles) 32.6 -> 40.1; two experts, 2048 x 2048, 300
+// rows (96 tiles) 11.0 -> 10.9; where the tiles are more than run at once, 2304 -> 5120: 8 experts, 64 rows 39.7 -> 42.0; 48 experts, 384 rows 176 -> 184;
+// six of them, 240 tiles, 29.1 -> 28.0.
+// 8 bits, 5120 x 5120 of one weight: 16 rows 15.8 -> 8.6, 64 16.2 -> 12.7, 128 16.6 -> 16.2, 192 16.8 -> 24.6; gated 5120 -> 2 x 2304: 8 experts, 256 rows 50.2 -> 35.8,
+// 500 62.5 -> 56.5, 600 62.7 -> 62.5; 48 experts, 384 rows 266 -> 186, 2304 280 -> 218, 3600 292 -> 266, 5000 315 -> 371.
 bool grouped_few_rows(const GroupedProduct& p, int sms) {
   if (p.w_k_rows || (p.kind != kLinear && p.kind != kGated)) return false;
   if (p.type == kGroupedE4m3) return p.rows <= std::max<int64_t>(128, 64 * (int64_t)p.experts);
-  return few_tiles(p) <= (p.rows <= kFewCols ? 2 * sms : sms);
+  return 3 * few_tiles(p) <= (p.rows <= kFewCols ? 6 : 2) * sms;
 }
 
 cudaError_t prepare_grouped_few() {
