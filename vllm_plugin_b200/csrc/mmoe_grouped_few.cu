@@ -412,7 +412,8 @@ cudaError_t for_each_few_kernel(F f) {
 // rows (96 tiles) 11.0 -> 10.9; where the tiles are more than run at once, 2304 -> 5120: 8 experts, 64 rows 39.7 -> 42.0; 48 experts, 384 rows 176 -> 184;
 // six of them, 240 tiles, 29.1 -> 28.0.
 // 8 bits, 5120 x 5120 of one weight: 16 rows 15.8 -> 8.6, 64 16.2 -> 12.7, 128 16.6 -> 16.2, 192 16.8 -> 24.6; gated 5120 -> 2 x 2304: 8 experts, 256 rows 50.2 -> 35.8,
-// 500 62.5 -> 56.5, 600 62.7 -> 62.5; 48 experts, 384 rows 266 -> 186, 2304 280 -> 218, 3600 292 -> 266, 5000 315 -> 371.
+// 500 62.5 -> 56.5, 600 62.7 -> 62.5; 48 experts, 384 rows 266 -> 186, 2304 280 -> 218, 3600 292 -> 266, 5000 315 -> 371.  Where all rows are one expert's
+// pairs are ahead (48 experts, 3000 rows 75 -> 181, 8 experts, 500 rows 19 -> 33), which is not known here; where half of them are, not (323 -> 261, 52 -> 53).
 bool grouped_few_rows(const GroupedProduct& p, int sms) {
   if (p.w_k_rows || (p.kind != kLinear && p.kind != kGated)) return false;
   if (p.type == kGroupedE4m3) return p.rows <= std::max<int64_t>(128, 64 * (int64_t)p.experts);
