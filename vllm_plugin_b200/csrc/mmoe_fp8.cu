@@ -112,6 +112,13 @@ __device__ __forceinline__ void arrive_twice(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0], 2;" ::"r"(bar) : "memory");
 }
 
+// tc_ld_wait, behind which alone v is used
+__device__ __forceinline__ void wait_for(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
+                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])::"memory");
+}
+
 // of a CTA's 128 rows, rounded up to the smallest box
 __device__ __forceinline__ int fp8_rows_staged(int valid, int cta) { return min(max(valid - cta * kGroupRows + 15, 0), kGroupRows) & ~15; }
 
@@ -222,12 +229,12 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
               to = fmaf(__uint_as_float(v[c & 1][i]), scale[c >> 1], to);
             }
           };
-          tc_ld_wait();
+          wait_for(v[0]);
 #pragma unroll
           for (int c = 1; c < 2 * kBlocks; ++c) {
             fetch(c);
             add(c - 1);
-            tc_ld_wait();
+            wait_for(v[c & 1]);
           }
           tc_fence_before();
           __syncwarp();
