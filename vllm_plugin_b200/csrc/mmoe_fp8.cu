@@ -23,10 +23,10 @@ namespace {
 // What bounds it: the power limit, in calls that last.  3840 rows, 2304 -> 5120 49 us in bursts and 54.5 repeated (1.66-1.85 PFLOP/s), gated 5120 -> 2 x 2304 90
 // and 103.5 us (1.75-2.01).  With nothing done by the epilogue warps, 38.5 and 70 us in bursts and 46 and 83 repeated (at 1.55 GHz): that is what
 // products and copies alone would take; with loads from tensor memory alone 45 and 79 in bursts.  Tried, linear and gated (49, 90): all warps with 64 columns of
-// each accumulator 56, 102; 24 columns at a time 51.6, 90.9, and 32, for which registers are short, 53.8, 94; waits of the issuing warp that put it to
-// sleep 53, 96; one thread that issues 66, 128.  Before columns came by sixteens (54.5, 93): packed pairs (fma.rn.f32x2), with each of which a
-// move goes, 66, 107; sixteen epilogue warps with 64 columns each 63, 97; tiles of 192 columns 88, 160; whole accumulators of 256 columns 60, 101; eight groups'
-// scales by the epilogue warps themselves 60, 102.
+// each accumulator 56, 102; one accumulator of 256 columns a group 51, 92; 24 columns at a time 51.6, 90.9, and 32, for which registers are short, 53.8, 94; packed
+// pairs (fma.rn.f32x2) 50, 89 and 55.3, 103 repeated; waits of the issuing warp that put it to sleep 53, 96; one thread that issues 66, 128.  Before columns
+// came by sixteens (54.5, 93): sixteen epilogue warps with 64 columns each 63, 97; tiles of 192 columns 88, 160; eight groups' scales by the epilogue
+// warps themselves 60, 102.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFp8Unit = 128;                         // columns of an accumulator
 constexpr int kFp8Units = kTmemCols / kFp8Unit;
