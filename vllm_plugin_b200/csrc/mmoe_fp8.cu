@@ -266,15 +266,16 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
         const int first = g.channel0 + (kWhole ? fp8_channel<kGate>(side, 2 * run) : fp8_half_channel<kGate>(side, 0, (t - whole) & 1));
         const int count = min(kRun, p.n - first);
         if (count <= 0) continue;
-        const auto value = [&](int j) {                  // of channel first + j
-          const float f = sum[2 * run + (j >> 5)][j & 31];
-          if (!kGate) return f;
-          const float u = sum[kBlocks / 2 + (j >> 5)][j & 31];
-          return p.epi.out_type == kDenseFp32 ? gated_value_fp32(f, u, p.epi.clamp) : gated_value(f, u, p.epi.clamp);
-        };
         const auto put = [&](auto* out) {
           using T = std::remove_pointer_t<decltype(out)>;
           constexpr int kEach = 16 / sizeof(T), kPart = 128 / sizeof(T), kStride = 144;       // 144: no two of eight rows in one bank
+          const auto value = [&](int j) {                // of channel first + j; no branch in it, so that the activations run beside each other (13.3 -> 10.4 us
+            const float f = sum[2 * run + (j >> 5)][j & 31];      // a tile of 2048 k's)
+            if constexpr (!kGate) return f;
+            const float u = sum[kBlocks / 2 + (j >> 5)][j & 31];
+            if constexpr (sizeof(T) == 4) return gated_value_fp32(f, u, p.epi.clamp);
+            else return gated_value(f, u, p.epi.clamp);
+          };
           out += (int64_t)row0 * p.epi.ld_out + first;
 #pragma unroll
           for (int part = 0; part < (kRun + kPart - 1) / kPart; ++part) {     // 128 bytes of every row
