@@ -20,13 +20,14 @@ namespace {
 // Where at most half of the pairs had a tile in the last turn, its tiles come in two halves of their columns: one accumulator a group, which all
 // warps share.  50.7 -> 49.2 us (300 tiles for 74 pairs); 1021 rows, 5120 -> 5003 (80) 52.8 -> 46.1.
 //
-// What bounds it: the power limit, in calls that last.  3840 rows, 2304 -> 5120 49 us in bursts and 54.5 repeated (1.66-1.85 PFLOP/s), gated 5120 -> 2 x 2304 90
-// and 103.5 us (1.75-2.01).  With nothing done by the epilogue warps, 38.5 and 70 us in bursts and 46 and 83 repeated (at 1.55 GHz): that is what
-// products and copies alone would take; with loads from tensor memory alone 45 and 79 in bursts.  Tried, linear and gated (49, 90): all warps with 64 columns of
+// What bounds it: the power limit, in calls that last.  3840 rows, 2304 -> 5120 49 us in bursts and 54.5 repeated (1.66-1.85 PFLOP/s), gated 5120 -> 2 x 2304 84
+// and 98 us (1.85-2.16).  With nothing done by the epilogue warps, 38.5 and 70 us in bursts and 46 and 83 repeated (at 1.55 GHz): that is what
+// products and copies alone would take.  Multiplications take another 6 and 9, writing the results, which the next tile's sums wait for, 6 and 6.
+// Tried, linear and gated (49 and then 90): all warps with 64 columns of
 // each accumulator 56, 102; one accumulator of 256 columns a group 51, 92; 24 columns at a time 51.6, 90.9, and 32, for which registers are short, 53.8, 94; packed
 // pairs (fma.rn.f32x2) 50, 89 and 55.3, 103 repeated; waits of the issuing warp that put it to sleep 53, 96; one thread that issues 66, 128.  Before columns
 // came by sixteens (54.5, 93): sixteen epilogue warps with 64 columns each 63, 97; tiles of 192 columns 88, 160; eight groups' scales by the epilogue
-// warps themselves 60, 102.
+// warps themselves 60, 102.  Results by one bulk copy a row, when these were 49 and 84: 55, 86.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFp8Unit = 128;                         // columns of an accumulator
 constexpr int kFp8Units = kTmemCols / kFp8Unit;
@@ -269,8 +270,9 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
         const auto put = [&](auto* out) {
           using T = std::remove_pointer_t<decltype(out)>;
           constexpr int kEach = 16 / sizeof(T), kPart = 128 / sizeof(T), kStride = 144;       // 144: no two of eight rows in one bank
-          const auto value = [&](int j) {                // of channel first + j; no branch in it, so that the activations run beside each other (13.3 -> 10.4 us
-            const float f = sum[2 * run + (j >> 5)][j & 31];      // a tile of 2048 k's)
+          // of channel first + j; no branch in it, so that the activations run beside each other: a tile of 2048 k's 13.3 -> 11.4 us
+          const auto value = [&](int j) {
+            const float f = sum[2 * run + (j >> 5)][j & 31];
             if constexpr (!kGate) return f;
             const float u = sum[kBlocks / 2 + (j >> 5)][j & 31];
             if constexpr (sizeof(T) == 4) return gated_value_fp32(f, u, p.epi.clamp);

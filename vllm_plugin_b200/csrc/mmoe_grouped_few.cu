@@ -411,12 +411,20 @@ cudaError_t for_each_few_kernel(F f) {
 // both products of a block of one, 5120 -> 2304 -> 5120: 64 rows 29.3 -> 21.3, 128 31.3 -> 29.1, 160 (108 and 120 tiles) 32.6 -> 40.1; two experts, 2048 x 2048, 300
 // rows (96 tiles) 11.0 -> 10.9; where the tiles are more than run at once, 2304 -> 5120: 8 experts, 64 rows 39.7 -> 42.0; 48 experts, 384 rows 176 -> 184;
 // six of them, 240 tiles, 29.1 -> 28.0.
-// 8 bits, 5120 x 5120 of one weight: 16 rows 15.8 -> 8.6, 64 16.2 -> 12.7, 128 16.6 -> 16.2, 192 16.8 -> 24.6; gated 5120 -> 2 x 2304: 8 experts, 256 rows 50.2 -> 35.8,
-// 500 62.5 -> 56.5, 600 62.7 -> 62.5; 48 experts, 384 rows 266 -> 186, 2304 280 -> 218, 3600 292 -> 266, 5000 315 -> 371.  Where all rows are one expert's
-// pairs are ahead (48 experts, 3000 rows 75 -> 181, 8 experts, 500 rows 19 -> 33), which is not known here; where half of them are, not (323 -> 261, 52 -> 53).
+// 8 bits, 5120 x 5120 of one weight: 16 rows 16.0 -> 8.6, 64 16.2 -> 12.7, 128 16.6 -> 16.2, 192 16.8 -> 24.6.  More experts: a tile of few rows costs 560 clk a group of k and
+// 6000, one of pairs (a half of it, which one SM has) 1026 and 2700.  16 experts, gated 1024 -> 2 x 512: 300 rows 11.1 -> 8.6.  48, gated 5120 -> 2 x 2304: 384
+// rows 257 -> 188, 2304 271 -> 219, 2976 274 -> 239, 5000 285 -> 339.  48, 2304 -> 5120: 384 133 -> 112, 2304 140 -> 128, 3000 143 -> 145.  128, gated 2048 -> 2 x 768: 512
+// 94 -> 77, 4096 104 -> 93, 8192 108 -> 121.  128, 768 -> 2048: 512 57 -> 60, 4096 64 -> 75.  Where all rows are one expert's pairs are ahead (48 experts, 3000 rows
+// 75 -> 181, 8 experts, 500 rows 19 -> 33), which is not known here; where half of them are, not (323 -> 261, 52 -> 53).
 bool grouped_few_rows(const GroupedProduct& p, int sms) {
   if (p.w_k_rows || (p.kind != kLinear && p.kind != kGated)) return false;
-  if (p.type == kGroupedE4m3) return p.rows <= std::max<int64_t>(128, 64 * (int64_t)p.experts);
+  if (p.type == kGroupedE4m3) {
+    if (p.rows <= 128) return true;
+    const int64_t each = (p.rows + p.experts - 1) / p.experts, groups = (p.k + kScaleBlock - 1) / kScaleBlock;
+    if (each > kFewCols) return false;
+    // an expert's rows come in each / 64 + 1/2 tiles on average, one at least
+    return few_tiles(p) <= 2 * sms || std::max<int64_t>(kFewCols, each + kFewCols / 2) * (560 * groups + 6000) <= kFewCols * (1026 * groups + 2700);
+  }
   return 3 * few_tiles(p) <= (p.rows <= kFewCols ? 6 : 2) * sms;
 }
 
