@@ -23,11 +23,11 @@ namespace {
 // What bounds it: the power limit, in calls that last.  3840 rows, 2304 -> 5120 49 us in bursts and 54.5 repeated (1.66-1.85 PFLOP/s), gated 5120 -> 2 x 2304 84
 // and 98 us (1.85-2.16).  With nothing done by the epilogue warps, 38.5 and 70 us in bursts and 46 and 83 repeated (at 1.55 GHz): that is what
 // products and copies alone would take.  Multiplications take another 6 and 9, writing the results, which the next tile's sums wait for, 6 and 6.
-// Tried, linear and gated (49 and then 90): all warps with 64 columns of
-// each accumulator 56, 102; one accumulator of 256 columns a group 51, 92; 24 columns at a time 51.6, 90.9, and 32, for which registers are short, 53.8, 94; packed
-// pairs (fma.rn.f32x2) 50, 89 and 55.3, 103 repeated; waits of the issuing warp that put it to sleep 53, 96; one thread that issues 66, 128.  Before columns
-// came by sixteens (54.5, 93): sixteen epilogue warps with 64 columns each 63, 97; tiles of 192 columns 88, 160; eight groups' scales by the epilogue
-// warps themselves 60, 102.  Results by one bulk copy a row, when these were 49 and 84: 55, 86.
+// Tried, linear and gated (49 and then 90): all warps with 64 columns of each accumulator 56, 102; one accumulator of 256 columns a group 51, 92; 24 columns at
+// a time 51.6, 90.9, and 32, for which registers are short, 53.8, 94; packed pairs (fma.rn.f32x2) 50, 89 and 55.3, 103 repeated; waits of the issuing warp
+// that put it to sleep 53, 96; one thread that issues 66, 128.  Before columns came by sixteens (54.5, 93): sixteen epilogue warps with 64 columns each 63, 97;
+// tiles of 192 columns 88, 160; eight groups' scales by the epilogue warps themselves 60, 102.  When these were 49 and 84: results by one bulk copy a row 55, 86; by a
+// warp of their own, with four stages instead of five, 50, 87.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFp8Unit = 128;                         // columns of an accumulator
 constexpr int kFp8Units = kTmemCols / kFp8Unit;
