@@ -487,7 +487,7 @@ __device__ __forceinline__ float odd_quotient(float x, float s, float inv) {
   const float rest = fmaf(-q, s, x);
   uint32_t bits = __float_as_uint(q);
   if (rest != 0.f) {
-    if ((rest < 0.f) != (q < 0.f)) --bits;       // towards zero ...
+    if ((rest < 0.f) != (x < 0.f)) --bits;       // towards zero (a q that is one, where the quotient leaves the numbers, has all of x left and stays) ...
     bits |= 1u;                                  // ... and marked
   }
   return __uint_as_float(bits);
