@@ -398,10 +398,10 @@ int mmoe_grouped_feed_forward_grad(const MmoeGroupedFeedForward* ff, const void*
 
 /* Quantiser: for each 128 values of a row (the last group may have fewer) scale = max|x| / 448 (1 for zeros), q = x / scale to the nearest E4M3 value,
  * ties to even, by that scale as it is in FP32.  A group that holds an infinity or a NaN gets the scale NaN and zeros.  x: `type` BF16 or FP16,
- * [M, K] with `x_stride` elements between rows, any K; q [M, K]; scales float [M, ceil(K / 128)]. */
+ * [M, K] with `x_stride` elements between rows, any K; q [M, K]; scales float [M, ceil(K / 128)].  x, q and scales on their elements' size. */
 int mmoe_quantize_fp8(const void* x, int32_t type, int64_t x_stride, void* q, float* scales, int32_t num_rows, int32_t width, void* stream);
 
-/* Products of E4M3 values with FP32 scales; sums over 128 values in the tensor core, over those in FP32. */
+/* Products of E4M3 values with FP32 scales (on 4 bytes); sums over 128 values in the tensor core, over those in FP32. */
 typedef struct MmoeFp8Product {
   int32_t num_rows;           /* T */
   int32_t num_experts;        /* E, 1 to 1024; 1 without ends */

@@ -5,13 +5,15 @@
 
 namespace {
 
+bool aligned(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
 // tiles and rows of all experts are 32-bit numbers
 constexpr int32_t kMostGroupedChannels = 1 << 20;
 
 int check_grouping(const char* what, int32_t rows, int32_t experts, const int32_t* ends) {
   if (rows < 0 || rows > kMostTokens) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: num_rows=%d outside [0, %d]", what, rows, kMostTokens);
   if (experts < 1 || experts > mmoe::kMaxExperts) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: num_experts=%d outside [1, %d]", what, experts, mmoe::kMaxExperts);
-  if (ends == nullptr || (reinterpret_cast<uintptr_t>(ends) & 3u) != 0) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: ends must not be NULL and on 4 bytes", what);
+  if (ends == nullptr || !aligned(ends, 4)) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: ends must not be NULL and on 4 bytes", what);
   return MMOE_OK;
 }
 
@@ -108,6 +110,7 @@ int fp8_product(const MmoeFp8Product* a, bool gated, void* stream) {
   if (a->num_rows == 0) return MMOE_OK;
   if (a->x_scales == nullptr || a->w == nullptr || a->w_scales == nullptr || a->out == nullptr) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: pointers must not be NULL", what);
   if (!aligned16(a->x) || !aligned16(a->w) || !aligned16(a->out)) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: x, w and out must be 16-byte aligned", what);
+  if (!aligned(a->x_scales, 4) || !aligned(a->w_scales, 4)) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: scales must be on 4 bytes", what);
   mmoe::GroupedProduct p = product_of(mmoe::kGroupedE4m3, a->num_rows, a->num_experts, a->ends, a->status, a->timeout_ms);
   p.kind = gated ? mmoe::kGated : mmoe::kLinear;
   p.n = a->channels, p.k = a->width, p.w = a->w, p.x = a->x, p.x_ld = a->x_stride, p.x_scales = a->x_scales, p.w_scales = a->w_scales;
@@ -196,6 +199,7 @@ int mmoe_quantize_fp8(const void* x, int32_t type, int64_t x_stride, void* q, fl
   if (x_stride < width) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: x_stride must be at least width=%d", what, width);
   if (num_rows == 0) return MMOE_OK;
   if (x == nullptr || q == nullptr || scales == nullptr) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: pointers must not be NULL", what);
+  if (!aligned(x, 2) || !aligned(scales, 4)) return fail(MMOE_ERR_INVALID_ARGUMENT, "%s: x must be on 2 bytes and scales on 4", what);
   const cudaError_t e = mmoe::launch_quantize_fp8(x, type, x_stride, static_cast<uint8_t*>(q), scales, num_rows, width, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MMOE_OK : cuda_fail(e, what);
 }
