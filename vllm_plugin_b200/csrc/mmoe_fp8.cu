@@ -138,11 +138,11 @@ __device__ __forceinline__ bool poll(DenseWaiter& w, uint32_t bar, uint32_t pari
 }
 
 // Where the phase has mostly completed: two probes, then as everybody waits, by a waiter of its own, which takes no registers meanwhile
-__device__ __forceinline__ bool probe_then_wait(volatile int32_t* abort_flag, int32_t* status, int64_t timeout_ns, uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool probe_then_wait(const Fp8Params& p, Fp8Control* ctl, uint32_t bar, uint32_t parity) {
   bool there = mbar_try_wait(bar, parity);
   if (!there) there = mbar_try_wait(bar, parity);
   if (__all_sync(0xffffffffu, there)) return true;
-  DenseWaiter slow{{abort_flag, status, 0, kStatusGrouped + 1, static_cast<int>(threadIdx.x >> 5)}, timeout_ns};
+  DenseWaiter slow{{&ctl->abort_flag, p.status, 0, kStatusGrouped + 1, static_cast<int>(threadIdx.x >> 5)}, p.timeout_ns};
   return slow.wait_uniform(bar, parity);
 }
 
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_pair_kernel(const __grid_c
     uint8_t* turn = smem + kFp8TurnAt + warp * kFp8Turn;
     const uint32_t full = smem_u32(&ctl->acc_full[0]), sums = tmem_base + lanes;
     uint32_t batch = 0, phase = 0, unit = side;       // the accumulator whose turn it is
-    const auto wait = [&](uint32_t bar, uint32_t parity) { return probe_then_wait(&ctl->abort_flag, p.status, p.timeout_ns, bar, parity); };
+    const auto wait = [&](uint32_t bar, uint32_t parity) { return probe_then_wait(p, ctl, bar, parity); };
     const auto tile = [&](auto all, int t) {           // a whole one, or half of one
       constexpr bool kWhole = all.value;
       constexpr int kBlocks = kWhole ? 4 : 2;            // of 32 columns; gated: the gate's, then the up rows'
