@@ -183,7 +183,8 @@ def grouped_projection(x, w, ends):
 
 def grouped_feed_forward(x, w13, w2, ends, *, activation_clamp: Optional[float] = None):
     """:func:`gated_feed_forward` with the weights of each row's expert, with its gradients: ``x`` ``(T, H)``, ``w13`` ``(E, 2 I, H)`` in checkpoint order, the
-    gate's rows first, ``w2`` ``(E, H, I)``; rows and ``ends`` as in :func:`grouped_projection`.  Returns ``(T, H)``."""
+    gate's rows first, ``w2`` ``(E, H, I)``; rows and ``ends`` as in :func:`grouped_projection`.  Returns ``(T, H)``.  As there, ``h`` and in the backward pass the
+    gradients of g and u are rounded to the type, as operands of the next product: in FP16 they overflow past 65504."""
     global _grouped_feed_forward
     if _grouped_feed_forward is None:
         from .backend.grouped import grouped_feed_forward as _grouped_feed_forward

@@ -23,12 +23,18 @@ namespace {
 //
 // What bounds it: the tensor cores, and in calls that last the power limit.  8 experts of 512 rows, gated 5120 -> 2 x 2304: 111 us (1.74 PFLOP/s; tensor
 // cores 90 % busy, 435 MB of memory where 420 are the least) alone, 158 at 1.24 GHz of one call after another; a dense product of as many operations by the
-// library 143.  46 experts with 23040 uneven rows, block 5120 -> 2304 -> 5120: 1.27 to 1.43 ms (1.14 to 1.28 PFLOP/s), all their weights read beside it.  3840 rows of
-// 8 experts with gradients: 710 to 740 us (1.1 PFLOP/s); through the second product 66 % and the gradients of the weights 68 to 73 % of the tensor cores' cycles,
+// library 143.  46 experts with 23040 uneven rows, block 5120 -> 2304 -> 5120: 1.24 to 1.30 ms in bursts (1.25 to 1.31 PFLOP/s), 1.55 to 1.74 in calls that last, all
+// their weights read beside it.  3840 rows of 7 experts with gradients: 710 to 720 us in bursts (1.1 PFLOP/s); through the second product 66 % and the gradients of the weights 68 to 73 % of the tensor cores' cycles,
 // the rest goes into tiles that do not come out even and sums that leave (dw13 writes 378 MB).
 // Where at most half of the pairs had a tile in the last turn, its tiles come in two halves of their columns (those of more than 128; fewer cost what the
 // weights' bytes cost): 1021 rows of one expert, block with gradients 207 -> 184 us, 300 rows 122 -> 117, 3840 576 -> 567; not so the gradients of the
-// weights, whose tiles are many.  Tried: the widest tile chosen from 256, 224 ... 128 by the turns of the pairs, 186 us, but 48 experts with 6000 rows 593 -> 602.
+// weights, whose tiles are many.
+//
+// h, and in the backward pass dg and du, leave in the type of the operands: the next product multiplies them as such.  FP32 operands would be rounded as well (to
+// TF32, eleven bits), at half the rate, with twice the bytes and weights that had to be widened.  The rounding takes a block's error against 64 bits from
+// 0.0017 to 0.0024 of the result's norm in BF16 and from 0.00021 to 0.00029 in FP16; in FP16 an h past 65504 is an infinity.
+//
+// Tried: the widest tile chosen from 256, 224 ... 128 by the turns of the pairs, 186 us, but 48 experts with 6000 rows 593 -> 602.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kGroupCols = 256;                       // most rows of B per tile
 constexpr int kGroupStageA = kGroupRows * 128;        // bytes
@@ -475,15 +481,15 @@ __global__ void __launch_bounds__(kGroupThreads, 1) grouped_pair_kernel(const __
 // ---------------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------------
-// Weights [experts][n][k], boxes of `box` rows by 128 bytes of K; stored as [k][n] (k_rows): of 64 rows by 64 k's.  In three dimensions, so that a box
+// Weights [experts][n][k], boxes of a CTA's rows by 128 bytes of K; stored as [k][n] (k_rows): of 64 rows by 64 k's.  In three dimensions, so that a box
 // ends with its expert.
-bool encode_weights(CUtensorMap* map, const GroupedProduct& p, uint32_t box) {
+bool encode_weights(CUtensorMap* map, const GroupedProduct& p) {
   const uint64_t n = p.n, k = p.k, e = p.experts;
   if (p.kind == kGated) {                      // eight gate rows, eight up rows, the next eight gate rows ...
-    return encode_map(map, p.type, p.w, 5, {k, 8, 2, n / 8, e}, {2 * k, 2 * n * k, 16 * k, 4 * n * k}, {64, 8, 2, box / 16, 1});
+    return encode_map(map, p.type, p.w, 5, {k, 8, 2, n / 8, e}, {2 * k, 2 * n * k, 16 * k, 4 * n * k}, {64, 8, 2, kGroupRows / 16, 1});
   }
   if (p.w_k_rows) return encode_map(map, p.type, p.w, 3, {n, k, e, 1, 1}, {2 * n, 2 * n * k, 0, 0}, {64, 64, 1, 1, 1});
-  return encode_map(map, p.type, p.w, 3, {k, n, e, 1, 1}, {2 * k, 2 * n * k, 0, 0}, {64, box, 1, 1, 1});
+  return encode_map(map, p.type, p.w, 3, {k, n, e, 1, 1}, {2 * k, 2 * n * k, 0, 0}, {64, kGroupRows, 1, 1, 1});
 }
 
 // Rows [rows][width], boxes of 128 bytes by `box` rows
@@ -528,7 +534,7 @@ cudaError_t launch_group_pairs(const GroupedProduct& p, int sms, cudaStream_t s)
     ok = encode_summed(&d.map_a, p, p.left, p.left_ld, p.n) && encode_summed(&d.map_b[0], p, p.x, p.x_ld, p.k);
     most = (int64_t)p.experts * d.row_tiles * d.col_tiles;
   } else {
-    ok = encode_weights(&d.map_a, p, kGroupRows);
+    ok = encode_weights(&d.map_a, p);
     for (int i = 0; ok && i < 4; ++i) ok = encode_rows(&d.map_b[i], p, 128 >> i);
     most = ((int64_t)p.rows / kGroupCols + std::min(p.experts, p.rows)) * d.row_tiles;
   }

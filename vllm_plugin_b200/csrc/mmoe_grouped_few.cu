@@ -1,6 +1,5 @@
 // Products of a layer's experts with few rows each, for sm_100a (see mmoe_grouped.cuh).
 #include <algorithm>
-#include <atomic>
 
 #include "mmoe_grouped_device.cuh"
 
@@ -12,7 +11,7 @@ namespace {
 // Bound by the bytes of the weights: a CTA has 128 rows of an expert's weights (operand A; gated: 64 gate and 64 up rows) and up to 64 of its rows
 // (operand B, padded to 16), so that a handful of rows costs what their weights cost.  Two CTAs to an SM.  Where that leaves SMs without one, K
 // is split over the CTAs of a cluster, whose partial sums meet in shared memory in the order of the CTAs, as those of the dense products
-// of few tokens do: no atomics, no workspace, the same bits in every call.  The grid has a CTA for every tile there could be; which one it is follows
+// of few tokens do: no atomics, no workspace, the same bits in every call.  h is rounded to its type, as on pairs.  The grid has a CTA for every tile there could be; which one it is follows
 // from `ends`, and those beyond the last leave at once.
 //
 // 8 bits: a group of 128 k's goes into one of four accumulators.  Four warps, a lane for each row of weights, multiply it by its scales and add it
@@ -382,7 +381,8 @@ int64_t few_tiles(const GroupedProduct& p) {
 
 // CTAs that share a tile's K, by what their stages cost (twice that where two share an SM) and what meeting costs, in clocks.  With 1, 2, 3, 4, 6 of them,
 // 8 bits, 5120 -> 5120 (40 tiles): one row 15.0, 10.0, 8.4, 8.4, 8.0 us, 64 rows 24.0, 14.9, 12.7, 13.9, 13.3; 128 rows (80 tiles) 24.2, 18.8, 16.0, 23.1, -; gated
-// 5120 -> 2 x 2304 (72) 24.4, 15.4, 16.0, 22.9, -; 2304 -> 1024 (8), one row 8.4, 6.6, 5.7, 5.3, 5.1, 64 rows 13.3, 9.6, 8.4, 7.8, 7.2.  Clusters of 7 and 8 take longer.
+// 5120 -> 2 x 2304 (72), 128 rows, 24.4, 15.4, 16.0, 22.9, -; 2304 -> 1024 (8), one row 8.4, 6.6, 5.7, 5.3, 5.1, 64 rows 13.3, 9.6, 8.4, 7.8, 7.2.  Clusters of 7 and 8 take longer.
+// The columns are those of a call of one expert; with more of them an expert's are fewer, and the cost of a stage is taken to be too high.
 int few_split(const GroupedProduct& p, int64_t tiles, int k_stages, int sms) {
   const int cols = std::min((p.rows + 15) & ~15, kFewCols);
   const int64_t stage = p.type == kGroupedE4m3 ? 475 + 6 * cols : 340 + cols;
@@ -411,7 +411,10 @@ cudaError_t for_each_few_kernel(F f) {
 // both products of a block of one, 5120 -> 2304 -> 5120: 64 rows 29.3 -> 21.3, 128 31.3 -> 29.1, 160 (108 and 120 tiles) 32.6 -> 40.1; two experts, 2048 x 2048, 300
 // rows (96 tiles) 11.0 -> 10.9; where the tiles are more than run at once, 2304 -> 5120: 8 experts, 64 rows 39.7 -> 42.0; 48 experts, 384 rows 176 -> 184;
 // six of them, 240 tiles, 29.1 -> 28.0.
-// 8 bits, 5120 x 5120 of one weight: 16 rows 16.0 -> 8.6, 64 16.2 -> 12.7, 128 16.6 -> 16.2, 192 16.8 -> 24.6.  More experts: a tile of few rows costs 560 clk a group of k and
+// 8 bits, 5120 x 5120 of one weight: 16 rows 16.0 -> 8.6, 64 16.2 -> 12.7, 128 16.6 -> 16.2, 192 16.8 -> 24.6.  That line at 128 rows was drawn there; between 64 and it
+// the weights are read for two tiles, which costs more the wider they are.  65 and 128 rows: 2304 -> 5120 10.3 -> 9.7, 10.4 -> 11.6; gated 5120 -> 2 x 2304 16.3 -> 13.8,
+// 16.3 -> 15.4; gated 2048 -> 2 x 768 9.2 -> 6.8, 9.3 -> 7.4; 1024 -> 16384 10.5 -> 9.6, 10.9 -> 10.8; gated 5120 -> 2 x 8192 26.5 -> 27.7, 26.6 -> 31.7; 8192 -> 8192
+// 24.1 -> 32.1, 24.1 -> 37.0; 8192 -> 16384 36.8 -> 40.3, 37.0 -> 46.1; gated 8192 -> 2 x 8192 37.3 -> 40.9, 37.7 -> 46.5.  More experts: a tile of few rows costs 560 clk a group of k and
 // 6000, one of pairs (a half of it, which one SM has) 1026 and 2700.  16 experts, gated 1024 -> 2 x 512: 300 rows 11.1 -> 8.6.  48, gated 5120 -> 2 x 2304: 384
 // rows 257 -> 188, 2304 271 -> 219, 2976 274 -> 239, 5000 285 -> 339.  48, 2304 -> 5120: 384 133 -> 112, 2304 140 -> 128, 3000 143 -> 145.  128, gated 2048 -> 2 x 768: 512
 // 94 -> 77, 4096 104 -> 93, 8192 108 -> 121.  128, 768 -> 2048: 512 57 -> 60, 4096 64 -> 75.  Where all rows are one expert's pairs are ahead (48 experts, 3000 rows
